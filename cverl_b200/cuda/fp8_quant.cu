@@ -1,0 +1,501 @@
+// Block-scaled 8-bit quantisation: one pass over a bf16 or fp32 matrix that writes its codes and scales in the row
+// form, the transposed form, or both, and the same with one scale per 128 x 128 block for weights.
+//
+// Bound by HBM: 2 bytes read and 1 written per element and form (bf16), no arithmetic to speak of.  One CTA takes a
+// 128 x 128 tile, the smallest piece that holds whole blocks of both forms: a thread keeps 8 rows x 8 columns in
+// registers, a half-warp covers the 128 columns of a row (256 bytes a load), so a row block's maximum is four
+// shuffles and a column block's is eight values per thread and one shared-memory maximum.  Both forms come from the
+// registers of the one read; only the transposed codes pass through shared memory.
+#include "fp8_common.cuh"
+
+namespace cvb {
+
+constexpr int QT = 128;            // tile edge
+constexpr int Q_THREADS = 256;
+
+struct QuantArgs {
+  const void* x;
+  long long rows, cols, x_stride;
+  int vec;                         // base and row stride are 16-byte aligned
+  uint8_t *q, *sf;                 // row form
+  long long q_ld;
+  int kgroups;                     // ceil(ceil(cols / 128) / 4)
+  uint8_t *qt, *sft;               // transposed form
+  long long qt_ld;
+  int kgroups_t;
+  int col_tiles;
+  // values are x * rstd[row] * (w_offset + w[col]) where rstd is given
+  const float* rstd;
+  const __nv_bfloat16* w;
+  float w_offset;
+};
+
+template <typename T, int FMT, bool ROWS, bool COLS, bool BLOCK>
+__global__ void __launch_bounds__(Q_THREADS)
+fp8_quant_kernel(const QuantArgs p) {
+  __shared__ uint32_t s_max[QT];                                   // column maxima; [0] is the tile's for BLOCK
+  __shared__ __align__(16) uint8_t s_t[COLS ? QT * QT : 16];       // transposed codes, 8-byte units XOR-swizzled
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cl = lane & 15, rg = warp * 2 + (lane >> 4);           // columns 8 cl .. + 7, rows 8 rg .. + 7 of the tile
+  const long long tile_r = blockIdx.x / p.col_tiles;
+  const int tile_c = blockIdx.x - static_cast<int>(tile_r * p.col_tiles);
+  const long long r0 = tile_r * QT + rg * 8;
+  const long long c0 = static_cast<long long>(tile_c) * QT + cl * 8;
+  if (COLS || BLOCK) {
+    if (threadIdx.x < QT) s_max[threadIdx.x] = 0u;
+    __syncthreads();
+  }
+  const int nc = static_cast<int>(max(0ll, min(8ll, p.cols - c0)));
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    fp8_load8(static_cast<const T*>(p.x) + (r0 + i) * p.x_stride + c0, r0 + i < p.rows ? nc : 0, p.vec, v[i]);
+  if (p.rstd != nullptr) {
+    float g[8];
+    fp8_load8(p.w + c0, nc, (reinterpret_cast<uintptr_t>(p.w) & 15) == 0, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float rs = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = r0 + i < p.rows && j < nc ? v[i][j] * rs * (p.w_offset + g[j]) : 0.f;
+    }
+  }
+  bool odd = false;
+  uint32_t rmax[8], cmax[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rmax[i] = cmax[i] = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t m = fp8_mag(v[i][j], &odd);
+      rmax[i] = max(rmax[i], m);
+      cmax[j] = max(cmax[j], m);
+    }
+  uint32_t tile_byte = 0;
+  if (BLOCK) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, rmax[i]);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) atomicMax(&s_max[0], m);
+    __syncthreads();
+    tile_byte = fp8_scale_byte<FMT>(s_max[0]);
+  }
+  if (ROWS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = rmax[i];
+      if (!BLOCK) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      }
+      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(m);
+      // the tile's rows all get a scale, those past the matrix too: the tensor core reads 128 at a time
+      if (cl == 0) p.sf[fp8_sf_offset(r0 + i, tile_c, p.kgroups)] = static_cast<uint8_t>(byte);
+      if (r0 + i < p.rows && c0 < p.q_ld)
+        *reinterpret_cast<uint2*>(p.q + (r0 + i) * p.q_ld + c0) = fp8_pack8<FMT>(v[i], fp8_inverse_scale(byte), odd);
+    }
+  }
+  if (COLS) {
+    if (!BLOCK) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t m = max(cmax[j], __shfl_xor_sync(0xffffffffu, cmax[j], 16));
+        if (lane < 16) atomicMax(&s_max[cl * 8 + j], m);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(s_max[cl * 8 + j]);
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = v[i][j];
+      // 8-byte unit rg of column 8 cl + j sits at unit rg ^ cl: the 16 lanes of a half-warp hit 16 different units
+      *reinterpret_cast<uint2*>(s_t + (cl * 8 + j) * QT + (rg ^ cl) * 8) = fp8_pack8<FMT>(t, fp8_inverse_scale(byte), odd);
+    }
+    __syncthreads();
+    const long long out_c = tile_r * QT;
+#pragma unroll
+    for (int it = 0; it < QT / 16; ++it) {
+      const int c = it * 16 + rg;                   // a half-warp writes the 128 bytes of one transposed row
+      const long long col = static_cast<long long>(tile_c) * QT + c;
+      if (col < p.cols && out_c + cl * 8 < p.qt_ld)
+        *reinterpret_cast<uint2*>(p.qt + col * p.qt_ld + out_c + cl * 8) =
+            *reinterpret_cast<const uint2*>(s_t + c * QT + (cl ^ ((c >> 3) & 15)) * 8);
+    }
+    if (threadIdx.x < QT)
+      p.sft[fp8_sf_offset(static_cast<long long>(tile_c) * QT + threadIdx.x, static_cast<int>(tile_r), p.kgroups_t)] =
+          static_cast<uint8_t>(BLOCK ? tile_byte : fp8_scale_byte<FMT>(s_max[threadIdx.x]));
+  }
+}
+
+// scale bytes in the plain order [rows, blocks] for inspection and for other programs
+__global__ void fp8_scales_kernel(const uint8_t* __restrict__ sf, uint8_t* __restrict__ out, long long rows, int nb) {
+  const int kgroups = (nb + 3) / 4;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows * nb;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long r = i / nb;
+    out[i] = sf[fp8_sf_offset(r, static_cast<int>(i - r * nb), kgroups)];
+  }
+}
+
+template <typename T, int FMT>
+static void quant_launch(const QuantArgs& p, int mode, long long grid, cudaStream_t s) {
+  const dim3 g(static_cast<unsigned>(grid));
+  switch (mode) {
+    case 1: fp8_quant_kernel<T, FMT, true, false, false><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 2: fp8_quant_kernel<T, FMT, false, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 3: fp8_quant_kernel<T, FMT, true, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 5: fp8_quant_kernel<T, FMT, true, false, true><<<g, Q_THREADS, 0, s>>>(p); break;
+    default: fp8_quant_kernel<T, FMT, true, true, true><<<g, Q_THREADS, 0, s>>>(p); break;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// h = x + resid (rounded to bf16, as a consumer reading it back would see it); y = h * rstd * (w_offset + w) in fp32,
+// quantised without a bf16 rounding between.  Bound by HBM: 2 (x) + 2 (resid) read, 2 (h) + 1 + 1/128 written per
+// element.  A row is held in registers from the read to the codes: TPR threads a row with NV vectors of 8 elements,
+// 16 lanes to a block of 128, so its maximum is four shuffles.
+// ---------------------------------------------------------------------------------------------------
+struct NormQuantArgs {
+  const __nv_bfloat16 *x, *resid, *w;
+  __nv_bfloat16* h;
+  uint8_t *q, *sf;
+  float* rstd;
+  long long rows, x_stride, r_stride, h_stride, q_ld;
+  int D, kgroups, vec;
+  float eps, w_offset;
+};
+
+template <int TPR, int NV, int FMT>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+fp8_norm_kernel(const NormQuantArgs p) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  constexpr int ROWS = THREADS / TPR;
+  __shared__ float s_part[ROWS][TPR / 32];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
+  const bool ok = row < p.rows;
+  float v[NV][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * 8;
+    const int n = ok ? max(0, min(8, p.D - c)) : 0;
+    fp8_load8(p.x + row * p.x_stride + c, n, p.vec, v[i]);
+    if (p.resid != nullptr) {
+      float b[8];
+      fp8_load8(p.resid + row * p.r_stride + c, n, p.vec, b);
+      __nv_bfloat16* hp = p.h + row * p.h_stride + c;
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(v[i][2 * j] + b[2 * j], v[i][2 * j + 1] + b[2 * j + 1]);
+      if (n == 8 && p.vec) {
+        *reinterpret_cast<uint4*>(hp) = make_uint4(o[0], o[1], o[2], o[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < n) reinterpret_cast<uint16_t*>(hp)[j] = static_cast<uint16_t>(o[j >> 1] >> ((j & 1) * 16));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[i][2 * j] = __uint_as_float(o[j] << 16);
+        v[i][2 * j + 1] = __uint_as_float(o[j] & 0xFFFF0000u);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+  }
+  ss = warp_sum(ss);
+  if (TPR > 32) {
+    if (lane == 0) s_part[sub][t >> 5] = ss;
+    __syncthreads();
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) ss += s_part[sub][i];
+  }
+  const float rstd = rsqrtf(ss / p.D + p.eps);
+  if (ok && t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * 8;
+    const int n = max(0, min(8, p.D - c));
+    float g[8];
+    fp8_load8(p.w + c, n, p.vec, g);
+    bool odd = false;
+    uint32_t m = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[i][j] = j < n ? v[i][j] * rstd * (p.w_offset + g[j]) : 0.f;
+      m = max(m, fp8_mag(v[i][j], &odd));
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t byte = fp8_scale_byte<FMT>(m);
+    if (ok && c < p.D && (t & 15) == 0) p.sf[fp8_sf_offset(row, c >> 7, p.kgroups)] = static_cast<uint8_t>(byte);
+    if (ok && c < p.q_ld)
+      *reinterpret_cast<uint2*>(p.q + row * p.q_ld + c) = fp8_pack8<FMT>(v[i], fp8_inverse_scale(byte), odd);
+  }
+}
+
+template <int TPR, int NV>
+static void norm_launch(const NormQuantArgs& p, int fmt, cudaStream_t s) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  const unsigned grid = static_cast<unsigned>((p.rows + THREADS / TPR - 1) / (THREADS / TPR));
+  if (fmt == FP8_E4M3) fp8_norm_kernel<TPR, NV, FP8_E4M3><<<grid, THREADS, 0, s>>>(p);
+  else fp8_norm_kernel<TPR, NV, FP8_E5M2><<<grid, THREADS, 0, s>>>(p);
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Backward of the norm, dn = gradient of its output:  g = dn * (w_offset + w), xh = h * rstd,
+//   dx = rstd * (g - xh * mean(g * xh)) + dh,        dw = sum over rows of dn * xh.
+// Bound by HBM: 2 (dn) + 2 (h) + 2 (dh) read, 2 written per element.  Same row layout as the forward kernel.  Every
+// CTA walks rows at a stride of the grid and keeps its share of dw in registers; the shares are written out and
+// summed in a fixed order by a second kernel, so that dw is the same from run to run.
+// ---------------------------------------------------------------------------------------------------
+struct NormBwdArgs {
+  const __nv_bfloat16 *dn, *h, *w, *dh;
+  const float* rstd;
+  __nv_bfloat16* dx;
+  float* part;       // [grid, D]
+  long long rows, dn_stride, h_stride, dh_stride;
+  int D, vec;
+  float w_offset;
+};
+
+template <int TPR, int NV>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+fp8_norm_bwd_kernel(const NormBwdArgs p) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  constexpr int ROWS = THREADS / TPR;
+  __shared__ float s_part[ROWS][TPR / 32];
+  __shared__ float s_dw[ROWS > 1 ? ROWS * TPR * NV * 8 : 1];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, lane = threadIdx.x & 31;
+  float acc[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+  // the trip count is the block's, not the row group's: TPR > 32 synchronises inside
+  for (long long r0 = static_cast<long long>(blockIdx.x) * ROWS; r0 < p.rows; r0 += static_cast<long long>(gridDim.x) * ROWS) {
+    const long long row = r0 + sub;
+    const bool ok = row < p.rows;
+    const float rstd = ok ? p.rstd[row] : 0.f;
+    float xh[NV][8], gn[NV][8];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * 8;
+      const int n = ok ? max(0, min(8, p.D - c)) : 0;
+      float w8[8];
+      fp8_load8(p.h + row * p.h_stride + c, n, p.vec, xh[i]);
+      fp8_load8(p.dn + row * p.dn_stride + c, n, p.vec, gn[i]);
+      fp8_load8(p.w + c, n, p.vec, w8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xh[i][j] *= rstd;
+        acc[i][j] += gn[i][j] * xh[i][j];
+        gn[i][j] *= p.w_offset + w8[j];
+        dot += j < n ? gn[i][j] * xh[i][j] : 0.f;
+      }
+    }
+    dot = warp_sum(dot);
+    if (TPR > 32) {
+      __syncthreads();          // the previous row's sums have been read
+      if (lane == 0) s_part[sub][t >> 5] = dot;
+      __syncthreads();
+      dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) dot += s_part[sub][i];
+    }
+    dot /= p.D;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * 8;
+      const int n = ok ? max(0, min(8, p.D - c)) : 0;
+      float d8[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d8[j] = 0.f;
+      if (p.dh != nullptr) fp8_load8(p.dh + row * p.dh_stride + c, n, p.vec, d8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d8[j] += rstd * (gn[i][j] - xh[i][j] * dot);
+      __nv_bfloat16* out = p.dx + row * p.D + c;
+      if (n == 8 && p.vec) {
+        *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(d8[0], d8[1]), pack_bf16x2(d8[2], d8[3]),
+                                                    pack_bf16x2(d8[4], d8[5]), pack_bf16x2(d8[6], d8[7]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < n) out[j] = __float2bfloat16_rn(d8[j]);
+      }
+    }
+  }
+  if (p.part == nullptr) return;
+  float* part = p.part + static_cast<long long>(blockIdx.x) * p.D;
+  if (ROWS > 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s_dw[(sub * NV * TPR + i * TPR + t) * 8 + j] = acc[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.D; c += THREADS) {
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) sum += s_dw[r * NV * TPR * 8 + c];
+      part[c] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = (i * TPR + t) * 8 + j;
+        if (c < p.D) part[c] = acc[i][j];
+      }
+  }
+}
+
+// dw[c] = sum over the parts in a fixed order: 32 groups of consecutive parts, then the groups; fp32 +=, or bf16
+__global__ void __launch_bounds__(1024)
+fp8_norm_dw_kernel(const float* __restrict__ part, int parts, int D, float* __restrict__ acc,
+                   __nv_bfloat16* __restrict__ out) {
+  __shared__ float s[32][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+  const int per = (parts + 31) / 32;
+  float sum = 0.f;
+  if (c < D)
+    for (int i = g * per; i < min(parts, (g + 1) * per); ++i) sum += part[static_cast<long long>(i) * D + c];
+  s[g][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (g == 0 && c < D) {
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) total += s[i][threadIdx.x & 31];
+    if (acc != nullptr) acc[c] += total;
+    else out[c] = __float2bfloat16_rn(total);
+  }
+}
+
+constexpr int NORM_BWD_MAX_PARTS = 592;   // 148 SMs with four CTAs each
+
+template <int TPR, int NV>
+static int norm_bwd_launch(const NormBwdArgs& p, cudaStream_t s) {
+  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  const long long want = (p.rows + THREADS / TPR - 1) / (THREADS / TPR);
+  const int grid = static_cast<int>(want < NORM_BWD_MAX_PARTS ? want : NORM_BWD_MAX_PARTS);
+  fp8_norm_bwd_kernel<TPR, NV><<<grid, THREADS, 0, s>>>(p);
+  return grid;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace cvb
+
+using namespace cvb;
+
+// mode: 1 row form, 2 transposed form, 3 both, 5 row form with 128 x 128 blocks, 7 both with 128 x 128 blocks
+extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, long long x_stride, int fmt,
+                                int mode, void* q, void* sf, long long q_ld, void* qt, void* sft, long long qt_ld,
+                                const float* rstd, const void* w, float w_offset, void* stream) {
+  if (rows <= 0 || cols <= 0) return 0;
+  if ((fmt != FP8_E4M3 && fmt != FP8_E5M2) || (mode != 1 && mode != 2 && mode != 3 && mode != 5 && mode != 7)) return -1;
+  if (((mode & 1) && (!q || !sf || !aligned16(q) || q_ld % 16 || q_ld < cols)) ||
+      ((mode & 2) && (!qt || !sft || !aligned16(qt) || qt_ld % 16 || qt_ld < rows)))
+    return -2;
+  if ((rstd != nullptr) != (w != nullptr)) return -3;
+  const long long row_tiles = (rows + QT - 1) / QT, col_tiles = (cols + QT - 1) / QT;
+  if (row_tiles * col_tiles > 0x7fffffffll) return -4;
+  const int elem = x_fp32 ? 4 : 2;
+  QuantArgs p = {};
+  p.x = x;
+  p.rows = rows, p.cols = cols, p.x_stride = x_stride;
+  p.vec = aligned16(x) && (x_stride * elem) % 16 == 0;
+  p.q = static_cast<uint8_t*>(q), p.sf = static_cast<uint8_t*>(sf), p.q_ld = q_ld;
+  p.kgroups = static_cast<int>((col_tiles + 3) / 4);
+  p.qt = static_cast<uint8_t*>(qt), p.sft = static_cast<uint8_t*>(sft), p.qt_ld = qt_ld;
+  p.kgroups_t = static_cast<int>((row_tiles + 3) / 4);
+  p.col_tiles = static_cast<int>(col_tiles);
+  p.rstd = rstd, p.w = static_cast<const __nv_bfloat16*>(w), p.w_offset = w_offset;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const long long grid = row_tiles * col_tiles;
+  if (x_fp32) {
+    if (fmt == FP8_E4M3) quant_launch<float, FP8_E4M3>(p, mode, grid, s);
+    else quant_launch<float, FP8_E5M2>(p, mode, grid, s);
+  } else {
+    if (fmt == FP8_E4M3) quant_launch<__nv_bfloat16, FP8_E4M3>(p, mode, grid, s);
+    else quant_launch<__nv_bfloat16, FP8_E5M2>(p, mode, grid, s);
+  }
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int cvb_fp8_scales(const void* sf, void* out, long long rows, int nb, void* stream) {
+  if (rows <= 0 || nb <= 0) return 0;
+  const long long n = rows * nb;
+  const unsigned grid = static_cast<unsigned>(n < 148ll * 8 * 256 ? (n + 255) / 256 : 148 * 8);
+  fp8_scales_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint8_t*>(sf),
+                                                                       static_cast<uint8_t*>(out), rows, nb);
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride,
+                                   const void* w, void* h, void* q, void* sf, long long q_ld, float* rstd,
+                                   long long rows, int D, int fmt, float eps, float w_offset, void* stream) {
+  if (rows <= 0 || D <= 0) return 0;
+  if (fmt != FP8_E4M3 && fmt != FP8_E5M2) return -1;
+  if (!aligned16(q) || q_ld % 16 || q_ld < D || (resid != nullptr) != (h != nullptr)) return -2;
+  if (D > 16384 || rows > 0x7fffffffll) return -3;
+  NormQuantArgs p = {};
+  p.x = static_cast<const __nv_bfloat16*>(x), p.resid = static_cast<const __nv_bfloat16*>(resid);
+  p.w = static_cast<const __nv_bfloat16*>(w), p.h = static_cast<__nv_bfloat16*>(h);
+  p.q = static_cast<uint8_t*>(q), p.sf = static_cast<uint8_t*>(sf), p.rstd = rstd;
+  p.rows = rows, p.x_stride = x_stride, p.r_stride = r_stride, p.h_stride = D, p.q_ld = q_ld;
+  p.D = D, p.kgroups = ((D + 127) / 128 + 3) / 4;
+  p.vec = aligned16(x) && aligned16(resid) && aligned16(w) && aligned16(h) && x_stride % 8 == 0 && r_stride % 8 == 0 &&
+          D % 8 == 0;
+  p.eps = eps, p.w_offset = w_offset;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // the fewest threads that hold a row with at most four vectors each
+  if (D <= 256) norm_launch<32, 1>(p, fmt, s);
+  else if (D <= 512) norm_launch<32, 2>(p, fmt, s);
+  else if (D <= 1024) norm_launch<32, 4>(p, fmt, s);
+  else if (D <= 2048) norm_launch<128, 2>(p, fmt, s);
+  else if (D <= 4096) norm_launch<128, 4>(p, fmt, s);
+  else if (D <= 8192) norm_launch<256, 4>(p, fmt, s);
+  else norm_launch<512, 4>(p, fmt, s);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// rows of the workspace [parts, D] that cvb_fp8_norm_bwd may fill
+extern "C" int cvb_fp8_norm_bwd_parts(void) { return NORM_BWD_MAX_PARTS; }
+
+// dw_acc (fp32, +=) or dw (bf16); both null: no weight gradient
+extern "C" int cvb_fp8_norm_bwd(const void* dn, long long dn_stride, const void* h, long long h_stride, const void* w,
+                                const float* rstd, const void* dh, long long dh_stride, void* dx, float* part,
+                                float* dw_acc, void* dw, long long rows, int D, float w_offset, void* stream) {
+  if (rows <= 0 || D <= 0) return 0;
+  if (D > 16384) return -3;
+  if ((dw_acc != nullptr || dw != nullptr) && part == nullptr) return -2;
+  NormBwdArgs p = {};
+  p.dn = static_cast<const __nv_bfloat16*>(dn), p.h = static_cast<const __nv_bfloat16*>(h);
+  p.w = static_cast<const __nv_bfloat16*>(w), p.dh = static_cast<const __nv_bfloat16*>(dh);
+  p.rstd = rstd, p.dx = static_cast<__nv_bfloat16*>(dx);
+  p.part = dw_acc != nullptr || dw != nullptr ? part : nullptr;
+  p.rows = rows, p.dn_stride = dn_stride, p.h_stride = h_stride, p.dh_stride = dh_stride, p.D = D;
+  p.vec = aligned16(dn) && aligned16(h) && aligned16(w) && aligned16(dh) && aligned16(dx) && dn_stride % 8 == 0 &&
+          h_stride % 8 == 0 && dh_stride % 8 == 0 && D % 8 == 0;
+  p.w_offset = w_offset;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int grid;
+  if (D <= 256) grid = norm_bwd_launch<32, 1>(p, s);
+  else if (D <= 512) grid = norm_bwd_launch<32, 2>(p, s);
+  else if (D <= 1024) grid = norm_bwd_launch<32, 4>(p, s);
+  else if (D <= 2048) grid = norm_bwd_launch<128, 2>(p, s);
+  else if (D <= 4096) grid = norm_bwd_launch<128, 4>(p, s);
+  else if (D <= 8192) grid = norm_bwd_launch<256, 4>(p, s);
+  else grid = norm_bwd_launch<512, 4>(p, s);
+  if (p.part != nullptr)
+    fp8_norm_dw_kernel<<<(D + 31) / 32, 1024, 0, s>>>(part, grid, D, dw_acc, static_cast<__nv_bfloat16*>(dw));
+  return static_cast<int>(cudaGetLastError());
+}

@@ -714,11 +714,6 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-// Tensor map with 128-byte swizzle over [outer, inner] rows, or over [depth, outer, inner] with depth > 0.
-static int encode_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
-                             uint64_t depth, uint64_t row_stride_bytes, uint64_t depth_stride_bytes, uint32_t box_inner,
-                             uint32_t box_outer);
-
 // A tensor map is a pure function of (base, element size, extents, row stride, box): training re-issues the same
 // few hundred (pointer, shape) pairs every step - weights, the flat gradient, cached activation buffers - so the
 // encoded maps are kept in a small per-thread table (the forward and the autograd thread each have one; no lock)
@@ -790,9 +785,10 @@ int make_tensor_map_3d(CUtensorMap* out, const void* base, int elem_bytes, uint6
   return rc;
 }
 
-static int encode_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
-                             uint64_t depth, uint64_t row_stride_bytes, uint64_t depth_stride_bytes, uint32_t box_inner,
-                             uint32_t box_outer) {
+// Tensor map with 128-byte swizzle over [outer, inner] rows, or over [depth, outer, inner] with depth > 0.
+int encode_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
+                      uint64_t depth, uint64_t row_stride_bytes, uint64_t depth_stride_bytes, uint32_t box_inner,
+                      uint32_t box_outer) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -1;
   // The driver call needs this thread to have a current context.  Autograd runs backward on
@@ -806,9 +802,13 @@ static int encode_tensor_map(CUtensorMap* out, const void* base, int elem_bytes,
   cuuint64_t strides[2] = {row_stride_bytes, depth_stride_bytes};
   cuuint32_t box[3] = {box_inner, box_outer, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const bool plain = elem_bytes == TMAP_U32_PLAIN;
+  CUtensorMapDataType dt = elem_bytes == 2   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                           : elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                           : plain           ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = fn(out, dt, depth > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  plain ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     fprintf(stderr,

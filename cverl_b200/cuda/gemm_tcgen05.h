@@ -105,5 +105,11 @@ int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint6
 int make_tensor_map_3d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
                        uint64_t depth, uint64_t row_stride_bytes, uint64_t depth_stride_bytes, uint32_t box_inner,
                        uint32_t box_outer);
+// the encoding itself, without the table of earlier ones.  elem_bytes: 1 uint8, 2 bf16, 4 fp32 (128-byte swizzle), or
+// TMAP_U32_PLAIN: 32-bit words without a swizzle
+constexpr int TMAP_U32_PLAIN = -4;
+int encode_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, uint64_t inner, uint64_t outer,
+                      uint64_t depth, uint64_t row_stride_bytes, uint64_t depth_stride_bytes, uint32_t box_inner,
+                      uint32_t box_outer);
 }  // namespace cvb
 #endif

@@ -272,6 +272,41 @@ __host__ __device__ constexpr uint32_t umma_idesc(int m, int n, int fmt, int a_m
 }
 
 // ---------------------------------------------------------------------------
+// Block-scaled 8-bit MMA (kind::mxf8f6f4): every row of A and of B has one power-of-two scale per 32 elements of K,
+// read from tensor memory.  A 32-bit cell (lane, column) of a scale operand holds four scale bytes; row r of 128 sits
+// in lane r % 32, column r / 32, and the instruction descriptor names the byte that applies.
+// ---------------------------------------------------------------------------
+// Instruction descriptor: operand types (0 = e4m3, 1 = e5m2), both K-major, fp32 accumulation, UE8M0 scales (bit 23).
+__host__ __device__ constexpr uint32_t umma_idesc_mxf8(int m, int n, int a_fmt, int b_fmt) {
+  return (static_cast<uint32_t>(a_fmt) << 7) | (static_cast<uint32_t>(b_fmt) << 10) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 7) << 27);
+}
+// the same descriptor with byte `id` (0-3) of the scale cells selected, for A and for B
+__host__ __device__ constexpr uint32_t umma_idesc_scale_id(uint32_t idesc, uint32_t id) {
+  return idesc | (id << 4) | (id << 29);
+}
+__device__ __forceinline__ void umma_mxf8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t"
+      "}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb)
+      : "memory");
+}
+// 512 bytes of scale cells, 32 rows of 16 bytes in shared memory, to four columns of all four lane quarters
+__device__ __forceinline__ uint64_t umma_scale_desc(uint32_t smem_addr) {
+  // no swizzle; eight-row groups of 16-byte rows follow each other at 128 bytes
+  return static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46);
+}
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+
+// ---------------------------------------------------------------------------
 // CTA pairs (cluster of two CTAs, cta_group::2): one UMMA spans both SMs.  The even CTA of the pair issues
 // the MMAs; each CTA stages its own 128 rows of A and its own half of B, and holds its 128 rows of D in TMEM.
 // ---------------------------------------------------------------------------
@@ -325,6 +360,21 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t adesc, 
       "}\n" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// the block-scaled 8-bit forms: scales of A are each CTA's own 128 rows, scales of B those of all N rows in both CTAs
+__device__ __forceinline__ void umma_mxf8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t"
+      "}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
 }
 // Arrives, once the pair's MMAs issued so far are done, on the barrier at this shared-memory offset in every
 // CTA of `cta_mask` (bit r = CTA rank r of the cluster).

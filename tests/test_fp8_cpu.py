@@ -1,0 +1,188 @@
+"""8-bit operators on the CPU path: format, gradients, refusals."""
+import pytest
+import torch
+
+import fp8_oracle as orc
+from cverl_b200 import ops
+from fp8_oracle import E4M3, E5M2
+
+
+def _rand(*shape, seed=0, std=1.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype)
+
+
+def _same(got, want):
+    return torch.equal(torch.nan_to_num(got.double(), nan=1e300), torch.nan_to_num(want, nan=1e300))
+
+
+def awkward(R, C, dtype):
+    """Rows that are zero, subnormal, huge, at the borders of a scale, infinite or NaN."""
+    x = _rand(R, C, seed=R * 1000 + C) * torch.exp2(torch.arange(R).float() % 40 - 20)[:, None]
+    rows = [torch.zeros(C), torch.full((C,), 2.0 ** -130), torch.full((C,), 3e38), torch.full((C,), 448.0 * 2 ** -9),
+            torch.full((C,), 450.0), torch.full((C,), -1.0)]
+    rows[5][::3] = float("inf")
+    rows[5][1::5] = float("nan")
+    rows[5][2::7] = float("-inf")
+    for i, row in enumerate(rows[:R]):
+        x[R - 1 - i] = row
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 128), (6, 129), (130, 300), (257, 640)])
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+def test_codes_and_scales_are_the_definition(shape, dtype, src):
+    x = awkward(*shape, src)
+    q, t = ops.quantize_fp8_pair(x, dtype)
+    for got, want in ((q, orc.quantize(x, dtype)), (t, orc.quantize(x.t(), dtype))):
+        assert _same(got.values, want[0])
+        assert torch.equal(got.scales().double(), want[1][:, ::128])
+    assert _same(ops.quantize_fp8(x, dtype).values, orc.quantize(x, dtype)[0])
+    assert _same(ops.quantize_fp8_t(x, dtype).values, orc.quantize(x.t(), dtype)[0])
+
+
+def test_weight_and_its_transpose_hold_the_same_values():
+    w = _rand(200, 300, seed=3)
+    q = ops.quantize_fp8_weight(w)
+    assert torch.equal(q.w.dequantize(), q.wt.dequantize().t())
+    assert torch.equal(orc.value(q.w), orc.through(w, tall=128))
+    assert ops.quantize_fp8_weight(w, transposed=False).wt is None
+
+
+def test_product_and_accumulation():
+    a, b = ops.quantize_fp8(_rand(5, 200)), ops.quantize_fp8(_rand(7, 200, seed=1), E5M2)
+    want = orc.value(a) @ orc.value(b).t()
+    # 200 products, each sum in fp32: at most 200 half steps of a sum of magnitudes
+    tol = 200 * 2.0 ** -24 * (orc.value(a).abs() @ orc.value(b).abs().t())
+    got = ops.gemm_fp8_nt(a, b, out_dtype=torch.float32)
+    assert ((got - want).abs() <= tol).all()
+    out = torch.ones(5, 7)
+    ops.gemm_fp8_nt(a, b, out, accumulate=True)
+    assert ((out - 1 - want).abs() <= tol + 2.0 ** -23 * (1 + want.abs())).all()
+
+
+@pytest.mark.parametrize("grad", [E4M3, E5M2])
+def test_linear_gradients_are_the_formula(grad):
+    x, w = _rand(3, 50, 140, seed=1).requires_grad_(), _rand(130, 140, seed=2).requires_grad_()
+    dy = _rand(3, 50, 130, seed=3, std=1e-3)
+    y = ops.linear_fp8(x, w, grad_dtype=grad)
+    y.backward(dy)
+    x2, dy2 = x.detach().view(150, 140), dy.view(150, 130)
+    qw = orc.through(w.detach(), tall=128)
+    for got, want in ((y.detach().view(150, 130), orc.through(x2) @ qw.t()),
+                      (x.grad.view(150, 140), orc.through(dy2, grad) @ qw),
+                      (w.grad, orc.through(dy2.t(), grad) @ orc.through(x2.t()).t())):
+        # fp32 sums of at most 150 terms, random signs: 150 half steps of 2^-24 of the norm at the very most
+        assert (got - want).norm() <= 150 * 2.0 ** -24 * want.norm()
+
+
+def test_gradients_agree_with_differences_of_the_smooth_layer():
+    """Every rounding is at most 2^-4 of its value, three a product, independent over 96 or more terms: the gradient of
+    the rounded layer lies within 3 * 2^-4 of the smooth layer's, whose gradient is taken by central differences."""
+    x, r = _rand(40, 96, seed=1), _rand(40, 96, seed=2)
+    wn, w = _rand(96, seed=3, std=0.1), _rand(100, 96, seed=4, std=0.1)
+    dy, dh = _rand(40, 100, seed=5), _rand(40, 96, seed=6)
+    leaves = [t.clone().requires_grad_() for t in (x, r, wn, w)]
+    y, h = ops.add_rmsnorm_linear_fp8(*leaves, 1e-6, 1.0)
+    grads = torch.autograd.grad((y, h), leaves, (dy, dh))
+
+    def loss(x, r, wn, w):
+        n, h, _ = orc.norm(x.double(), r.double(), wn, 1e-6, 1.0)
+        return ((n @ w.double().t()) * dy.double()).sum() + (h * dh.double()).sum()
+
+    for i, g in enumerate(grads):
+        d = _rand(*g.shape, seed=10 + i).double()
+        d = 1e-5 * (d + g.double() / g.double().norm() * d.norm())      # not orthogonal to the gradient
+        args = [t.double() for t in (x, r, wn, w)]
+        hi, lo = list(args), list(args)
+        hi[i], lo[i] = args[i] + d, args[i] - d
+        want = (loss(*hi) - loss(*lo)) / 2
+        got = (g.double() * d).sum()
+        assert abs(got - want) <= 3 * 2.0 ** -4 * abs(want)
+
+
+def test_norm_then_linear_is_the_joint_layer():
+    x, r = _rand(33, 200, seed=1), _rand(33, 200, seed=2)
+    wn, w = _rand(200, seed=3, std=0.1), _rand(70, 200, seed=4)
+    q, h = ops.add_rmsnorm_fp8(x, r, wn)
+    kept = ops.quantize_fp8_weight(w)
+    y = ops.linear_fp8(q, kept)
+    y2, h2 = ops.add_rmsnorm_linear_fp8(x, r, wn, w)
+    assert torch.equal(h, h2) and torch.equal(y.float(), y2.to(y.dtype).float())
+    y3, h3 = ops.add_rmsnorm_linear_fp8(x, None, wn, kept)
+    assert h3 is x and y3.shape == (33, 70)
+
+
+def test_main_grad_takes_the_weight_gradients():
+    x, w, wn = _rand(20, 130, seed=1), _rand(40, 130, seed=2), _rand(130, seed=3)
+    plain = [t.clone().requires_grad_() for t in (wn, w)]
+    y, _ = ops.add_rmsnorm_linear_fp8(x, None, *plain)
+    want = torch.autograd.grad(y.sum(), plain)
+    kept = [t.clone().requires_grad_() for t in (wn, w)]
+    for p in kept:
+        p.main_grad = torch.ones_like(p)
+    y, _ = ops.add_rmsnorm_linear_fp8(x, None, *kept)
+    y.sum().backward()
+    for p, g in zip(kept, want):
+        assert p.grad is None
+        assert torch.allclose(p.main_grad - 1, g, rtol=1e-5, atol=1e-5)
+
+
+def test_frozen_weights_pass_gradients_of_the_input():
+    x, w = _rand(9, 150, seed=1).requires_grad_(), _rand(30, 150, seed=2)
+    kept = ops.quantize_fp8_weight(w)
+    y = ops.linear_fp8(x, kept)
+    y.sum().backward()
+    want = orc.through(torch.ones(9, 30)) @ orc.through(w, tall=128)
+    assert (x.grad - want).norm() <= 30 * 2.0 ** -24 * want.norm()
+    with pytest.raises(ValueError, match="transposed"):
+        ops.linear_fp8(x, ops.quantize_fp8_weight(w, transposed=False))
+
+
+@pytest.mark.parametrize("m,n,k", [(0, 5, 7), (5, 0, 7), (5, 7, 0)])
+def test_empty_matrices(m, n, k):
+    a, b = ops.quantize_fp8(torch.ones(m, k)), ops.quantize_fp8(torch.ones(n, k))
+    y = ops.gemm_fp8_nt(a, b, out_dtype=torch.float32)
+    assert y.shape == (m, n) and not y.any()
+    assert a.values.shape == (m, k) and a.scales().shape == (m, (k + 127) // 128)
+
+
+def test_no_tokens_give_zero_gradients():
+    x, w = torch.zeros(0, 64, requires_grad=True), torch.randn(32, 64, requires_grad=True)
+    y = ops.linear_fp8(x, w)
+    y.sum().backward()
+    assert y.shape == (0, 32) and x.grad.shape == (0, 64) and w.grad.shape == (32, 64) and not w.grad.any()
+
+
+def test_refusals():
+    a, b = ops.quantize_fp8(torch.ones(4, 8)), ops.quantize_fp8(torch.ones(3, 9))
+    good = ops.quantize_fp8(torch.ones(3, 8))
+    bad = [
+        (TypeError, lambda: ops.quantize_fp8(torch.ones(2, 2), torch.float16)),
+        (TypeError, lambda: ops.quantize_fp8(torch.ones(2, 2, dtype=torch.float16))),
+        (TypeError, lambda: ops.quantize_fp8(torch.ones(2, 2, dtype=torch.int32))),
+        (TypeError, lambda: ops.quantize_fp8([1.0])),
+        (ValueError, lambda: ops.quantize_fp8(torch.ones(2))),
+        (ValueError, lambda: ops.quantize_fp8_weight(torch.ones(2, 2, 2))),
+        (TypeError, lambda: ops.gemm_fp8_nt(torch.ones(4, 8), good)),
+        (ValueError, lambda: ops.gemm_fp8_nt(a, b)),
+        (TypeError, lambda: ops.gemm_fp8_nt(a, good, out_dtype=torch.float16)),
+        (ValueError, lambda: ops.gemm_fp8_nt(a, good, accumulate=True)),
+        (TypeError, lambda: ops.gemm_fp8_nt(a, good, torch.ones(4, 3, dtype=torch.bfloat16), accumulate=True)),
+        (ValueError, lambda: ops.gemm_fp8_nt(a, good, torch.ones(3, 4))),
+        (ValueError, lambda: ops.gemm_fp8_nt(a, good, torch.ones(3, 4).t())),
+        (ValueError, lambda: ops.gemm_fp8_nt(a, good, torch.ones(1, 3).expand(4, 3))),
+        (ValueError, lambda: ops.add_rmsnorm_fp8(torch.ones(2, 8), None, torch.ones(9))),
+        (ValueError, lambda: ops.add_rmsnorm_fp8(torch.ones(2, 8), torch.ones(3, 8), torch.ones(8))),
+        (ValueError, lambda: ops.add_rmsnorm_fp8(torch.ones(2, 16385), None, torch.ones(16385))),
+        (ValueError, lambda: ops.linear_fp8(torch.ones(2, 8), torch.ones(4, 9))),
+        (TypeError, lambda: ops.linear_fp8(torch.ones(2, 8), torch.ones(4, 8), grad_dtype=torch.bfloat16)),
+        (TypeError, lambda: ops.linear_fp8(torch.ones(2, 8).half(), torch.ones(4, 8))),
+        (TypeError, lambda: ops.linear_fp8(torch.ones(2, 8), torch.ones(4, 8).half())),
+        (ValueError, lambda: ops.linear_fp8(torch.ones(2, 8), torch.ones(4, 8), weight=ops.quantize_fp8_weight(torch.ones(5, 8)))),
+        (ValueError, lambda: ops.linear_fp8(torch.ones(2, 8), ops.quantize_fp8_weight(torch.ones(4, 8)),
+                                            weight=ops.quantize_fp8_weight(torch.ones(4, 8)))),
+    ]
+    for err, call in bad:
+        with pytest.raises(err):
+            call()

@@ -1,0 +1,386 @@
+"""8-bit operators on the kernels against plain 64-bit statements."""
+import pytest
+import torch
+
+import fp8_oracle as orc
+from cverl_b200 import ops
+from fp8_oracle import E4M3, E5M2
+from test_fp8_cpu import awkward
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-6
+
+
+def _rand(*shape, seed=0, std=1.0, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, device="cuda", generator=g) * std).to(dtype)
+
+
+def _same(got, want):
+    return torch.equal(torch.nan_to_num(got.double(), nan=1e300), torch.nan_to_num(want, nan=1e300))
+
+
+def _check_quantised(got, want):
+    assert _same(got.values, want[0])
+    assert torch.equal(got.scales().double(), want[1][:, ::128])
+
+
+# ----------------------------------------------------------------------------- quantisation: exact
+SHAPES = [(1, 1), (1, 128), (1, 1024), (7, 129), (128, 128), (129, 127), (300, 1000), (257, 513), (515, 2055)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+def test_codes_and_scales_are_the_definition(shape, dtype, src):
+    x = awkward(*shape, src).cuda()
+    rows, cols = orc.quantize(x, dtype), orc.quantize(x.t(), dtype)
+    q, t = ops.quantize_fp8_pair(x, dtype)
+    _check_quantised(q, rows)
+    _check_quantised(t, cols)
+    _check_quantised(ops.quantize_fp8(x, dtype), rows)
+    _check_quantised(ops.quantize_fp8_t(x, dtype), cols)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+def test_weight_blocks(shape, src):
+    w = awkward(*shape, src).cuda()
+    kept = ops.quantize_fp8_weight(w)
+    _check_quantised(kept.w, orc.quantize(w, tall=128))
+    assert _same(kept.wt.values, orc.quantize(w, tall=128)[0].t())
+    assert _same(orc.value(kept.wt), orc.value(kept.w).t())
+    _check_quantised(ops.quantize_fp8_weight(w, transposed=False).w, orc.quantize(w, tall=128))
+
+
+def test_strides_and_alignments():
+    base = _rand(300, 700, seed=1)
+    for x in (base[:, 3:640], base[5:, 8:136], base[::3, 1:2], base.t(), base[:1].expand(140, 700), base[7]
+              .unsqueeze(0), base.view(-1)[1:1 + 256 * 800].view(256, 800)):
+        q, t = ops.quantize_fp8_pair(x)
+        _check_quantised(q, orc.quantize(x))
+        _check_quantised(t, orc.quantize(x.t()))
+
+
+# ----------------------------------------------------------------------------- product
+def _whole(rows, cols, seed):
+    """Whole numbers up to 8 times a power of two per block: codes, scales and every partial sum are exact."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    v = torch.randint(-8, 9, (rows, cols), device="cuda", generator=g).float()
+    s = torch.randint(0, 4, (rows, -(-cols // 128)), device="cuda", generator=g).float()
+    return v * torch.exp2(s).repeat_interleave(128, 1)[:, :cols]
+
+
+PRODUCTS = [(1, 1, 1), (1, 128, 128), (1, 7168, 1024), (2, 129, 513), (15, 300, 130), (16, 256, 2048), (17, 65, 16),
+            (33, 127, 640), (64, 1000, 1000), (65, 512, 129), (128, 1024, 3584), (129, 130, 4096), (200, 4000, 256),
+            (333, 1003, 1111), (512, 512, 512), (1000, 257, 385), (2049, 260, 131), (257, 2304, 1024),
+            (1536, 1600, 640), (4100, 1024, 512), (300, 300, 9000)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_product_of_whole_numbers_is_exact(m, n, k):
+    x, w = _whole(m, k, 1), _whole(n, k, 2)
+    want = x.double() @ w.double().t()
+    assert want.abs().max() < 2 ** 24                       # every sum is a whole number that fp32 holds
+    a, b = ops.quantize_fp8(x), ops.quantize_fp8(w)
+    got = ops.gemm_fp8_nt(a, b, out_dtype=torch.float32)
+    assert torch.equal(got.double(), want)
+    assert torch.equal(ops.gemm_fp8_nt(a, b), want.float().bfloat16())
+    out = torch.full((m, n), 3.0, device="cuda")
+    ops.gemm_fp8_nt(a, b, out, accumulate=True)
+    assert torch.equal(out.double(), (want.float() + 3.0).double())
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("fa,fb", [(E4M3, E5M2), (E5M2, E4M3), (E5M2, E5M2), (E4M3, E4M3)])
+def test_product_of_random_values(m, n, k, fa, fb):
+    a = ops.quantize_fp8(_rand(m, k, seed=m) * torch.exp(_rand(m, 1, seed=5)), fa)
+    b = ops.quantize_fp8(_rand(n, k, seed=n, std=0.05), fb)
+    x, w = orc.value(a), orc.value(b)
+    got = ops.gemm_fp8_nt(a, b, out_dtype=torch.float32).double()
+    # products of two 8-bit values are exact in fp32; each of the k additions is off by at most one step (2^-23) of a
+    # partial sum, which is at most the sum of magnitudes
+    assert ((got - x @ w.t()).abs() <= k * 2.0 ** -23 * (x.abs() @ w.abs().t())).all()
+
+
+def test_output_that_is_a_range_of_a_wider_tensor():
+    """Rows behind the last and columns beside the range keep what they held."""
+    for m, n, k, c0 in [(5, 37, 200, 3), (300, 515, 140, 1), (129, 100, 128, 8), (700, 700, 300, 5)]:
+        a, b = ops.quantize_fp8(_whole(m, k, 1)), ops.quantize_fp8(_whole(n, k, 2))
+        want = ops.gemm_fp8_nt(a, b, out_dtype=torch.float32)
+        for dt in (torch.float32, torch.bfloat16):
+            wide = torch.full((m + 3, n + 11), 7.0, dtype=dt, device="cuda")
+            ops.gemm_fp8_nt(a, b, wide[1:m + 1, c0:c0 + n])
+            assert torch.equal(wide[1:m + 1, c0:c0 + n], want.to(dt))
+            wide[1:m + 1, c0:c0 + n] = 7.0
+            assert (wide == 7.0).all()
+
+
+def test_non_finite_values_stay_in_their_rows():
+    x, w = _rand(150, 300, seed=1), _rand(140, 300, seed=2)
+    clean = ops.gemm_fp8_nt(ops.quantize_fp8(x), ops.quantize_fp8(w), out_dtype=torch.float32)
+    x[3, 7], x[131, 299], w[5, 100] = float("inf"), float("nan"), float("-inf")
+    got = ops.gemm_fp8_nt(ops.quantize_fp8(x), ops.quantize_fp8(w), out_dtype=torch.float32)
+    bad = torch.zeros(150, 140, dtype=torch.bool, device="cuda")
+    bad[3], bad[131], bad[:, 5] = True, True, True
+    assert got[bad].isnan().all() and not got[~bad].isnan().any()
+    same = ~bad
+    same[[3, 131]] = False
+    assert torch.equal(got[same], clean[same])
+
+
+def test_product_is_the_same_from_run_to_run():
+    for m, n, k in [(1, 1000, 3584), (128, 1024, 3584), (700, 900, 2000), (2048, 2048, 1024)]:
+        a, b = ops.quantize_fp8(_rand(m, k, seed=1)), ops.quantize_fp8(_rand(n, k, seed=2))
+        first = ops.gemm_fp8_nt(a, b, out_dtype=torch.float32)
+        for _ in range(3):
+            assert torch.equal(ops.gemm_fp8_nt(a, b, out_dtype=torch.float32), first)
+
+
+# ----------------------------------------------------------------------------- norm
+@pytest.mark.parametrize("rows,d", [(1, 1), (1, 1024), (3, 129), (9, 128), (130, 256), (77, 500), (64, 513), (257, 1024),
+                                    (31, 1111), (20, 2048), (33, 2560), (5, 4096), (7, 5000), (4, 8192), (3, 16384),
+                                    (2, 16001), (5000, 64)])
+@pytest.mark.parametrize("resid", [True, False])
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+def test_norm(rows, d, resid, dtype):
+    x = _rand(rows, d, seed=rows, std=3.0)
+    r = _rand(rows, d, seed=d) if resid else None
+    w = _rand(d, seed=7, std=0.2)
+    x[rows // 2] = 0.0
+    if resid:
+        r[rows // 2] = 0.0
+    q, h = ops.add_rmsnorm_fp8(x, r, w, EPS, 1.0, dtype)
+    y, want_h, _ = orc.norm(x, r, w, EPS, 1.0)
+    assert torch.equal(h, want_h)
+    # the fp32 row: sum of d squares (d half steps at most, one in practice halved by the root), root, two products
+    fp32 = (d / 2 + 8) * 2.0 ** -24
+    s = q.scales().double().repeat_interleave(128, 1)[:, :d]
+    _, exact_s = orc.quantize(y, dtype)
+    # a scale is the definition's, or the neighbour where the block's maximum is that close to the border
+    big = torch.stack([b.abs().amax(1) for b in y.split(128, 1)], 1).repeat_interleave(128, 1)[:, :d]
+    edge = orc.FMAX[dtype] * torch.minimum(s, exact_s)
+    assert ((s == exact_s) | ((big / edge - 1).abs() <= fp32)).all()
+    step, low = (2.0 ** -4, 2.0 ** -10) if dtype == E4M3 else (2.0 ** -3, 2.0 ** -17)
+    assert ((orc.value(q) - y).abs() <= y.abs() * (step + 2 * fp32) + low * s).all()
+
+
+def test_norm_strides_and_rows_of_no_number():
+    x, r, w = _rand(40, 600, seed=1), _rand(40, 600, seed=2), _rand(512, seed=3, std=0.1)
+    x[3, 9], x[4, 20] = float("nan"), float("inf")
+    cols = (x[:, 5:517], r[:, 8:520])
+    q, h = ops.add_rmsnorm_fp8(*cols, w)
+    q2, h2 = ops.add_rmsnorm_fp8(cols[0].contiguous(), cols[1].contiguous(), w)
+    assert _same(q.values, q2.values.double()) and torch.equal(q.scales().view(torch.uint8), q2.scales().view(torch.uint8))
+    assert _same(h, h2.double())
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[3] = True
+    assert q.values[3].isnan().all()
+    assert q.values[4].isnan().any() and not q.values[5:].float().isnan().any()
+
+
+# ----------------------------------------------------------------------------- linear layers
+def _near(got, want, terms):
+    """bf16 result of fp32 sums: half a step of 2^-8, and the sums' 2^-24 a term of the norm."""
+    assert (got.double() - want).norm() <= (2.0 ** -8 + terms * 2.0 ** -24) * want.norm()
+
+
+LAYERS = [(1, 128, 64), (5, 100, 33), (77, 512, 1536), (130, 257, 129), (300, 1000, 520), (1301, 640, 384), (2100, 1024, 2048)]
+
+
+@pytest.mark.parametrize("m,k,n", LAYERS)
+@pytest.mark.parametrize("grad", [E4M3, E5M2])
+def test_linear_and_gradients(m, k, n, grad):
+    x, w, dy = _rand(m, k, seed=1), _rand(n, k, seed=2, std=k ** -0.5), _rand(m, n, seed=3, std=1e-3)
+    x.requires_grad_(), w.requires_grad_()
+    y = ops.linear_fp8(x, w, grad_dtype=grad)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    qw = orc.through(w.detach(), tall=128)
+    _near(y.detach(), orc.through(x.detach()) @ qw.t(), k)
+    _near(dx, orc.through(dy, grad) @ qw, n)
+    _near(dw, orc.through(dy.t(), grad) @ orc.through(x.detach().t()).t(), m)
+    assert torch.equal(ops.linear_fp8(x.detach(), ops.quantize_fp8_weight(w.detach())), y.detach())
+    w.main_grad = torch.ones(n, k, device="cuda")
+    dw32 = ops.linear_fp8(x, w, grad_dtype=grad, weight=ops.quantize_fp8_weight(w))
+    dw32.backward(dy)
+    assert w.grad is None
+    want = orc.through(dy.t(), grad) @ orc.through(x.detach().t()).t()
+    assert (w.main_grad.double() - 1 - want).norm() <= (m + 1) * 2.0 ** -24 * (want.norm() + (n * k) ** 0.5)
+
+
+@pytest.mark.parametrize("m,k,n", LAYERS + [(40, 4100, 96), (9, 8192, 64), (6, 16384, 32)])
+@pytest.mark.parametrize("resid", [True, False])
+def test_norm_linear_and_gradients(m, k, n, resid):
+    x, w, wn = _rand(m, k, seed=1), _rand(n, k, seed=2, std=k ** -0.5), _rand(k, seed=3, std=0.1)
+    r = _rand(m, k, seed=4) if resid else None
+    dy, dh = _rand(m, n, seed=5, std=1e-2), _rand(m, k, seed=6, std=1e-2)
+    leaves = [t.requires_grad_() for t in (x, r, wn, w) if t is not None]
+    y, h = ops.add_rmsnorm_linear_fp8(x, r, wn, w, EPS, 1.0)
+    outs, seeds = ((y, h), (dy, dh)) if resid else ((y,), (dy,))
+    grads = torch.autograd.grad(outs, leaves, seeds)
+    with torch.no_grad():
+        nrm, want_h, rstd = orc.norm(x, r, wn, EPS, 1.0)
+        assert torch.equal(h, want_h)
+        # what the kernel rounded, from its own fp32 norm: at a rounding border it may differ from the 64-bit norm's by
+        # a step of 2^-3 of a value, which happens to at most one in 2^14 of them (fp32 steps against e4m3 steps)
+        few = 2.0 ** -3 * 2.0 ** -7
+        qw = orc.through(w, tall=128)
+        want_y = orc.through(nrm) @ qw.t()
+        assert (y.double() - want_y).norm() <= (2.0 ** -8 + k * 2.0 ** -24 + few) * want_y.norm()
+        dn = orc.through(dy) @ qw
+        want_dw = orc.through(dy.t()) @ orc.through(nrm.t()).t()
+        dx, dwn = orc.norm_grads(want_h, rstd, wn, 1.0, dn, dh if resid else None)
+        assert (grads[-1].double() - want_dw).norm() <= (2.0 ** -8 + m * 2.0 ** -24 + few) * want_dw.norm()
+        # dn is bf16 between the product and the norm: one more half step of it, and of what it is subtracted from
+        size = (rstd * dn * (1.0 + wn.double())).norm()
+        tol = 2.0 ** -8 * dx.norm() + (2 * 2.0 ** -8 + n * 2.0 ** -24) * size
+        for g in grads[:2 if resid else 1]:
+            assert (g.double() - dx).norm() <= tol
+        xh = want_h.double() * rstd
+        assert (grads[-2].double() - dwn).norm() <= 2.0 ** -8 * dwn.norm() + 2.0 ** -8 * (dn * xh).abs().sum(0).norm()
+
+
+def test_norm_weight_gradient_is_the_same_from_run_to_run():
+    x, wn, w = _rand(3000, 384, seed=1), _rand(384, seed=2).requires_grad_(), _rand(64, 384, seed=3)
+    kept = ops.quantize_fp8_weight(w)
+    runs = []
+    for _ in range(3):
+        y, _ = ops.add_rmsnorm_linear_fp8(x, None, wn, kept)
+        runs.append(torch.autograd.grad(y, wn, torch.ones_like(y))[0])
+    assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+    wn.main_grad = torch.zeros(384, device="cuda")
+    y, _ = ops.add_rmsnorm_linear_fp8(x, None, wn, kept)
+    y.backward(torch.ones_like(y))
+    assert torch.equal(wn.main_grad.bfloat16(), runs[0])
+
+
+# ----------------------------------------------------------------------------- together
+def _mlp(x, r, wn, w1, w2):
+    gu, h = ops.add_rmsnorm_linear_fp8(x, r, wn, w1)
+    return ops.linear_fp8(ops.swiglu(gu), w2), h
+
+
+def test_feed_forward_block_trains():
+    """Norm, gate|up, SwiGLU and down projection as a model runs them, against the same block in 64 bits."""
+    m, d, f = 700, 512, 896
+    x, r = _rand(m, d, seed=1).requires_grad_(), _rand(m, d, seed=2).requires_grad_()
+    wn = _rand(d, seed=3, std=0.1).requires_grad_()
+    w1, w2 = _rand(2 * f, d, seed=4, std=d ** -0.5).requires_grad_(), _rand(d, f, seed=5, std=f ** -0.5).requires_grad_()
+    leaves = (x, r, wn, w1, w2)
+    y, h = _mlp(*leaves)
+    dy = _rand(m, d, seed=6)
+    grads = torch.autograd.grad((y, h), leaves, (dy, dy))
+    l64 = [t.detach().double().requires_grad_() for t in leaves]
+    h64 = l64[0] + l64[1]
+    n64 = h64 * torch.rsqrt((h64 * h64).mean(-1, keepdim=True) + EPS) * (1 + l64[2])
+    g64, u64 = (n64 @ l64[3].t()).chunk(2, -1)
+    y64 = (torch.nn.functional.silu(g64) * u64) @ l64[4].t()
+    want = torch.autograd.grad((y64, h64), l64, (dy.double(), dy.double()))
+    # each 8-bit rounding is at most 2^-4 of its value; the chain has at most 6 of them in any gradient
+    for g, e in zip((y.detach(), *grads), (y64.detach(), *want)):
+        assert (g.double() - e).norm() <= 6 * 2.0 ** -4 * e.norm()
+
+
+def test_decoding_and_prefill_of_a_block_agree():
+    """Tokens one by one give what they give together: rows do not depend on each other."""
+    d, f, m = 1024, 3584, 9
+    wn, w1, w2 = _rand(d, seed=1, std=0.1), _rand(2 * f, d, seed=2, std=0.03), _rand(d, f, seed=3, std=0.02)
+    kept = ops.quantize_fp8_weight(w1, transposed=False), ops.quantize_fp8_weight(w2, transposed=False)
+    x, r = _rand(m, d, seed=4), _rand(m, d, seed=5)
+
+    def block(x, r):
+        q, h = ops.add_rmsnorm_fp8(x, r, wn)
+        return ops.linear_fp8(ops.swiglu(ops.linear_fp8(q, kept[0])), kept[1]), h
+
+    with torch.no_grad():
+        y, h = block(x, r)
+        for i in range(m):
+            yi, hi = block(x[i:i + 1], r[i:i + 1])
+            assert torch.equal(hi, h[i:i + 1])
+            assert (yi.double() - y[i:i + 1].double()).norm() <= 2.0 ** -7 * y[i].double().norm()
+
+
+# ----------------------------------------------------------------------------- streams, graphs, refusals
+def test_other_stream():
+    x, w = _rand(300, 512, seed=1), _rand(256, 512, seed=2)
+    want = ops.linear_fp8(x, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.linear_fp8(x, w)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+
+
+def test_two_captured_graphs_replayed_in_turn():
+    w = ops.quantize_fp8_weight(_rand(700, 512, seed=1))
+    wn = _rand(512, seed=2)
+    xs = [_rand(5, 512, seed=3), _rand(130, 512, seed=4)]
+    ops.linear_fp8(xs[0], w)
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            q, _ = ops.add_rmsnorm_fp8(x, None, wn)
+            outs.append(ops.linear_fp8(q, w) + ops.linear_fp8(x, w))
+        graphs.append(g)
+    for seed in (10, 11):
+        for x, g, out in zip(xs, graphs, outs):
+            x.copy_(_rand(*x.shape, seed=seed))
+            g.replay()
+        for x, out in zip(xs, outs):
+            want = ops.linear_fp8(ops.add_rmsnorm_fp8(x, None, wn)[0], w) + ops.linear_fp8(x, w)
+            assert torch.equal(out, want)
+
+
+def test_captured_training_step():
+    x, w = _rand(200, 256, seed=1).requires_grad_(), _rand(300, 256, seed=2).requires_grad_()
+    dy = _rand(200, 300, seed=3)
+    want = torch.autograd.grad(ops.linear_fp8(x, w), (x, w), dy)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(ops.linear_fp8(x, w), (x, w), dy)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(ops.linear_fp8(x, w), (x, w), dy)
+    for _ in range(2):
+        g.replay()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_backward_twice_and_expanded_gradient():
+    x, w = _rand(20, 200, seed=1).requires_grad_(), _rand(30, 200, seed=2).requires_grad_()
+    y = ops.linear_fp8(x, w)
+    first = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)
+    again = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_empty_calls():
+    w = _rand(30, 200, seed=2).requires_grad_()
+    x = torch.empty(0, 200, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    y, _ = ops.add_rmsnorm_linear_fp8(x, None, _rand(200), w)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+    assert dx.shape == (0, 200) and not dw.any()
+    a, b = ops.quantize_fp8(_rand(4, 0)), ops.quantize_fp8(_rand(5, 0))
+    assert not ops.gemm_fp8_nt(a, b).any()
+
+
+def test_refusals():
+    h = _rand(4, 64).half()
+    for call in (lambda: ops.quantize_fp8(h), lambda: ops.linear_fp8(h, _rand(8, 64)),
+                 lambda: ops.linear_fp8(_rand(4, 64).float(), _rand(8, 64)),
+                 lambda: ops.add_rmsnorm_fp8(_rand(4, 64).float(), None, _rand(64).float()),
+                 lambda: ops.linear_fp8(_rand(4, 64), _rand(8, 64), grad_dtype=torch.float16)):
+        with pytest.raises(TypeError):
+            call()
+    a = ops.quantize_fp8(_rand(4, 64))
+    for call in (lambda: ops.gemm_fp8_nt(a, ops.quantize_fp8(torch.ones(4, 64))),
+                 lambda: ops.gemm_fp8_nt(a, ops.quantize_fp8(_rand(4, 65))),
+                 lambda: ops.linear_fp8(torch.ones(4, 64), _rand(8, 64)),
+                 lambda: ops.add_rmsnorm_fp8(_rand(4, 64), None, torch.ones(64))):
+        with pytest.raises((TypeError, ValueError)):
+            call()
