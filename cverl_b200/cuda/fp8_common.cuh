@@ -22,13 +22,16 @@ __device__ __forceinline__ long long fp8_sf_offset(long long row, int b, int kgr
   return ((row >> 7) * kgroups + (b >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (b & 3);
 }
 
-// scale byte of a block from the bits of its largest finite magnitude: the exponent field, one more where the
-// mantissa is above 1.75, less TOP.  Integer arithmetic: subnormal magnitudes (field 0) end at the smallest scale.
+// A block's maximum is carried as the upper 16 bits of the magnitude, rounded up: what the scale asks of it, its
+// exponent and whether its mantissa is above 1.75, is the same, and two blocks' maxima fit a register.
+__device__ __forceinline__ uint32_t fp8_max16(uint32_t mag_bits) { return (mag_bits + 0xFFFFu) >> 16; }
+
+// scale byte of a block from the largest finite magnitude: the exponent field, one more where the mantissa is above
+// 1.75, less TOP.  Integer arithmetic: subnormal magnitudes (field 0) end at the smallest scale.
 template <int FMT>
-__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits) {
+__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t max16) {
   constexpr int TOP = FMT == FP8_E4M3 ? 8 : 15;
-  const int e = static_cast<int>((amax_bits + 0x1FFFFFu) >> 23) - TOP;
-  return static_cast<uint32_t>(max(e, 1));
+  return static_cast<uint32_t>(max(static_cast<int>((max16 + 0x1Fu) >> 7) - TOP, 1));
 }
 // 2^-e as a float; byte <= 247, so the exponent field stays positive
 __device__ __forceinline__ float fp8_inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
@@ -79,12 +82,24 @@ __device__ __forceinline__ uint2 fp8_pack8(const float (&v)[8], float inv, bool 
   return o;
 }
 
-// bits of |v| where v is finite, 0 where it is not (and *odd is set): what a block's maximum is taken over
-__device__ __forceinline__ uint32_t fp8_mag(float v, bool* odd) {
-  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-  if (b < 0x7F800000u) return b;
-  *odd = true;
-  return 0u;
+// maximum of |v| over the finite ones of n values, as bits; *odd says that there were others.  The common case costs
+// one maximum a value: fmaxf passes over NaN, and an infinity shows in the result and is then left out.
+template <int N>
+__device__ __forceinline__ uint32_t fp8_finite_max(const float (&v)[N], bool* odd) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
+  uint32_t bits = __float_as_uint(m);
+  if (bits >= 0x7F800000u) {
+    *odd = true;
+    bits = 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+      if (b < 0x7F800000u) bits = max(bits, b);
+    }
+  }
+  return bits;
 }
 
 // eight consecutive elements from `p`, of which the first `n` exist (the others read as zero)

@@ -30,93 +30,225 @@ struct QuantArgs {
   float w_offset;
 };
 
-template <typename T, int FMT, bool ROWS, bool COLS, bool BLOCK>
-__global__ void __launch_bounds__(Q_THREADS)
+// A thread's 8 x 8 piece of the tile as it was read.  bf16 stays packed (32 registers), so that two CTAs with 64 KB
+// of loads in flight fit an SM; values are formed where they are used, once for each form.
+template <typename T, bool NORM>
+struct Piece;
+
+template <bool NORM>
+struct Piece<__nv_bfloat16, NORM> {
+  uint32_t raw[8][4];
+  float rstd[NORM ? 8 : 1], gain[NORM ? 8 : 1];
+  __device__ __forceinline__ void load(const QuantArgs& p, long long r0, long long c0, int nc) {
+    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + r0 * p.x_stride + c0;
+    if (p.vec && nc == 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        if (r0 + i < p.rows) u = __ldg(reinterpret_cast<const uint4*>(x + i * p.x_stride));
+        raw[i][0] = u.x, raw[i][1] = u.y, raw[i][2] = u.z, raw[i][3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t* row = reinterpret_cast<const uint16_t*>(x + i * p.x_stride);
+        const int n = r0 + i < p.rows ? nc : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          raw[i][j] = (2 * j < n ? row[2 * j] : 0u) | ((2 * j + 1 < n ? row[2 * j + 1] : 0u) << 16);
+      }
+    }
+    if constexpr (NORM) {
+      fp8_load8(p.w + c0, nc, (reinterpret_cast<uintptr_t>(p.w) & 15) == 0, gain);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        gain[i] += p.w_offset;       // columns and rows outside hold zeros: whatever they are multiplied by is finite
+        rstd[i] = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
+      }
+    }
+  }
+  // the packed words are what stays live from here on, not the values formed from them
+  __device__ __forceinline__ void keep_packed() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(raw[i][0]), "+r"(raw[i][1]), "+r"(raw[i][2]), "+r"(raw[i][3]));
+  }
+  __device__ __forceinline__ float get(int i, int j) const {
+    const uint32_t w = raw[i][j >> 1];
+    const float v = __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+    if constexpr (NORM) return v * rstd[i] * gain[j];
+    else return v;
+  }
+};
+
+template <>
+struct Piece<float, false> {
+  float raw[8][8];
+  __device__ __forceinline__ void load(const QuantArgs& p, long long r0, long long c0, int nc) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      fp8_load8(static_cast<const float*>(p.x) + (r0 + i) * p.x_stride + c0, r0 + i < p.rows ? nc : 0, p.vec, raw[i]);
+  }
+  __device__ __forceinline__ void keep_packed() {}
+  __device__ __forceinline__ float get(int i, int j) const { return raw[i][j]; }
+};
+
+// Maxima of the piece's rows and columns over finite values, two 16-bit maxima a word: rows 2i, 2i + 1 in rmax[i],
+// columns 2j, 2j + 1 in cmax[j].  Returns whether a value was not finite.
+template <typename T, bool NORM>
+__device__ __forceinline__ bool piece_maxima(const Piece<T, NORM>& x, uint32_t (&rmax)[4], uint32_t (&cmax)[4]) {
+  float rm[8], cm[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rm[i] = cm[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = fabsf(x.get(i, j));
+      rm[i] = fmaxf(rm[i], a);
+      cm[j] = fmaxf(cm[j], a);
+    }
+  float all = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) all = fmaxf(all, rm[i]);
+  const bool odd = __float_as_uint(all) >= 0x7F800000u;
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rm[i] = cm[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(x.get(i, j));
+        if (__float_as_uint(a) < 0x7F800000u) {
+          rm[i] = fmaxf(rm[i], a);
+          cm[j] = fmaxf(cm[j], a);
+        }
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    rmax[i] = fp8_max16(__float_as_uint(rm[2 * i])) | (fp8_max16(__float_as_uint(rm[2 * i + 1])) << 16);
+    cmax[i] = fp8_max16(__float_as_uint(cm[2 * i])) | (fp8_max16(__float_as_uint(cm[2 * i + 1])) << 16);
+  }
+  return odd;
+}
+
+// bf16 as read: magnitudes are compared as pairs of 16-bit integers, half the instructions of the above
+__device__ __forceinline__ bool piece_maxima(const Piece<__nv_bfloat16, false>& x, uint32_t (&rmax)[4], uint32_t (&cmax)[4]) {
+  uint32_t row[8], all = 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) cmax[j] = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    row[i] = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t m = x.raw[i][j] & 0x7FFF7FFFu;
+      row[i] = __vmaxu2(row[i], m);
+      cmax[j] = __vmaxu2(cmax[j], m);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) all = __vmaxu2(all, cmax[j]);
+  const bool odd = (all & 0xFFFFu) >= 0x7F80u || (all >> 16) >= 0x7F80u;
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row[i] = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) cmax[j] = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t m = x.raw[i][j] & 0x7FFF7FFFu;
+        if ((m & 0xFFFFu) >= 0x7F80u) m &= 0xFFFF0000u;
+        if ((m >> 16) >= 0x7F80u) m &= 0xFFFFu;
+        row[i] = __vmaxu2(row[i], m);
+        cmax[j] = __vmaxu2(cmax[j], m);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)     // the larger half of each row's word: rows 2i and 2i + 1 side by side
+    rmax[i] = __vmaxu2(__byte_perm(row[2 * i], row[2 * i + 1], 0x5410), __byte_perm(row[2 * i], row[2 * i + 1], 0x7632));
+  return odd;
+}
+
+__device__ __forceinline__ uint32_t half16(const uint32_t (&w)[4], int i) { return (w[i >> 1] >> ((i & 1) * 16)) & 0xFFFFu; }
+
+template <typename T, int FMT, bool NORM, bool ROWS, bool COLS, bool BLOCK>
+__global__ void __launch_bounds__(Q_THREADS, sizeof(T) == 2 ? 3 : 1)
 fp8_quant_kernel(const QuantArgs p) {
-  __shared__ uint32_t s_max[QT];                                   // column maxima; [0] is the tile's for BLOCK
+  __shared__ __align__(16) uint32_t s_max[COLS || BLOCK ? Q_THREADS / 32 : 1][QT / 2];   // column maxima by warp
   __shared__ __align__(16) uint8_t s_t[COLS ? QT * QT : 16];       // transposed codes, 8-byte units XOR-swizzled
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cl = lane & 15, rg = warp * 2 + (lane >> 4);           // columns 8 cl .. + 7, rows 8 rg .. + 7 of the tile
-  const long long tile_r = blockIdx.x / p.col_tiles;
-  const int tile_c = blockIdx.x - static_cast<int>(tile_r * p.col_tiles);
-  const long long r0 = tile_r * QT + rg * 8;
+  const int tile_r = blockIdx.x / p.col_tiles;
+  const int tile_c = blockIdx.x - tile_r * p.col_tiles;
+  const long long r0 = static_cast<long long>(tile_r) * QT + rg * 8;
   const long long c0 = static_cast<long long>(tile_c) * QT + cl * 8;
-  if (COLS || BLOCK) {
-    if (threadIdx.x < QT) s_max[threadIdx.x] = 0u;
-    __syncthreads();
-  }
-  const int nc = static_cast<int>(max(0ll, min(8ll, p.cols - c0)));
-  float v[8][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    fp8_load8(static_cast<const T*>(p.x) + (r0 + i) * p.x_stride + c0, r0 + i < p.rows ? nc : 0, p.vec, v[i]);
-  if (p.rstd != nullptr) {
-    float g[8];
-    fp8_load8(p.w + c0, nc, (reinterpret_cast<uintptr_t>(p.w) & 15) == 0, g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float rs = r0 + i < p.rows ? p.rstd[r0 + i] : 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = r0 + i < p.rows && j < nc ? v[i][j] * rs * (p.w_offset + g[j]) : 0.f;
-    }
-  }
-  bool odd = false;
-  uint32_t rmax[8], cmax[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) rmax[i] = cmax[i] = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t m = fp8_mag(v[i][j], &odd);
-      rmax[i] = max(rmax[i], m);
-      cmax[j] = max(cmax[j], m);
-    }
+  Piece<T, NORM> x;
+  x.load(p, r0, c0, static_cast<int>(max(0ll, min(8ll, p.cols - c0))));
+  uint32_t rmax[4], cmax[4];
+  const bool odd = piece_maxima(x, rmax, cmax);
+  x.keep_packed();
   uint32_t tile_byte = 0;
   if (BLOCK) {
-    uint32_t m = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, rmax[i]);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) atomicMax(&s_max[0], m);
+    uint32_t m = __vmaxu2(__vmaxu2(rmax[0], rmax[1]), __vmaxu2(rmax[2], rmax[3]));
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+    if (lane == 0) s_max[warp][0] = m;
     __syncthreads();
-    tile_byte = fp8_scale_byte<FMT>(s_max[0]);
+#pragma unroll
+    for (int w = 0; w < Q_THREADS / 32; ++w) m = max(m, s_max[w][0]);
+    tile_byte = fp8_scale_byte<FMT>(m);
+  } else if (COLS) {
+    uint32_t c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = __vmaxu2(cmax[j], __shfl_xor_sync(0xffffffffu, cmax[j], 16));
+    if (lane < 16) *reinterpret_cast<uint4*>(&s_max[warp][cl * 4]) = make_uint4(c[0], c[1], c[2], c[3]);
   }
   if (ROWS) {
+    if (!BLOCK) {
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rmax[i] = __vmaxu2(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t m = rmax[i];
-      if (!BLOCK) {
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      }
-      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(m);
+      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(half16(rmax, i));
       // the tile's rows all get a scale, those past the matrix too: the tensor core reads 128 at a time
       if (cl == 0) p.sf[fp8_sf_offset(r0 + i, tile_c, p.kgroups)] = static_cast<uint8_t>(byte);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = x.get(i, j);
       if (r0 + i < p.rows && c0 < p.q_ld)
-        *reinterpret_cast<uint2*>(p.q + (r0 + i) * p.q_ld + c0) = fp8_pack8<FMT>(v[i], fp8_inverse_scale(byte), odd);
+        *reinterpret_cast<uint2*>(p.q + (r0 + i) * p.q_ld + c0) = fp8_pack8<FMT>(v, fp8_inverse_scale(byte), odd);
     }
   }
   if (COLS) {
+    x.keep_packed();
     if (!BLOCK) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t m = max(cmax[j], __shfl_xor_sync(0xffffffffu, cmax[j], 16));
-        if (lane < 16) atomicMax(&s_max[cl * 8 + j], m);
-      }
       __syncthreads();
+#pragma unroll
+      for (int w = 0; w < Q_THREADS / 32; ++w) {
+        const uint4 m = *reinterpret_cast<const uint4*>(&s_max[w][cl * 4]);
+        cmax[0] = __vmaxu2(cmax[0], m.x), cmax[1] = __vmaxu2(cmax[1], m.y);
+        cmax[2] = __vmaxu2(cmax[2], m.z), cmax[3] = __vmaxu2(cmax[3], m.w);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(s_max[cl * 8 + j]);
-      float t[8];
+      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(half16(cmax, j));
+      if (rg == 0)
+        p.sft[fp8_sf_offset(c0 + j, tile_r, p.kgroups_t)] = static_cast<uint8_t>(byte);
+      float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = v[i][j];
+      for (int i = 0; i < 8; ++i) v[i] = x.get(i, j);
       // 8-byte unit rg of column 8 cl + j sits at unit rg ^ cl: the 16 lanes of a half-warp hit 16 different units
-      *reinterpret_cast<uint2*>(s_t + (cl * 8 + j) * QT + (rg ^ cl) * 8) = fp8_pack8<FMT>(t, fp8_inverse_scale(byte), odd);
+      *reinterpret_cast<uint2*>(s_t + (cl * 8 + j) * QT + (rg ^ cl) * 8) = fp8_pack8<FMT>(v, fp8_inverse_scale(byte), odd);
     }
     __syncthreads();
-    const long long out_c = tile_r * QT;
+    const long long out_c = static_cast<long long>(tile_r) * QT;
 #pragma unroll
     for (int it = 0; it < QT / 16; ++it) {
       const int c = it * 16 + rg;                   // a half-warp writes the 128 bytes of one transposed row
@@ -125,9 +257,6 @@ fp8_quant_kernel(const QuantArgs p) {
         *reinterpret_cast<uint2*>(p.qt + col * p.qt_ld + out_c + cl * 8) =
             *reinterpret_cast<const uint2*>(s_t + c * QT + (cl ^ ((c >> 3) & 15)) * 8);
     }
-    if (threadIdx.x < QT)
-      p.sft[fp8_sf_offset(static_cast<long long>(tile_c) * QT + threadIdx.x, static_cast<int>(tile_r), p.kgroups_t)] =
-          static_cast<uint8_t>(BLOCK ? tile_byte : fp8_scale_byte<FMT>(s_max[threadIdx.x]));
   }
 }
 
@@ -145,11 +274,11 @@ template <typename T, int FMT>
 static void quant_launch(const QuantArgs& p, int mode, long long grid, cudaStream_t s) {
   const dim3 g(static_cast<unsigned>(grid));
   switch (mode) {
-    case 1: fp8_quant_kernel<T, FMT, true, false, false><<<g, Q_THREADS, 0, s>>>(p); break;
-    case 2: fp8_quant_kernel<T, FMT, false, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
-    case 3: fp8_quant_kernel<T, FMT, true, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
-    case 5: fp8_quant_kernel<T, FMT, true, false, true><<<g, Q_THREADS, 0, s>>>(p); break;
-    default: fp8_quant_kernel<T, FMT, true, true, true><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 1: fp8_quant_kernel<T, FMT, false, true, false, false><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 2: fp8_quant_kernel<T, FMT, false, false, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 3: fp8_quant_kernel<T, FMT, false, true, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 5: fp8_quant_kernel<T, FP8_E4M3, false, true, false, true><<<g, Q_THREADS, 0, s>>>(p); break;
+    default: fp8_quant_kernel<T, FP8_E4M3, false, true, true, true><<<g, Q_THREADS, 0, s>>>(p); break;
   }
 }
 
@@ -216,7 +345,7 @@ fp8_norm_kernel(const NormQuantArgs p) {
 #pragma unroll
     for (int i = 0; i < TPR / 32; ++i) ss += s_part[sub][i];
   }
-  const float rstd = rsqrtf(ss / p.D + p.eps);
+  const float rstd = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
   if (ok && t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -225,12 +354,9 @@ fp8_norm_kernel(const NormQuantArgs p) {
     float g[8];
     fp8_load8(p.w + c, n, p.vec, g);
     bool odd = false;
-    uint32_t m = 0u;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[i][j] = j < n ? v[i][j] * rstd * (p.w_offset + g[j]) : 0.f;
-      m = max(m, fp8_mag(v[i][j], &odd));
-    }
+    for (int j = 0; j < 8; ++j) v[i][j] = j < n ? v[i][j] * rstd * (p.w_offset + g[j]) : 0.f;
+    uint32_t m = fp8_max16(fp8_finite_max(v[i], &odd));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const uint32_t byte = fp8_scale_byte<FMT>(m);
@@ -401,10 +527,11 @@ extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long 
                                 const float* rstd, const void* w, float w_offset, void* stream) {
   if (rows <= 0 || cols <= 0) return 0;
   if ((fmt != FP8_E4M3 && fmt != FP8_E5M2) || (mode != 1 && mode != 2 && mode != 3 && mode != 5 && mode != 7)) return -1;
+  if (mode > 3 && fmt != FP8_E4M3) return -1;
   if (((mode & 1) && (!q || !sf || !aligned16(q) || q_ld % 16 || q_ld < cols)) ||
       ((mode & 2) && (!qt || !sft || !aligned16(qt) || qt_ld % 16 || qt_ld < rows)))
     return -2;
-  if ((rstd != nullptr) != (w != nullptr)) return -3;
+  if ((rstd != nullptr) != (w != nullptr) || (rstd != nullptr && (x_fp32 || mode != 2 || fmt != FP8_E4M3))) return -3;
   const long long row_tiles = (rows + QT - 1) / QT, col_tiles = (cols + QT - 1) / QT;
   if (row_tiles * col_tiles > 0x7fffffffll) return -4;
   const int elem = x_fp32 ? 4 : 2;
@@ -420,7 +547,9 @@ extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long 
   p.rstd = rstd, p.w = static_cast<const __nv_bfloat16*>(w), p.w_offset = w_offset;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long grid = row_tiles * col_tiles;
-  if (x_fp32) {
+  if (rstd != nullptr) {     // the transposed form of a norm's result: what a weight gradient reads
+    fp8_quant_kernel<__nv_bfloat16, FP8_E4M3, true, false, true, false><<<static_cast<unsigned>(grid), Q_THREADS, 0, s>>>(p);
+  } else if (x_fp32) {
     if (fmt == FP8_E4M3) quant_launch<float, FP8_E4M3>(p, mode, grid, s);
     else quant_launch<float, FP8_E5M2>(p, mode, grid, s);
   } else {
