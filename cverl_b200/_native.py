@@ -124,6 +124,8 @@ _CUDA_PROTOS = {
     "cvb_fp8_norm_bwd_parts": "",
     "cvb_fp8_norm_bwd": "pl pl pp pl pp pp l i f p",
     "cvb_fp8_gemm": "ppli ppli iii p l i p p",
+    "cvb_fp8_linear_fwd": "pil pil iii pppp p l i p p",
+    "cvb_fp8_linear_bwd": "pil i iii pppp pl pp f pli pli p p",
 }
 
 
@@ -187,6 +189,12 @@ def ptr(t) -> int | None:
 
 def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def raw_stream(device_index: int) -> int:
+    """The device's current stream as ``stream()`` gives it for the current device, without the Python stream object
+    (which costs a small operator more than its launch)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 _status_words = {}

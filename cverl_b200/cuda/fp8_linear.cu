@@ -1,0 +1,69 @@
+// The launches of an 8-bit linear layer, forward and backward, each behind one call: a small layer spends more time in
+// the calls than in the kernels (five ctypes calls of a 77-token layer's step took longer than its ten launches).
+//
+// Buffers of 8-bit matrices are codes (rows padded to 16 bytes) followed by the scale cells.
+#include <cuda_runtime.h>
+
+extern "C" {
+int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, long long x_stride, int fmt, int mode,
+                     void* q, void* sf, long long q_ld, void* qt, void* sft, long long qt_ld, const float* rstd,
+                     const void* w, float w_offset, void* stream);
+int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
+                 long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int* status,
+                 void* stream);
+}
+
+namespace {
+constexpr int E4M3 = 0;
+enum { ROWS = 1, COLS = 2, BLOCKS = 4 };
+
+struct Mat8 {      // [rows, cols] in a buffer; null buffer: absent
+  char* codes;
+  char* sf;
+  long long ld;
+  Mat8(void* buf, long long rows, long long cols) : codes(static_cast<char*>(buf)), sf(nullptr), ld((cols + 15) / 16 * 16) {
+    if (codes) sf = codes + rows * ld;
+  }
+};
+
+int quantize(const void* x, int x_fp32, long long rows, long long cols, long long stride, int fmt, int extra,
+             const Mat8& q, const Mat8& t, void* stream) {
+  const int mode = (q.codes ? ROWS : 0) | (t.codes ? COLS : 0) | extra;
+  return cvb_fp8_quantize(x, x_fp32, rows, cols, stride, fmt, mode, q.codes, q.sf, q.ld, t.codes, t.sf, t.ld, nullptr,
+                          nullptr, 0.f, stream);
+}
+int product(const Mat8& a, int a_fmt, const Mat8& b, int b_fmt, int M, int N, int K, void* c, long long ldc,
+            int out_kind, int* status, void* stream) {
+  return cvb_fp8_gemm(a.codes, a.sf, a.ld, a_fmt, b.codes, b.sf, b.ld, b_fmt, M, N, K, c, ldc, out_kind, status, stream);
+}
+}  // namespace
+
+// y [M, N] = x [M, K] w [N, K]^T.  x null: `xq` holds its 8-bit form already.  w null: `wq` does.  `xt` and `wt`
+// (both may be null) take the transposed forms that the backward pass reads.
+extern "C" int cvb_fp8_linear_fwd(const void* x, int x_fp32, long long x_stride, const void* w, int w_fp32,
+                                  long long w_stride, int M, int N, int K, void* xq, void* xt, void* wq, void* wt,
+                                  void* y, long long ldy, int out_kind, int* status, void* stream) {
+  const Mat8 mxq(xq, M, K), mxt(xt, K, M), mwq(wq, N, K), mwt(wt, K, N);
+  int rc = 0;
+  if (w && (rc = quantize(w, w_fp32, N, K, w_stride, E4M3, BLOCKS, mwq, mwt, stream))) return rc;
+  if (x && (rc = quantize(x, x_fp32, M, K, x_stride, E4M3, 0, mxq, mxt, stream))) return rc;
+  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, status, stream);
+}
+
+// dx [M, K] = dy w (where wt is given) and dw [N, K] (+)= dy^T x (where dw is given).  `dyq` and `dyt` are workspaces
+// for the two forms of dy.  h given: x is h * rstd * (w_offset + wn), formed into the workspace `xt`.
+extern "C" int cvb_fp8_linear_bwd(const void* dy, int dy_fp32, long long dy_stride, int grad_fmt, int M, int N, int K,
+                                  void* dyq, void* dyt, void* wt, void* xt, const void* h, long long h_stride,
+                                  const float* rstd, const void* wn, float w_offset, void* dx, long long lddx,
+                                  int dx_kind, void* dw, long long lddw, int dw_kind, int* status, void* stream) {
+  const Mat8 mdq(wt ? dyq : nullptr, M, N), mdt(dw ? dyt : nullptr, N, M), mwt(wt, K, N), mxt(xt, K, M);
+  if (!mdq.codes && !mdt.codes) return 0;
+  int rc = quantize(dy, dy_fp32, M, N, dy_stride, grad_fmt, 0, mdq, mdt, stream);
+  if (rc) return rc;
+  if (wt && (rc = product(mdq, grad_fmt, mwt, E4M3, M, K, N, dx, lddx, dx_kind, status, stream))) return rc;
+  if (!dw) return 0;
+  if (h && (rc = cvb_fp8_quantize(h, 0, M, K, h_stride, E4M3, COLS, nullptr, nullptr, 0, mxt.codes, mxt.sf, mxt.ld,
+                                  rstd, wn, w_offset, stream)))
+    return rc;
+  return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, status, stream);
+}

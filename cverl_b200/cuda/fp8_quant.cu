@@ -298,44 +298,84 @@ struct NormQuantArgs {
   float eps, w_offset;
 };
 
-template <int TPR, int NV, int FMT>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+// eight bf16 as read, of which the first n exist.  VEC: rows are whole 16-byte vectors, n is 0 or 8; the load is then
+// one predicated instruction, and those of a row are all in flight before the first is used.
+template <bool VEC>
+__device__ __forceinline__ uint4 load_raw8(const __nv_bfloat16* p, int n) {
+  uint4 u = make_uint4(0u, 0u, 0u, 0u);
+  if (VEC) {
+    if (n > 0) u = __ldg(reinterpret_cast<const uint4*>(p));
+  } else {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+    u.x = (n > 0 ? e[0] : 0u) | ((n > 1 ? e[1] : 0u) << 16);
+    u.y = (n > 2 ? e[2] : 0u) | ((n > 3 ? e[3] : 0u) << 16);
+    u.z = (n > 4 ? e[4] : 0u) | ((n > 5 ? e[5] : 0u) << 16);
+    u.w = (n > 6 ? e[6] : 0u) | ((n > 7 ? e[7] : 0u) << 16);
+  }
+  return u;
+}
+template <bool VEC>
+__device__ __forceinline__ void store_raw8(__nv_bfloat16* p, const uint4& u, int n) {
+  if (VEC) {
+    if (n > 0) *reinterpret_cast<uint4*>(p) = u;
+  } else {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) reinterpret_cast<uint16_t*>(p)[j] = static_cast<uint16_t>(w[j >> 1] >> ((j & 1) * 16));
+  }
+}
+__device__ __forceinline__ void widen8(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(w[j] << 16);
+    v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint4 narrow8(const float (&v)[8]) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+template <int TPR>
+struct RowBlock {
+  static constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  static constexpr int ROWS = THREADS / TPR;
+};
+
+template <int TPR, int NV, int FMT, bool VEC>
+__global__ void __launch_bounds__(RowBlock<TPR>::THREADS)
 fp8_norm_kernel(const NormQuantArgs p) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
-  constexpr int ROWS = THREADS / TPR;
+  constexpr int ROWS = RowBlock<TPR>::ROWS;
   __shared__ float s_part[ROWS][TPR / 32];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
   const bool ok = row < p.rows;
-  float v[NV][8];
+  uint4 xr[NV], rr[NV], wr[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * 8, n = max(0, min(8, p.D - c));
+    xr[i] = load_raw8<VEC>(p.x + row * p.x_stride + c, ok ? n : 0);
+    rr[i] = load_raw8<VEC>(p.resid + row * p.r_stride + c, ok && p.resid != nullptr ? n : 0);
+    wr[i] = load_raw8<VEC>(p.w + c, n);
+  }
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * 8;
-    const int n = ok ? max(0, min(8, p.D - c)) : 0;
-    fp8_load8(p.x + row * p.x_stride + c, n, p.vec, v[i]);
+    float v[8];
+    widen8(xr[i], v);
     if (p.resid != nullptr) {
+      const int c = (i * TPR + t) * 8, n = ok ? max(0, min(8, p.D - c)) : 0;
       float b[8];
-      fp8_load8(p.resid + row * p.r_stride + c, n, p.vec, b);
-      __nv_bfloat16* hp = p.h + row * p.h_stride + c;
-      uint32_t o[4];
+      widen8(rr[i], b);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(v[i][2 * j] + b[2 * j], v[i][2 * j + 1] + b[2 * j + 1]);
-      if (n == 8 && p.vec) {
-        *reinterpret_cast<uint4*>(hp) = make_uint4(o[0], o[1], o[2], o[3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < n) reinterpret_cast<uint16_t*>(hp)[j] = static_cast<uint16_t>(o[j >> 1] >> ((j & 1) * 16));
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[i][2 * j] = __uint_as_float(o[j] << 16);
-        v[i][2 * j + 1] = __uint_as_float(o[j] & 0xFFFF0000u);
-      }
+      for (int j = 0; j < 8; ++j) v[j] += b[j];
+      xr[i] = narrow8(v);
+      store_raw8<VEC>(p.h + row * p.h_stride + c, xr[i], n);
+      widen8(xr[i], v);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+    for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
   }
   ss = warp_sum(ss);
   if (TPR > 32) {
@@ -349,40 +389,47 @@ fp8_norm_kernel(const NormQuantArgs p) {
   if (ok && t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * 8;
-    const int n = max(0, min(8, p.D - c));
-    float g[8];
-    fp8_load8(p.w + c, n, p.vec, g);
+    const int c = (i * TPR + t) * 8, n = max(0, min(8, p.D - c));
+    float v[8], g[8];
+    widen8(xr[i], v);
+    widen8(wr[i], g);
     bool odd = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = j < n ? v[i][j] * rstd * (p.w_offset + g[j]) : 0.f;
-    uint32_t m = fp8_max16(fp8_finite_max(v[i], &odd));
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? v[j] * rstd * (p.w_offset + g[j]) : 0.f;
+    uint32_t m = fp8_max16(fp8_finite_max(v, &odd));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const uint32_t byte = fp8_scale_byte<FMT>(m);
     if (ok && c < p.D && (t & 15) == 0) p.sf[fp8_sf_offset(row, c >> 7, p.kgroups)] = static_cast<uint8_t>(byte);
     if (ok && c < p.q_ld)
-      *reinterpret_cast<uint2*>(p.q + row * p.q_ld + c) = fp8_pack8<FMT>(v[i], fp8_inverse_scale(byte), odd);
+      *reinterpret_cast<uint2*>(p.q + row * p.q_ld + c) = fp8_pack8<FMT>(v, fp8_inverse_scale(byte), odd);
   }
 }
 
 template <int TPR, int NV>
 static void norm_launch(const NormQuantArgs& p, int fmt, cudaStream_t s) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  constexpr int THREADS = RowBlock<TPR>::THREADS;
   const unsigned grid = static_cast<unsigned>((p.rows + THREADS / TPR - 1) / (THREADS / TPR));
-  if (fmt == FP8_E4M3) fp8_norm_kernel<TPR, NV, FP8_E4M3><<<grid, THREADS, 0, s>>>(p);
-  else fp8_norm_kernel<TPR, NV, FP8_E5M2><<<grid, THREADS, 0, s>>>(p);
+  if (p.vec) {
+    if (fmt == FP8_E4M3) fp8_norm_kernel<TPR, NV, FP8_E4M3, true><<<grid, THREADS, 0, s>>>(p);
+    else fp8_norm_kernel<TPR, NV, FP8_E5M2, true><<<grid, THREADS, 0, s>>>(p);
+  } else {
+    if (fmt == FP8_E4M3) fp8_norm_kernel<TPR, NV, FP8_E4M3, false><<<grid, THREADS, 0, s>>>(p);
+    else fp8_norm_kernel<TPR, NV, FP8_E5M2, false><<<grid, THREADS, 0, s>>>(p);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Backward of the norm, dn = gradient of its output:  g = dn * (w_offset + w), xh = h * rstd,
+// Backward of the norm, dn (fp32) = gradient of its output:  g = dn * (w_offset + w), xh = h * rstd,
 //   dx = rstd * (g - xh * mean(g * xh)) + dh,        dw = sum over rows of dn * xh.
-// Bound by HBM: 2 (dn) + 2 (h) + 2 (dh) read, 2 written per element.  Same row layout as the forward kernel.  Every
-// CTA walks rows at a stride of the grid and keeps its share of dw in registers; the shares are written out and
-// summed in a fixed order by a second kernel, so that dw is the same from run to run.
+// dn comes straight from the product's fp32 sums: rounding it to bf16 between the two would put a second rounding, as
+// large as the result's own, into every gradient.  Bound by HBM: 4 (dn) + 2 (h) + 2 (dh) read, 2 written per element.
+// Every CTA walks rows at a stride of the grid; a thread keeps a row's values packed as they were read and its share
+// of dw in registers.  The shares are summed in a fixed order by a second kernel, so dw is the same from run to run.
 // ---------------------------------------------------------------------------------------------------
 struct NormBwdArgs {
-  const __nv_bfloat16 *dn, *h, *w, *dh;
+  const float* dn;
+  const __nv_bfloat16 *h, *w, *dh;
   const float* rstd;
   __nv_bfloat16* dx;
   float* part;       // [grid, D]
@@ -391,95 +438,102 @@ struct NormBwdArgs {
   float w_offset;
 };
 
-template <int TPR, int NV>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+template <bool VEC>
+__device__ __forceinline__ void load_f32x8(const float* p, int n, float (&v)[8]) {
+  if (VEC) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (n > 0) {
+      a = __ldg(reinterpret_cast<const float4*>(p));
+      b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    }
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.f;
+  }
+}
+
+// A thread holds one vector of a row up to 8192 elements (two beyond): few registers, so that an SM has 1024 threads
+// with 64 bytes of loads each in flight.
+template <int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(RowBlock<TPR>::THREADS, 1024 / RowBlock<TPR>::THREADS)
 fp8_norm_bwd_kernel(const NormBwdArgs p) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
-  constexpr int ROWS = THREADS / TPR;
-  __shared__ float s_part[ROWS][TPR / 32];
-  __shared__ float s_dw[ROWS > 1 ? ROWS * TPR * NV * 8 : 1];
+  constexpr int ROWS = RowBlock<TPR>::ROWS;
+  __shared__ float s_part[2][ROWS][TPR / 32];
+  __shared__ float s_dw[ROWS > 1 ? TPR * NV * 8 : 1];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, lane = threadIdx.x & 31;
   float acc[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+  int flip = 0;
   // the trip count is the block's, not the row group's: TPR > 32 synchronises inside
   for (long long r0 = static_cast<long long>(blockIdx.x) * ROWS; r0 < p.rows; r0 += static_cast<long long>(gridDim.x) * ROWS) {
     const long long row = r0 + sub;
     const bool ok = row < p.rows;
+    uint4 hr[NV], dr[NV];
+    float gn[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * 8, n = ok ? max(0, min(8, p.D - c)) : 0;
+      hr[i] = load_raw8<VEC>(p.h + row * p.h_stride + c, n);
+      load_f32x8<VEC>(p.dn + row * p.dn_stride + c, n, gn[i]);
+      dr[i] = load_raw8<VEC>(p.dh + row * p.dh_stride + c, p.dh != nullptr ? n : 0);
+    }
     const float rstd = ok ? p.rstd[row] : 0.f;
-    float xh[NV][8], gn[NV][8];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * 8;
-      const int n = ok ? max(0, min(8, p.D - c)) : 0;
-      float w8[8];
-      fp8_load8(p.h + row * p.h_stride + c, n, p.vec, xh[i]);
-      fp8_load8(p.dn + row * p.dn_stride + c, n, p.vec, gn[i]);
-      fp8_load8(p.w + c, n, p.vec, w8);
+      float xh[8], w8[8];
+      widen8(hr[i], xh);
+      widen8(load_raw8<VEC>(p.w + c, max(0, min(8, p.D - c))), w8);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        xh[i][j] *= rstd;
-        acc[i][j] += gn[i][j] * xh[i][j];
+        const float x = xh[j] * rstd;
+        acc[i][j] += gn[i][j] * x;
         gn[i][j] *= p.w_offset + w8[j];
-        dot += j < n ? gn[i][j] * xh[i][j] : 0.f;
+        dot += gn[i][j] * x;             // both are zero outside the row
       }
     }
     dot = warp_sum(dot);
     if (TPR > 32) {
-      __syncthreads();          // the previous row's sums have been read
-      if (lane == 0) s_part[sub][t >> 5] = dot;
-      __syncthreads();
+      if (lane == 0) s_part[flip][sub][t >> 5] = dot;
+      __syncthreads();                   // the other buffer's readers are all past the barrier before this one
       dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < TPR / 32; ++i) dot += s_part[sub][i];
+      for (int i = 0; i < TPR / 32; ++i) dot += s_part[flip][sub][i];
+      flip ^= 1;
     }
-    dot /= p.D;
+    dot *= rstd / p.D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * 8;
-      const int n = ok ? max(0, min(8, p.D - c)) : 0;
-      float d8[8];
+      const int c = (i * TPR + t) * 8, n = ok ? max(0, min(8, p.D - c)) : 0;
+      float xh[8], d8[8];
+      widen8(hr[i], xh);
+      widen8(dr[i], d8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d8[j] = 0.f;
-      if (p.dh != nullptr) fp8_load8(p.dh + row * p.dh_stride + c, n, p.vec, d8);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d8[j] += rstd * (gn[i][j] - xh[i][j] * dot);
-      __nv_bfloat16* out = p.dx + row * p.D + c;
-      if (n == 8 && p.vec) {
-        *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(d8[0], d8[1]), pack_bf16x2(d8[2], d8[3]),
-                                                    pack_bf16x2(d8[4], d8[5]), pack_bf16x2(d8[6], d8[7]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < n) out[j] = __float2bfloat16_rn(d8[j]);
-      }
+      for (int j = 0; j < 8; ++j) d8[j] += rstd * (gn[i][j] - xh[j] * dot);
+      store_raw8<VEC>(p.dx + row * p.D + c, narrow8(d8), n);
     }
   }
   if (p.part == nullptr) return;
   float* part = p.part + static_cast<long long>(blockIdx.x) * p.D;
-  if (ROWS > 1) {
+  // the row groups add their shares one after the other, in the same order every time
+  for (int g = 0; g < ROWS; ++g) {
+    if (sub == g) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s_dw[(sub * NV * TPR + i * TPR + t) * 8 + j] = acc[i][j];
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.D; c += THREADS) {
-      float sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) sum += s_dw[r * NV * TPR * 8 + c];
-      part[c] = sum;
+        for (int j = 0; j < 8; ++j) {
+          const int c = (i * TPR + t) * 8 + j;
+          const float v = g > 0 ? s_dw[ROWS > 1 ? (i * 8 + j) * TPR + t : 0] + acc[i][j] : acc[i][j];
+          if (g < ROWS - 1) s_dw[ROWS > 1 ? (i * 8 + j) * TPR + t : 0] = v;
+          else if (c < p.D) part[c] = v;
+        }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = (i * TPR + t) * 8 + j;
-        if (c < p.D) part[c] = acc[i][j];
-      }
+    if (ROWS > 1) __syncthreads();
   }
 }
 
@@ -508,10 +562,12 @@ constexpr int NORM_BWD_MAX_PARTS = 592;   // 148 SMs with four CTAs each
 
 template <int TPR, int NV>
 static int norm_bwd_launch(const NormBwdArgs& p, cudaStream_t s) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  constexpr int THREADS = RowBlock<TPR>::THREADS;
   const long long want = (p.rows + THREADS / TPR - 1) / (THREADS / TPR);
-  const int grid = static_cast<int>(want < NORM_BWD_MAX_PARTS ? want : NORM_BWD_MAX_PARTS);
-  fp8_norm_bwd_kernel<TPR, NV><<<grid, THREADS, 0, s>>>(p);
+  const int resident = 148 * (1024 / THREADS);
+  const int grid = static_cast<int>(want < resident ? want : resident);
+  if (p.vec) fp8_norm_bwd_kernel<TPR, NV, true><<<grid, THREADS, 0, s>>>(p);
+  else fp8_norm_bwd_kernel<TPR, NV, false><<<grid, THREADS, 0, s>>>(p);
   return grid;
 }
 
@@ -600,30 +656,30 @@ extern "C" int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void
 extern "C" int cvb_fp8_norm_bwd_parts(void) { return NORM_BWD_MAX_PARTS; }
 
 // dw_acc (fp32, +=) or dw (bf16); both null: no weight gradient
-extern "C" int cvb_fp8_norm_bwd(const void* dn, long long dn_stride, const void* h, long long h_stride, const void* w,
+extern "C" int cvb_fp8_norm_bwd(const float* dn, long long dn_stride, const void* h, long long h_stride, const void* w,
                                 const float* rstd, const void* dh, long long dh_stride, void* dx, float* part,
                                 float* dw_acc, void* dw, long long rows, int D, float w_offset, void* stream) {
   if (rows <= 0 || D <= 0) return 0;
   if (D > 16384) return -3;
   if ((dw_acc != nullptr || dw != nullptr) && part == nullptr) return -2;
   NormBwdArgs p = {};
-  p.dn = static_cast<const __nv_bfloat16*>(dn), p.h = static_cast<const __nv_bfloat16*>(h);
+  p.dn = dn, p.h = static_cast<const __nv_bfloat16*>(h);
   p.w = static_cast<const __nv_bfloat16*>(w), p.dh = static_cast<const __nv_bfloat16*>(dh);
   p.rstd = rstd, p.dx = static_cast<__nv_bfloat16*>(dx);
   p.part = dw_acc != nullptr || dw != nullptr ? part : nullptr;
   p.rows = rows, p.dn_stride = dn_stride, p.h_stride = h_stride, p.dh_stride = dh_stride, p.D = D;
-  p.vec = aligned16(dn) && aligned16(h) && aligned16(w) && aligned16(dh) && aligned16(dx) && dn_stride % 8 == 0 &&
+  p.vec = aligned16(dn) && aligned16(h) && aligned16(w) && aligned16(dh) && aligned16(dx) && dn_stride % 4 == 0 &&
           h_stride % 8 == 0 && dh_stride % 8 == 0 && D % 8 == 0;
   p.w_offset = w_offset;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int grid;
   if (D <= 256) grid = norm_bwd_launch<32, 1>(p, s);
-  else if (D <= 512) grid = norm_bwd_launch<32, 2>(p, s);
-  else if (D <= 1024) grid = norm_bwd_launch<32, 4>(p, s);
-  else if (D <= 2048) grid = norm_bwd_launch<128, 2>(p, s);
-  else if (D <= 4096) grid = norm_bwd_launch<128, 4>(p, s);
-  else if (D <= 8192) grid = norm_bwd_launch<256, 4>(p, s);
-  else grid = norm_bwd_launch<512, 4>(p, s);
+  else if (D <= 512) grid = norm_bwd_launch<64, 1>(p, s);
+  else if (D <= 1024) grid = norm_bwd_launch<128, 1>(p, s);
+  else if (D <= 2048) grid = norm_bwd_launch<256, 1>(p, s);
+  else if (D <= 4096) grid = norm_bwd_launch<512, 1>(p, s);
+  else if (D <= 8192) grid = norm_bwd_launch<1024, 1>(p, s);
+  else grid = norm_bwd_launch<1024, 2>(p, s);
   if (p.part != nullptr)
     fp8_norm_dw_kernel<<<(D + 31) / 32, 1024, 0, s>>>(part, grid, D, dw_acc, static_cast<__nv_bfloat16*>(dw));
   return static_cast<int>(cudaGetLastError());

@@ -21,14 +21,13 @@ statement of the same math, which is also the test oracle.  The reference has no
 """
 from __future__ import annotations
 
-import contextlib
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _native as nv
-from .gemm import _alloc_out, count_launch
+from .gemm import count_launch
 
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
 BLOCK = 128
@@ -43,11 +42,37 @@ def _ceil(a: int, b: int) -> int:
     return (a + b - 1) // b
 
 
-def _device(t: torch.Tensor):
-    """Launches go to the tensor's device and to that device's current stream."""
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+class _On:
+    """Launches of a block go to one device: ``stream`` is that device's current stream, ``status`` its status word."""
+
+    __slots__ = ("index", "before", "stream", "status")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.get_device()
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        self.stream = nv.raw_stream(self.index)
+        self.status = nv.status_word(self.index).data_ptr()
+        return self
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _bytes(n: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _alloc_rows(M: int, N: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """``[M, N]`` whose rows start on 16 bytes (what the vector stores of the product want)."""
+    per16 = 8 if dtype == torch.bfloat16 else 4
+    if N % per16 == 0:
+        return torch.empty((M, N), dtype=dtype, device=device)
+    return torch.empty((M, _ceil(N, per16) * per16), dtype=dtype, device=device)[:, :N]
 
 
 # ----------------------------------------------------------------------------
@@ -91,9 +116,8 @@ class Fp8Tensor:
         if out.numel() == 0:
             pass
         elif self.buf.is_cuda:
-            with _device(self.buf):
-                nv.check(nv.cuda().cvb_fp8_scales(self.sf_ptr, out.data_ptr(), self.rows, nb, nv.stream()),
-                         "cvb_fp8_scales")
+            with _On(out) as on:
+                nv.check(nv.cuda().cvb_fp8_scales(self.sf_ptr, out.data_ptr(), self.rows, nb, on.stream), "cvb_fp8_scales")
             count_launch()
         else:
             out.copy_(_scale_cells(self.buf, self.rows, self.cols, self.ld)[:self.rows, :nb])
@@ -171,51 +195,49 @@ def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int, rstd=None, w=None,
     R, C = x.shape
     tall = BLOCK if mode & _TILES else 1
     if not x.is_cuda:
+        x = x.detach()
         v = x.float() if rstd is None else x.float() * rstd[:, None] * (w_offset + w.float())
         return (_pack_ref(v, dtype, tall) if mode & _ROWS else None,
                 _pack_ref(v.t(), dtype, tall) if mode & _COLS else None)
-    n_q = Fp8Tensor.nbytes_of(R, C) if mode & _ROWS else 0
-    n_t = Fp8Tensor.nbytes_of(C, R) if mode & _COLS else 0
-    q = Fp8Tensor(torch.empty(n_q, dtype=torch.uint8, device=x.device), R, C, dtype) if n_q or mode & _ROWS else None
-    t = Fp8Tensor(torch.empty(n_t, dtype=torch.uint8, device=x.device), C, R, dtype) if n_t or mode & _COLS else None
+    q = t = None
+    q_args = t_args = (None, None, 0)
+    if mode & _ROWS:
+        q = Fp8Tensor(_bytes(Fp8Tensor.nbytes_of(R, C), x.device), R, C, dtype)
+        q_args = (q.buf.data_ptr(), q.sf_ptr, q.ld)
+    if mode & _COLS:
+        t = Fp8Tensor(_bytes(Fp8Tensor.nbytes_of(C, R), x.device), C, R, dtype)
+        t_args = (t.buf.data_ptr(), t.sf_ptr, t.ld)
     if R and C:
-        with _device(x):
+        with _On(x) as on:
             nv.check(nv.cuda().cvb_fp8_quantize(
-                x.data_ptr(), int(x.dtype == torch.float32), R, C, x.stride(0), _FMT[dtype], mode,
-                q.buf.data_ptr() if q else None, q.sf_ptr if q else None, q.ld if q else 0,
-                t.buf.data_ptr() if t else None, t.sf_ptr if t else None, t.ld if t else 0,
-                nv.ptr(rstd), nv.ptr(w), w_offset, nv.stream()), "cvb_fp8_quantize")
+                x.data_ptr(), x.dtype == torch.float32, R, C, x.stride(0), _FMT[dtype], mode, *q_args, *t_args,
+                nv.ptr(rstd), nv.ptr(w), w_offset, on.stream), "cvb_fp8_quantize")
         count_launch()
     return q, t
 
 
-@torch.no_grad()
 def quantize_fp8(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
     """``x [R, C]`` (bf16 or fp32) in 8 bits, one scale per 128 elements of a row."""
     _check_dtype(dtype, "quantize_fp8")
     return _quantize(_check_matrix(x, "quantize_fp8"), dtype, _ROWS)[0]
 
 
-@torch.no_grad()
 def quantize_fp8_t(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
     """``x.T [C, R]`` in 8 bits, one scale per 128 rows of ``x``."""
     _check_dtype(dtype, "quantize_fp8_t")
     return _quantize(_check_matrix(x, "quantize_fp8_t"), dtype, _COLS)[1]
 
 
-@torch.no_grad()
 def quantize_fp8_pair(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Tuple[Fp8Tensor, Fp8Tensor]:
     """``(quantize_fp8(x), quantize_fp8_t(x))`` from one read of ``x``."""
     _check_dtype(dtype, "quantize_fp8_pair")
     return _quantize(_check_matrix(x, "quantize_fp8_pair"), dtype, _ROWS | _COLS)
 
 
-@torch.no_grad()
 def quantize_fp8_weight(w: torch.Tensor, transposed: bool = True) -> Fp8Weight:
     """A weight ``[N, K]`` in e4m3 with one scale per 128 x 128 block.  ``transposed=False`` leaves the transpose out,
     which only gradients of the layer's input need."""
-    w = _check_matrix(w, "quantize_fp8_weight")
-    q, t = _quantize(w, E4M3, _ROWS | _TILES | (_COLS if transposed else 0))
+    q, t = _quantize(_check_matrix(w, "quantize_fp8_weight"), E4M3, _ROWS | _TILES | (_COLS if transposed else 0))
     return Fp8Weight(q, t)
 
 
@@ -239,7 +261,7 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
         dt = out_dtype or torch.bfloat16
         if dt not in _OUT:
             raise TypeError(f"gemm_fp8_nt: the result is bfloat16 or float32, not {dt}")
-        out = _alloc_out(M, N, dt, a.device)
+        out = _alloc_rows(M, N, dt, a.device)
     else:
         if tuple(out.shape) != (M, N) or out.device != a.device:
             raise ValueError(f"gemm_fp8_nt: out is {tuple(out.shape)} on {out.device}, not {(M, N)} on {a.device}")
@@ -256,11 +278,11 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
     if not a.buf.is_cuda:
         r = a.dequantize() @ b.dequantize().t()
         return out.add_(r) if accumulate else out.copy_(r)
-    with _device(a.buf):
+    with _On(out) as on:
         nv.check(nv.cuda().cvb_fp8_gemm(
             a.buf.data_ptr(), a.sf_ptr, a.ld, _FMT[a.dtype], b.buf.data_ptr(), b.sf_ptr, b.ld, _FMT[b.dtype], M, N, K,
-            out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype],
-            nv.status_word(a.device).data_ptr(), nv.stream()), "cvb_fp8_gemm")
+            out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype], on.status, on.stream),
+            "cvb_fp8_gemm")
     count_launch()
     return out
 
@@ -292,28 +314,28 @@ def _norm_forward(x2, r2, w, eps, w_offset, dtype, need_rstd: bool):
         h = x2 if r2 is None else (x2.float() + r2.float()).to(x2.dtype)
         rstd = torch.rsqrt(h.float().pow(2).mean(-1) + eps)
         return _pack_ref(h.float() * rstd[:, None] * (w_offset + w.float()), dtype), h, rstd
-    q = Fp8Tensor(torch.empty(Fp8Tensor.nbytes_of(R, D), dtype=torch.uint8, device=x2.device), R, D, dtype)
+    q = Fp8Tensor(_bytes(Fp8Tensor.nbytes_of(R, D), x2.device), R, D, dtype)
     h = torch.empty((R, D), dtype=x2.dtype, device=x2.device) if r2 is not None else None
     rstd = torch.empty(R, dtype=torch.float32, device=x2.device) if need_rstd else None
     if R:
         w = w.contiguous()
-        with _device(x2):
+        with _On(x2) as on:
             nv.check(nv.cuda().cvb_fp8_add_rmsnorm(
                 x2.data_ptr(), x2.stride(0), nv.ptr(r2), r2.stride(0) if r2 is not None else 0, w.data_ptr(),
                 nv.ptr(h), q.buf.data_ptr(), q.sf_ptr, q.ld, nv.ptr(rstd), R, D, _FMT[dtype], eps, w_offset,
-                nv.stream()), "cvb_fp8_add_rmsnorm")
+                on.stream), "cvb_fp8_add_rmsnorm")
         count_launch()
     return q, (h if h is not None else x2), rstd
 
 
-@torch.no_grad()
 def add_rmsnorm_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], w: torch.Tensor, eps: float = 1e-6,
                     w_offset: float = 1.0, dtype: torch.dtype = E4M3) -> Tuple[Fp8Tensor, torch.Tensor]:
     """``(Q(rmsnorm(x + resid)), x + resid)``; ``resid`` may be None.  The norm is rounded once, from fp32 to 8 bits;
     rows of the result are the rows of ``x`` flattened to a matrix.  For gradients see ``add_rmsnorm_linear_fp8``."""
     _check_dtype(dtype, "add_rmsnorm_fp8")
     _check_norm(x, resid, w, "add_rmsnorm_fp8")
-    q, h, _ = _norm_forward(_rows2d(x), _rows2d(resid) if resid is not None else None, w, eps, w_offset, dtype, False)
+    r2 = _rows2d(resid.detach()) if resid is not None else None
+    q, h, _ = _norm_forward(_rows2d(x.detach()), r2, w.detach(), eps, w_offset, dtype, False)
     return q, (x if resid is None else h.view(x.shape))
 
 
@@ -333,46 +355,107 @@ def _check_linear(K: int, device, w, weight: Optional[Fp8Weight], grad_dtype, wh
         raise ValueError(f"{what}: the 8-bit weight is {weight.shape} on {weight.w.device}, the weight {shape} on {device}")
 
 
-def _weight_grad(qdyt: Fp8Tensor, qxt: Fp8Tensor, w: torch.Tensor):
-    """dw = dy^T x: added to ``w.main_grad`` (fp32) where the parameter has one, else returned in its dtype."""
-    main = getattr(w, "main_grad", None)
-    if main is not None:
-        gemm_fp8_nt(qdyt, qxt, main.view(w.shape), accumulate=True)
-        return None
-    return gemm_fp8_nt(qdyt, qxt, torch.empty(w.shape, dtype=w.dtype, device=w.device))
+def _forward(x2, xq, w, weight: Optional[Fp8Weight], M, N, K, need_wt: bool, need_xt: bool, dtype):
+    """``(y, xt, wt)``: the product and the transposed 8-bit forms that gradients read (buffers or None).  ``x2`` is the
+    input's rows or None where ``xq`` is its 8-bit form; ``w`` the weight or None where ``weight`` is."""
+    device = (x2 if x2 is not None else xq.buf).device
+    y = _alloc_rows(M, N, dtype, device)
+    if not y.is_cuda:
+        xt = None
+        if x2 is not None:
+            xq, xt = _quantize(x2, E4M3, _ROWS | (_COLS if need_xt else 0))
+        weight = weight or quantize_fp8_weight(w, transposed=need_wt)
+        gemm_fp8_nt(xq, weight.w, y)
+        return y, xt.buf if xt else None, weight.wt.buf if need_wt else None
+    xt = _bytes(Fp8Tensor.nbytes_of(K, M), device) if need_xt else None
+    xb = xq.buf if xq is not None else _bytes(Fp8Tensor.nbytes_of(M, K), device)
+    if weight is None:
+        w = _check_matrix(w, "linear_fp8 weight")
+        wq = _bytes(Fp8Tensor.nbytes_of(N, K), device)
+        wt = _bytes(Fp8Tensor.nbytes_of(K, N), device) if need_wt else None
+    else:
+        w, wq, wt = None, weight.w.buf, weight.wt.buf if need_wt else None
+    if M and N and K:
+        with _On(y) as on:
+            nv.check(nv.cuda().cvb_fp8_linear_fwd(
+                nv.ptr(x2), x2 is not None and x2.dtype == torch.float32, x2.stride(0) if x2 is not None else 0,
+                nv.ptr(w), w is not None and w.dtype == torch.float32, w.stride(0) if w is not None else 0, M, N, K,
+                xb.data_ptr(), nv.ptr(xt), wq.data_ptr(), nv.ptr(wt) if weight is None else None,
+                y.data_ptr(), max(y.stride(0), N), _OUT[dtype], on.status, on.stream), "cvb_fp8_linear_fwd")
+        count_launch(1 + (x2 is not None) + (w is not None))
+    else:
+        if weight is None:      # no rows: the gradient of the input is empty too, and reads nothing
+            weight = quantize_fp8_weight(w, transposed=need_wt)
+            wt = weight.wt.buf if need_wt else None
+        y.zero_()
+    return y, xt, wt
 
 
-def _quantize_dy(dy, N, grad_dtype, need_dx, need_dw):
+def _backward(dy, M, N, K, grad_dtype, wt, xt, w, dx_dtype, norm=None):
+    """``(dx or None, dw or None)`` of ``y = x w^T``: dx where ``wt`` is given, dw where the parameter ``w`` is (added
+    to its fp32 ``main_grad`` where it has one, and then None).  ``norm = (h, rstd, wn, w_offset)`` stands for ``xt``."""
     dy2 = _check_matrix(dy.reshape(-1, N) if dy.numel() else dy.reshape(0, N), "linear_fp8 gradient")
-    return _quantize(dy2, grad_dtype, (_ROWS if need_dx else 0) | (_COLS if need_dw else 0))
+    dx = _alloc_rows(M, K, dx_dtype, dy.device) if wt is not None else None
+    main = getattr(w, "main_grad", None) if w is not None else None
+    target = None
+    if w is not None:
+        target = main.view(N, K) if main is not None else _alloc_rows(N, K, w.dtype, dy.device)
+    if not (M and N and K):
+        if dx is not None:
+            dx.zero_()
+        if target is not None and main is None:
+            target.zero_()
+    elif not dy2.is_cuda:
+        qdy, qdyt = _quantize(dy2, grad_dtype, (_ROWS if wt is not None else 0) | (_COLS if w is not None else 0))
+        if dx is not None:
+            gemm_fp8_nt(qdy, Fp8Tensor(wt, K, N, E4M3), dx)
+        if target is not None:
+            if norm is not None:
+                xt = _quantize(norm[0], E4M3, _COLS, *norm[1:])[1].buf
+            gemm_fp8_nt(qdyt, Fp8Tensor(xt, K, M, E4M3), target, accumulate=main is not None)
+    else:
+        if main is not None and (main.dtype != torch.float32 or not main.is_contiguous()):
+            raise TypeError("linear_fp8: main_grad is a contiguous float32 tensor")
+        dyq = _bytes(Fp8Tensor.nbytes_of(M, N), dy.device) if wt is not None else None
+        dyt = _bytes(Fp8Tensor.nbytes_of(N, M), dy.device) if w is not None else None
+        h = rstd = wn = None
+        w_offset = 0.0
+        if norm is not None and w is not None:
+            h, rstd, wn, w_offset = norm
+            xt = _bytes(Fp8Tensor.nbytes_of(K, M), dy.device)
+        with _On(dy2) as on:
+            nv.check(nv.cuda().cvb_fp8_linear_bwd(
+                dy2.data_ptr(), dy2.dtype == torch.float32, dy2.stride(0), _FMT[grad_dtype], M, N, K, nv.ptr(dyq),
+                nv.ptr(dyt), nv.ptr(wt), nv.ptr(xt), nv.ptr(h), h.stride(0) if h is not None else 0, nv.ptr(rstd),
+                nv.ptr(wn), w_offset, nv.ptr(dx), max(dx.stride(0), K) if dx is not None else 0,
+                _OUT[dx_dtype], nv.ptr(target), max(target.stride(0), K) if target is not None else 0,
+                2 if main is not None else _OUT[w.dtype] if w is not None else 0, on.status, on.stream),
+                "cvb_fp8_linear_bwd")
+        count_launch(1 + (wt is not None) + (w is not None) + (h is not None))
+    return dx, (target if main is None else None)
 
 
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, weight, grad_dtype):
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        x2 = _rows2d(x)
-        if weight is None:
-            weight = quantize_fp8_weight(w, transposed=need_dx)
-        elif need_dx and weight.wt is None:
+        if need_dx and weight is not None and weight.wt is None:
             raise ValueError("linear_fp8: the gradient of the input needs the transposed 8-bit weight")
-        qx, qxt = _quantize(x2, E4M3, _ROWS | (_COLS if need_dw else 0))
-        y = gemm_fp8_nt(qx, weight.w, out_dtype=torch.bfloat16 if x.is_cuda else x.dtype)
-        # what the gradients need: x^T and w^T in 8 bits, half of what the bf16 layer keeps of x
-        ctx.save_for_backward(w if need_dw else None, qxt.buf if need_dw else None, weight.wt.buf if need_dx else None)
-        ctx.cfg = (x.shape, x.dtype, x2.shape[0], w.shape, grad_dtype)
-        return y.reshape(*x.shape[:-1], w.shape[0])
+        x2 = _rows2d(x)
+        (M, K), N = x2.shape, w.shape[0]
+        y, xt, wt = _forward(x2, None, w, weight, M, N, K, need_dx, need_dw, x.dtype)
+        # what the gradients read: x^T and w^T in 8 bits, half of what the bf16 layer keeps of x
+        ctx.save_for_backward(w if need_dw else None, xt, wt)
+        ctx.cfg = (x.shape, x.dtype, M, N, K, grad_dtype)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
 
     @staticmethod
     def backward(ctx, dy):
-        w, qxt, wt = ctx.saved_tensors
-        shape, xdtype, M, (N, K), grad_dtype = ctx.cfg
-        qdy, qdyt = _quantize_dy(dy, N, grad_dtype, wt is not None, qxt is not None)
-        dx = dw = None
-        if wt is not None:
-            dx = gemm_fp8_nt(qdy, Fp8Tensor(wt, K, N, E4M3), out_dtype=xdtype).reshape(shape)
-        if qxt is not None:
-            dw = _weight_grad(qdyt, Fp8Tensor(qxt, K, M, E4M3), w)
+        w, xt, wt = ctx.saved_tensors
+        shape, xdtype, M, N, K, grad_dtype = ctx.cfg
+        dx, dw = _backward(dy, M, N, K, grad_dtype, wt, xt, w, xdtype)
+        if dx is not None and len(shape) != 2:
+            dx = dx.reshape(shape)
         return dx, dw, None, None
 
 
@@ -387,21 +470,23 @@ def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dt
     if weight is not None and isinstance(w, Fp8Weight):
         raise ValueError(f"{what}: the 8-bit weight is given twice")
     frozen = w if isinstance(w, Fp8Weight) else None
+    N = w.shape[0] if len(w.shape) else 0
     if isinstance(x, Fp8Tensor):
         _check_linear(x.cols, x.device, w, weight, grad_dtype, what)
-        if frozen is None:
-            frozen = weight or quantize_fp8_weight(w, transposed=False)
-        return gemm_fp8_nt(x, frozen.w)
+        if x.dtype != E4M3:
+            raise TypeError(f"{what}: inputs are torch.float8_e4m3fn, got {x.dtype}")
+        with torch.no_grad():
+            return _forward(None, x, w, frozen or weight, x.rows, N, x.cols, False, False, torch.bfloat16)[0]
     if x.dim() < 1:
         raise ValueError(f"{what}: x has no dimensions")
     if x.dtype != torch.bfloat16 and (x.is_cuda or x.dtype != torch.float32):
         raise TypeError(f"{what}: bfloat16 is wanted, got {x.dtype}")
     _check_linear(x.shape[-1], x.device, w, weight, grad_dtype, what)
+    if not (torch.is_grad_enabled() and (x.requires_grad or (frozen is None and w.requires_grad))):
+        x2 = _rows2d(x)
+        y = _forward(x2, None, w, frozen or weight, x2.shape[0], N, x2.shape[1], False, False, x.dtype)[0]
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
     if frozen is not None:
-        if not (torch.is_grad_enabled() and x.requires_grad):
-            x2 = _rows2d(x)
-            y = gemm_fp8_nt(_quantize(x2, E4M3, _ROWS)[0], frozen.w, out_dtype=x.dtype)
-            return y.reshape(*x.shape[:-1], w.shape[0])
         return _LinearFp8.apply(x, _Shape(w.shape), frozen, grad_dtype)
     return _LinearFp8.apply(x, w, weight, grad_dtype)
 
@@ -418,39 +503,33 @@ class _NormLinearFp8(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, resid, wn, w, weight, eps, w_offset, grad_dtype):
-        need_dn = any(ctx.needs_input_grad[:3])
-        need_dw = ctx.needs_input_grad[3]
-        if weight is None:
-            weight = quantize_fp8_weight(w, transposed=need_dn)
-        elif need_dn and weight.wt is None:
+        need_dn, need_dw = any(ctx.needs_input_grad[:3]), ctx.needs_input_grad[3]
+        if need_dn and weight is not None and weight.wt is None:
             raise ValueError("add_rmsnorm_linear_fp8: the gradient of the input needs the transposed 8-bit weight")
         x2 = _rows2d(x)
-        q, h, rstd = _norm_forward(x2, _rows2d(resid) if resid is not None else None, wn, eps, w_offset, E4M3, True)
-        y = gemm_fp8_nt(q, weight.w, out_dtype=torch.bfloat16 if x.is_cuda else x.dtype)
-        ctx.save_for_backward(h, rstd, wn, w if need_dw else None, weight.wt.buf if need_dn else None)
-        ctx.cfg = (x.shape, w.shape, w_offset, grad_dtype, resid is not None, need_dn, need_dw)
-        y = y.reshape(*x.shape[:-1], w.shape[0])
-        if resid is None:
-            return y
-        return y, h.view(x.shape)
+        (M, K), N = x2.shape, w.shape[0]
+        q, h, rstd = _norm_forward(x2, _rows2d(resid) if resid is not None else None, wn, eps, w_offset, E4M3,
+                                   need_dn or need_dw)
+        y, _, wt = _forward(None, q, w, weight, M, N, K, need_dn, False, x.dtype)
+        ctx.save_for_backward(h, rstd, wn, w if need_dw else None, wt)
+        ctx.cfg = (x.shape, M, N, K, w_offset, grad_dtype)
+        if x.dim() != 2:
+            y = y.reshape(*x.shape[:-1], N)
+        return y if resid is None else (y, h.view(x.shape))
 
     @staticmethod
     def backward(ctx, dy, dh=None):
         h, rstd, wn, w, wt = ctx.saved_tensors
-        shape, (N, K), w_offset, grad_dtype, has_resid, need_dn, need_dw = ctx.cfg
-        qdy, qdyt = _quantize_dy(dy, N, grad_dtype, need_dn, need_dw)
-        dx = dwn = dw = None
-        if need_dw:
-            # the norm's result is formed again from h and rstd while its transpose is quantised: it is never stored
-            qnt = _quantize(h, E4M3, _COLS, rstd, wn.contiguous(), w_offset)[1]
-            dw = _weight_grad(qdyt, qnt, w)
-        if need_dn:
-            # bf16 between the product and the norm's backward, as between the bf16 layers: half the traffic of fp32
-            dn = gemm_fp8_nt(qdy, Fp8Tensor(wt, K, N, E4M3), out_dtype=h.dtype)
-            dx, dwn = _norm_backward(dn, h, wn, rstd, dh, w_offset, ctx.needs_input_grad[2])
+        shape, M, N, K, w_offset, grad_dtype = ctx.cfg
+        need_x, need_r, need_wn = ctx.needs_input_grad[:3]
+        # The norm's result is formed again from h and rstd while its transpose is quantised: it is never stored.  Its
+        # gradient stays fp32 between the product and the norm's backward.
+        dn, dw = _backward(dy, M, N, K, grad_dtype, wt, None, w, torch.float32, (h, rstd, wn.contiguous(), w_offset))
+        dx = dwn = None
+        if dn is not None:
+            dx, dwn = _norm_backward(dn, h, wn, rstd, dh, w_offset, need_wn)
             dx = dx.view(shape)
-        need_x, need_r = ctx.needs_input_grad[:2]
-        return (dx if need_x else None), (dx if need_r and has_resid else None), dwn, dw, None, None, None, None
+        return (dx if need_x else None), (dx if need_r else None), dwn, dw, None, None, None, None
 
 
 def _norm_backward(dn, h, wn, rstd, dh, w_offset, need_dwn):
@@ -473,12 +552,14 @@ def _norm_backward(dn, h, wn, rstd, dh, w_offset, need_dwn):
     if R == 0:
         return dx, dwn.zero_() if dwn is not None else None
     part = torch.empty((min(R, lib.cvb_fp8_norm_bwd_parts()), D), dtype=torch.float32, device=h.device) if need_dwn else None
+    if main is not None and (main.dtype != torch.float32 or not main.is_contiguous()):
+        raise TypeError("add_rmsnorm_linear_fp8: main_grad is a contiguous float32 tensor")
     wc = wn.contiguous()
-    with _device(h):
+    with _On(h) as on:
         nv.check(lib.cvb_fp8_norm_bwd(dn.data_ptr(), dn.stride(0), h.data_ptr(), h.stride(0), wc.data_ptr(),
                                       rstd.data_ptr(), nv.ptr(dh2), dh2.stride(0) if dh2 is not None else 0,
                                       dx.data_ptr(), nv.ptr(part), nv.ptr(main), nv.ptr(dwn), R, D, w_offset,
-                                      nv.stream()), "cvb_fp8_norm_bwd")
+                                      on.stream), "cvb_fp8_norm_bwd")
     count_launch(2 if need_dwn else 1)
     return dx, dwn
 
@@ -495,5 +576,9 @@ def add_rmsnorm_linear_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], norm_
     _check_linear(x.shape[-1], x.device, w, weight, grad_dtype, what)
     if isinstance(w, Fp8Weight):
         w, weight = _Shape(w.shape), w
+    if not (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, resid, norm_w, w))):
+        q, h = add_rmsnorm_fp8(x, resid, norm_w, eps, w_offset)
+        y = _forward(None, q, w, weight, q.rows, w.shape[0], q.cols, False, False, x.dtype)[0]
+        return (y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])), h
     out = _NormLinearFp8.apply(x, resid, norm_w, w, weight, eps, w_offset, grad_dtype)
     return (out, x) if resid is None else out
