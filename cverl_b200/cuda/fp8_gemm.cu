@@ -280,64 +280,79 @@ struct F8PairCfg {
   static constexpr int SF_BYTES = 3 * 512;                  // A's rows of this CTA, B's two groups of 128 rows
   static constexpr int STAGES = 5;
   static constexpr int ACC1 = 192, SF_COL = 448;            // second accumulator, scales (two slots of 16 columns)
-  static constexpr int STG_ROW = 144, STG_WARP = 32 * STG_ROW;
-  static constexpr int SF_OFF = STAGES * TILE_BYTES;
+  static constexpr int EPI_WARPS = 8;                       // two to a lane quarter, each with every other 64 columns
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int STG_BUFS = 8 / EPI_WARPS;            // 4 KB store buffers of an epilogue warp
+  static constexpr int STG_OFF = STAGES * TILE_BYTES;
+  static constexpr int SF_OFF = STG_OFF + EPI_WARPS * STG_BUFS * 4096;
   static constexpr int BAR_OFF = SF_OFF + STAGES * SF_BYTES;
-  static constexpr int STG_OFF = BAR_OFF + 256;
-  static constexpr int SMEM_BYTES = STG_OFF + 4 * STG_WARP + 1024;
+  static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
 };
 
-// 32 rows x 64 columns of one epilogue warp, lane = row, through shared memory as 128-byte row segments
-__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const uint32_t (&r)[64], uint8_t* stg, int row0,
-                                               int col0, int lane) {
-  using Cfg = F8PairCfg;
-  if (p.out_kind == FP8_OUT_BF16) {
-    uint4* mine = reinterpret_cast<uint4*>(stg + lane * Cfg::STG_ROW);
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, const void* smem_src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* m, const void* smem_src, int x, int y) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+               : "memory");
+}
+// the stores committed by this thread before its last one have read their shared memory
+__device__ __forceinline__ void tma_store_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+
+// 32 rows x 64 columns of one epilogue warp, lane = row, out of registers.  Where C allows it, as boxes of 32 rows of
+// 128 bytes (128-byte swizzle, two buffers a warp) that TMA stores, or adds for accumulation (one addition an
+// element: the result does not depend on the order); TMA drops what lies outside C.  Else value by value.
+__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUtensorMap* tmC, const uint32_t (&r)[64],
+                                               uint8_t* stg, int* buf, int row0, int col0, int lane) {
+  if (p.vec) {
+    const int boxes = p.out_kind == FP8_OUT_BF16 ? 1 : 2;
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
-      mine[g] = make_uint4(pack_bf16x2(__uint_as_float(r[g * 8]), __uint_as_float(r[g * 8 + 1])),
-                           pack_bf16x2(__uint_as_float(r[g * 8 + 2]), __uint_as_float(r[g * 8 + 3])),
-                           pack_bf16x2(__uint_as_float(r[g * 8 + 4]), __uint_as_float(r[g * 8 + 5])),
-                           pack_bf16x2(__uint_as_float(r[g * 8 + 6]), __uint_as_float(r[g * 8 + 7])));
-    __syncwarp();
-    const int ch = lane & 7, n = p.N - (col0 + ch * 8);
-#pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int rr = it * 4 + (lane >> 3), row = row0 + rr;
-      if (row < p.M && n > 0) {
-        const uint4 o = *reinterpret_cast<const uint4*>(stg + rr * Cfg::STG_ROW + ch * 16);
-        uint16_t* dst = reinterpret_cast<uint16_t*>(p.C) + static_cast<long long>(row) * p.ldc + col0 + ch * 8;
-        if (p.vec && n >= 8) {
-          *reinterpret_cast<uint4*>(dst) = o;
-        } else {
-          const uint32_t w[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < n) dst[i] = static_cast<uint16_t>(w[i >> 1] >> ((i & 1) * 16));
-        }
+    for (int half = 0; half < 2; ++half) {
+      if (half == boxes) break;
+      if (lane == 0) {     // this buffer's last store has read it; with two, the other's may still be reading
+        if (F8PairCfg::STG_BUFS == 2) tma_store_wait_read1();
+        else tma_store_wait_read();
       }
+      __syncwarp();
+      uint8_t* row = stg + *buf * 4096 + lane * 128;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        uint4 o;
+        if (p.out_kind == FP8_OUT_BF16)
+          o = make_uint4(pack_bf16x2(__uint_as_float(r[g * 8]), __uint_as_float(r[g * 8 + 1])),
+                         pack_bf16x2(__uint_as_float(r[g * 8 + 2]), __uint_as_float(r[g * 8 + 3])),
+                         pack_bf16x2(__uint_as_float(r[g * 8 + 4]), __uint_as_float(r[g * 8 + 5])),
+                         pack_bf16x2(__uint_as_float(r[g * 8 + 6]), __uint_as_float(r[g * 8 + 7])));
+        else
+          o = make_uint4(r[half * 32 + g * 4], r[half * 32 + g * 4 + 1], r[half * 32 + g * 4 + 2], r[half * 32 + g * 4 + 3]);
+        *reinterpret_cast<uint4*>(row + ((g ^ (lane & 7)) << 4)) = o;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        const void* src = stg + *buf * 4096;
+        if (row0 < p.M && col0 + half * 32 < p.N) {
+          if (p.out_kind == FP8_OUT_F32_ACC) tma_add_2d(tmC, src, col0 + half * 32, row0);
+          else tma_store_2d(tmC, src, col0 + half * 32, row0);
+        }
+        tma_store_commit();
+      }
+      *buf ^= F8PairCfg::STG_BUFS - 1;
     }
-    __syncwarp();
     return;
   }
+  if (row0 + lane >= p.M) return;
+  const long long off = static_cast<long long>(row0 + lane) * p.ldc + col0;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float4* mine = reinterpret_cast<float4*>(stg + lane * Cfg::STG_ROW);
-#pragma unroll
-    for (int g = 0; g < 8; ++g)
-      mine[g] = make_float4(__uint_as_float(r[half * 32 + g * 4]), __uint_as_float(r[half * 32 + g * 4 + 1]),
-                            __uint_as_float(r[half * 32 + g * 4 + 2]), __uint_as_float(r[half * 32 + g * 4 + 3]));
-    __syncwarp();
-    const int ch = lane & 7, col = col0 + half * 32 + ch * 4, n = min(4, p.N - col);
-#pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int rr = it * 4 + (lane >> 3), row = row0 + rr;
-      if (row < p.M && n > 0)
-        fp8_store4(p, static_cast<long long>(row) * p.ldc + col,
-                   *reinterpret_cast<const float4*>(stg + rr * Cfg::STG_ROW + ch * 16), n);
-    }
-    __syncwarp();
-  }
+  for (int g = 0; g < 16; ++g)
+    fp8_store4(p, off + g * 4, make_float4(__uint_as_float(r[g * 4]), __uint_as_float(r[g * 4 + 1]),
+                                           __uint_as_float(r[g * 4 + 2]), __uint_as_float(r[g * 4 + 3])),
+               p.N - col0 - g * 4);
 }
 
 __device__ __forceinline__ void fp8_pair_tile(const Fp8GemmParams& p, int t, int* mb, int* nb) {
@@ -348,10 +363,10 @@ __device__ __forceinline__ void fp8_pair_tile(const Fp8GemmParams& p, int t, int
   *nb = r / size;
 }
 
-__global__ void __launch_bounds__(F8_THREADS, 1)
+__global__ void __launch_bounds__(F8PairCfg::THREADS, 1)
 fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                     const Fp8GemmParams p) {
+                     const __grid_constant__ CUtensorMap tmC, const Fp8GemmParams p) {
   using Cfg = F8PairCfg;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -371,13 +386,14 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       mbar_init(&empty_bar[s], 1);
     }
     mbar_init(tfull_bar, 1);
-    mbar_init(tfree_bar, 8);     // four epilogue warps in each CTA
+    mbar_init(tfree_bar, 2 * Cfg::EPI_WARPS);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmSA);
     tma_prefetch_desc(&tmSB);
+    if (p.vec) tma_prefetch_desc(&tmC);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -482,8 +498,10 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       }
     }
   } else {
-    const int q = warp & 3;
-    uint8_t* stg = smem + Cfg::STG_OFF + q * Cfg::STG_WARP;
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    constexpr int PARTS = Cfg::EPI_WARPS / 4;
+    uint8_t* stg = smem + Cfg::STG_OFF + (warp - 2) * Cfg::STG_BUFS * 4096;
+    int buf = 0;
     int local = 0;
     for (int t = pair; t < p.total; t += pairs, ++local) {
       int mb, nb;
@@ -501,21 +519,22 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + (local & 1 ? Cfg::ACC1 : 0);
       const int row0 = mb * 256 + rank * 128 + q * 32, n0 = nb * 256;
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
+      for (int i = part; i < 4; i += PARTS) {
         const int c = ((i + (local & 1 ? 0 : 3)) & 3) * 64;     // the shared columns first: 192-255, or 0-63
         uint32_t r[64];
         __syncwarp();
         tmem_ld_32x32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
         tmem_ld_32x32(taddr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
         tmem_ld_wait();
-        if (i == 0) {
+        if (i == part) {   // the shared columns are in registers, and the tile before has been read by this warp
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa_cluster(smem_u32(tfree_bar), 0));
         }
-        if (n0 + c < p.N) fp8_pair_store(p, r, stg, row0, n0 + c, lane);
+        if (n0 + c < p.N) fp8_pair_store(p, &tmC, r, stg, &buf, row0, n0 + c, lane);
       }
     }
+    if (lane == 0) tma_store_wait_read();
   }
   __syncwarp();
   tc_fence_before();
@@ -532,7 +551,7 @@ struct Fp8Operands {
   int M, N, K;
 };
 
-static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, unsigned grid, int cluster, size_t smem,
+static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, unsigned grid, int threads, int cluster, size_t smem,
                                          cudaStream_t stream) {
   at->id = cudaLaunchAttributeClusterDimension;
   at->val.clusterDim.x = cluster;
@@ -540,7 +559,7 @@ static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, unsigned grid,
   at->val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(F8_THREADS, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = at;
@@ -569,7 +588,7 @@ static int launch_small(const Fp8Operands& o, Fp8GemmParams p, cudaStream_t stre
   if (tiles * p.split > 0x7fffffffll) return -11;
   cudaLaunchAttribute at;
   const cudaLaunchConfig_t cfg =
-      cluster_config(&at, static_cast<unsigned>(tiles * p.split), p.split, Cfg::SMEM_BYTES, stream);
+      cluster_config(&at, static_cast<unsigned>(tiles * p.split), F8_THREADS, p.split, Cfg::SMEM_BYTES, stream);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, p));
 }
 
@@ -580,7 +599,7 @@ static int fp8_pair_capacity() {
         cudaSuccess)
       return 0;
     cudaLaunchAttribute at;
-    cudaLaunchConfig_t cfg = cluster_config(&at, 2 * 148, 2, F8PairCfg::SMEM_BYTES, nullptr);
+    cudaLaunchConfig_t cfg = cluster_config(&at, 2 * 148, F8PairCfg::THREADS, 2, F8PairCfg::SMEM_BYTES, nullptr);
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, fp8_gemm_pair_kernel, &cfg) != cudaSuccess) n = 0;
     return n;
@@ -589,7 +608,7 @@ static int fp8_pair_capacity() {
 }
 
 static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int pairs, cudaStream_t stream) {
-  CUtensorMap ta, tb, sa, sb;
+  CUtensorMap ta, tb, sa, sb, tc = {};
   const uint64_t ra = static_cast<uint64_t>((o.M + 127) / 128) * p.kgroups;
   const uint64_t rb = static_cast<uint64_t>((o.N + 127) / 128) * p.kgroups;
   if (encode_tensor_map(&ta, o.a, 1, o.K, o.M, 0, o.lda, 0, 128, 128) ||
@@ -597,6 +616,8 @@ static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int pairs, cudaStr
       encode_tensor_map(&sa, p.a_sf, TMAP_U32_PLAIN, 128, ra, 0, 512, 0, 128, 1) ||
       encode_tensor_map(&sb, p.b_sf, TMAP_U32_PLAIN, 128, rb, 0, 512, 0, 128, 1))
     return -10;
+  const int elem = p.out_kind == FP8_OUT_BF16 ? 2 : 4;
+  if (p.vec && encode_tensor_map(&tc, p.C, elem, p.N, p.M, 0, p.ldc * elem, 0, 128 / elem, 32)) return -10;
   const cudaError_t e =
       cudaFuncSetAttribute(fp8_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F8PairCfg::SMEM_BYTES);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -607,8 +628,8 @@ static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int pairs, cudaStr
   p.group_m = p.m_tiles < 16 ? p.m_tiles : 16;
   const int n = p.total < pairs ? p.total : pairs;
   cudaLaunchAttribute at;
-  const cudaLaunchConfig_t cfg = cluster_config(&at, 2u * n, 2, F8PairCfg::SMEM_BYTES, stream);
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel, ta, tb, sa, sb, p));
+  const cudaLaunchConfig_t cfg = cluster_config(&at, 2u * n, F8PairCfg::THREADS, 2, F8PairCfg::SMEM_BYTES, stream);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel, ta, tb, sa, sb, tc, p));
 }
 
 }  // namespace cvb
