@@ -20,9 +20,9 @@ struct Fp8GemmParams {
   long long ldc;
   int M, N, kblocks, kgroups;
   int a_fmt, b_fmt, out_kind;
-  int vec;                 // C and its row stride are 16-byte aligned
+  int vec;                 // bytes that C and its row stride are aligned to: 32, 16 or less
   int m_tiles, n_tiles;
-  int split, kb_per_split; // small kernel: CTAs of a cluster that share a tile's K, and K blocks of each
+  int split, kb_per_split; // CTAs (or CTA pairs) of a cluster that share a tile's K, and K blocks of each
   int group_m, total;      // pair kernel: M tiles walked per N tile, tiles in all
   int* status;
 };
@@ -35,6 +35,34 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                    smem_u32(smem_dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
+}
+
+// The warp that issues MMAs walks its loop with all lanes and one elected lane issues: loop state and descriptors are
+// then the same in every lane as far as the compiler can tell, and stay in uniform registers.  With the loop inside
+// `if (lane == 0)` the issue took 600 cycles for the four MMAs of a K block, whatever their width: more than the
+// tensor cores take for 256 columns.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ uint32_t warp_uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+  if (!ok) {
+    if (elect_one()) {
+      if (!*abort_flag) atomicCAS(status, 0, code);
+      *abort_flag = 1;
+    }
+    __syncwarp();
+  }
+  return ok;
 }
 
 // `n` (1 to 4) consecutive results of one row
@@ -66,6 +94,11 @@ __device__ __forceinline__ void fp8_store4(const Fp8GemmParams& p, long long off
     if (i < n) c[i] = acc ? c[i] + f[i] : f[i];
 }
 
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -89,12 +122,14 @@ struct F8SmallCfg {
   static constexpr int B_BYTES = 128 * 128;
   static constexpr int A_BYTES = TN * 128;
   static constexpr int SF_BYTES = 1024;                     // 512 for B, 512 for A
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SF_BYTES;
-  static constexpr int STAGES = 5;
+  static constexpr int TILE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = TN == 128 ? 3 : TN == 64 ? 4 : 5;   // two CTAs fit an SM
   static constexpr int SF_SLOTS = 3;                        // TMEM copies of the scales of four K blocks
+  // as in the pair kernel below; a CTA's first group may be shorter than four blocks, its later ones are not
+  static_assert(4 * (SF_SLOTS - 1) + 1 >= STAGES, "scale slot reused before its readers retired");
   static constexpr int TMEM_USED = TN + SF_SLOTS * 8;
   static constexpr int TMEM_COLS = TMEM_USED <= 64 ? 64 : TMEM_USED <= 128 ? 128 : 256;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+  static constexpr int SMEM_BYTES = STAGES * (TILE_BYTES + SF_BYTES) + 1024 + 256;
 };
 
 template <int TN>
@@ -104,14 +139,14 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   using Cfg = F8SmallCfg<TN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sf_smem = smem + Cfg::STAGES * (Cfg::A_BYTES + Cfg::B_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES);
+  uint8_t* sf_smem = smem + Cfg::STAGES * Cfg::TILE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sf_smem + Cfg::STAGES * Cfg::SF_BYTES);
   uint64_t* full_bar = bars;
   uint64_t* empty_bar = bars + Cfg::STAGES;
   uint64_t* done_bar = bars + 2 * Cfg::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = static_cast<int>(warp_uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::STAGES; ++s) {
@@ -131,91 +166,83 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int rank = static_cast<int>(cluster_ctarank());
+  const uint32_t tmem = warp_uniform(*tmem_slot);
+  const int rank = static_cast<int>(warp_uniform(cluster_ctarank()));
   const int tile = blockIdx.x / p.split;
   const int m0 = (tile % p.m_tiles) * TN;
   const int n0 = (tile / p.m_tiles) * 128;
   const int kb0 = rank * p.kb_per_split, kb1 = min(p.kblocks, kb0 + p.kb_per_split);   // never empty
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, armed = 0, armed_parity = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag)) {
-          if (!*abort_flag) atomicCAS(p.status, 0, ERR_WAIT_EMPTY);
-          *abort_flag = 1;
-          ok = false;
-          break;
-        }
-        uint8_t* sb = smem + stage * (Cfg::A_BYTES + Cfg::B_BYTES);
-        const bool scales = kb == kb0 || (kb & 3) == 0;
-        mbar_arrive_expect_tx(&full_bar[stage], Cfg::A_BYTES + Cfg::B_BYTES + (scales ? Cfg::SF_BYTES : 0));
+    const bool leader = elect_one();
+    const uint8_t* b_sf = p.b_sf + static_cast<long long>(n0 >> 7) * p.kgroups * 512;
+    const uint8_t* a_sf = p.a_sf + static_cast<long long>(m0 >> 7) * p.kgroups * 512;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, ERR_WAIT_EMPTY)) {
+        ok = false;
+        break;
+      }
+      uint8_t* sb = smem + stage * Cfg::TILE_BYTES;
+      uint8_t* sf = sf_smem + stage * Cfg::SF_BYTES;
+      const bool scales = kb == kb0 || (kb & 3) == 0;
+      const long long kg = static_cast<long long>(kb >> 2) * 512;
+      if (leader) {
+        mbar_arrive_expect_tx(&full_bar[stage], Cfg::TILE_BYTES + (scales ? Cfg::SF_BYTES : 0));
         tma_load_2d(sb, &tmB, &full_bar[stage], kb * 128, n0);
         tma_load_2d(sb + Cfg::B_BYTES, &tmA, &full_bar[stage], kb * 128, m0);
         if (scales) {
-          uint8_t* sf = sf_smem + stage * Cfg::SF_BYTES;
-          bulk_load(sf, p.b_sf + (static_cast<long long>(n0 >> 7) * p.kgroups + (kb >> 2)) * 512, 512, &full_bar[stage]);
-          bulk_load(sf + 512, p.a_sf + (static_cast<long long>(m0 >> 7) * p.kgroups + (kb >> 2)) * 512, 512,
-                    &full_bar[stage]);
-        }
-        armed |= 1u << stage;
-        armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == Cfg::STAGES) {
-          stage = 0;
-          phase ^= 1;
+          bulk_load(sf, b_sf + kg, 512, &full_bar[stage]);
+          bulk_load(sf + 512, a_sf + kg, 512, &full_bar[stage]);
         }
       }
-      if (!ok || *abort_flag) {
-        for (int s = 0; s < Cfg::STAGES; ++s) {
-          if (armed & (1u << s)) {
-            int dummy = 0;
-            mbar_wait_bounded(&full_bar[s], (armed_parity >> s) & 1, &dummy);
-          }
-        }
+      __syncwarp();
+      if (++stage == Cfg::STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (!ok || *abort_flag) {
+      // leave no copy in flight: give those that are a bounded time to land before the CTA ends
+      const long long t0 = clock64();
+      while (clock64() - t0 < (1ll << 21)) {
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_mxf8(128, TN, p.b_fmt, p.a_fmt);
-      int stage = 0;
-      uint32_t phase = 0;
-      int slot = -1;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag)) {
-          if (!*abort_flag) atomicCAS(p.status, 0, ERR_WAIT_FULL);
-          *abort_flag = 1;
-          ok = false;
-          break;
+    const uint32_t idesc = umma_idesc_mxf8(128, TN, p.b_fmt, p.a_fmt);
+    const bool leader = elect_one();
+    const uint64_t db0 = umma_smem_desc(smem_u32(smem), 16, 1024);
+    const uint64_t da0 = umma_smem_desc(smem_u32(smem) + Cfg::B_BYTES, 16, 1024);
+    const uint64_t ds0 = umma_scale_desc(smem_u32(sf_smem));
+    int stage = 0, slot = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(&full_bar[stage], phase, abort_flag, p.status, ERR_WAIT_FULL)) break;
+      tc_fence_after();
+      const bool scales = kb == kb0 || (kb & 3) == 0, last = kb + 1 == kb1;
+      if (scales) slot = slot + 1 == Cfg::SF_SLOTS ? 0 : slot + 1;
+      const uint64_t db = db0 + stage * (Cfg::TILE_BYTES >> 4), da = da0 + stage * (Cfg::TILE_BYTES >> 4);
+      const uint64_t ds = ds0 + stage * (Cfg::SF_BYTES >> 4);
+      const uint32_t id = umma_idesc_scale_id(idesc, kb & 3);
+      const uint32_t sfb = tmem + TN + slot * 8, sfa = sfb + 4;   // m0 is a multiple of 128: TN < 128 has one tile
+      if (leader) {
+        if (scales) {
+          tmem_cp_scales(sfb, ds);
+          tmem_cp_scales(sfb + 4, ds + 32);
         }
-        tc_fence_after();
-        const uint32_t sb = smem_u32(smem + stage * (Cfg::A_BYTES + Cfg::B_BYTES));
-        const uint32_t sa = sb + Cfg::B_BYTES;
-        if (kb == kb0 || (kb & 3) == 0) {
-          // A slot is written again SF_SLOTS groups later.  This stage was filled after the MMAs STAGES blocks back
-          // had retired, and the slot's last reader is at least 4 * (SF_SLOTS - 1) + 1 >= STAGES blocks back.
-          static_assert(4 * (Cfg::SF_SLOTS - 1) + 1 >= Cfg::STAGES, "scale slot reused before its readers retired");
-          slot = slot + 1 == Cfg::SF_SLOTS ? 0 : slot + 1;
-          const uint32_t sf = smem_u32(sf_smem + stage * Cfg::SF_BYTES);
-          tmem_cp_scales(tmem + TN + slot * 8, umma_scale_desc(sf));
-          tmem_cp_scales(tmem + TN + slot * 8 + 4, umma_scale_desc(sf + 512));
-        }
-        const uint32_t id = umma_idesc_scale_id(idesc, kb & 3);
-        const uint32_t sfb = tmem + TN + slot * 8, sfa = sfb + 4;   // m0 is a multiple of 128: TN < 128 has one tile
+        umma_mxf8(tmem, db, da, id, sfb, sfa, kb > kb0 ? 1u : 0u);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_mxf8(tmem, umma_smem_desc(sb + k * 32, 16, 1024), umma_smem_desc(sa + k * 32, 16, 1024), id, sfb, sfa,
-                    (kb > kb0 || k > 0) ? 1u : 0u);
+        for (int k = 1; k < 4; ++k) umma_mxf8(tmem, db + 2 * k, da + 2 * k, id, sfb, sfa, 1u);
         umma_commit(&empty_bar[stage]);
-        if (++stage == Cfg::STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
+        if (last) umma_commit(done_bar);
       }
-      if (ok) umma_commit(done_bar);
+      __syncwarp();
+      if (++stage == Cfg::STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
   } else {
     const int q = warp & 3;
@@ -264,95 +291,109 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Many rows: 256 x 256 tiles over a CTA pair (cta_group::2), persistent.
+// Many rows: 256 x BN tiles over a CTA pair (cta_group::2), persistent.
 //
-// Bound by the tensor cores; per K block of 128 an SM moves 32 KB through shared memory for 128 x 256 x 128 products,
-// the most an accumulator of 256 columns allows.  CTA r of a pair stages rows [128 r, + 128) of A and of B, holds the
-// scales of its own rows of A and of all 256 of B, and owns 128 rows of the accumulator.
+// Bound by the tensor cores; per K block of 128 an SM moves 16 KB + BN / 2 * 128 bytes through shared memory for
+// 128 x BN x 128 products.  CTA r of a pair stages rows [128 r, + 128) of A and [BN / 2 * r, + BN / 2) of B, holds
+// the scales of its own rows of A and of all BN of B, and owns 128 rows of the accumulator.
 //
-// Tensor memory: two accumulators of 256 columns and the scales do not fit 512 columns side by side, so the
-// accumulators overlap: columns 0-255 and 192-447, scales in 448-479.  The epilogue reads the shared 64 columns
-// first and then lets the next tile's MMAs start; the rest of its work runs under them.
+// Tensor memory: two accumulators, so that a tile's results leave under the next tile's MMAs, and the scales.  At
+// BN = 256 they do not fit 512 columns side by side: the accumulators overlap (columns 0-255 and 192-447), the
+// epilogue reads the shared 64 columns first and then lets the next tile begin.  That hand-over costs about 1.4 us a
+// tile; BN = 192 has none, but loads more for a product and pads other widths.
+// Four epilogue warps belong to each accumulator, so they have two tiles' time for one.
+//
+// SPLIT: few tiles and a long K (weight gradients).  `split` pairs of a cluster share a tile's K, one tile a cluster;
+// their partial tiles meet in shared memory as in the kernel above.
 // ---------------------------------------------------------------------------------------------------
+template <int BN>
 struct F8PairCfg {
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = 128 * 128;
+  static constexpr bool OVERLAP = BN == 256;
+  static constexpr int HALF = BN / 2;                       // rows of B that each CTA stages
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = HALF * 128;
   static constexpr int TILE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int SF_BYTES = 3 * 512;                  // A's rows of this CTA, B's two groups of 128 rows
-  static constexpr int STAGES = 5;
-  static constexpr int ACC1 = 192, SF_COL = 448;            // second accumulator, scales (two slots of 16 columns)
-  static constexpr int EPI_WARPS = 8;                       // two to a lane quarter, each with every other 64 columns
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STG_BUFS = 8 / EPI_WARPS;            // 4 KB store buffers of an epilogue warp
-  static constexpr int STG_OFF = STAGES * TILE_BYTES;
-  static constexpr int SF_OFF = STG_OFF + EPI_WARPS * STG_BUFS * 4096;
+  static constexpr int SF_GROUPS = BN == 128 ? 1 : 2;       // groups of 128 rows of B whose scales a tile reads
+  static constexpr int SF_BYTES = (1 + SF_GROUPS) * 512;    // and those of A's rows of this CTA
+  static constexpr int STAGES = OVERLAP ? 6 : BN == 192 ? 7 : 8;
+  static constexpr int SF_SLOTS = 3;                        // TMEM copies of the scales of four K blocks
+  static constexpr int ACC1 = OVERLAP ? 192 : BN;
+  static constexpr int SF_COL = ACC1 + BN;                  // 16 columns a slot
+  static constexpr int THREADS = 64 + 32 * 8;
+  static constexpr int SF_OFF = STAGES * TILE_BYTES;
   static constexpr int BAR_OFF = SF_OFF + STAGES * SF_BYTES;
   static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
+  static_assert(SF_COL + 16 * SF_SLOTS <= 512, "tensor memory");
+  // A slot is written again SF_SLOTS groups of four K blocks later.  The stage that brings the new scales was filled
+  // after the MMAs STAGES blocks back had retired; the slot's last reader is at least 4 (SF_SLOTS - 1) + 1 back.
+  static_assert(4 * (SF_SLOTS - 1) + 1 >= STAGES, "scale slot reused before its readers retired");
 };
 
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, const void* smem_src, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(m)),
-               "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+// Arrival that orders nothing but tensor memory (its reads are complete, tcgen05.fence::before_thread_sync precedes):
+// a releasing one would first wait for the result stores of the chunk before.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void st_global_32b(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e,
+                                              uint32_t f, uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d),
+               "r"(e), "r"(f), "r"(g), "r"(h)
                : "memory");
 }
-__device__ __forceinline__ void tma_add_2d(const CUtensorMap* m, const void* smem_src, int x, int y) {
-  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(m)),
-               "r"(smem_u32(smem_src)), "r"(x), "r"(y)
-               : "memory");
-}
-// the stores committed by this thread before its last one have read their shared memory
-__device__ __forceinline__ void tma_store_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 
-// 32 rows x 64 columns of one epilogue warp, lane = row, out of registers.  Where C allows it, as boxes of 32 rows of
-// 128 bytes (128-byte swizzle, two buffers a warp) that TMA stores, or adds for accumulation (one addition an
-// element: the result does not depend on the order); TMA drops what lies outside C.  Else value by value.
-__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUtensorMap* tmC, const uint32_t (&r)[64],
-                                               uint8_t* stg, int* buf, int row0, int col0, int lane) {
-  if (p.vec) {
-    const int boxes = p.out_kind == FP8_OUT_BF16 ? 1 : 2;
+// 32 rows x 64 columns of one epilogue warp, lane = row, straight from registers: a lane's 64 results are 128 (or
+// 256) bytes of its row, stored as whole 32-byte sectors.  An accumulating product adds by reduction, one addition an
+// element: the result does not depend on the order.  Value by value where C is not aligned or the columns end.
+__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const uint32_t (&r)[64], int row, int col) {
+  if (row >= p.M) return;
+  const long long off = static_cast<long long>(row) * p.ldc + col;
+  const int n = p.N - col;
+  if (p.out_kind == FP8_OUT_BF16) {
+    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.C) + off;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (half == boxes) break;
-      if (lane == 0) {     // this buffer's last store has read it; with two, the other's may still be reading
-        if (F8PairCfg::STG_BUFS == 2) tma_store_wait_read1();
-        else tma_store_wait_read();
-      }
-      __syncwarp();
-      uint8_t* row = stg + *buf * 4096 + lane * 128;
+    for (int g = 0; g < 4; ++g) {
+      uint32_t w[8];
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        uint4 o;
-        if (p.out_kind == FP8_OUT_BF16)
-          o = make_uint4(pack_bf16x2(__uint_as_float(r[g * 8]), __uint_as_float(r[g * 8 + 1])),
-                         pack_bf16x2(__uint_as_float(r[g * 8 + 2]), __uint_as_float(r[g * 8 + 3])),
-                         pack_bf16x2(__uint_as_float(r[g * 8 + 4]), __uint_as_float(r[g * 8 + 5])),
-                         pack_bf16x2(__uint_as_float(r[g * 8 + 6]), __uint_as_float(r[g * 8 + 7])));
-        else
-          o = make_uint4(r[half * 32 + g * 4], r[half * 32 + g * 4 + 1], r[half * 32 + g * 4 + 2], r[half * 32 + g * 4 + 3]);
-        *reinterpret_cast<uint4*>(row + ((g ^ (lane & 7)) << 4)) = o;
+      for (int i = 0; i < 8; ++i)
+        w[i] = pack_bf16x2(__uint_as_float(r[g * 16 + 2 * i]), __uint_as_float(r[g * 16 + 2 * i + 1]));
+      if (p.vec == 32 && g * 16 + 16 <= n) {
+        st_global_32b(dst + g * 16, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+      } else if (p.vec >= 16 && g * 16 + 16 <= n) {
+        *reinterpret_cast<uint4*>(dst + g * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(dst + g * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (g * 16 + i < n)
+            reinterpret_cast<uint16_t*>(dst)[g * 16 + i] = static_cast<uint16_t>(w[i >> 1] >> ((i & 1) * 16));
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        const void* src = stg + *buf * 4096;
-        if (row0 < p.M && col0 + half * 32 < p.N) {
-          if (p.out_kind == FP8_OUT_F32_ACC) tma_add_2d(tmC, src, col0 + half * 32, row0);
-          else tma_store_2d(tmC, src, col0 + half * 32, row0);
-        }
-        tma_store_commit();
-      }
-      *buf ^= F8PairCfg::STG_BUFS - 1;
     }
     return;
   }
-  if (row0 + lane >= p.M) return;
-  const long long off = static_cast<long long>(row0 + lane) * p.ldc + col0;
+  float* dst = reinterpret_cast<float*>(p.C) + off;
+  const bool acc = p.out_kind == FP8_OUT_F32_ACC;
 #pragma unroll
-  for (int g = 0; g < 16; ++g)
-    fp8_store4(p, off + g * 4, make_float4(__uint_as_float(r[g * 4]), __uint_as_float(r[g * 4 + 1]),
-                                           __uint_as_float(r[g * 4 + 2]), __uint_as_float(r[g * 4 + 3])),
-               p.N - col0 - g * 4);
+  for (int g = 0; g < 8; ++g) {
+    const uint32_t* w = r + g * 8;
+    if (p.vec >= 16 && g * 8 + 8 <= n) {
+      if (acc) {
+        red_add_v4_f32(dst + g * 8, __uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+        red_add_v4_f32(dst + g * 8 + 4, __uint_as_float(w[4]), __uint_as_float(w[5]), __uint_as_float(w[6]),
+                       __uint_as_float(w[7]));
+      } else if (p.vec == 32) {
+        st_global_32b(dst + g * 8, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+      } else {
+        *reinterpret_cast<uint4*>(dst + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(dst + g * 8 + 4) = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (g * 8 + i < n) {
+          if (acc) atomicAdd(dst + g * 8 + i, __uint_as_float(w[i]));
+          else dst[g * 8 + i] = __uint_as_float(w[i]);
+        }
+    }
+  }
 }
 
 __device__ __forceinline__ void fp8_pair_tile(const Fp8GemmParams& p, int t, int* mb, int* nb) {
@@ -363,37 +404,46 @@ __device__ __forceinline__ void fp8_pair_tile(const Fp8GemmParams& p, int t, int
   *nb = r / size;
 }
 
-__global__ void __launch_bounds__(F8PairCfg::THREADS, 1)
+template <int BN, bool SPLIT>
+__global__ void __launch_bounds__(F8PairCfg<BN>::THREADS, 1)
 fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                     const __grid_constant__ CUtensorMap tmC, const Fp8GemmParams p) {
-  using Cfg = F8PairCfg;
+                     const Fp8GemmParams p) {
+  using Cfg = F8PairCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFF);   // even CTA's: bytes of both CTAs
   uint64_t* empty_bar = full_bar + Cfg::STAGES;                            // each CTA's, committed to both
-  uint64_t* tfull_bar = empty_bar + Cfg::STAGES;                           // each CTA's: a tile is complete
-  uint64_t* tfree_bar = tfull_bar + 1;                                     // even CTA's: the shared columns are read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree_bar + 1);
+  uint64_t* tfull_bar = empty_bar + Cfg::STAGES;                           // [2] each CTA's: an accumulator is complete
+  uint64_t* tdone_bar = tfull_bar + 2;                                     // [2] even CTA's: it has been read
+  uint64_t* tfree_bar = tdone_bar + 2;                                     // [2] even CTA's: its shared columns have
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank());
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int warp = static_cast<int>(warp_uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  const int crank = static_cast<int>(warp_uniform(cluster_ctarank()));
+  const int rank = crank & 1, even = crank & ~1;                // within the pair; the pair's CTA that issues
+  // first tile and stride of this pair's walk; SPLIT: the cluster's only tile, this pair's range of its K
+  const int pair = SPLIT ? blockIdx.x / (2 * p.split) : blockIdx.x >> 1, pairs = SPLIT ? p.total : gridDim.x >> 1;
+  const int kb0 = SPLIT ? (crank >> 1) * p.kb_per_split : 0;
+  const int kb1 = SPLIT ? min(p.kblocks, kb0 + p.kb_per_split) : p.kblocks;
+  const uint16_t both = static_cast<uint16_t>(3 << even);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    mbar_init(tfull_bar, 1);
-    mbar_init(tfree_bar, 2 * Cfg::EPI_WARPS);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tdone_bar[a], 8);     // an accumulator's four epilogue warps in each CTA
+      mbar_init(&tfree_bar[a], 8);
+    }
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmSA);
     tma_prefetch_desc(&tmSB);
-    if (p.vec) tma_prefetch_desc(&tmC);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -403,110 +453,136 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   tc_fence_before();
   cluster_sync_all();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = warp_uniform(*tmem_slot);
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = pair; ok && t < p.total; t += pairs) {
-        int mb, nb;
-        fp8_pair_tile(p, t, &mb, &nb);
-        const int ra = mb * 2 + rank, rb = nb * 2;              // groups of 128 rows
-        for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag)) {
-            if (!*abort_flag) atomicCAS(p.status, 0, ERR_WAIT_EMPTY);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          uint8_t* sa = smem + stage * Cfg::TILE_BYTES;
-          uint8_t* sf = smem + Cfg::SF_OFF + stage * Cfg::SF_BYTES;
-          const bool scales = (kb & 3) == 0;
+    const bool leader = elect_one();
+    const uint32_t full0 = mapa_cluster(smem_u32(full_bar), even);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = pair; ok && t < p.total; t += pairs) {
+      int mb, nb;
+      fp8_pair_tile(p, t, &mb, &nb);
+      const int ra = mb * 2 + rank, rb = nb * BN / 128;         // groups of 128 rows
+      const int row_a = ra * 128, row_b = nb * BN + rank * Cfg::HALF;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!warp_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, ERR_WAIT_EMPTY)) {
+          ok = false;
+          break;
+        }
+        const bool scales = kb == kb0 || (kb & 3) == 0;
+        uint8_t* sa = smem + stage * Cfg::TILE_BYTES;
+        uint8_t* sf = smem + Cfg::SF_OFF + stage * Cfg::SF_BYTES;
+        const uint32_t fb = full0 + stage * 8;
+        const int kg = kb >> 2;
+        if (leader) {
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (Cfg::TILE_BYTES + (scales ? Cfg::SF_BYTES : 0)));
-          const uint32_t fb = mapa_cluster(smem_u32(&full_bar[stage]), 0);
-          tma_load_2d_pair(sa, &tmA, fb, kb * 128, ra * 128);
-          tma_load_2d_pair(sa + Cfg::A_BYTES, &tmB, fb, kb * 128, (rb + rank) * 128);
+          tma_load_2d_pair(sa, &tmA, fb, kb * 128, row_a);
+          tma_load_2d_pair(sa + Cfg::A_BYTES, &tmB, fb, kb * 128, row_b);
           if (scales) {   // rows of scale cells past the last read as zero: they belong to rows that are not stored
-            tma_load_2d_pair(sf, &tmSA, fb, 0, ra * p.kgroups + (kb >> 2));
-            tma_load_2d_pair(sf + 512, &tmSB, fb, 0, rb * p.kgroups + (kb >> 2));
-            tma_load_2d_pair(sf + 1024, &tmSB, fb, 0, (rb + 1) * p.kgroups + (kb >> 2));
-          }
-          if (++stage == Cfg::STAGES) {
-            stage = 0;
-            phase ^= 1;
+            tma_load_2d_pair(sf, &tmSA, fb, 0, ra * p.kgroups + kg);
+            tma_load_2d_pair(sf + 512, &tmSB, fb, 0, rb * p.kgroups + kg);
+            if (Cfg::SF_GROUPS == 2) tma_load_2d_pair(sf + 1024, &tmSB, fb, 0, (rb + 1) * p.kgroups + kg);
           }
         }
-      }
-      if (!ok || *abort_flag) {
-        // This CTA's copies report to the even CTA's barriers, so it cannot wait on them itself: give those in
-        // flight a bounded time to land before the CTA ends.
-        const long long t0 = clock64();
-        while (clock64() - t0 < (1ll << 21)) {
+        __syncwarp();
+        if (++stage == Cfg::STAGES) {
+          stage = 0;
+          phase ^= 1;
         }
       }
     }
+    if (!ok || *abort_flag) {
+      // This CTA's copies report to the even CTA's barriers, so it cannot wait on them itself: give those in flight a
+      // bounded time to land before the CTA ends.
+      const long long t0 = clock64();
+      while (clock64() - t0 < (1ll << 21)) {
+      }
+    }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = umma_idesc_mxf8(256, 256, p.a_fmt, p.b_fmt);
+    if (rank == 0) {
+      const uint32_t idesc = umma_idesc_mxf8(256, BN, p.a_fmt, p.b_fmt);
+      const bool leader = elect_one();
+      // descriptors of stage 0: a stage adds TILE_BYTES / 16 to the address field, 32 elements of K two
+      const uint64_t da0 = umma_smem_desc(smem_u32(smem), 16, 1024);
+      const uint64_t db0 = umma_smem_desc(smem_u32(smem) + Cfg::A_BYTES, 16, 1024);
+      const uint64_t ds0 = umma_scale_desc(smem_u32(smem) + Cfg::SF_OFF);
       int stage = 0, local = 0, slot = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; ok && t < p.total; t += pairs, ++local) {
-        // the tile before has been read where the accumulators overlap; the one before that was read entirely then
-        if (local > 0 && !mbar_wait_bounded(tfree_bar, (local - 1) & 1, abort_flag)) {
-          if (!*abort_flag) atomicCAS(p.status, 0, ERR_WAIT_TMEM_EMPTY);
-          *abort_flag = 1;
+        const int a = local & 1, use = local >> 1;
+        // this accumulator's last tile has been read, and the other's where the two overlap
+        if (use > 0 && !warp_wait(&tdone_bar[a], (use - 1) & 1, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY)) break;
+        if (Cfg::OVERLAP && local > 0 &&
+            !warp_wait(&tfree_bar[a ^ 1], ((local - 1) >> 1) & 1, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY))
           break;
-        }
         tc_fence_after();
-        const uint32_t acc = tmem + (local & 1 ? Cfg::ACC1 : 0);
-        for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag)) {
-            if (!*abort_flag) atomicCAS(p.status, 0, ERR_WAIT_FULL);
-            *abort_flag = 1;
+        const uint32_t acc = tmem + (a ? Cfg::ACC1 : 0);
+        uint32_t sfb_col = 0;                                   // the tile's first row in its group's scale cells
+        if (BN % 128 != 0) {
+          int mb, nb;
+          fp8_pair_tile(p, t, &mb, &nb);
+          sfb_col = ((nb * BN) & 127) >> 5;
+        }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!warp_wait(&full_bar[stage], phase, abort_flag, p.status, ERR_WAIT_FULL)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * Cfg::TILE_BYTES), sb = sa + Cfg::A_BYTES;
-          if ((kb & 3) == 0) {
-            // The slot's last readers are at least five K blocks back in this tile, or in a tile whose MMAs have
-            // retired; this stage was filled after the MMAs five blocks back had.
-            static_assert(Cfg::STAGES <= 5, "scale slot reused before its readers retired");
-            slot ^= 1;
-            const uint32_t sf = smem_u32(smem + Cfg::SF_OFF + stage * Cfg::SF_BYTES);
-            const uint32_t col = tmem + Cfg::SF_COL + slot * 16;
-            tmem_cp_scales_pair(col, umma_scale_desc(sf));
-            tmem_cp_scales_pair(col + 4, umma_scale_desc(sf + 512));
-            tmem_cp_scales_pair(col + 8, umma_scale_desc(sf + 1024));
-          }
+          const bool scales = kb == kb0 || (kb & 3) == 0;
+          if (scales) slot = slot + 1 == Cfg::SF_SLOTS ? 0 : slot + 1;
+          const uint32_t sfa = tmem + Cfg::SF_COL + slot * 16, sfb = sfa + 4 + sfb_col;
+          const uint64_t ds = ds0 + stage * (Cfg::SF_BYTES >> 4);
+          const uint64_t da = da0 + stage * (Cfg::TILE_BYTES >> 4), db = db0 + stage * (Cfg::TILE_BYTES >> 4);
           const uint32_t id = umma_idesc_scale_id(idesc, kb & 3);
-          const uint32_t sfa = tmem + Cfg::SF_COL + slot * 16;
+          const bool last = kb + 1 == kb1;
+          if (leader) {
+            if (scales) {
+              tmem_cp_scales_pair(sfa, ds);
+              tmem_cp_scales_pair(sfa + 4, ds + 32);
+              if (Cfg::SF_GROUPS == 2) tmem_cp_scales_pair(sfa + 8, ds + 64);
+            }
+            umma_mxf8_pair(acc, da, db, id, sfa, sfb, kb > kb0 ? 1u : 0u);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_mxf8_pair(acc, umma_smem_desc(sa + k * 32, 16, 1024), umma_smem_desc(sb + k * 32, 16, 1024), id, sfa,
-                           sfa + 4, (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit_pair(&empty_bar[stage], 3);
+            for (int k = 1; k < 4; ++k) umma_mxf8_pair(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, 1u);
+            umma_commit_pair(&empty_bar[stage], both);
+            if (last) umma_commit_pair(&tfull_bar[a], both);
+          }
+          __syncwarp();
           if (++stage == Cfg::STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (ok) umma_commit_pair(tfull_bar, 3);
       }
     }
   } else {
-    const int q = warp & 3, part = (warp - 2) >> 2;
-    constexpr int PARTS = Cfg::EPI_WARPS / 4;
-    uint8_t* stg = smem + Cfg::STG_OFF + (warp - 2) * Cfg::STG_BUFS * 4096;
-    int buf = 0;
-    int local = 0;
-    for (int t = pair; t < p.total; t += pairs, ++local) {
+    const int q = warp & 3, a = (warp - 2) >> 2;             // lane quarter, accumulator
+    const uint32_t tfree = mapa_cluster(smem_u32(&tfree_bar[a]), even), tdone = mapa_cluster(smem_u32(&tdone_bar[a]), even);
+    uint32_t use = 0;
+    if (SPLIT) {
+      const bool ok = warp_wait(&tfull_bar[0], 0, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+      tc_fence_after();
+      // this pair's partial tile as [column][128 rows of this CTA]: the stages are free, every copy has been read.
+      // The two sets of warps take half of the columns each.
+      float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
+#pragma unroll 1
+      for (int c = a * Cfg::HALF; ok && c < (a + 1) * Cfg::HALF; c += 32) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_32x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) part[(c + i) * 128] = __uint_as_float(r[i]);
+      }
+    }
+    for (int t = pair + a * pairs; !SPLIT && t < p.total; t += 2 * pairs, ++use) {
       int mb, nb;
       fp8_pair_tile(p, t, &mb, &nb);
-      bool ok = mbar_wait_bounded(tfull_bar, local & 1, abort_flag);
+      bool ok = mbar_wait_bounded(&tfull_bar[a], use & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         if (lane == 0) {
@@ -516,25 +592,25 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         break;
       }
       tc_fence_after();
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + (local & 1 ? Cfg::ACC1 : 0);
-      const int row0 = mb * 256 + rank * 128 + q * 32, n0 = nb * 256;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + (a ? Cfg::ACC1 : 0);
+      const int row0 = mb * 256 + rank * 128 + q * 32, n0 = nb * BN;
 #pragma unroll 1
-      for (int i = part; i < 4; i += PARTS) {
-        const int c = ((i + (local & 1 ? 0 : 3)) & 3) * 64;     // the shared columns first: 192-255, or 0-63
+      for (int i = 0; i < BN / 64; ++i) {
+        // the shared columns first: 192-255 of the first accumulator, 0-63 of the second
+        const int c = (Cfg::OVERLAP && a == 0 ? (i + 3) & 3 : i) * 64;
         uint32_t r[64];
         __syncwarp();
         tmem_ld_32x32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
         tmem_ld_32x32(taddr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
         tmem_ld_wait();
-        if (i == part) {   // the shared columns are in registers, and the tile before has been read by this warp
+        if ((Cfg::OVERLAP && i == 0) || i == BN / 64 - 1) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(mapa_cluster(smem_u32(tfree_bar), 0));
+          if (lane == 0) mbar_arrive_cluster_relaxed(i == 0 ? tfree : tdone);
         }
-        if (n0 + c < p.N) fp8_pair_store(p, &tmC, r, stg, &buf, row0, n0 + c, lane);
+        if (n0 + c < p.N) fp8_pair_store(p, r, row0 + lane, n0 + c);
       }
     }
-    if (lane == 0) tma_store_wait_read();
   }
   __syncwarp();
   tc_fence_before();
@@ -542,6 +618,27 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
+  }
+  if (SPLIT) {
+    // 64 columns at a time: chunk i belongs to pair i % split, there to the set of warps i / split
+    if (warp >= 2) {
+      const int q = warp & 3, a = (warp - 2) >> 2;
+      int mb, nb;
+      fp8_pair_tile(p, pair, &mb, &nb);
+      for (int i = (crank >> 1) + a * p.split; i < BN / 64; i += 2 * p.split) {
+        uint32_t r[64];
+#pragma unroll
+        for (int c = 0; c < 64; ++c) r[c] = 0u;
+        for (int z = 0; z < p.split; ++z) {       // in the order of the ranks
+          const uint32_t src = mapa_cluster(smem_u32(smem) + (i * 64 * 128 + q * 32 + lane) * 4, 2 * z + rank);
+#pragma unroll
+          for (int c = 0; c < 64; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + ld_cluster(src + c * 512));
+        }
+        if (nb * BN + i * 64 < p.N) fp8_pair_store(p, r, mb * 256 + rank * 128 + q * 32 + lane, nb * BN + i * 64);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();   // nobody leaves while a peer reads its tile
   }
 }
 
@@ -570,7 +667,7 @@ static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, unsigned grid,
 template <int TN>
 static int launch_small(const Fp8Operands& o, Fp8GemmParams p, cudaStream_t stream) {
   using Cfg = F8SmallCfg<TN>;
-  static_assert(TN * 512 <= Cfg::STAGES * (Cfg::A_BYTES + Cfg::B_BYTES), "the partial tile fits the stages");
+  static_assert(TN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
   CUtensorMap ta, tb;
   if (encode_tensor_map(&ta, o.a, 1, o.K, o.M, 0, o.lda, 0, 128, TN) ||
       encode_tensor_map(&tb, o.b, 1, o.K, o.N, 0, o.ldb, 0, 128, 128))
@@ -581,8 +678,16 @@ static int launch_small(const Fp8Operands& o, Fp8GemmParams p, cudaStream_t stre
   p.m_tiles = (p.M + TN - 1) / TN;
   p.n_tiles = (p.N + 127) / 128;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  // Fill the SMs: one CTA each (two where each still has 8 K blocks), clusters of eight only where few of them have to
+  // find room.  One token, N = 1024, K = 3584: 10.2 us with one CTA a tile, 4.5 with eight; 128 rows, N = K = 2048:
+  // 12.2 with one, 7.4 with four, 8.8 with eight; 128 rows, N = K = 8192: 27.0 with one, 17.6 with two, 14.6 with four.
   p.split = 1;
-  while (p.split < 8 && tiles * p.split * 2 <= 148 && p.split * 2 <= p.kblocks) p.split *= 2;
+  while (p.split < 8) {
+    const int next = p.split * 2, per = p.kblocks / next;
+    const long long room = next == 8 ? 74 : per >= 8 ? 296 : 148;
+    if (per < 1 || tiles * next > room) break;
+    p.split = next;
+  }
   p.kb_per_split = (p.kblocks + p.split - 1) / p.split;
   p.split = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
   if (tiles * p.split > 0x7fffffffll) return -11;
@@ -593,43 +698,72 @@ static int launch_small(const Fp8Operands& o, Fp8GemmParams p, cudaStream_t stre
 }
 
 // CTA pairs that can be resident at once
+template <int BN>
 static int fp8_pair_capacity() {
   static const int cached = [] {
-    if (cudaFuncSetAttribute(fp8_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F8PairCfg::SMEM_BYTES) !=
-        cudaSuccess)
-      return 0;
+    using Cfg = F8PairCfg<BN>;
+    auto kern = fp8_gemm_pair_kernel<BN, false>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess) return 0;
     cudaLaunchAttribute at;
-    cudaLaunchConfig_t cfg = cluster_config(&at, 2 * 148, F8PairCfg::THREADS, 2, F8PairCfg::SMEM_BYTES, nullptr);
+    cudaLaunchConfig_t cfg = cluster_config(&at, 2 * 148, Cfg::THREADS, 2, Cfg::SMEM_BYTES, nullptr);
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, fp8_gemm_pair_kernel, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
     return n;
   }();
   return cached;
 }
 
-static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int pairs, cudaStream_t stream) {
-  CUtensorMap ta, tb, sa, sb, tc = {};
+template <int BN, bool SPLIT>
+static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int split, cudaStream_t stream) {
+  using Cfg = F8PairCfg<BN>;
+  static_assert(BN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
+  const int pairs = fp8_pair_capacity<BN>();
+  if (pairs <= 0) return -12;
+  CUtensorMap ta, tb, sa, sb;
   const uint64_t ra = static_cast<uint64_t>((o.M + 127) / 128) * p.kgroups;
   const uint64_t rb = static_cast<uint64_t>((o.N + 127) / 128) * p.kgroups;
   if (encode_tensor_map(&ta, o.a, 1, o.K, o.M, 0, o.lda, 0, 128, 128) ||
-      encode_tensor_map(&tb, o.b, 1, o.K, o.N, 0, o.ldb, 0, 128, 128) ||
+      encode_tensor_map(&tb, o.b, 1, o.K, o.N, 0, o.ldb, 0, 128, Cfg::HALF) ||
       encode_tensor_map(&sa, p.a_sf, TMAP_U32_PLAIN, 128, ra, 0, 512, 0, 128, 1) ||
       encode_tensor_map(&sb, p.b_sf, TMAP_U32_PLAIN, 128, rb, 0, 512, 0, 128, 1))
     return -10;
-  const int elem = p.out_kind == FP8_OUT_BF16 ? 2 : 4;
-  if (p.vec && encode_tensor_map(&tc, p.C, elem, p.N, p.M, 0, p.ldc * elem, 0, 128 / elem, 32)) return -10;
-  const cudaError_t e =
-      cudaFuncSetAttribute(fp8_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F8PairCfg::SMEM_BYTES);
+  auto kern = fp8_gemm_pair_kernel<BN, SPLIT>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
   if (e != cudaSuccess) return static_cast<int>(e);
   p.m_tiles = (p.M + 255) / 256;
-  p.n_tiles = (p.N + 255) / 256;
-  if (static_cast<long long>(p.m_tiles) * p.n_tiles > 0x3fffffffll) return -11;
+  p.n_tiles = (p.N + BN - 1) / BN;
+  if (static_cast<long long>(p.m_tiles) * p.n_tiles > 0x0fffffffll) return -11;
   p.total = p.m_tiles * p.n_tiles;
   p.group_m = p.m_tiles < 16 ? p.m_tiles : 16;
-  const int n = p.total < pairs ? p.total : pairs;
+  p.split = split;
+  p.kb_per_split = (p.kblocks + split - 1) / split;
+  p.split = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
+  const int n = SPLIT ? p.total * p.split : p.total < pairs ? p.total : pairs;
   cudaLaunchAttribute at;
-  const cudaLaunchConfig_t cfg = cluster_config(&at, 2u * n, F8PairCfg::THREADS, 2, F8PairCfg::SMEM_BYTES, stream);
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel, ta, tb, sa, sb, tc, p));
+  const cudaLaunchConfig_t cfg = cluster_config(&at, 2u * n, Cfg::THREADS, 2 * p.split, Cfg::SMEM_BYTES, stream);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, sa, sb, p));
+}
+
+// Tile width and split for the pair kernel: the least of waves * (K blocks * c + o), in cycles.  c is what a K block
+// takes once the pipeline runs and o what a tile adds, both from timing the variants over K = 1024 ... 20480 at one and
+// at many waves; a split halves K and adds the meeting of the partial tiles.  Two pairs sharing K pay only while all
+// clusters are resident: [1024, 20480] x [2048, 20480]^T takes 53 us in 32 tiles of 256 columns, 36 with two pairs each.
+struct PairChoice {
+  int bn, split;
+};
+static PairChoice choose_pair(int M, int N, int kblocks) {
+  static const struct { int bn, split, c, o; } ways[] = {
+      {256, 1, 530, 1250}, {192, 1, 418, 750}, {128, 1, 408, 650}, {256, 2, 530, 5250}, {128, 2, 408, 3150}};
+  PairChoice best = {256, 1};
+  long long least = -1;
+  for (const auto& w : ways) {
+    const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + w.bn - 1) / w.bn);
+    if (w.split > 1 && (tiles * w.split > 74 || kblocks < 2 * w.split)) continue;
+    const long long waves = (tiles * w.split + 73) / 74;
+    const long long cost = waves * (static_cast<long long>((kblocks + w.split - 1) / w.split) * w.c + w.o);
+    if (least < 0 || cost < least) least = cost, best = {w.bn, w.split};
+  }
+  return best;
 }
 
 }  // namespace cvb
@@ -653,13 +787,20 @@ extern "C" int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int 
   p.kblocks = (K + 127) / 128, p.kgroups = (p.kblocks + 3) / 4;
   p.a_fmt = a_fmt, p.b_fmt = b_fmt, p.out_kind = out_kind, p.status = status;
   const int elem = out_kind == FP8_OUT_BF16 ? 2 : 4;
-  p.vec = (reinterpret_cast<uintptr_t>(c) & 15) == 0 && (ldc * elem) % 16 == 0;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(ldc * elem);
+  p.vec = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
   const Fp8Operands o = {a, b, lda, ldb, M, N, K};
-  // Pairs where their tiles fill at least half of the SMs: 8 tiles (512 x 1024, K 1024) take 12.3 us against 10.2 us
-  // with the other kernel, 64 (2048 x 2048, K 2048) 16.4 against 30.7.
-  const long long pair_tiles = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
-  const int pairs = M > 128 && N > 128 && pair_tiles >= 37 ? fp8_pair_capacity() : 0;
-  if (pairs > 0) return launch_pair(o, p, pairs, stream);
+  const PairChoice pick = choose_pair(p.M, p.N, p.kblocks);
+  // Above 128 rows always pairs; from 65 where tiles of 128 columns fill half of the SMs and K is short (128 rows,
+  // N = 7168, K = 1024: 6.4 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 7.9; N = K = 8192:
+  // 19.2 against 14.6).
+  if (M > 128 || (M > 64 && N >= 37 * 128 && p.kblocks <= 12)) {
+    if (pick.split == 2)
+      return pick.bn == 256 ? launch_pair<256, true>(o, p, 2, stream) : launch_pair<128, true>(o, p, 2, stream);
+    if (pick.bn == 256) return launch_pair<256, false>(o, p, 1, stream);
+    if (pick.bn == 192) return launch_pair<192, false>(o, p, 1, stream);
+    return launch_pair<128, false>(o, p, 1, stream);
+  }
   if (M <= 16) return launch_small<16>(o, p, stream);
   if (M <= 32) return launch_small<32>(o, p, stream);
   if (M <= 64) return launch_small<64>(o, p, stream);

@@ -68,11 +68,11 @@ def _bytes(n: int, device: torch.device) -> torch.Tensor:
 
 
 def _alloc_rows(M: int, N: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """``[M, N]`` whose rows start on 16 bytes (what the vector stores of the product want)."""
-    per16 = 8 if dtype == torch.bfloat16 else 4
-    if N % per16 == 0:
+    """``[M, N]`` whose rows start on 32 bytes (what the vector stores of the product want)."""
+    per32 = 16 if dtype == torch.bfloat16 else 8
+    if N % per32 == 0:
         return torch.empty((M, N), dtype=dtype, device=device)
-    return torch.empty((M, _ceil(N, per16) * per16), dtype=dtype, device=device)[:, :N]
+    return torch.empty((M, _ceil(N, per32) * per32), dtype=dtype, device=device)[:, :N]
 
 
 # ----------------------------------------------------------------------------
