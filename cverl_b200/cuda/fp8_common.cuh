@@ -26,15 +26,18 @@ __device__ __forceinline__ long long fp8_sf_offset(long long row, int b, int kgr
 // exponent and whether its mantissa is above 1.75, is the same, and two blocks' maxima fit a register.
 __device__ __forceinline__ uint32_t fp8_max16(uint32_t mag_bits) { return (mag_bits + 0xFFFFu) >> 16; }
 
-// scale byte of a block from the largest finite magnitude: the exponent field, one more where the mantissa is above
-// 1.75, less TOP.  Integer arithmetic: subnormal magnitudes (field 0) end at the smallest scale.
+// Scale bytes of two blocks from their maxima (one in each half of the word): the exponent field, one more where the
+// mantissa is above 1.75, less TOP, at least 1.  Subnormal magnitudes (field 0) end at the smallest scale too.
 template <int FMT>
-__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t max16) {
-  constexpr int TOP = FMT == FP8_E4M3 ? 8 : 15;
-  return static_cast<uint32_t>(max(static_cast<int>((max16 + 0x1Fu) >> 7) - TOP, 1));
+__device__ __forceinline__ uint32_t fp8_scale_bytes(uint32_t max16x2) {
+  constexpr uint32_t TOP = FMT == FP8_E4M3 ? 8 : 15;
+  const uint32_t e = ((max16x2 + 0x001F001Fu) >> 7) & 0x01FF01FFu;
+  return __vmaxu2(e, (TOP + 1) * 0x00010001u) - TOP * 0x00010001u;
 }
-// 2^-e as a float; byte <= 247, so the exponent field stays positive
-__device__ __forceinline__ float fp8_inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// 2^-e of each as a bf16, whose exponent field is 254 - byte (7 or more: the byte is at most 247)
+__device__ __forceinline__ uint32_t fp8_inverse_scales(uint32_t bytes) { return (0x00FE00FEu - bytes) << 7; }
+__device__ __forceinline__ float fp8_low(uint32_t bf16x2) { return __uint_as_float(bf16x2 << 16); }
+__device__ __forceinline__ float fp8_high(uint32_t bf16x2) { return __uint_as_float(bf16x2 & 0xFFFF0000u); }
 
 // product without the flush of subnormal inputs that this library is otherwise compiled with
 __device__ __forceinline__ float fp8_mul(float a, float b) {
@@ -43,43 +46,41 @@ __device__ __forceinline__ float fp8_mul(float a, float b) {
   return r;
 }
 
+// four values as codes, saturating: infinities come out as the largest finite code here, see fp8_fix_inf
 template <int FMT>
-__device__ __forceinline__ uint32_t fp8_pack2(float lo, float hi) {
-  uint16_t r;
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
+  uint32_t r;
   if (FMT == FP8_E4M3)
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
   else
-    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e5m2x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e5m2x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
   return r;
 }
-
-// code of an infinity: e4m3 has none and takes NaN; e5m2 keeps it (the conversion itself would saturate)
 template <int FMT>
-__device__ __forceinline__ uint32_t fp8_inf_code(uint32_t bits) {
-  return (FMT == FP8_E4M3 ? 0x7Fu : 0x7Cu) | ((bits >> 24) & 0x80u);
-}
-
-// eight values times `inv` as eight codes.  `odd` says that one of them may be infinite.
-template <int FMT>
-__device__ __forceinline__ uint2 fp8_pack8(const float (&v)[8], float inv, bool odd) {
-  float s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = fp8_mul(v[i], inv);
+__device__ __forceinline__ uint2 fp8_pack8(const float (&v)[8], float inv) {
   uint2 o;
-  o.x = fp8_pack2<FMT>(s[0], s[1]) | (fp8_pack2<FMT>(s[2], s[3]) << 16);
-  o.y = fp8_pack2<FMT>(s[4], s[5]) | (fp8_pack2<FMT>(s[6], s[7]) << 16);
-  if (odd) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t bits = __float_as_uint(v[i]);
-      if ((bits & 0x7FFFFFFFu) == 0x7F800000u) {
-        uint32_t& word = i < 4 ? o.x : o.y;
-        const int at = (i & 3) * 8;
-        word = (word & ~(0xFFu << at)) | (fp8_inf_code<FMT>(bits) << at);
-      }
-    }
-  }
+  o.x = fp8_pack4<FMT>(fp8_mul(v[0], inv), fp8_mul(v[1], inv), fp8_mul(v[2], inv), fp8_mul(v[3], inv));
+  o.y = fp8_pack4<FMT>(fp8_mul(v[4], inv), fp8_mul(v[5], inv), fp8_mul(v[6], inv), fp8_mul(v[7], inv));
   return o;
+}
+// the codes of infinite values among eight, put in afterwards by the few threads that hold one: e4m3 has no infinity
+// and takes NaN; e5m2 keeps it
+template <int FMT>
+__device__ __forceinline__ void fp8_fix_inf(const float (&v)[8], uint8_t* codes, int n) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t bits = __float_as_uint(v[i]);
+    if (i < n && (bits & 0x7FFFFFFFu) == 0x7F800000u)
+      codes[i] = static_cast<uint8_t>((FMT == FP8_E4M3 ? 0x7Fu : 0x7Cu) | ((bits >> 24) & 0x80u));
+  }
 }
 
 // maximum of |v| over the finite ones of n values, as bits; *odd says that there were others.  The common case costs

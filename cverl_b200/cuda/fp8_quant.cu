@@ -72,6 +72,16 @@ struct Piece<__nv_bfloat16, NORM> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(raw[i][0]), "+r"(raw[i][1]), "+r"(raw[i][2]), "+r"(raw[i][3]));
   }
+  // get() with an index that is not known when compiling
+  __device__ __forceinline__ float at(int i, int j) const {
+    float v = 0.f;
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+        if (a == i && b == j) v = get(a, b);
+    return v;
+  }
   __device__ __forceinline__ float get(int i, int j) const {
     const uint32_t w = raw[i][j >> 1];
     const float v = __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
@@ -89,6 +99,15 @@ struct Piece<float, false> {
       fp8_load8(static_cast<const float*>(p.x) + (r0 + i) * p.x_stride + c0, r0 + i < p.rows ? nc : 0, p.vec, raw[i]);
   }
   __device__ __forceinline__ void keep_packed() {}
+  __device__ __forceinline__ float at(int i, int j) const {
+    float v = 0.f;
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+        if (a == i && b == j) v = raw[a][b];
+    return v;
+  }
   __device__ __forceinline__ float get(int i, int j) const { return raw[i][j]; }
 };
 
@@ -173,12 +192,14 @@ __device__ __forceinline__ bool piece_maxima(const Piece<__nv_bfloat16, false>& 
   return odd;
 }
 
-__device__ __forceinline__ uint32_t half16(const uint32_t (&w)[4], int i) { return (w[i >> 1] >> ((i & 1) * 16)) & 0xFFFFu; }
-
+// Instructions bound this kernel before HBM does (71 % of the issue slots and 65 % of the integer pipe at 4.1 TB/s in
+// an earlier form), so scales are computed two to a word, a column's once for the tile, addresses advance by a stride,
+// and an infinity costs nothing where there is none.
 template <typename T, int FMT, bool NORM, bool ROWS, bool COLS, bool BLOCK>
-__global__ void __launch_bounds__(Q_THREADS, sizeof(T) == 2 ? 3 : 1)
+__global__ void __launch_bounds__(Q_THREADS, sizeof(T) == 4 ? 1 : NORM ? 2 : 3)
 fp8_quant_kernel(const QuantArgs p) {
   __shared__ __align__(16) uint32_t s_max[COLS || BLOCK ? Q_THREADS / 32 : 1][QT / 2];   // column maxima by warp
+  __shared__ __align__(16) uint32_t s_inv[COLS ? QT / 2 : 4];      // 2^-e of two columns a word, as bf16
   __shared__ __align__(16) uint8_t s_t[COLS ? QT * QT : 16];       // transposed codes, 8-byte units XOR-swizzled
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cl = lane & 15, rg = warp * 2 + (lane >> 4);           // columns 8 cl .. + 7, rows 8 rg .. + 7 of the tile
@@ -186,12 +207,13 @@ fp8_quant_kernel(const QuantArgs p) {
   const int tile_c = blockIdx.x - tile_r * p.col_tiles;
   const long long r0 = static_cast<long long>(tile_r) * QT + rg * 8;
   const long long c0 = static_cast<long long>(tile_c) * QT + cl * 8;
+  const int nr = static_cast<int>(max(0ll, min(8ll, p.rows - r0))), nc = static_cast<int>(max(0ll, min(8ll, p.cols - c0)));
   Piece<T, NORM> x;
-  x.load(p, r0, c0, static_cast<int>(max(0ll, min(8ll, p.cols - c0))));
+  x.load(p, r0, c0, nc);
   uint32_t rmax[4], cmax[4];
   const bool odd = piece_maxima(x, rmax, cmax);
   x.keep_packed();
-  uint32_t tile_byte = 0;
+  uint32_t tile_bytes = 0;      // BLOCK: the tile's scale in both halves
   if (BLOCK) {
     uint32_t m = __vmaxu2(__vmaxu2(rmax[0], rmax[1]), __vmaxu2(rmax[2], rmax[3]));
     m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
@@ -199,12 +221,23 @@ fp8_quant_kernel(const QuantArgs p) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < Q_THREADS / 32; ++w) m = max(m, s_max[w][0]);
-    tile_byte = fp8_scale_byte<FMT>(m);
+    tile_bytes = fp8_scale_bytes<FMT>(m * 0x00010001u);
   } else if (COLS) {
     uint32_t c[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) c[j] = __vmaxu2(cmax[j], __shfl_xor_sync(0xffffffffu, cmax[j], 16));
     if (lane < 16) *reinterpret_cast<uint4*>(&s_max[warp][cl * 4]) = make_uint4(c[0], c[1], c[2], c[3]);
+    __syncthreads();
+    if (threadIdx.x < QT / 2) {            // two columns a thread
+      uint32_t m = s_max[0][threadIdx.x];
+#pragma unroll
+      for (int w = 1; w < Q_THREADS / 32; ++w) m = __vmaxu2(m, s_max[w][threadIdx.x]);
+      const uint32_t bytes = fp8_scale_bytes<FMT>(m);
+      s_inv[threadIdx.x] = fp8_inverse_scales(bytes);
+      uint8_t* sf = p.sft + fp8_sf_offset(static_cast<long long>(tile_c) * QT + threadIdx.x * 2, tile_r, p.kgroups_t);
+      sf[0] = static_cast<uint8_t>(bytes);
+      sf[16] = static_cast<uint8_t>(bytes >> 16);
+    }
   }
   if (ROWS) {
     if (!BLOCK) {
@@ -213,49 +246,81 @@ fp8_quant_kernel(const QuantArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) rmax[i] = __vmaxu2(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], o));
     }
+    uint32_t bytes[4], inv[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(half16(rmax, i));
-      // the tile's rows all get a scale, those past the matrix too: the tensor core reads 128 at a time
-      if (cl == 0) p.sf[fp8_sf_offset(r0 + i, tile_c, p.kgroups)] = static_cast<uint8_t>(byte);
-      float v[8];
+    for (int i = 0; i < 4; ++i) {
+      bytes[i] = BLOCK ? tile_bytes : fp8_scale_bytes<FMT>(rmax[i]);
+      inv[i] = fp8_inverse_scales(bytes[i]);
+    }
+    if (cl == 0) {      // the tile's rows all get a scale, those past the matrix too: the tensor core reads 128 at a time
+      uint8_t* sf = p.sf + fp8_sf_offset(r0, tile_c, p.kgroups);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = x.get(i, j);
-      if (r0 + i < p.rows && c0 < p.q_ld)
-        *reinterpret_cast<uint2*>(p.q + (r0 + i) * p.q_ld + c0) = fp8_pack8<FMT>(v, fp8_inverse_scale(byte), odd);
+      for (int i = 0; i < 8; ++i) sf[i * 16] = static_cast<uint8_t>(bytes[i >> 1] >> ((i & 1) * 16));
+    }
+    if (c0 < p.q_ld) {
+      uint8_t* out = p.q + r0 * p.q_ld + c0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i, out += p.q_ld) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x.get(i, j);
+        if (i < nr)
+          *reinterpret_cast<uint2*>(out) = fp8_pack8<FMT>(v, i & 1 ? fp8_high(inv[i >> 1]) : fp8_low(inv[i >> 1]));
+      }
+      if (odd) {
+        out = p.q + r0 * p.q_ld + c0;
+#pragma unroll 1
+        for (int i = 0; i < nr; ++i, out += p.q_ld) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = x.at(i, j);
+          fp8_fix_inf<FMT>(v, out, nc);
+        }
+      }
     }
   }
   if (COLS) {
     x.keep_packed();
-    if (!BLOCK) {
+    uint4 inv = make_uint4(0u, 0u, 0u, 0u);
+    if (BLOCK) {
+      inv.x = inv.y = inv.z = inv.w = fp8_inverse_scales(tile_bytes);
+      if (threadIdx.x < QT)
+        p.sft[fp8_sf_offset(static_cast<long long>(tile_c) * QT + threadIdx.x, tile_r, p.kgroups_t)] =
+            static_cast<uint8_t>(tile_bytes);
+    } else {
       __syncthreads();
-#pragma unroll
-      for (int w = 0; w < Q_THREADS / 32; ++w) {
-        const uint4 m = *reinterpret_cast<const uint4*>(&s_max[w][cl * 4]);
-        cmax[0] = __vmaxu2(cmax[0], m.x), cmax[1] = __vmaxu2(cmax[1], m.y);
-        cmax[2] = __vmaxu2(cmax[2], m.z), cmax[3] = __vmaxu2(cmax[3], m.w);
-      }
+      inv = *reinterpret_cast<const uint4*>(&s_inv[cl * 4]);
     }
+    const uint32_t iw[4] = {inv.x, inv.y, inv.z, inv.w};
+    // 8-byte unit rg of column 8 cl + j sits at unit rg ^ cl: the 16 lanes of a half-warp hit 16 different units
+    uint8_t* mine = s_t + cl * 8 * QT + (rg ^ cl) * 8;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t byte = BLOCK ? tile_byte : fp8_scale_byte<FMT>(half16(cmax, j));
-      if (rg == 0)
-        p.sft[fp8_sf_offset(c0 + j, tile_r, p.kgroups_t)] = static_cast<uint8_t>(byte);
       float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = x.get(i, j);
-      // 8-byte unit rg of column 8 cl + j sits at unit rg ^ cl: the 16 lanes of a half-warp hit 16 different units
-      *reinterpret_cast<uint2*>(s_t + (cl * 8 + j) * QT + (rg ^ cl) * 8) = fp8_pack8<FMT>(v, fp8_inverse_scale(byte), odd);
+      *reinterpret_cast<uint2*>(mine + j * QT) = fp8_pack8<FMT>(v, j & 1 ? fp8_high(iw[j >> 1]) : fp8_low(iw[j >> 1]));
+    }
+    if (odd) {
+#pragma unroll 1
+      for (int j = 0; j < 8; ++j) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x.at(i, j);
+        fp8_fix_inf<FMT>(v, mine + j * QT, 8);
+      }
     }
     __syncthreads();
-    const long long out_c = static_cast<long long>(tile_r) * QT;
+    const long long out_c = static_cast<long long>(tile_r) * QT + cl * 8;
+    const long long left = p.cols - static_cast<long long>(tile_c) * QT;
+    if (out_c < p.qt_ld) {
+      uint8_t* out = p.qt + (static_cast<long long>(tile_c) * QT + rg) * p.qt_ld + out_c;
 #pragma unroll
-    for (int it = 0; it < QT / 16; ++it) {
-      const int c = it * 16 + rg;                   // a half-warp writes the 128 bytes of one transposed row
-      const long long col = static_cast<long long>(tile_c) * QT + c;
-      if (col < p.cols && out_c + cl * 8 < p.qt_ld)
-        *reinterpret_cast<uint2*>(p.qt + col * p.qt_ld + out_c + cl * 8) =
-            *reinterpret_cast<const uint2*>(s_t + c * QT + (cl ^ ((c >> 3) & 15)) * 8);
+      for (int it = 0; it < QT / 16; ++it, out += 16 * p.qt_ld) {
+        const int c = it * 16 + rg;                   // a half-warp writes the 128 bytes of one transposed row
+        if (c < left)
+          *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(s_t + c * QT + (cl ^ ((c >> 3) & 15)) * 8);
+      }
     }
   }
 }
@@ -359,23 +424,22 @@ fp8_norm_kernel(const NormQuantArgs p) {
     rr[i] = load_raw8<VEC>(p.resid + row * p.r_stride + c, ok && p.resid != nullptr ? n : 0);
     wr[i] = load_raw8<VEC>(p.w + c, n);
   }
-  float ss = 0.f;
+  float ss = 0.f, v[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float v[8];
-    widen8(xr[i], v);
+    widen8(xr[i], v[i]);
     if (p.resid != nullptr) {
       const int c = (i * TPR + t) * 8, n = ok ? max(0, min(8, p.D - c)) : 0;
       float b[8];
       widen8(rr[i], b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += b[j];
-      xr[i] = narrow8(v);
-      store_raw8<VEC>(p.h + row * p.h_stride + c, xr[i], n);
-      widen8(xr[i], v);
+      for (int j = 0; j < 8; ++j) v[i][j] += b[j];
+      const uint4 h = narrow8(v[i]);
+      store_raw8<VEC>(p.h + row * p.h_stride + c, h, n);
+      widen8(h, v[i]);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += v[j] * v[j];
+    for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
   }
   ss = warp_sum(ss);
   if (TPR > 32) {
@@ -387,22 +451,25 @@ fp8_norm_kernel(const NormQuantArgs p) {
   }
   const float rstd = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
   if (ok && t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+  uint8_t* q = p.q + row * p.q_ld;
+  uint8_t* sf = p.sf + fp8_sf_offset(row, 0, p.kgroups);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + t) * 8, n = max(0, min(8, p.D - c));
-    float v[8], g[8];
-    widen8(xr[i], v);
+    float g[8];
     widen8(wr[i], g);
     bool odd = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? v[j] * rstd * (p.w_offset + g[j]) : 0.f;
-    uint32_t m = fp8_max16(fp8_finite_max(v, &odd));
+    for (int j = 0; j < 8; ++j) v[i][j] = VEC || j < n ? v[i][j] * rstd * (p.w_offset + g[j]) : 0.f;
+    uint32_t m = fp8_max16(fp8_finite_max(v[i], &odd));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t byte = fp8_scale_byte<FMT>(m);
-    if (ok && c < p.D && (t & 15) == 0) p.sf[fp8_sf_offset(row, c >> 7, p.kgroups)] = static_cast<uint8_t>(byte);
-    if (ok && c < p.q_ld)
-      *reinterpret_cast<uint2*>(p.q + row * p.q_ld + c) = fp8_pack8<FMT>(v, fp8_inverse_scale(byte), odd);
+    const uint32_t byte = fp8_scale_bytes<FMT>(m) & 0xFFu;
+    if (ok && c < p.D && (t & 15) == 0) sf[(c >> 9) * 512 + ((c >> 7) & 3)] = static_cast<uint8_t>(byte);
+    if (ok && c < p.q_ld) {
+      *reinterpret_cast<uint2*>(q + c) = fp8_pack8<FMT>(v[i], fp8_low(fp8_inverse_scales(byte)));
+      if (odd) fp8_fix_inf<FMT>(v[i], q + c, n);
+    }
   }
 }
 
