@@ -1,6 +1,6 @@
 """Rollout (generation) throughput of the cached native decode, in tokens per second.
 
-``python -m cverl_b200.bench_rollout [--batch 128] [--prompt-len 256] [--new-tokens 1024] [--baseline-tokens 8]``
+``python -m cverl_b200.bench_rollout [--batch 128] [--prompt-len 256] [--new-tokens 1024] [--baseline-tokens 8] [--fp8]``
 
 Qwen3.5-0.8B shape, random-init bf16 weights, uniform random prompt ids.  Timed with CUDA events after a warm-up
 generation: the prompt prefill, then ``new-tokens`` decode steps replayed from one CUDA graph (tcgen05 GEMMs,
@@ -25,13 +25,14 @@ def main(argv=None) -> int:
     ap.add_argument("--new-tokens", type=int, default=1024)
     ap.add_argument("--baseline-tokens", type=int, default=4)
     ap.add_argument("--layers", type=int, default=0, help="debug: fewer layers")
+    ap.add_argument("--fp8", action="store_true", help="projections of the decode steps in 8 bits")
     a = ap.parse_args(argv)
     if not torch.cuda.is_available():
         print(json.dumps({"error": "no CUDA device"}))
         return 1
     from . import _native as nv
     from .models.config import Qwen35TextConfig
-    from .models.decode import GraphedDecoder, prefill
+    from .models.decode import GraphedDecoder, fp8_decode_weights, prefill
     from .models.qwen3_5 import Qwen35Model
     dev = torch.device("cuda", 0)
     cfg = Qwen35TextConfig.qwen3_5_0_8b() if not a.layers else Qwen35TextConfig(num_hidden_layers=a.layers)
@@ -40,10 +41,13 @@ def main(argv=None) -> int:
     g = torch.Generator(device=dev).manual_seed(0)
     prompts = torch.randint(1, cfg.vocab_size, (a.batch, a.prompt_len), device=dev, generator=g)
 
+    def decoder(state):
+        return GraphedDecoder(model, state, a.batch, fp8=fp8_decode_weights(model) if a.fp8 else None)
+
     def generate(n):
         with torch.no_grad():
             state, logits = prefill(model, prompts, max_len=a.prompt_len + n)
-            dec = GraphedDecoder(model, state, a.batch)
+            dec = decoder(state)
             tok = logits.argmax(-1)
             for _ in range(n - 1):
                 tok = dec.step(tok).argmax(-1)
@@ -55,7 +59,7 @@ def main(argv=None) -> int:
     e0.record()
     with torch.no_grad():
         state, logits = prefill(model, prompts, max_len=a.prompt_len + a.new_tokens)
-        dec = GraphedDecoder(model, state, a.batch)
+        dec = decoder(state)
     e1.record()
     with torch.no_grad():
         tok = logits.argmax(-1)
@@ -69,7 +73,8 @@ def main(argv=None) -> int:
            "prompt_len": a.prompt_len, "new_tokens": a.new_tokens, "prefill_and_capture_ms": setup_ms,
            "decode_ms": decode_ms, "ms_per_token_step": decode_ms / max(1, a.new_tokens - 1),
            "decode_tokens_per_s": a.batch * (a.new_tokens - 1) / (decode_ms / 1e3),
-           "end_to_end_tokens_per_s": a.batch * a.new_tokens / ((setup_ms + decode_ms) / 1e3), "dtype": "bf16",
+           "end_to_end_tokens_per_s": a.batch * a.new_tokens / ((setup_ms + decode_ms) / 1e3),
+           "dtype": "fp8 projections, bf16 elsewhere" if a.fp8 else "bf16",
            "data": "uniform random prompt ids, random-init weights, greedy sampling"}
     if a.baseline_tokens > 0:
         from .models.policy import Qwen3_5CausalLmPolicy

@@ -732,7 +732,7 @@ static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int split, cudaStr
   if (e != cudaSuccess) return static_cast<int>(e);
   p.m_tiles = (p.M + 255) / 256;
   p.n_tiles = (p.N + BN - 1) / BN;
-  if (static_cast<long long>(p.m_tiles) * p.n_tiles > 0x0fffffffll) return -11;
+  if (static_cast<long long>(p.m_tiles) * p.n_tiles > 0x0fffffffll || ra > 0x7fffffffull || rb > 0x7fffffffull) return -11;
   p.total = p.m_tiles * p.n_tiles;
   p.group_m = p.m_tiles < 16 ? p.m_tiles : 16;
   p.split = split;

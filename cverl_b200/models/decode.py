@@ -35,6 +35,7 @@ class DecodeState:
     length: int                      # tokens already in the caches
     layers: List[dict] = field(default_factory=list)
     dev: Optional[dict] = None       # device-side step counters and tables of the native path
+    fp8: Optional[dict] = None       # the projections' weights in 8 bits (``fp8_decode_weights``); None: bf16
 
     def to_native(self, model) -> None:
         """Device copies of what the native step reads: the length after this step (int32 [1]), the position of
@@ -213,14 +214,43 @@ def _linear_attention_step(model, x, i, c):
 # ---------------------------------------------------------------------------------------------------------
 # native one-token step
 # ---------------------------------------------------------------------------------------------------------
-def _native_full_attention(model, x, i, c, dv):
+@torch.no_grad()
+def fp8_decode_weights(model) -> dict:
+    """The weights of every projection that the native step runs, in 8 bits with 128 x 128 block scales; embedding,
+    norms, convolution and LM head stay bf16.  A copy: made again after the parameters change."""
+    if not native_decode_supported(model):
+        raise RuntimeError("the native decode path does not support this model / device")
+    cfg = model.cfg
+    out = {}
+    for i in range(model.layer_begin, model.layer_end):
+        p = f"{cfg.layer_root}{i}."
+        named = {f"{i}.gate_up": model.fused[f"{i}.gate_up"], p + "mlp.down_proj.weight": None}
+        if cfg.layer_types[i] == "full_attention":
+            named |= {f"{i}.qkv": model.fused[f"{i}.qkv"], p + "self_attn.o_proj.weight": None}
+        else:
+            named |= {f"{i}.lin_in": model.fused[f"{i}.lin_in"], p + "linear_attn.out_proj.weight": None}
+        for name, w in named.items():
+            out[name] = ops.quantize_fp8_weight(model.param(name) if w is None else w, transposed=False)
+    return out
+
+
+def _proj(fp8, name, x, w):
+    return ops.linear(x, w) if fp8 is None else ops.linear_fp8(x, fp8[name])
+
+
+def _norm(fp8, x, resid, w, eps, off):
+    """Residual add + norm; its result in 8 bits where the projections that read it are."""
+    return ops.add_rmsnorm(x, resid, w, eps, off) if fp8 is None else ops.add_rmsnorm_fp8(x, resid, w, eps, off)
+
+
+def _native_full_attention(model, x, i, c, dv, fp8=None):
     from .. import _native as nv
     from ..ops.gemm import count_launch
     cfg = model.cfg
     p = f"{cfg.layer_root}{i}.self_attn."
     d, h, kvh = cfg.head_dim, cfg.num_attention_heads, cfg.num_key_value_heads
     B = x.shape[0]
-    qkv = ops.linear(x, model.fused[f"{i}.qkv"])                       # [B, h*d*2 + 2*kvh*d] bf16
+    qkv = _proj(fp8, f"{i}.qkv", x, model.fused[f"{i}.qkv"])           # [B, h*d*2 + 2*kvh*d] bf16
     q_all, k, v = qkv.split([h * d * 2, kvh * d, kvh * d], dim=-1)
     q, gate = q_all.view(B, h, 2 * d).split([d, d], dim=-1)            # strided views into the projection
     off = cfg.norm_weight_offset
@@ -228,7 +258,7 @@ def _native_full_attention(model, x, i, c, dv):
                           cfg.rms_norm_eps, off)
     k = ops.headnorm_rope(k.view(B, kvh, d), model.param(p + "k_norm.weight"), dv["cos"], dv["sin"], dv["pos"],
                           cfg.rotary_dim, cfg.rms_norm_eps, off)
-    o = torch.empty((B, h, d), dtype=x.dtype, device=x.device)
+    o = torch.empty((B, h, d), dtype=model.dtype, device=x.device)
     if k.stride(0) != v.stride(0):           # the kernel takes one row stride for the new key and value
         v = v.contiguous()
         k = k.contiguous()
@@ -239,10 +269,10 @@ def _native_full_attention(model, x, i, c, dv):
              "cvb_decode_attention")
     count_launch()
     o = ops.siggate(o, gate)
-    return ops.linear(o.reshape(B, h * d), model.param(p + "o_proj.weight"))
+    return _proj(fp8, p + "o_proj.weight", o.reshape(B, h * d), model.param(p + "o_proj.weight"))
 
 
-def _native_linear_attention(model, x, i, c, dv):
+def _native_linear_attention(model, x, i, c, dv, fp8=None):
     from .. import _native as nv
     from ..ops.gemm import count_launch
     cfg = model.cfg
@@ -252,9 +282,9 @@ def _native_linear_attention(model, x, i, c, dv):
     key_dim, value_dim = kh * kd, vh * vd
     conv_dim = 2 * key_dim + value_dim
     B = x.shape[0]
-    proj = ops.linear(x, model.fused[f"{i}.lin_in"])                   # [B, conv_dim + value_dim + 2 vh]
+    proj = _proj(fp8, f"{i}.lin_in", x, model.fused[f"{i}.lin_in"])    # [B, conv_dim + value_dim + 2 vh]
     mixed, z, b, a = proj.split([conv_dim, value_dim, vh, vh], dim=-1)
-    o = torch.empty((B, vh, vd), dtype=x.dtype, device=x.device)
+    o = torch.empty((B, vh, vd), dtype=model.dtype, device=x.device)
     # convolution (ring cache of raw rows) + SiLU + l2norm + gates + state update + read-out: one kernel
     nv.check(nv.cuda().cvb_gdn_decode_step(proj.data_ptr(), proj.stride(0), kh, vh,
                                            model.param(p + "conv1d.weight").data_ptr(), c["conv_ring"].data_ptr(),
@@ -264,15 +294,16 @@ def _native_linear_attention(model, x, i, c, dv):
                                            o.data_ptr(), B, nv.stream()), "cvb_gdn_decode_step")
     count_launch()
     y = ops.gated_rmsnorm(o, z, model.param(p + "norm.weight"), cfg.rms_norm_eps)
-    return ops.linear(y.reshape(B, value_dim), model.param(p + "out_proj.weight"))
+    return _proj(fp8, p + "out_proj.weight", y.reshape(B, value_dim), model.param(p + "out_proj.weight"))
 
 
 @torch.no_grad()
 def decode_step_native(model, state: DecodeState, tokens: torch.Tensor, advance: bool = True) -> torch.Tensor:
     """One token per sequence on the native kernels; logits ``[B, V]`` fp32.  Every length / position is read
-    from ``state.dev`` on the device and advanced there, so the same launches serve every step."""
+    from ``state.dev`` on the device and advanced there, so the same launches serve every step.  With ``state.fp8``
+    the projections and the norms before them run in 8 bits."""
     cfg = model.cfg
-    dv = state.dev
+    dv, fp8 = state.dev, state.fp8
     B = tokens.shape[0]
     eps, off = cfg.rms_norm_eps, cfg.norm_weight_offset
     delta = ops.embedding(tokens.view(B), model.param(cfg.embed_name))
@@ -280,13 +311,16 @@ def decode_step_native(model, state: DecodeState, tokens: torch.Tensor, advance:
     for li, i in enumerate(range(model.layer_begin, model.layer_end)):
         p = f"{cfg.layer_root}{i}."
         c = state.layers[li]
-        n1, resid = ops.add_rmsnorm(delta, resid, model.param(p + "input_layernorm.weight"), eps, off)
+        n1, resid = _norm(fp8, delta, resid, model.param(p + "input_layernorm.weight"), eps, off)
         if cfg.layer_types[i] == "full_attention":
-            a = _native_full_attention(model, n1, i, c, dv)
+            a = _native_full_attention(model, n1, i, c, dv, fp8)
         else:
-            a = _native_linear_attention(model, n1, i, c, dv)
-        n2, resid = ops.add_rmsnorm(a, resid, model.param(p + "post_attention_layernorm.weight"), eps, off)
-        delta = model.mlp(n2, i)
+            a = _native_linear_attention(model, n1, i, c, dv, fp8)
+        n2, resid = _norm(fp8, a, resid, model.param(p + "post_attention_layernorm.weight"), eps, off)
+        if fp8 is None:
+            delta = model.mlp(n2, i)
+        else:
+            delta = ops.linear_fp8(ops.swiglu(ops.linear_fp8(n2, fp8[f"{i}.gate_up"])), fp8[p + "mlp.down_proj.weight"])
     out, _ = ops.add_rmsnorm(delta, resid, model.param(cfg.final_norm_name), eps, off)
     logits = ops.gemm_nt(out, model.lm_head_weight(), out_dtype=torch.float32)
     if advance:
@@ -301,12 +335,15 @@ class GraphedDecoder:
 
     ``step(tokens)`` copies the tokens into the graph's input buffer, replays, and returns the graph's logits
     buffer (valid until the next ``step``).  The caches, the recurrent states, the length counter and the position
-    vector are the tensors of ``state``; the graph updates them in place.
+    vector are the tensors of ``state``; the graph updates them in place.  ``fp8`` takes the result of
+    ``fp8_decode_weights(model)``: the projections then read 8-bit weights, half the bytes of a step.
     """
 
-    def __init__(self, model, state: DecodeState, batch: int, warmup: int = 2):
+    def __init__(self, model, state: DecodeState, batch: int, warmup: int = 2, fp8: Optional[dict] = None):
         if not native_decode_supported(model):
             raise RuntimeError("the native decode path does not support this model / device")
+        if fp8 is not None:
+            state.fp8 = fp8
         if state.dev is None:
             state.to_native(model)
         self.model, self.state = model, state

@@ -21,10 +21,11 @@ statement of the same math, which is also the test oracle.  The reference has no
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+import functools
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native as nv
 from .gemm import count_launch
@@ -32,35 +33,45 @@ from .gemm import count_launch
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
 BLOCK = 128
 MAX_NORM_WIDTH = 16384
+MAX_EXTENT = 2 ** 31 - 1024                # rows or columns; sizes are 32-bit in the product
 _FMT = {E4M3: 0, E5M2: 1}
 _TOP = {E4M3: 8, E5M2: 15}                 # FMAX = 1.75 * 2^TOP
 _ROWS, _COLS, _TILES = 1, 2, 4             # mode bits of cvb_fp8_quantize
 _OUT = {torch.bfloat16: 0, torch.float32: 1}
+_status_ptr: dict = {}
 
 
 def _ceil(a: int, b: int) -> int:
     return (a + b - 1) // b
 
 
-class _On:
-    """Launches of a block go to one device: ``stream`` is that device's current stream, ``status`` its status word."""
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
 
-    __slots__ = ("index", "before", "stream", "status")
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.get_device()
+def _on_device(fn):
+    """Runs ``fn`` with the device of its first argument as the current one: launches go to the tensors' device and to
+    that device's current stream."""
+    @functools.wraps(fn)
+    def call(x, *args, **kwargs):
+        t = x.buf if isinstance(x, Fp8Tensor) else x
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != _current_device():
+            with torch.cuda.device(t.device):
+                return fn(x, *args, **kwargs)
+        return fn(x, *args, **kwargs)
+    return call
 
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        self.stream = nv.raw_stream(self.index)
-        self.status = nv.status_word(self.index).data_ptr()
-        return self
 
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _stream() -> int:
+    return nv.raw_stream(_current_device())
+
+
+def _status() -> int:
+    index = _current_device()
+    p = _status_ptr.get(index)
+    if p is None:
+        p = _status_ptr[index] = nv.status_word(index).data_ptr()      # one per device, never replaced
+    return p
 
 
 def _bytes(n: int, device: torch.device) -> torch.Tensor:
@@ -78,6 +89,10 @@ def _alloc_rows(M: int, N: int, dtype: torch.dtype, device: torch.device) -> tor
 # ----------------------------------------------------------------------------
 # the 8-bit matrix
 # ----------------------------------------------------------------------------
+def _nbytes(rows: int, cols: int) -> int:
+    return rows * ((cols + 15) // 16 * 16) + ((rows + 127) // 128) * ((cols + 511) // 512) * 512
+
+
 class Fp8Tensor:
     """``[rows, cols]`` in 8 bits.  One buffer: codes, row-major with rows padded to 16 bytes, then the scale bytes in
     the order in which the tensor core reads them (see ``cuda/fp8_common.cuh``)."""
@@ -86,11 +101,7 @@ class Fp8Tensor:
 
     def __init__(self, buf: torch.Tensor, rows: int, cols: int, dtype: torch.dtype):
         self.buf, self.rows, self.cols, self.dtype = buf, rows, cols, dtype
-        self.ld = _ceil(cols, 16) * 16
-
-    @staticmethod
-    def nbytes_of(rows: int, cols: int) -> int:
-        return rows * _ceil(cols, 16) * 16 + _ceil(rows, BLOCK) * _ceil(cols, 4 * BLOCK) * 512
+        self.ld = (cols + 15) // 16 * 16
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -107,43 +118,40 @@ class Fp8Tensor:
     @property
     def values(self) -> torch.Tensor:
         """The codes as an 8-bit float view ``[rows, cols]`` (in units of their scales)."""
-        return self.buf[:self.rows * self.ld].view(self.dtype).view(self.rows, self.ld)[:, :self.cols]
+        return self.buf.view(self.dtype).as_strided((self.rows, self.cols), (self.ld, 1))
 
     def scales(self) -> torch.Tensor:
         """The scales ``[rows, ceil(cols / 128)]`` as ``torch.float8_e8m0fnu`` (powers of two)."""
-        nb = _ceil(self.cols, BLOCK)
-        out = torch.empty((self.rows, nb), dtype=torch.uint8, device=self.device)
-        if out.numel() == 0:
-            pass
-        elif self.buf.is_cuda:
-            with _On(out) as on:
-                nv.check(nv.cuda().cvb_fp8_scales(self.sf_ptr, out.data_ptr(), self.rows, nb, on.stream), "cvb_fp8_scales")
-            count_launch()
-        else:
-            out.copy_(_scale_cells(self.buf, self.rows, self.cols, self.ld)[:self.rows, :nb])
-        return out.view(torch.float8_e8m0fnu)
+        return _scales(self).view(torch.float8_e8m0fnu)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         s = self.scales().float().repeat_interleave(BLOCK, 1)[:, :self.cols]
         return (self.values.float() * s).to(dtype)
 
 
-@dataclass
 class Fp8Weight:
     """A weight ``[N, K]`` in 8 bits (``w``) and, for gradients of the input, its transpose ``[K, N]`` (``wt``)."""
-    w: Fp8Tensor
-    wt: Optional[Fp8Tensor]
 
-    @property
-    def shape(self) -> Tuple[int, int]:
-        return self.w.shape
+    __slots__ = ("w", "wt", "shape", "device")
+
+    def __init__(self, w: Fp8Tensor, wt: Optional[Fp8Tensor]):
+        self.w, self.wt = w, wt
+        self.shape, self.device = w.shape, w.device
 
 
-def _scale_cells(buf: torch.Tensor, rows: int, cols: int, ld: int) -> torch.Tensor:
-    """CPU: the scale bytes of a buffer as a fresh plain ``[rows up to 128, blocks up to 4]`` matrix."""
-    rt, kg = _ceil(rows, BLOCK), _ceil(cols, 4 * BLOCK)
-    cells = buf[rows * ld:rows * ld + rt * kg * 512].view(rt, kg, 32, 4, 4)       # [.., r % 32, r / 32, b % 4]
-    return cells.permute(0, 3, 2, 1, 4).reshape(rt * BLOCK, kg * 4)
+@_on_device
+def _scales(q: Fp8Tensor) -> torch.Tensor:
+    nb = _ceil(q.cols, BLOCK)
+    out = torch.empty((q.rows, nb), dtype=torch.uint8, device=q.device)
+    if q.rows == 0 or nb == 0:
+        return out
+    if q.buf.is_cuda:
+        nv.check(nv.cuda().cvb_fp8_scales(q.sf_ptr, out.data_ptr(), q.rows, nb, _stream()), "cvb_fp8_scales")
+        count_launch()
+        return out
+    rt, kg = _ceil(q.rows, BLOCK), _ceil(q.cols, 4 * BLOCK)
+    cells = q.buf[q.rows * q.ld:].view(rt, kg, 32, 4, 4)                           # [.., r % 32, r / 32, b % 4]
+    return out.copy_(cells.permute(0, 3, 2, 1, 4).reshape(rt * BLOCK, kg * 4)[:q.rows, :nb])
 
 
 def _quantize_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1):
@@ -162,7 +170,7 @@ def _quantize_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1):
 
 def _pack_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1) -> Fp8Tensor:
     R, C = x.shape
-    out = Fp8Tensor(torch.zeros(Fp8Tensor.nbytes_of(R, C), dtype=torch.uint8, device=x.device), R, C, dtype)
+    out = Fp8Tensor(torch.zeros(_nbytes(R, C), dtype=torch.uint8, device=x.device), R, C, dtype)
     if R == 0 or C == 0:
         return out
     codes, byte = _quantize_ref(x, dtype, block_rows)
@@ -179,8 +187,10 @@ def _check_matrix(x: torch.Tensor, what: str) -> torch.Tensor:
         raise TypeError(f"{what}: a tensor is wanted, got {type(x).__name__}")
     if x.dim() != 2:
         raise ValueError(f"{what}: a matrix is wanted, got shape {tuple(x.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float32):
+    if x.dtype not in _OUT:
         raise TypeError(f"{what}: bfloat16 or float32 is wanted, got {x.dtype}")
+    if x.shape[0] > MAX_EXTENT or x.shape[1] > MAX_EXTENT:
+        raise ValueError(f"{what}: at most {MAX_EXTENT} rows and columns, got {tuple(x.shape)}")
     return x if x.stride(1) == 1 or x.shape[1] <= 1 else x.contiguous()
 
 
@@ -190,11 +200,11 @@ def _check_dtype(dtype: torch.dtype, what: str) -> None:
 
 
 def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int, rstd=None, w=None, w_offset: float = 0.0):
-    """(row form or None, transposed form or None) by the mode's bits.  With ``rstd`` the values are
+    """(row form or None, transposed form or None) by the mode's bits.  With ``rstd`` (on the CPU) the values are
     ``x * rstd[row] * (w_offset + w[col])``."""
     R, C = x.shape
-    tall = BLOCK if mode & _TILES else 1
     if not x.is_cuda:
+        tall = BLOCK if mode & _TILES else 1
         x = x.detach()
         v = x.float() if rstd is None else x.float() * rstd[:, None] * (w_offset + w.float())
         return (_pack_ref(v, dtype, tall) if mode & _ROWS else None,
@@ -202,38 +212,41 @@ def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int, rstd=None, w=None,
     q = t = None
     q_args = t_args = (None, None, 0)
     if mode & _ROWS:
-        q = Fp8Tensor(_bytes(Fp8Tensor.nbytes_of(R, C), x.device), R, C, dtype)
+        q = Fp8Tensor(_bytes(_nbytes(R, C), x.device), R, C, dtype)
         q_args = (q.buf.data_ptr(), q.sf_ptr, q.ld)
     if mode & _COLS:
-        t = Fp8Tensor(_bytes(Fp8Tensor.nbytes_of(C, R), x.device), C, R, dtype)
+        t = Fp8Tensor(_bytes(_nbytes(C, R), x.device), C, R, dtype)
         t_args = (t.buf.data_ptr(), t.sf_ptr, t.ld)
     if R and C:
-        with _On(x) as on:
-            nv.check(nv.cuda().cvb_fp8_quantize(
-                x.data_ptr(), x.dtype == torch.float32, R, C, x.stride(0), _FMT[dtype], mode, *q_args, *t_args,
-                nv.ptr(rstd), nv.ptr(w), w_offset, on.stream), "cvb_fp8_quantize")
+        nv.check(nv.cuda().cvb_fp8_quantize(
+            x.data_ptr(), x.dtype == torch.float32, R, C, x.stride(0), _FMT[dtype], mode, *q_args, *t_args, None, None,
+            0.0, _stream()), "cvb_fp8_quantize")
         count_launch()
     return q, t
 
 
+@_on_device
 def quantize_fp8(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
     """``x [R, C]`` (bf16 or fp32) in 8 bits, one scale per 128 elements of a row."""
     _check_dtype(dtype, "quantize_fp8")
     return _quantize(_check_matrix(x, "quantize_fp8"), dtype, _ROWS)[0]
 
 
+@_on_device
 def quantize_fp8_t(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
     """``x.T [C, R]`` in 8 bits, one scale per 128 rows of ``x``."""
     _check_dtype(dtype, "quantize_fp8_t")
     return _quantize(_check_matrix(x, "quantize_fp8_t"), dtype, _COLS)[1]
 
 
+@_on_device
 def quantize_fp8_pair(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Tuple[Fp8Tensor, Fp8Tensor]:
     """``(quantize_fp8(x), quantize_fp8_t(x))`` from one read of ``x``."""
     _check_dtype(dtype, "quantize_fp8_pair")
     return _quantize(_check_matrix(x, "quantize_fp8_pair"), dtype, _ROWS | _COLS)
 
 
+@_on_device
 def quantize_fp8_weight(w: torch.Tensor, transposed: bool = True) -> Fp8Weight:
     """A weight ``[N, K]`` in e4m3 with one scale per 128 x 128 block.  ``transposed=False`` leaves the transpose out,
     which only gradients of the layer's input need."""
@@ -244,6 +257,7 @@ def quantize_fp8_weight(w: torch.Tensor, transposed: bool = True) -> Fp8Weight:
 # ----------------------------------------------------------------------------
 # product
 # ----------------------------------------------------------------------------
+@_on_device
 def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, *,
                 out_dtype: Optional[torch.dtype] = None, accumulate: bool = False) -> torch.Tensor:
     """``a [M, K] @ b [N, K].T -> [M, N]`` in bf16 (default) or fp32; ``accumulate`` adds to an fp32 ``out``.
@@ -278,11 +292,10 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
     if not a.buf.is_cuda:
         r = a.dequantize() @ b.dequantize().t()
         return out.add_(r) if accumulate else out.copy_(r)
-    with _On(out) as on:
-        nv.check(nv.cuda().cvb_fp8_gemm(
-            a.buf.data_ptr(), a.sf_ptr, a.ld, _FMT[a.dtype], b.buf.data_ptr(), b.sf_ptr, b.ld, _FMT[b.dtype], M, N, K,
-            out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype], on.status, on.stream),
-            "cvb_fp8_gemm")
+    nv.check(nv.cuda().cvb_fp8_gemm(
+        a.buf.data_ptr(), a.sf_ptr, a.ld, _FMT[a.dtype], b.buf.data_ptr(), b.sf_ptr, b.ld, _FMT[b.dtype], M, N, K,
+        out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype], _status(), _stream()),
+        "cvb_fp8_gemm")
     count_launch()
     return out
 
@@ -291,19 +304,21 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
 # residual add + RMSNorm with 8-bit output
 # ----------------------------------------------------------------------------
 def _check_norm(x, resid, w, what):
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_WIDTH:
-        raise ValueError(f"{what}: a last dimension of 1 to {MAX_NORM_WIDTH} is wanted, got shape {tuple(x.shape)}")
-    if x.is_cuda and (x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16):
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= MAX_NORM_WIDTH:
+        raise ValueError(f"{what}: a last dimension of 1 to {MAX_NORM_WIDTH} is wanted, got shape {tuple(shape)}")
+    if (x.is_cuda or w.is_cuda) and (x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16):
         raise TypeError(f"{what}: bfloat16 is wanted on the GPU, got {x.dtype} and a weight in {w.dtype}")
-    if tuple(w.shape) != (x.shape[-1],) or w.device != x.device:
-        raise ValueError(f"{what}: the weight is {tuple(w.shape)} on {w.device}, the rows have {x.shape[-1]} on {x.device}")
-    if resid is not None and (resid.shape != x.shape or resid.dtype != x.dtype or resid.device != x.device):
+    if w.dim() != 1 or w.shape[0] != shape[-1] or w.device != x.device:
+        raise ValueError(f"{what}: the weight is {tuple(w.shape)} on {w.device}, the rows have {shape[-1]} on {x.device}")
+    if resid is not None and (resid.shape != shape or resid.dtype != x.dtype or resid.device != x.device):
         raise ValueError(f"{what}: resid is {tuple(resid.shape)} {resid.dtype} on {resid.device}, "
-                         f"x is {tuple(x.shape)} {x.dtype} on {x.device}")
+                         f"x is {tuple(shape)} {x.dtype} on {x.device}")
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    t = t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
@@ -311,95 +326,119 @@ def _norm_forward(x2, r2, w, eps, w_offset, dtype, need_rstd: bool):
     """(8-bit rows, h or x2, rstd or None) of matrices."""
     R, D = x2.shape
     if not x2.is_cuda:
-        h = x2 if r2 is None else (x2.float() + r2.float()).to(x2.dtype)
+        x2, w = x2.detach(), w.detach()
+        h = x2 if r2 is None else (x2.float() + r2.detach().float()).to(x2.dtype)
         rstd = torch.rsqrt(h.float().pow(2).mean(-1) + eps)
         return _pack_ref(h.float() * rstd[:, None] * (w_offset + w.float()), dtype), h, rstd
-    q = Fp8Tensor(_bytes(Fp8Tensor.nbytes_of(R, D), x2.device), R, D, dtype)
+    q = Fp8Tensor(_bytes(_nbytes(R, D), x2.device), R, D, dtype)
     h = torch.empty((R, D), dtype=x2.dtype, device=x2.device) if r2 is not None else None
     rstd = torch.empty(R, dtype=torch.float32, device=x2.device) if need_rstd else None
     if R:
-        w = w.contiguous()
-        with _On(x2) as on:
-            nv.check(nv.cuda().cvb_fp8_add_rmsnorm(
-                x2.data_ptr(), x2.stride(0), nv.ptr(r2), r2.stride(0) if r2 is not None else 0, w.data_ptr(),
-                nv.ptr(h), q.buf.data_ptr(), q.sf_ptr, q.ld, nv.ptr(rstd), R, D, _FMT[dtype], eps, w_offset,
-                on.stream), "cvb_fp8_add_rmsnorm")
+        if w.stride(0) != 1:
+            w = w.contiguous()
+        nv.check(nv.cuda().cvb_fp8_add_rmsnorm(
+            x2.data_ptr(), x2.stride(0), nv.ptr(r2), r2.stride(0) if r2 is not None else 0, w.data_ptr(), nv.ptr(h),
+            q.buf.data_ptr(), q.sf_ptr, q.ld, nv.ptr(rstd), R, D, _FMT[dtype], eps, w_offset, _stream()),
+            "cvb_fp8_add_rmsnorm")
         count_launch()
     return q, (h if h is not None else x2), rstd
 
 
+@_on_device
 def add_rmsnorm_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], w: torch.Tensor, eps: float = 1e-6,
                     w_offset: float = 1.0, dtype: torch.dtype = E4M3) -> Tuple[Fp8Tensor, torch.Tensor]:
     """``(Q(rmsnorm(x + resid)), x + resid)``; ``resid`` may be None.  The norm is rounded once, from fp32 to 8 bits;
-    rows of the result are the rows of ``x`` flattened to a matrix.  For gradients see ``add_rmsnorm_linear_fp8``."""
+    rows of the result are the rows of ``x`` flattened to a matrix.  It has no gradient and refuses inputs that ask for
+    one: see ``add_rmsnorm_linear_fp8``."""
     _check_dtype(dtype, "add_rmsnorm_fp8")
     _check_norm(x, resid, w, "add_rmsnorm_fp8")
-    r2 = _rows2d(resid.detach()) if resid is not None else None
-    q, h, _ = _norm_forward(_rows2d(x.detach()), r2, w.detach(), eps, w_offset, dtype, False)
-    return q, (x if resid is None else h.view(x.shape))
+    if _needs_grad(x, resid, w):
+        raise RuntimeError("add_rmsnorm_fp8 has no gradient: call it under torch.no_grad(), or add_rmsnorm_linear_fp8")
+    q, h, _ = _norm_forward(_rows2d(x), _rows2d(resid) if resid is not None else None, w, eps, w_offset, dtype, False)
+    if resid is None:
+        return q, x
+    return q, h if x.dim() == 2 else h.view(x.shape)
 
 
 # ----------------------------------------------------------------------------
 # linear layers
 # ----------------------------------------------------------------------------
 def _check_linear(K: int, device, w, weight: Optional[Fp8Weight], grad_dtype, what: str) -> None:
-    _check_dtype(grad_dtype, what)
-    shape = tuple(w.shape)
+    if grad_dtype not in _FMT:
+        _check_dtype(grad_dtype, what)
+    shape = w.shape
     if len(shape) != 2 or shape[1] != K:
-        raise ValueError(f"{what}: a weight [N, {K}] is wanted, got {shape}")
-    if isinstance(w, torch.Tensor) and w.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"{what}: the weight is bfloat16 or float32, not {w.dtype}")
-    if (w.w.device if isinstance(w, Fp8Weight) else w.device) != device:
-        raise ValueError(f"{what}: the weight and the input are on different devices")
-    if weight is not None and (tuple(weight.shape) != shape or weight.w.device != device):
-        raise ValueError(f"{what}: the 8-bit weight is {weight.shape} on {weight.w.device}, the weight {shape} on {device}")
+        raise ValueError(f"{what}: a weight [N, {K}] is wanted, got {tuple(shape)}")
+    if w.device != device:
+        raise ValueError(f"{what}: the weight is on {w.device}, the input on {device}")
+    if not isinstance(w, Fp8Weight):
+        if w.dtype not in _OUT:
+            raise TypeError(f"{what}: the weight is bfloat16 or float32, not {w.dtype}")
+        if weight is not None and (weight.shape != tuple(shape) or weight.device != device):
+            raise ValueError(f"{what}: the 8-bit weight is {weight.shape} on {weight.device}, the weight {tuple(shape)} on {device}")
+    elif weight is not None:
+        raise ValueError(f"{what}: the 8-bit weight is given twice")
 
 
 def _forward(x2, xq, w, weight: Optional[Fp8Weight], M, N, K, need_wt: bool, need_xt: bool, dtype):
-    """``(y, xt, wt)``: the product and the transposed 8-bit forms that gradients read (buffers or None).  ``x2`` is the
-    input's rows or None where ``xq`` is its 8-bit form; ``w`` the weight or None where ``weight`` is."""
+    """``(y, xt, wt, wt_off)``: the product, and the transposed 8-bit forms that gradients read: ``xt`` at the start of
+    its buffer, ``wt`` at ``wt_off`` bytes of its (buffers or None).  ``x2`` is the input's rows or None where ``xq`` is
+    its 8-bit form; ``w`` the weight or None where ``weight`` is."""
     device = (x2 if x2 is not None else xq.buf).device
     y = _alloc_rows(M, N, dtype, device)
-    if not y.is_cuda:
+    if not y.is_cuda or not (M and N and K):
         xt = None
         if x2 is not None:
             xq, xt = _quantize(x2, E4M3, _ROWS | (_COLS if need_xt else 0))
         weight = weight or quantize_fp8_weight(w, transposed=need_wt)
         gemm_fp8_nt(xq, weight.w, y)
-        return y, xt.buf if xt else None, weight.wt.buf if need_wt else None
-    xt = _bytes(Fp8Tensor.nbytes_of(K, M), device) if need_xt else None
-    xb = xq.buf if xq is not None else _bytes(Fp8Tensor.nbytes_of(M, K), device)
+        return y, xt.buf if need_xt else None, weight.wt.buf if need_wt else None, 0
+    # workspaces: 8-bit x and w for this product; 8-bit x^T and w^T kept for the gradients
+    xq_n = 0 if xq is not None else _nbytes(M, K)
+    xt_n = _nbytes(K, M) if need_xt else 0
+    wq_n = wt_n = x_stride = w_stride = 0
+    x_fp32 = w_fp32 = False
     if weight is None:
         w = _check_matrix(w, "linear_fp8 weight")
-        wq = _bytes(Fp8Tensor.nbytes_of(N, K), device)
-        wt = _bytes(Fp8Tensor.nbytes_of(K, N), device) if need_wt else None
+        wq_n, wt_n = _nbytes(N, K), _nbytes(K, N) if need_wt else 0
+        w_ptr, w_stride, w_fp32 = w.data_ptr(), w.stride(0), w.dtype == torch.float32
     else:
-        w, wq, wt = None, weight.w.buf, weight.wt.buf if need_wt else None
-    if M and N and K:
-        with _On(y) as on:
-            nv.check(nv.cuda().cvb_fp8_linear_fwd(
-                nv.ptr(x2), x2 is not None and x2.dtype == torch.float32, x2.stride(0) if x2 is not None else 0,
-                nv.ptr(w), w is not None and w.dtype == torch.float32, w.stride(0) if w is not None else 0, M, N, K,
-                xb.data_ptr(), nv.ptr(xt), wq.data_ptr(), nv.ptr(wt) if weight is None else None,
-                y.data_ptr(), max(y.stride(0), N), _OUT[dtype], on.status, on.stream), "cvb_fp8_linear_fwd")
-        count_launch(1 + (x2 is not None) + (w is not None))
+        w_ptr = None
+    temp = _bytes(xq_n + wq_n, device) if xq_n + wq_n else None
+    keep = _bytes(xt_n + wt_n, device) if xt_n + wt_n else None
+    temp_ptr = temp.data_ptr() if temp is not None else 0
+    keep_ptr = keep.data_ptr() if keep is not None else 0
+    if x2 is not None:
+        x_ptr, x_stride, x_fp32 = x2.data_ptr(), x2.stride(0), x2.dtype == torch.float32
     else:
-        if weight is None:      # no rows: the gradient of the input is empty too, and reads nothing
-            weight = quantize_fp8_weight(w, transposed=need_wt)
-            wt = weight.wt.buf if need_wt else None
-        y.zero_()
-    return y, xt, wt
+        x_ptr = None
+    nv.check(nv.cuda().cvb_fp8_linear_fwd(
+        x_ptr, x_fp32, x_stride, w_ptr, w_fp32, w_stride, M, N, K, temp_ptr if xq_n else xq.buf.data_ptr(),
+        keep_ptr if xt_n else None, temp_ptr + xq_n if weight is None else weight.w.buf.data_ptr(),
+        keep_ptr + xt_n if wt_n else None, y.data_ptr(), max(y.stride(0), N), _OUT[dtype], _status(), _stream()),
+        "cvb_fp8_linear_fwd")
+    count_launch(1 + (x_ptr is not None) + (w_ptr is not None))
+    if need_wt and weight is not None:
+        return y, keep, weight.wt.buf, 0
+    return y, keep if need_xt else None, keep if need_wt else None, xt_n
 
 
-def _backward(dy, M, N, K, grad_dtype, wt, xt, w, dx_dtype, norm=None):
+def _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, dx_dtype, norm=None):
     """``(dx or None, dw or None)`` of ``y = x w^T``: dx where ``wt`` is given, dw where the parameter ``w`` is (added
     to its fp32 ``main_grad`` where it has one, and then None).  ``norm = (h, rstd, wn, w_offset)`` stands for ``xt``."""
-    dy2 = _check_matrix(dy.reshape(-1, N) if dy.numel() else dy.reshape(0, N), "linear_fp8 gradient")
+    if dy.is_cuda and dy.get_device() != _current_device():
+        with torch.cuda.device(dy.device):
+            return _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, dx_dtype, norm)
+    dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N) if dy.numel() else dy.reshape(0, N), "linear_fp8 gradient")
     dx = _alloc_rows(M, K, dx_dtype, dy.device) if wt is not None else None
     main = getattr(w, "main_grad", None) if w is not None else None
     target = None
-    if w is not None:
-        target = main.view(N, K) if main is not None else _alloc_rows(N, K, w.dtype, dy.device)
+    if main is not None:
+        if main.dtype != torch.float32 or not main.is_contiguous():
+            raise TypeError("linear_fp8: main_grad is a contiguous float32 tensor")
+        target = main.view(N, K)
+    elif w is not None:
+        target = _alloc_rows(N, K, w.dtype, dy.device)
     if not (M and N and K):
         if dx is not None:
             dx.zero_()
@@ -414,24 +453,28 @@ def _backward(dy, M, N, K, grad_dtype, wt, xt, w, dx_dtype, norm=None):
                 xt = _quantize(norm[0], E4M3, _COLS, *norm[1:])[1].buf
             gemm_fp8_nt(qdyt, Fp8Tensor(xt, K, M, E4M3), target, accumulate=main is not None)
     else:
-        if main is not None and (main.dtype != torch.float32 or not main.is_contiguous()):
-            raise TypeError("linear_fp8: main_grad is a contiguous float32 tensor")
-        dyq = _bytes(Fp8Tensor.nbytes_of(M, N), dy.device) if wt is not None else None
-        dyt = _bytes(Fp8Tensor.nbytes_of(N, M), dy.device) if w is not None else None
-        h = rstd = wn = None
+        dyq_n = _nbytes(M, N) if wt is not None else 0
+        dyt_n = _nbytes(N, M) if w is not None else 0
+        from_norm = norm is not None and w is not None
+        temp = _bytes(dyq_n + dyt_n + (_nbytes(K, M) if from_norm else 0), dy.device)
+        base = temp.data_ptr()
+        xt_ptr = base + dyq_n + dyt_n if from_norm else nv.ptr(xt)
+        h_ptr = rstd_ptr = wn_ptr = dx_ptr = dw_ptr = wt_ptr = None
+        h_stride = dx_stride = dw_stride = dw_kind = 0
         w_offset = 0.0
-        if norm is not None and w is not None:
+        if from_norm:
             h, rstd, wn, w_offset = norm
-            xt = _bytes(Fp8Tensor.nbytes_of(K, M), dy.device)
-        with _On(dy2) as on:
-            nv.check(nv.cuda().cvb_fp8_linear_bwd(
-                dy2.data_ptr(), dy2.dtype == torch.float32, dy2.stride(0), _FMT[grad_dtype], M, N, K, nv.ptr(dyq),
-                nv.ptr(dyt), nv.ptr(wt), nv.ptr(xt), nv.ptr(h), h.stride(0) if h is not None else 0, nv.ptr(rstd),
-                nv.ptr(wn), w_offset, nv.ptr(dx), max(dx.stride(0), K) if dx is not None else 0,
-                _OUT[dx_dtype], nv.ptr(target), max(target.stride(0), K) if target is not None else 0,
-                2 if main is not None else _OUT[w.dtype] if w is not None else 0, on.status, on.stream),
-                "cvb_fp8_linear_bwd")
-        count_launch(1 + (wt is not None) + (w is not None) + (h is not None))
+            h_ptr, h_stride, rstd_ptr, wn_ptr = h.data_ptr(), h.stride(0), rstd.data_ptr(), wn.data_ptr()
+        if wt is not None:
+            wt_ptr, dx_ptr, dx_stride = wt.data_ptr() + wt_off, dx.data_ptr(), max(dx.stride(0), K)
+        if w is not None:
+            dw_ptr, dw_stride = target.data_ptr(), max(target.stride(0), K)
+            dw_kind = 2 if main is not None else _OUT[w.dtype]
+        nv.check(nv.cuda().cvb_fp8_linear_bwd(
+            dy2.data_ptr(), dy2.dtype == torch.float32, dy2.stride(0), _FMT[grad_dtype], M, N, K, base, base + dyq_n,
+            wt_ptr, xt_ptr, h_ptr, h_stride, rstd_ptr, wn_ptr, w_offset, dx_ptr, dx_stride, _OUT[dx_dtype], dw_ptr,
+            dw_stride, dw_kind, _status(), _stream()), "cvb_fp8_linear_bwd")
+        count_launch(1 + (wt is not None) + (w is not None) + from_norm)
     return dx, (target if main is None else None)
 
 
@@ -443,22 +486,40 @@ class _LinearFp8(torch.autograd.Function):
             raise ValueError("linear_fp8: the gradient of the input needs the transposed 8-bit weight")
         x2 = _rows2d(x)
         (M, K), N = x2.shape, w.shape[0]
-        y, xt, wt = _forward(x2, None, w, weight, M, N, K, need_dx, need_dw, x.dtype)
+        y, xt, wt, wt_off = _forward(x2, None, w, weight, M, N, K, need_dx, need_dw, x.dtype)
         # what the gradients read: x^T and w^T in 8 bits, half of what the bf16 layer keeps of x
         ctx.save_for_backward(w if need_dw else None, xt, wt)
-        ctx.cfg = (x.shape, x.dtype, M, N, K, grad_dtype)
+        ctx.cfg = (x.shape, x.dtype, M, N, K, grad_dtype, wt_off)
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         w, xt, wt = ctx.saved_tensors
-        shape, xdtype, M, N, K, grad_dtype = ctx.cfg
-        dx, dw = _backward(dy, M, N, K, grad_dtype, wt, xt, w, xdtype)
+        shape, xdtype, M, N, K, grad_dtype, wt_off = ctx.cfg
+        dx, dw = _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, xdtype)
         if dx is not None and len(shape) != 2:
             dx = dx.reshape(shape)
         return dx, dw, None, None
 
 
+class _Shape:
+    """Stands for a frozen weight in the autograd functions: only its shape is asked for."""
+
+    def __init__(self, shape):
+        self.shape = shape
+
+
+def _needs_grad(*tensors) -> bool:
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            return True
+    return False
+
+
+@_on_device
 def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dtype = E4M3) -> torch.Tensor:
     """``x [..., K] @ w [N, K].T`` with both operands rounded to 8 bits.
 
@@ -467,35 +528,29 @@ def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dt
     gradients, an ``Fp8Tensor`` (from ``add_rmsnorm_fp8``) with a matrix as the result.  Gradients of ``y`` are rounded
     to ``grad_dtype``; the weight's gradient goes to ``w.main_grad`` when the parameter has one."""
     what = "linear_fp8"
-    if weight is not None and isinstance(w, Fp8Weight):
-        raise ValueError(f"{what}: the 8-bit weight is given twice")
-    frozen = w if isinstance(w, Fp8Weight) else None
-    N = w.shape[0] if len(w.shape) else 0
+    kept = w if isinstance(w, Fp8Weight) else weight
     if isinstance(x, Fp8Tensor):
         _check_linear(x.cols, x.device, w, weight, grad_dtype, what)
         if x.dtype != E4M3:
             raise TypeError(f"{what}: inputs are torch.float8_e4m3fn, got {x.dtype}")
-        with torch.no_grad():
-            return _forward(None, x, w, frozen or weight, x.rows, N, x.cols, False, False, torch.bfloat16)[0]
-    if x.dim() < 1:
+        if _needs_grad(w):
+            raise RuntimeError(f"{what}: an 8-bit input carries no gradient: call it under torch.no_grad()")
+        return _forward(None, x, w, kept, x.rows, w.shape[0], x.cols, False, False, torch.bfloat16)[0]
+    shape = x.shape
+    if not shape:
         raise ValueError(f"{what}: x has no dimensions")
     if x.dtype != torch.bfloat16 and (x.is_cuda or x.dtype != torch.float32):
         raise TypeError(f"{what}: bfloat16 is wanted, got {x.dtype}")
-    _check_linear(x.shape[-1], x.device, w, weight, grad_dtype, what)
-    if not (torch.is_grad_enabled() and (x.requires_grad or (frozen is None and w.requires_grad))):
+    K = shape[-1]
+    _check_linear(K, x.device, w, weight, grad_dtype, what)
+    if not _needs_grad(x, w):
         x2 = _rows2d(x)
-        y = _forward(x2, None, w, frozen or weight, x2.shape[0], N, x2.shape[1], False, False, x.dtype)[0]
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
-    if frozen is not None:
-        return _LinearFp8.apply(x, _Shape(w.shape), frozen, grad_dtype)
-    return _LinearFp8.apply(x, w, weight, grad_dtype)
-
-
-class _Shape:
-    """Stands for a frozen weight in the autograd function: only its shape is asked for."""
-
-    def __init__(self, shape):
-        self.shape = shape
+        N = w.shape[0]
+        y = _forward(x2, None, w, kept, x2.shape[0], N, K, False, False, x.dtype)[0]
+        return y if len(shape) == 2 else y.reshape(*shape[:-1], N)
+    if kept is w:
+        w = _Shape(w.shape)
+    return _LinearFp8.apply(x, w, kept, grad_dtype)
 
 
 class _NormLinearFp8(torch.autograd.Function):
@@ -510,29 +565,34 @@ class _NormLinearFp8(torch.autograd.Function):
         (M, K), N = x2.shape, w.shape[0]
         q, h, rstd = _norm_forward(x2, _rows2d(resid) if resid is not None else None, wn, eps, w_offset, E4M3,
                                    need_dn or need_dw)
-        y, _, wt = _forward(None, q, w, weight, M, N, K, need_dn, False, x.dtype)
+        y, _, wt, wt_off = _forward(None, q, w, weight, M, N, K, need_dn, False, x.dtype)
         ctx.save_for_backward(h, rstd, wn, w if need_dw else None, wt)
-        ctx.cfg = (x.shape, M, N, K, w_offset, grad_dtype)
+        ctx.cfg = (x.shape, M, N, K, w_offset, grad_dtype, wt_off)
         if x.dim() != 2:
-            y = y.reshape(*x.shape[:-1], N)
-        return y if resid is None else (y, h.view(x.shape))
+            y, h = y.reshape(*x.shape[:-1], N), h.view(x.shape)
+        return y if resid is None else (y, h)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh=None):
         h, rstd, wn, w, wt = ctx.saved_tensors
-        shape, M, N, K, w_offset, grad_dtype = ctx.cfg
+        shape, M, N, K, w_offset, grad_dtype, wt_off = ctx.cfg
         need_x, need_r, need_wn = ctx.needs_input_grad[:3]
         # The norm's result is formed again from h and rstd while its transpose is quantised: it is never stored.  Its
         # gradient stays fp32 between the product and the norm's backward.
-        dn, dw = _backward(dy, M, N, K, grad_dtype, wt, None, w, torch.float32, (h, rstd, wn.contiguous(), w_offset))
+        dn, dw = _backward(dy, M, N, K, grad_dtype, wt, wt_off, None, w, torch.float32, (h, rstd, wn.contiguous(), w_offset))
         dx = dwn = None
         if dn is not None:
             dx, dwn = _norm_backward(dn, h, wn, rstd, dh, w_offset, need_wn)
-            dx = dx.view(shape)
+            if len(shape) != 2:
+                dx = dx.view(shape)
         return (dx if need_x else None), (dx if need_r else None), dwn, dw, None, None, None, None
 
 
 def _norm_backward(dn, h, wn, rstd, dh, w_offset, need_dwn):
+    if h.is_cuda and h.get_device() != _current_device():
+        with torch.cuda.device(h.device):
+            return _norm_backward(dn, h, wn, rstd, dh, w_offset, need_dwn)
     R, D = h.shape
     main = getattr(wn, "main_grad", None) if need_dwn else None
     dh2 = _rows2d(dh) if dh is not None else None
@@ -546,39 +606,38 @@ def _norm_backward(dn, h, wn, rstd, dh, w_offset, need_dwn):
         if main is not None:
             main.view(D).add_(dwn)
         return dx.to(h.dtype), dwn.to(wn.dtype) if need_dwn and main is None else None
+    if main is not None and (main.dtype != torch.float32 or not main.is_contiguous()):
+        raise TypeError("add_rmsnorm_linear_fp8: main_grad is a contiguous float32 tensor")
     lib = nv.cuda()
     dx = torch.empty((R, D), dtype=h.dtype, device=h.device)
     dwn = torch.empty(D, dtype=wn.dtype, device=h.device) if need_dwn and main is None else None
     if R == 0:
         return dx, dwn.zero_() if dwn is not None else None
     part = torch.empty((min(R, lib.cvb_fp8_norm_bwd_parts()), D), dtype=torch.float32, device=h.device) if need_dwn else None
-    if main is not None and (main.dtype != torch.float32 or not main.is_contiguous()):
-        raise TypeError("add_rmsnorm_linear_fp8: main_grad is a contiguous float32 tensor")
     wc = wn.contiguous()
-    with _On(h) as on:
-        nv.check(lib.cvb_fp8_norm_bwd(dn.data_ptr(), dn.stride(0), h.data_ptr(), h.stride(0), wc.data_ptr(),
-                                      rstd.data_ptr(), nv.ptr(dh2), dh2.stride(0) if dh2 is not None else 0,
-                                      dx.data_ptr(), nv.ptr(part), nv.ptr(main), nv.ptr(dwn), R, D, w_offset,
-                                      on.stream), "cvb_fp8_norm_bwd")
+    nv.check(lib.cvb_fp8_norm_bwd(dn.data_ptr(), dn.stride(0), h.data_ptr(), h.stride(0), wc.data_ptr(), rstd.data_ptr(),
+                                  nv.ptr(dh2), dh2.stride(0) if dh2 is not None else 0, dx.data_ptr(), nv.ptr(part),
+                                  nv.ptr(main), nv.ptr(dwn), R, D, w_offset, _stream()), "cvb_fp8_norm_bwd")
     count_launch(2 if need_dwn else 1)
     return dx, dwn
 
 
+@_on_device
 def add_rmsnorm_linear_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], norm_w: torch.Tensor, w, eps: float = 1e-6,
                            w_offset: float = 1.0, *, weight: Optional[Fp8Weight] = None,
                            grad_dtype: torch.dtype = E4M3) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(rmsnorm(x + resid) @ w.T, x + resid)``; ``resid`` may be None.  The norm's result exists in 8 bits only: the
     backward pass forms it again from ``x + resid``.  ``w``, ``weight`` and ``grad_dtype`` as in ``linear_fp8``."""
     what = "add_rmsnorm_linear_fp8"
-    if weight is not None and isinstance(w, Fp8Weight):
-        raise ValueError(f"{what}: the 8-bit weight is given twice")
     _check_norm(x, resid, norm_w, what)
-    _check_linear(x.shape[-1], x.device, w, weight, grad_dtype, what)
-    if isinstance(w, Fp8Weight):
-        w, weight = _Shape(w.shape), w
-    if not (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, resid, norm_w, w))):
-        q, h = add_rmsnorm_fp8(x, resid, norm_w, eps, w_offset)
-        y = _forward(None, q, w, weight, q.rows, w.shape[0], q.cols, False, False, x.dtype)[0]
-        return (y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])), h
-    out = _NormLinearFp8.apply(x, resid, norm_w, w, weight, eps, w_offset, grad_dtype)
+    K, N = x.shape[-1], w.shape[0] if len(w.shape) else 0
+    _check_linear(K, x.device, w, weight, grad_dtype, what)
+    kept = w if isinstance(w, Fp8Weight) else weight
+    if not _needs_grad(x, resid, norm_w, w):
+        q, h, _ = _norm_forward(_rows2d(x), _rows2d(resid) if resid is not None else None, norm_w, eps, w_offset, E4M3, False)
+        y = _forward(None, q, w, kept, q.rows, N, K, False, False, x.dtype)[0]
+        if x.dim() != 2:
+            y, h = y.reshape(*x.shape[:-1], N), h.view(x.shape)
+        return y, x if resid is None else h
+    out = _NormLinearFp8.apply(x, resid, norm_w, _Shape(w.shape) if kept is w else w, kept, eps, w_offset, grad_dtype)
     return (out, x) if resid is None else out

@@ -132,11 +132,14 @@ class PolicyRolloutWorker(RolloutWorker):
 
 
 class CachedQwenRolloutWorker(RolloutWorker):
-    """Cached decode over a ``Qwen35Model`` (see ``cverl_b200.models.decode``)."""
+    """Cached decode over a ``Qwen35Model`` (see ``cverl_b200.models.decode``).  With ``fp8`` the decode steps read the
+    projections' weights in 8 bits, converted from the parameters at the start of every ``generate``; the log-probs
+    are then those of the 8-bit policy."""
 
-    def __init__(self, model, pad_id: int = 0):
+    def __init__(self, model, pad_id: int = 0, fp8: bool = False):
         self.model = model
         self.pad_id = pad_id
+        self.fp8 = fp8
 
     def actor_parameters(self) -> List[ParameterView]:
         return [ParameterView(n, t) for n, t in self.model.flat.named_tensors()]
@@ -155,6 +158,9 @@ class CachedQwenRolloutWorker(RolloutWorker):
         gen = _generator(dev, config.seed)
         state, logits = prefill(self.model, prompts, max_len=prompts.shape[1] + N)
         graphed = None
+        if self.fp8:
+            from ..models.decode import fp8_decode_weights
+            state.fp8 = fp8_decode_weights(self.model)
         if prompts.is_cuda and N > 4:
             from ..models.decode import GraphedDecoder, native_decode_supported
             if native_decode_supported(self.model):

@@ -154,6 +154,20 @@ def test_no_tokens_give_zero_gradients():
     assert y.shape == (0, 32) and x.grad.shape == (0, 64) and w.grad.shape == (32, 64) and not w.grad.any()
 
 
+def test_what_has_no_gradient_says_so():
+    x, w, wn = torch.ones(4, 8, requires_grad=True), torch.ones(3, 8, requires_grad=True), torch.ones(8)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.add_rmsnorm_fp8(x, None, wn)
+    with torch.no_grad():
+        q, _ = ops.add_rmsnorm_fp8(x, None, wn)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.linear_fp8(q, w)
+    assert not ops.linear_fp8(q, ops.quantize_fp8_weight(w)).requires_grad
+    g, = torch.autograd.grad(ops.linear_fp8(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        g.sum().backward()
+
+
 def test_refusals():
     a, b = ops.quantize_fp8(torch.ones(4, 8)), ops.quantize_fp8(torch.ones(3, 9))
     good = ops.quantize_fp8(torch.ones(3, 8))
