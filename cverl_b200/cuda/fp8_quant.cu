@@ -520,10 +520,36 @@ __device__ __forceinline__ void load_f32x8(const float* p, int n, float (&v)[8])
   }
 }
 
-// A thread holds one vector of a row up to 8192 elements (two beyond): few registers, so that an SM has 1024 threads
-// with 64 bytes of loads each in flight.
+// The next row's vectors are loaded before this row's are used: a CTA waits for its row's sum in between, and without
+// them the SM had loads in flight for half of the time ([40960, 1024]: 93 us, 65 % of HBM).  TPR = 1024 has no registers
+// for that.
+template <int TPR, int NV>
+struct NormBwd {
+  static constexpr bool AHEAD = TPR < 1024;
+  static constexpr int MIN_CTAS = TPR >= 512 ? 1 : NV == 2 ? 2 : 3;
+};
+template <int NV>
+struct NormBwdRow {
+  uint4 h[NV], dh[NV];
+  float dn[NV][8];
+  float rstd;
+};
+
 template <int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(RowBlock<TPR>::THREADS, 1024 / RowBlock<TPR>::THREADS)
+__device__ __forceinline__ void norm_bwd_load(const NormBwdArgs& p, long long row, int t, NormBwdRow<NV>& r) {
+  const bool ok = row < p.rows;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * 8, n = ok ? max(0, min(8, p.D - c)) : 0;
+    r.h[i] = load_raw8<VEC>(p.h + row * p.h_stride + c, n);
+    load_f32x8<VEC>(p.dn + row * p.dn_stride + c, n, r.dn[i]);
+    r.dh[i] = load_raw8<VEC>(p.dh + row * p.dh_stride + c, p.dh != nullptr ? n : 0);
+  }
+  r.rstd = ok ? p.rstd[row] : 0.f;
+}
+
+template <int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(RowBlock<TPR>::THREADS, NormBwd<TPR, NV>::MIN_CTAS)
 fp8_norm_bwd_kernel(const NormBwdArgs p) {
   constexpr int ROWS = RowBlock<TPR>::ROWS;
   __shared__ float s_part[2][ROWS][TPR / 32];
@@ -534,34 +560,30 @@ fp8_norm_bwd_kernel(const NormBwdArgs p) {
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+  uint4 wr[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) wr[i] = load_raw8<VEC>(p.w + (i * TPR + t) * 8, max(0, min(8, p.D - (i * TPR + t) * 8)));
   int flip = 0;
+  const long long step = static_cast<long long>(gridDim.x) * ROWS;
+  NormBwdRow<NV> cur, next;
+  norm_bwd_load<TPR, NV, VEC>(p, static_cast<long long>(blockIdx.x) * ROWS + sub, t, cur);
   // the trip count is the block's, not the row group's: TPR > 32 synchronises inside
-  for (long long r0 = static_cast<long long>(blockIdx.x) * ROWS; r0 < p.rows; r0 += static_cast<long long>(gridDim.x) * ROWS) {
+  for (long long r0 = static_cast<long long>(blockIdx.x) * ROWS; r0 < p.rows; r0 += step) {
     const long long row = r0 + sub;
     const bool ok = row < p.rows;
-    uint4 hr[NV], dr[NV];
-    float gn[NV][8];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * 8, n = ok ? max(0, min(8, p.D - c)) : 0;
-      hr[i] = load_raw8<VEC>(p.h + row * p.h_stride + c, n);
-      load_f32x8<VEC>(p.dn + row * p.dn_stride + c, n, gn[i]);
-      dr[i] = load_raw8<VEC>(p.dh + row * p.dh_stride + c, p.dh != nullptr ? n : 0);
-    }
-    const float rstd = ok ? p.rstd[row] : 0.f;
+    if (NormBwd<TPR, NV>::AHEAD) norm_bwd_load<TPR, NV, VEC>(p, row + step, t, next);
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * 8;
       float xh[8], w8[8];
-      widen8(hr[i], xh);
-      widen8(load_raw8<VEC>(p.w + c, max(0, min(8, p.D - c))), w8);
+      widen8(cur.h[i], xh);
+      widen8(wr[i], w8);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = xh[j] * rstd;
-        acc[i][j] += gn[i][j] * x;
-        gn[i][j] *= p.w_offset + w8[j];
-        dot += gn[i][j] * x;             // both are zero outside the row
+        const float x = xh[j] * cur.rstd;
+        acc[i][j] += cur.dn[i][j] * x;
+        cur.dn[i][j] *= p.w_offset + w8[j];
+        dot += cur.dn[i][j] * x;             // both are zero outside the row
       }
     }
     dot = warp_sum(dot);
@@ -573,17 +595,19 @@ fp8_norm_bwd_kernel(const NormBwdArgs p) {
       for (int i = 0; i < TPR / 32; ++i) dot += s_part[flip][sub][i];
       flip ^= 1;
     }
-    dot *= rstd / p.D;
+    dot *= cur.rstd / p.D;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * 8, n = ok ? max(0, min(8, p.D - c)) : 0;
       float xh[8], d8[8];
-      widen8(hr[i], xh);
-      widen8(dr[i], d8);
+      widen8(cur.h[i], xh);
+      widen8(cur.dh[i], d8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d8[j] += rstd * (gn[i][j] - xh[j] * dot);
+      for (int j = 0; j < 8; ++j) d8[j] += cur.rstd * (cur.dn[i][j] - xh[j] * dot);
       store_raw8<VEC>(p.dx + row * p.D + c, narrow8(d8), n);
     }
+    if (NormBwd<TPR, NV>::AHEAD) cur = next;
+    else norm_bwd_load<TPR, NV, VEC>(p, row + step, t, cur);
   }
   if (p.part == nullptr) return;
   float* part = p.part + static_cast<long long>(blockIdx.x) * p.D;
@@ -625,13 +649,13 @@ fp8_norm_dw_kernel(const float* __restrict__ part, int parts, int D, float* __re
   }
 }
 
-constexpr int NORM_BWD_MAX_PARTS = 592;   // 148 SMs with four CTAs each
+constexpr int NORM_BWD_MAX_PARTS = 444;   // 148 SMs with three CTAs each
 
 template <int TPR, int NV>
 static int norm_bwd_launch(const NormBwdArgs& p, cudaStream_t s) {
   constexpr int THREADS = RowBlock<TPR>::THREADS;
   const long long want = (p.rows + THREADS / TPR - 1) / (THREADS / TPR);
-  const int resident = 148 * (1024 / THREADS);
+  const int resident = 148 * NormBwd<TPR, NV>::MIN_CTAS;
   const int grid = static_cast<int>(want < resident ? want : resident);
   if (p.vec) fp8_norm_bwd_kernel<TPR, NV, true><<<grid, THREADS, 0, s>>>(p);
   else fp8_norm_bwd_kernel<TPR, NV, false><<<grid, THREADS, 0, s>>>(p);
@@ -744,8 +768,8 @@ extern "C" int cvb_fp8_norm_bwd(const float* dn, long long dn_stride, const void
   else if (D <= 512) grid = norm_bwd_launch<64, 1>(p, s);
   else if (D <= 1024) grid = norm_bwd_launch<128, 1>(p, s);
   else if (D <= 2048) grid = norm_bwd_launch<256, 1>(p, s);
-  else if (D <= 4096) grid = norm_bwd_launch<512, 1>(p, s);
-  else if (D <= 8192) grid = norm_bwd_launch<1024, 1>(p, s);
+  else if (D <= 4096) grid = norm_bwd_launch<256, 2>(p, s);
+  else if (D <= 8192) grid = norm_bwd_launch<512, 2>(p, s);
   else grid = norm_bwd_launch<1024, 2>(p, s);
   if (p.part != nullptr)
     fp8_norm_dw_kernel<<<(D + 31) / 32, 1024, 0, s>>>(part, grid, D, dw_acc, static_cast<__nv_bfloat16*>(dw));
