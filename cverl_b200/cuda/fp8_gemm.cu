@@ -9,6 +9,7 @@
 // stays in TMEM over all of K.
 #include "fp8_common.cuh"
 #include "gemm_tcgen05.h"
+#include <atomic>
 
 namespace cvb {
 
@@ -648,6 +649,20 @@ struct Fp8Operands {
   int M, N, K;
 };
 
+// The shared-memory opt-in of a kernel, made once per device: a call costs as much as an eighth of a small product.
+template <auto KERN>
+static int opt_in_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};       // one bit a device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return 0;
+  e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return static_cast<int>(e);
+}
+
 static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, unsigned grid, int threads, int cluster, size_t smem,
                                          cudaStream_t stream) {
   at->id = cudaLaunchAttributeClusterDimension;
@@ -673,8 +688,7 @@ static int launch_small(const Fp8Operands& o, Fp8GemmParams p, cudaStream_t stre
       encode_tensor_map(&tb, o.b, 1, o.K, o.N, 0, o.ldb, 0, 128, 128))
     return -10;
   auto kern = fp8_gemm_small_kernel<TN>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
-  if (e != cudaSuccess) return static_cast<int>(e);
+  if (const int e = opt_in_smem<fp8_gemm_small_kernel<TN>>(Cfg::SMEM_BYTES)) return e;
   p.m_tiles = (p.M + TN - 1) / TN;
   p.n_tiles = (p.N + 127) / 128;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
@@ -703,7 +717,7 @@ static int fp8_pair_capacity() {
   static const int cached = [] {
     using Cfg = F8PairCfg<BN>;
     auto kern = fp8_gemm_pair_kernel<BN, false>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess) return 0;
+    if (opt_in_smem<fp8_gemm_pair_kernel<BN, false>>(Cfg::SMEM_BYTES)) return 0;
     cudaLaunchAttribute at;
     cudaLaunchConfig_t cfg = cluster_config(&at, 2 * 148, Cfg::THREADS, 2, Cfg::SMEM_BYTES, nullptr);
     int n = 0;
@@ -728,8 +742,7 @@ static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int split, cudaStr
       encode_tensor_map(&sb, p.b_sf, TMAP_U32_PLAIN, 128, rb, 0, 512, 0, 128, 1))
     return -10;
   auto kern = fp8_gemm_pair_kernel<BN, SPLIT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
-  if (e != cudaSuccess) return static_cast<int>(e);
+  if (const int e = opt_in_smem<fp8_gemm_pair_kernel<BN, SPLIT>>(Cfg::SMEM_BYTES)) return e;
   p.m_tiles = (p.M + 255) / 256;
   p.n_tiles = (p.N + BN - 1) / BN;
   if (static_cast<long long>(p.m_tiles) * p.n_tiles > 0x0fffffffll || ra > 0x7fffffffull || rb > 0x7fffffffull) return -11;

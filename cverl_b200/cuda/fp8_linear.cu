@@ -11,6 +11,12 @@ int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, 
 int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                  long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int* status,
                  void* stream);
+int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride, const void* w, void* h,
+                        void* q, void* sf, long long q_ld, float* rstd, long long rows, int D, int fmt, float eps,
+                        float w_offset, void* stream);
+int cvb_fp8_norm_bwd(const float* dn, long long dn_stride, const void* h, long long h_stride, const void* w,
+                     const float* rstd, const void* dh, long long dh_stride, void* dx, float* part, float* dw_acc,
+                     void* dw, long long rows, int D, float w_offset, void* stream);
 }
 
 namespace {
@@ -50,6 +56,19 @@ extern "C" int cvb_fp8_linear_fwd(const void* x, int x_fp32, long long x_stride,
   return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, status, stream);
 }
 
+// h = x + resid, y = norm(h) w^T; without resid, h is null and the norm reads x.
+extern "C" int cvb_fp8_norm_linear_fwd(const void* x, long long x_stride, const void* resid, long long r_stride,
+                                       const void* wn, void* h, float* rstd, float eps, float w_offset, const void* w,
+                                       int w_fp32, long long w_stride, int M, int N, int K, void* xq, void* wq, void* wt,
+                                       void* y, long long ldy, int out_kind, int* status, void* stream) {
+  const Mat8 mxq(xq, M, K);
+  const int rc = cvb_fp8_add_rmsnorm(x, x_stride, resid, r_stride, wn, h, mxq.codes, mxq.sf, mxq.ld, rstd, M, K, E4M3,
+                                     eps, w_offset, stream);
+  if (rc) return rc;
+  return cvb_fp8_linear_fwd(nullptr, 0, 0, w, w_fp32, w_stride, M, N, K, xq, nullptr, wq, wt, y, ldy, out_kind, status,
+                            stream);
+}
+
 // dx [M, K] = dy w (where wt is given) and dw [N, K] (+)= dy^T x (where dw is given).  `dyq` and `dyt` are workspaces
 // for the two forms of dy.  h given: x is h * rstd * (w_offset + wn), formed into the workspace `xt`.
 extern "C" int cvb_fp8_linear_bwd(const void* dy, int dy_fp32, long long dy_stride, int grad_fmt, int M, int N, int K,
@@ -66,4 +85,20 @@ extern "C" int cvb_fp8_linear_bwd(const void* dy, int dy_fp32, long long dy_stri
                                   rstd, wn, w_offset, stream)))
     return rc;
   return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, status, stream);
+}
+
+// The gradients of the norm + linear layer.  wt given: `dn` (fp32 [M, lddn], a workspace) takes the gradient of the
+// norm's result, dx that of x + resid (with dh added), and dwn (or dwn_acc, +=) that of the norm's weight, by way of
+// the workspace `part`.  dw given: as above, with the workspace `xt`.
+extern "C" int cvb_fp8_norm_linear_bwd(const void* dy, int dy_fp32, long long dy_stride, int grad_fmt, int M, int N,
+                                       int K, void* dyq, void* dyt, void* wt, void* xt, const void* h,
+                                       long long h_stride, const float* rstd, const void* wn, float w_offset, float* dn,
+                                       long long lddn, void* dw, long long lddw, int dw_kind, const void* dh,
+                                       long long dh_stride, void* dx, float* part, float* dwn_acc, void* dwn, int* status,
+                                       void* stream) {
+  constexpr int F32 = 1;
+  const int rc = cvb_fp8_linear_bwd(dy, dy_fp32, dy_stride, grad_fmt, M, N, K, dyq, dyt, wt, xt, h, h_stride, rstd, wn,
+                                    w_offset, dn, lddn, F32, dw, lddw, dw_kind, status, stream);
+  if (rc || !wt) return rc;
+  return cvb_fp8_norm_bwd(dn, lddn, h, h_stride, wn, rstd, dh, dh_stride, dx, part, dwn_acc, dwn, M, K, w_offset, stream);
 }

@@ -134,7 +134,9 @@ class Fp8Weight:
 
     __slots__ = ("w", "wt", "shape", "device")
 
-    def __init__(self, w: Fp8Tensor, wt: Optional[Fp8Tensor]):
+    def __init__(self, w: Fp8Tensor, wt: Optional[Fp8Tensor] = None):
+        if w.dtype != E4M3 or (wt is not None and (wt.dtype != E4M3 or wt.shape != w.shape[::-1] or wt.device != w.device)):
+            raise ValueError("Fp8Weight: a weight and its transpose in torch.float8_e4m3fn on one device are wanted")
         self.w, self.wt = w, wt
         self.shape, self.device = w.shape, w.device
 
@@ -363,7 +365,7 @@ def add_rmsnorm_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], w: torch.Ten
 # ----------------------------------------------------------------------------
 # linear layers
 # ----------------------------------------------------------------------------
-def _check_linear(K: int, device, w, weight: Optional[Fp8Weight], grad_dtype, what: str) -> None:
+def _check_linear(rows: int, K: int, device, w, weight: Optional[Fp8Weight], grad_dtype, what: str) -> None:
     if grad_dtype not in _FMT:
         _check_dtype(grad_dtype, what)
     shape = w.shape
@@ -371,6 +373,8 @@ def _check_linear(K: int, device, w, weight: Optional[Fp8Weight], grad_dtype, wh
         raise ValueError(f"{what}: a weight [N, {K}] is wanted, got {tuple(shape)}")
     if w.device != device:
         raise ValueError(f"{what}: the weight is on {w.device}, the input on {device}")
+    if shape[0] > MAX_EXTENT or K > MAX_EXTENT or rows > MAX_EXTENT:
+        raise ValueError(f"{what}: at most {MAX_EXTENT} rows and columns")
     if not isinstance(w, Fp8Weight):
         if w.dtype not in _OUT:
             raise TypeError(f"{what}: the weight is bfloat16 or float32, not {w.dtype}")
@@ -425,24 +429,17 @@ def _forward(x2, xq, w, weight: Optional[Fp8Weight], M, N, K, need_wt: bool, nee
 
 def _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, dx_dtype, norm=None):
     """``(dx or None, dw or None)`` of ``y = x w^T``: dx where ``wt`` is given, dw where the parameter ``w`` is (added
-    to its fp32 ``main_grad`` where it has one, and then None).  ``norm = (h, rstd, wn, w_offset)`` stands for ``xt``."""
+    to its fp32 ``main_grad`` where it has one, and then None).  ``norm = (h, rstd, wn, w_offset)`` stands for ``xt`` on the CPU."""
     if dy.is_cuda and dy.get_device() != _current_device():
         with torch.cuda.device(dy.device):
             return _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, dx_dtype, norm)
     dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N) if dy.numel() else dy.reshape(0, N), "linear_fp8 gradient")
     dx = _alloc_rows(M, K, dx_dtype, dy.device) if wt is not None else None
-    main = getattr(w, "main_grad", None) if w is not None else None
-    target = None
-    if main is not None:
-        if main.dtype != torch.float32 or not main.is_contiguous():
-            raise TypeError("linear_fp8: main_grad is a contiguous float32 tensor")
-        target = main.view(N, K)
-    elif w is not None:
-        target = _alloc_rows(N, K, w.dtype, dy.device)
+    target, is_main = _grad_target(w, N, K, "linear_fp8") if w is not None else (None, False)
     if not (M and N and K):
         if dx is not None:
             dx.zero_()
-        if target is not None and main is None:
+        if target is not None and not is_main:
             target.zero_()
     elif not dy2.is_cuda:
         qdy, qdyt = _quantize(dy2, grad_dtype, (_ROWS if wt is not None else 0) | (_COLS if w is not None else 0))
@@ -451,31 +448,24 @@ def _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, dx_dtype, norm=None):
         if target is not None:
             if norm is not None:
                 xt = _quantize(norm[0], E4M3, _COLS, *norm[1:])[1].buf
-            gemm_fp8_nt(qdyt, Fp8Tensor(xt, K, M, E4M3), target, accumulate=main is not None)
+            gemm_fp8_nt(qdyt, Fp8Tensor(xt, K, M, E4M3), target, accumulate=is_main)
     else:
         dyq_n = _nbytes(M, N) if wt is not None else 0
         dyt_n = _nbytes(N, M) if w is not None else 0
-        from_norm = norm is not None and w is not None
-        temp = _bytes(dyq_n + dyt_n + (_nbytes(K, M) if from_norm else 0), dy.device)
+        temp = _bytes(dyq_n + dyt_n, dy.device)
         base = temp.data_ptr()
-        xt_ptr = base + dyq_n + dyt_n if from_norm else nv.ptr(xt)
-        h_ptr = rstd_ptr = wn_ptr = dx_ptr = dw_ptr = wt_ptr = None
-        h_stride = dx_stride = dw_stride = dw_kind = 0
-        w_offset = 0.0
-        if from_norm:
-            h, rstd, wn, w_offset = norm
-            h_ptr, h_stride, rstd_ptr, wn_ptr = h.data_ptr(), h.stride(0), rstd.data_ptr(), wn.data_ptr()
+        dx_ptr = dw_ptr = wt_ptr = None
+        dx_stride = dw_stride = dw_kind = 0
         if wt is not None:
             wt_ptr, dx_ptr, dx_stride = wt.data_ptr() + wt_off, dx.data_ptr(), max(dx.stride(0), K)
         if w is not None:
-            dw_ptr, dw_stride = target.data_ptr(), max(target.stride(0), K)
-            dw_kind = 2 if main is not None else _OUT[w.dtype]
+            dw_ptr, dw_stride, dw_kind = target.data_ptr(), max(target.stride(0), K), 2 if is_main else _OUT[w.dtype]
         nv.check(nv.cuda().cvb_fp8_linear_bwd(
             dy2.data_ptr(), dy2.dtype == torch.float32, dy2.stride(0), _FMT[grad_dtype], M, N, K, base, base + dyq_n,
-            wt_ptr, xt_ptr, h_ptr, h_stride, rstd_ptr, wn_ptr, w_offset, dx_ptr, dx_stride, _OUT[dx_dtype], dw_ptr,
+            wt_ptr, nv.ptr(xt), None, 0, None, None, 0.0, dx_ptr, dx_stride, _OUT[dx_dtype], dw_ptr,
             dw_stride, dw_kind, _status(), _stream()), "cvb_fp8_linear_bwd")
-        count_launch(1 + (wt is not None) + (w is not None) + from_norm)
-    return dx, (target if main is None else None)
+        count_launch(1 + (wt is not None) + (w is not None))
+    return dx, (None if is_main else target)
 
 
 class _LinearFp8(torch.autograd.Function):
@@ -530,7 +520,7 @@ def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dt
     what = "linear_fp8"
     kept = w if isinstance(w, Fp8Weight) else weight
     if isinstance(x, Fp8Tensor):
-        _check_linear(x.cols, x.device, w, weight, grad_dtype, what)
+        _check_linear(x.rows, x.cols, x.device, w, weight, grad_dtype, what)
         if x.dtype != E4M3:
             raise TypeError(f"{what}: inputs are torch.float8_e4m3fn, got {x.dtype}")
         if _needs_grad(w):
@@ -542,7 +532,7 @@ def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dt
     if x.dtype != torch.bfloat16 and (x.is_cuda or x.dtype != torch.float32):
         raise TypeError(f"{what}: bfloat16 is wanted, got {x.dtype}")
     K = shape[-1]
-    _check_linear(K, x.device, w, weight, grad_dtype, what)
+    _check_linear(x.numel() // K if K else 0, K, x.device, w, weight, grad_dtype, what)
     if not _needs_grad(x, w):
         x2 = _rows2d(x)
         N = w.shape[0]
@@ -553,6 +543,42 @@ def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dt
     return _LinearFp8.apply(x, w, kept, grad_dtype)
 
 
+def _norm_linear_forward(x2, r2, wn, w, weight, eps, w_offset, need_wt: bool, need_rstd: bool):
+    """``(y, h, rstd, wt, wt_off)`` of matrices; ``h`` is ``x2`` without a residual, ``rstd`` None where not asked for."""
+    (M, K), N = x2.shape, w.shape[0]
+    if not x2.is_cuda or not (M and N and K):
+        q, h, rstd = _norm_forward(x2, r2, wn, eps, w_offset, E4M3, need_rstd)
+        y, _, wt, wt_off = _forward(None, q, w, weight, M, N, K, need_wt, False, x2.dtype)
+        return y, h, rstd, wt, wt_off
+    device = x2.device
+    y = _alloc_rows(M, N, x2.dtype, device)
+    h = torch.empty((M, K), dtype=x2.dtype, device=device) if r2 is not None else None
+    if wn.stride(0) != 1:
+        wn = wn.contiguous()
+    rstd = torch.empty(M, dtype=torch.float32, device=device) if need_rstd else None
+    xq_n = _nbytes(M, K)
+    w_ptr = wt_ptr = keep = None
+    wq_n = w_stride = 0
+    w_fp32 = False
+    if weight is None:
+        w = _check_matrix(w, "linear_fp8 weight")
+        w_ptr, w_stride, w_fp32, wq_n = w.data_ptr(), w.stride(0), w.dtype == torch.float32, _nbytes(N, K)
+        if need_wt:
+            keep = _bytes(_nbytes(K, N), device)
+            wt_ptr = keep.data_ptr()
+    temp = _bytes(xq_n + wq_n, device)
+    temp_ptr = temp.data_ptr()
+    nv.check(nv.cuda().cvb_fp8_norm_linear_fwd(
+        x2.data_ptr(), x2.stride(0), nv.ptr(r2), r2.stride(0) if r2 is not None else 0, wn.data_ptr(), nv.ptr(h),
+        nv.ptr(rstd), eps, w_offset, w_ptr, w_fp32, w_stride, M, N, K, temp_ptr,
+        temp_ptr + xq_n if weight is None else weight.w.buf.data_ptr(), wt_ptr, y.data_ptr(), max(y.stride(0), N),
+        _OUT[x2.dtype], _status(), _stream()), "cvb_fp8_norm_linear_fwd")
+    count_launch(2 + (w_ptr is not None))
+    if need_wt and weight is not None:
+        keep = weight.wt.buf
+    return y, (h if h is not None else x2), rstd, keep, 0
+
+
 class _NormLinearFp8(torch.autograd.Function):
     """(linear(rmsnorm(x + resid)), x + resid) with the norm's result in 8 bits only."""
 
@@ -561,15 +587,12 @@ class _NormLinearFp8(torch.autograd.Function):
         need_dn, need_dw = any(ctx.needs_input_grad[:3]), ctx.needs_input_grad[3]
         if need_dn and weight is not None and weight.wt is None:
             raise ValueError("add_rmsnorm_linear_fp8: the gradient of the input needs the transposed 8-bit weight")
-        x2 = _rows2d(x)
-        (M, K), N = x2.shape, w.shape[0]
-        q, h, rstd = _norm_forward(x2, _rows2d(resid) if resid is not None else None, wn, eps, w_offset, E4M3,
-                                   need_dn or need_dw)
-        y, _, wt, wt_off = _forward(None, q, w, weight, M, N, K, need_dn, False, x.dtype)
+        y, h, rstd, wt, wt_off = _norm_linear_forward(
+            _rows2d(x), _rows2d(resid) if resid is not None else None, wn, w, weight, eps, w_offset, need_dn, True)
         ctx.save_for_backward(h, rstd, wn, w if need_dw else None, wt)
-        ctx.cfg = (x.shape, M, N, K, w_offset, grad_dtype, wt_off)
+        ctx.cfg = (x.shape, h.shape[0], w.shape[0], h.shape[1], w_offset, grad_dtype, wt_off)
         if x.dim() != 2:
-            y, h = y.reshape(*x.shape[:-1], N), h.view(x.shape)
+            y, h = y.reshape(*x.shape[:-1], w.shape[0]), h.view(x.shape)
         return y if resid is None else (y, h)
 
     @staticmethod
@@ -580,46 +603,90 @@ class _NormLinearFp8(torch.autograd.Function):
         need_x, need_r, need_wn = ctx.needs_input_grad[:3]
         # The norm's result is formed again from h and rstd while its transpose is quantised: it is never stored.  Its
         # gradient stays fp32 between the product and the norm's backward.
-        dn, dw = _backward(dy, M, N, K, grad_dtype, wt, wt_off, None, w, torch.float32, (h, rstd, wn.contiguous(), w_offset))
-        dx = dwn = None
-        if dn is not None:
-            dx, dwn = _norm_backward(dn, h, wn, rstd, dh, w_offset, need_wn)
-            if len(shape) != 2:
-                dx = dx.view(shape)
+        norm = (h, rstd, wn if wn.stride(0) == 1 else wn.contiguous(), w_offset)
+        if dy.is_cuda and M and N and K:
+            dx, dwn, dw = _norm_linear_backward(dy, dh, M, N, K, grad_dtype, wt, wt_off, w, norm, wn if need_wn else None)
+        else:
+            dn, dw = _backward(dy, M, N, K, grad_dtype, wt, wt_off, None, w, torch.float32, norm)
+            dx, dwn = _norm_backward_ref(dn, h, wn, rstd, dh, w_offset, need_wn) if dn is not None else (None, None)
+        if dx is not None and len(shape) != 2:
+            dx = dx.view(shape)
         return (dx if need_x else None), (dx if need_r else None), dwn, dw, None, None, None, None
 
 
-def _norm_backward(dn, h, wn, rstd, dh, w_offset, need_dwn):
-    if h.is_cuda and h.get_device() != _current_device():
-        with torch.cuda.device(h.device):
-            return _norm_backward(dn, h, wn, rstd, dh, w_offset, need_dwn)
-    R, D = h.shape
-    main = getattr(wn, "main_grad", None) if need_dwn else None
-    dh2 = _rows2d(dh) if dh is not None else None
-    if not h.is_cuda:
-        xh, d32 = h.float() * rstd[:, None], dn.float()
-        g = d32 * (w_offset + wn.float())
-        dx = rstd[:, None] * (g - xh * (g * xh).mean(-1, keepdim=True))
-        if dh2 is not None:
-            dx = dx + dh2.float()
+def _grad_target(w, rows: int, cols: int, what: str):
+    """(where a weight's gradient goes, whether that is its main_grad)."""
+    main = getattr(w, "main_grad", None)
+    if main is None:
+        return _alloc_rows(rows, cols, w.dtype, w.device), False
+    if main.dtype != torch.float32 or not main.is_contiguous():
+        raise TypeError(f"{what}: main_grad is a contiguous float32 tensor")
+    return main.view(rows, cols), True
+
+
+def _norm_linear_backward(dy, dh, M, N, K, grad_dtype, wt, wt_off, w, norm, wn_param):
+    """``(dx, dwn, dw)``, each None where it is not wanted or went to a main_grad."""
+    if dy.get_device() != _current_device():
+        with torch.cuda.device(dy.device):
+            return _norm_linear_backward(dy, dh, M, N, K, grad_dtype, wt, wt_off, w, norm, wn_param)
+    h, rstd, wn, w_offset = norm
+    device = dy.device
+    dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N), "linear_fp8 gradient")
+    dh2 = _rows2d(dh) if dh is not None and wt is not None else None
+    lib = nv.cuda()
+    # one workspace: dy in both forms, the norm's result transposed, its gradient, and the parts of dwn
+    dyq_n = _nbytes(M, N) if wt is not None else 0
+    dyt_n, xt_n = (_nbytes(N, M), _nbytes(K, M)) if w is not None else (0, 0)
+    lddn = _ceil(K, 8) * 8
+    dn_n = M * lddn * 4 if wt is not None else 0
+    parts = min(M, lib.cvb_fp8_norm_bwd_parts()) if wn_param is not None else 0
+    temp = _bytes(_ceil(dyq_n + dyt_n + xt_n, 32) * 32 + dn_n + parts * K * 4, device)
+    base = temp.data_ptr()
+    dn_at = base + _ceil(dyq_n + dyt_n + xt_n, 32) * 32
+    wt_ptr = dx = dx_ptr = dw = dw_ptr = dwn = acc_ptr = dwn_ptr = part_ptr = None
+    dw_stride = dw_kind = 0
+    if wt is not None:
+        wt_ptr = wt.data_ptr() + wt_off
+        dx = torch.empty((M, K), dtype=h.dtype, device=device)
+        dx_ptr = dx.data_ptr()
+    if w is not None:
+        target, is_main = _grad_target(w, N, K, "linear_fp8")
+        dw_ptr, dw_stride, dw_kind = target.data_ptr(), max(target.stride(0), K), 2 if is_main else _OUT[w.dtype]
+        dw = None if is_main else target
+    if wn_param is not None:
+        part_ptr = dn_at + dn_n
+        if getattr(wn_param, "main_grad", None) is not None:
+            acc_ptr = _grad_target(wn_param, 1, K, "add_rmsnorm_linear_fp8")[0].data_ptr()
+        else:
+            dwn = torch.empty(K, dtype=wn_param.dtype, device=device)
+            dwn_ptr = dwn.data_ptr()
+    nv.check(lib.cvb_fp8_norm_linear_bwd(
+        dy2.data_ptr(), dy2.dtype == torch.float32, dy2.stride(0), _FMT[grad_dtype], M, N, K, base, base + dyq_n, wt_ptr,
+        base + dyq_n + dyt_n, h.data_ptr(), h.stride(0), rstd.data_ptr(), wn.data_ptr(), w_offset, dn_at, lddn, dw_ptr,
+        dw_stride, dw_kind, nv.ptr(dh2), dh2.stride(0) if dh2 is not None else 0, dx_ptr, part_ptr, acc_ptr, dwn_ptr,
+        _status(), _stream()), "cvb_fp8_norm_linear_bwd")
+    count_launch(1 + (2 if wt is not None else 0) + (2 if w is not None else 0) + (wn_param is not None))
+    return dx, dwn, dw
+
+
+def _norm_backward_ref(dn, h, wn, rstd, dh, w_offset, need_dwn):
+    """``(dx, dwn)`` of the norm in PyTorch; without rows on any device."""
+    D = h.shape[1]
+    xh, d32 = h.float() * rstd[:, None], dn.float()
+    g = d32 * (w_offset + wn.float())
+    dx = rstd[:, None] * (g - xh * (g * xh).mean(-1, keepdim=True))
+    if dh is not None:
+        dx = dx + _rows2d(dh).float()
+    dwn = None
+    if need_dwn:
         dwn = (d32 * xh).sum(0)
+        main = getattr(wn, "main_grad", None)
         if main is not None:
             main.view(D).add_(dwn)
-        return dx.to(h.dtype), dwn.to(wn.dtype) if need_dwn and main is None else None
-    if main is not None and (main.dtype != torch.float32 or not main.is_contiguous()):
-        raise TypeError("add_rmsnorm_linear_fp8: main_grad is a contiguous float32 tensor")
-    lib = nv.cuda()
-    dx = torch.empty((R, D), dtype=h.dtype, device=h.device)
-    dwn = torch.empty(D, dtype=wn.dtype, device=h.device) if need_dwn and main is None else None
-    if R == 0:
-        return dx, dwn.zero_() if dwn is not None else None
-    part = torch.empty((min(R, lib.cvb_fp8_norm_bwd_parts()), D), dtype=torch.float32, device=h.device) if need_dwn else None
-    wc = wn.contiguous()
-    nv.check(lib.cvb_fp8_norm_bwd(dn.data_ptr(), dn.stride(0), h.data_ptr(), h.stride(0), wc.data_ptr(), rstd.data_ptr(),
-                                  nv.ptr(dh2), dh2.stride(0) if dh2 is not None else 0, dx.data_ptr(), nv.ptr(part),
-                                  nv.ptr(main), nv.ptr(dwn), R, D, w_offset, _stream()), "cvb_fp8_norm_bwd")
-    count_launch(2 if need_dwn else 1)
-    return dx, dwn
+            dwn = None
+        else:
+            dwn = dwn.to(wn.dtype)
+    return dx.to(h.dtype), dwn
 
 
 @_on_device
@@ -631,11 +698,11 @@ def add_rmsnorm_linear_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], norm_
     what = "add_rmsnorm_linear_fp8"
     _check_norm(x, resid, norm_w, what)
     K, N = x.shape[-1], w.shape[0] if len(w.shape) else 0
-    _check_linear(K, x.device, w, weight, grad_dtype, what)
+    _check_linear(x.numel() // K, K, x.device, w, weight, grad_dtype, what)
     kept = w if isinstance(w, Fp8Weight) else weight
     if not _needs_grad(x, resid, norm_w, w):
-        q, h, _ = _norm_forward(_rows2d(x), _rows2d(resid) if resid is not None else None, norm_w, eps, w_offset, E4M3, False)
-        y = _forward(None, q, w, kept, q.rows, N, K, False, False, x.dtype)[0]
+        y, h, *_ = _norm_linear_forward(_rows2d(x), _rows2d(resid) if resid is not None else None, norm_w, w, kept, eps,
+                                        w_offset, False, False)
         if x.dim() != 2:
             y, h = y.reshape(*x.shape[:-1], N), h.view(x.shape)
         return y, x if resid is None else h

@@ -312,6 +312,43 @@ def test_other_stream():
     assert torch.equal(got, want)
 
 
+def test_two_streams_at_once():
+    """Products and quantisations of two streams run side by side: nothing is shared between calls."""
+    jobs = []
+    for seed, (m, n, k) in enumerate([(700, 1500, 1024), (3, 2048, 2048)]):
+        jobs.append((_rand(m, k, seed=seed), ops.quantize_fp8_weight(_rand(n, k, seed=seed + 10))))
+    want = [ops.linear_fp8(x, w) for x, w in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for _ in range(20):
+        for i, (s, (x, w)) in enumerate(zip(streams, jobs)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.linear_fp8(x, w))
+    torch.cuda.synchronize()
+    for outs, e in zip(got, want):
+        assert all(torch.equal(o, e) for o in outs)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in the input of a quantisation, in its codes and in a product's result."""
+    rows, cols = 70016, 32768
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    tail = _rand(200, cols, seed=1)
+    x[-200:] = tail
+    q, t = ops.quantize_fp8_pair(x)
+    del x
+    want = orc.quantize(tail)
+    assert _same(q.values[-200:], want[0]) and torch.equal(q.scales()[-200:].double(), want[1][:, ::128])
+    # 70016 = 547 * 128: the last block of a transposed row is the last 128 rows
+    assert _same(t.values[:, -128:], orc.quantize(tail[-128:].t())[0])
+    del q, t
+    a, b = _whole(rows, 128, 1), _whole(cols, 128, 2)
+    y = ops.gemm_fp8_nt(ops.quantize_fp8(a), ops.quantize_fp8(b))
+    at = [0, 1, 65535, 65537, rows - 129, rows - 1]
+    assert torch.equal(y[at], (a[at] @ b.t()).bfloat16())
+
+
 def test_two_captured_graphs_replayed_in_turn():
     w = ops.quantize_fp8_weight(_rand(700, 512, seed=1))
     wn = _rand(512, seed=2)
