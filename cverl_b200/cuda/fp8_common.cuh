@@ -129,4 +129,29 @@ __device__ __forceinline__ void fp8_load8(const float* p, int n, bool vec, float
   }
 }
 
+// eight bf16 as read, of which the first n exist.  VEC: rows are whole 16-byte vectors, n is 0 or 8; the load is then
+// one predicated instruction, and those of a row are all in flight before the first is used.
+template <bool VEC>
+__device__ __forceinline__ uint4 load_raw8(const __nv_bfloat16* p, int n) {
+  uint4 u = make_uint4(0u, 0u, 0u, 0u);
+  if (VEC) {
+    if (n > 0) u = __ldg(reinterpret_cast<const uint4*>(p));
+  } else {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+    u.x = (n > 0 ? e[0] : 0u) | ((n > 1 ? e[1] : 0u) << 16);
+    u.y = (n > 2 ? e[2] : 0u) | ((n > 3 ? e[3] : 0u) << 16);
+    u.z = (n > 4 ? e[4] : 0u) | ((n > 5 ? e[5] : 0u) << 16);
+    u.w = (n > 6 ? e[6] : 0u) | ((n > 7 ? e[7] : 0u) << 16);
+  }
+  return u;
+}
+__device__ __forceinline__ void widen8(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(w[j] << 16);
+    v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+
 }  // namespace cvb

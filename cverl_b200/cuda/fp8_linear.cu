@@ -11,6 +11,8 @@ int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, 
 int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                  long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int* status,
                  void* stream);
+int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* b, const void* b_sf, long long ldb, int b_fmt,
+                      int M, int N, int K, void* c, long long ldc, int out_kind, int* status, void* stream);
 int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride, const void* w, void* h,
                         void* q, void* sf, long long q_ld, float* rstd, long long rows, int D, int fmt, float eps,
                         float w_offset, void* stream);
@@ -45,13 +47,18 @@ int product(const Mat8& a, int a_fmt, const Mat8& b, int b_fmt, int M, int N, in
 }  // namespace
 
 // y [M, N] = x [M, K] w [N, K]^T.  x null: `xq` holds its 8-bit form already.  w null: `wq` does.  `xt` and `wt`
-// (both may be null) take the transposed forms that the backward pass reads.
+// (both may be null) take the transposed forms that the backward pass reads.  xq null: up to 32 bf16 rows, quantised
+// within the product.
 extern "C" int cvb_fp8_linear_fwd(const void* x, int x_fp32, long long x_stride, const void* w, int w_fp32,
                                   long long w_stride, int M, int N, int K, void* xq, void* xt, void* wq, void* wt,
                                   void* y, long long ldy, int out_kind, int* status, void* stream) {
   const Mat8 mxq(xq, M, K), mxt(xt, K, M), mwq(wq, N, K), mwt(wt, K, N);
   int rc = 0;
   if (w && (rc = quantize(w, w_fp32, N, K, w_stride, E4M3, BLOCKS, mwq, mwt, stream))) return rc;
+  if (x && !xq) {
+    if (x_fp32 || xt) return -1;
+    return cvb_fp8_gemm_rows(x, x_stride, mwq.codes, mwq.sf, mwq.ld, E4M3, M, N, K, y, ldy, out_kind, status, stream);
+  }
   if (x && (rc = quantize(x, x_fp32, M, K, x_stride, E4M3, 0, mxq, mxt, stream))) return rc;
   return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, status, stream);
 }

@@ -384,6 +384,14 @@ def _check_linear(rows: int, K: int, device, w, weight: Optional[Fp8Weight], gra
         raise ValueError(f"{what}: the 8-bit weight is given twice")
 
 
+def _quantised_within(M: int, K: int) -> bool:
+    """Whether the product quantises its bf16 rows itself (rows whose transpose nobody needs): every tile of 128 columns
+    does it for its share of K, in series, so for few rows of moderate length.  Back to back, against two kernels: one row,
+    K = 1024, N = 7168: 5.3 us against 6.6; 16 rows, K = 3584, N = 1024: 6.1 against 7.3; 32 rows, K = 2048: 7.2 against
+    7.5; 64 rows: 10.6 against 8.2; 16 rows, K = N = 8192: 14.2 against 11.9.  And one launch less."""
+    return M <= 16 and K <= 4096 or M <= 32 and K <= 2048
+
+
 def _forward(x2, xq, w, weight: Optional[Fp8Weight], M, N, K, need_wt: bool, need_xt: bool, dtype):
     """``(y, xt, wt, wt_off)``: the product, and the transposed 8-bit forms that gradients read: ``xt`` at the start of
     its buffer, ``wt`` at ``wt_off`` bytes of its (buffers or None).  ``x2`` is the input's rows or None where ``xq`` is
@@ -398,7 +406,8 @@ def _forward(x2, xq, w, weight: Optional[Fp8Weight], M, N, K, need_wt: bool, nee
         gemm_fp8_nt(xq, weight.w, y)
         return y, xt.buf if need_xt else None, weight.wt.buf if need_wt else None, 0
     # workspaces: 8-bit x and w for this product; 8-bit x^T and w^T kept for the gradients
-    xq_n = 0 if xq is not None else _nbytes(M, K)
+    fused = xq is None and not need_xt and x2.dtype == torch.bfloat16 and _quantised_within(M, K)
+    xq_n = 0 if xq is not None or fused else _nbytes(M, K)
     xt_n = _nbytes(K, M) if need_xt else 0
     wq_n = wt_n = x_stride = w_stride = 0
     x_fp32 = w_fp32 = False
@@ -417,11 +426,12 @@ def _forward(x2, xq, w, weight: Optional[Fp8Weight], M, N, K, need_wt: bool, nee
     else:
         x_ptr = None
     nv.check(nv.cuda().cvb_fp8_linear_fwd(
-        x_ptr, x_fp32, x_stride, w_ptr, w_fp32, w_stride, M, N, K, temp_ptr if xq_n else xq.buf.data_ptr(),
+        x_ptr, x_fp32, x_stride, w_ptr, w_fp32, w_stride, M, N, K,
+        None if fused else temp_ptr if xq_n else xq.buf.data_ptr(),
         keep_ptr if xt_n else None, temp_ptr + xq_n if weight is None else weight.w.buf.data_ptr(),
         keep_ptr + xt_n if wt_n else None, y.data_ptr(), max(y.stride(0), N), _OUT[dtype], _status(), _stream()),
         "cvb_fp8_linear_fwd")
-    count_launch(1 + (x_ptr is not None) + (w_ptr is not None))
+    count_launch(1 + (x_ptr is not None and not fused) + (w_ptr is not None))
     if need_wt and weight is not None:
         return y, keep, weight.wt.buf, 0
     return y, keep if need_xt else None, keep if need_wt else None, xt_n

@@ -137,6 +137,39 @@ def test_product_is_the_same_from_run_to_run():
             assert torch.equal(ops.gemm_fp8_nt(a, b, out_dtype=torch.float32), first)
 
 
+# ----------------------------------------------------------------------------- rows quantised within the product
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 32, 33, 63, 64, 65, 127, 128])
+@pytest.mark.parametrize("n,k", [(1, 1), (129, 127), (300, 130), (1000, 1000), (128, 4096), (7168, 1024), (520, 8200)])
+def test_rows_quantised_within_the_product(m, n, k):
+    kept = ops.quantize_fp8_weight(_whole(n, k, 2))
+    x = _whole(m, k, 1).bfloat16()
+    x[m // 2] = 0
+    want = (orc.value(ops.quantize_fp8(x)) @ orc.value(kept.w).t()).float().bfloat16()
+    assert torch.equal(ops.linear_fp8(x, kept), want)
+    wide = torch.full((m, k + 3), 5.0, dtype=torch.bfloat16, device="cuda")
+    wide[:, 1:k + 1] = x
+    assert torch.equal(ops.linear_fp8(wide[:, 1:k + 1], kept), want)
+    # random values: the same codes and scales as the separate quantisation, fp32 sums of k products
+    x = _rand(m, k, seed=m) * torch.exp(_rand(m, 1, seed=3))
+    kept = ops.quantize_fp8_weight(_rand(n, k, seed=4))
+    a, w = orc.value(ops.quantize_fp8(x)), orc.value(kept.w)
+    got = ops.linear_fp8(x, kept).double()
+    e = a @ w.t()
+    assert ((got - e).abs() <= 2.0 ** -8 * e.abs() + k * 2.0 ** -23 * (1 + 2.0 ** -8) * (a.abs() @ w.abs().t())).all()
+
+
+def test_rows_that_are_not_finite_within_the_product():
+    kept = ops.quantize_fp8_weight(_rand(140, 300, seed=2))
+    for m in (5, 20, 50, 128):
+        x = _rand(m, 300, seed=1)
+        clean = ops.linear_fp8(x, kept)
+        x[1, 7], x[3, 299], x[4, 128] = float("inf"), float("nan"), float("-inf")
+        got = ops.linear_fp8(x, kept)
+        assert got[[1, 3, 4]].isnan().all()
+        rest = [0, 2, *range(5, m)]
+        assert torch.equal(got[rest], clean[rest])
+
+
 # ----------------------------------------------------------------------------- norm
 @pytest.mark.parametrize("rows,d", [(1, 1), (1, 1024), (3, 129), (9, 128), (130, 256), (77, 500), (64, 513), (257, 1024),
                                     (31, 1111), (20, 2048), (33, 2560), (5, 4096), (7, 5000), (4, 8192), (3, 16384),
