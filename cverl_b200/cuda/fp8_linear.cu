@@ -6,15 +6,15 @@
 
 extern "C" {
 int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, long long x_stride, int fmt, int mode,
-                     void* q, void* sf, long long q_ld, void* qt, void* sft, long long qt_ld, const float* rstd,
-                     const void* w, float w_offset, void* stream);
+                     void* q, void* sf, void* ps, long long q_ld, void* qt, void* sft, void* pst, long long qt_ld,
+                     const float* rstd, const void* w, float w_offset, void* stream);
 int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                  long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int* status,
                  void* stream);
 int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* b, const void* b_sf, long long ldb, int b_fmt,
                       int M, int N, int K, void* c, long long ldc, int out_kind, int* status, void* stream);
 int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride, const void* w, void* h,
-                        void* q, void* sf, long long q_ld, float* rstd, long long rows, int D, int fmt, float eps,
+                        void* q, void* sf, void* ps, long long q_ld, float* rstd, long long rows, int D, int fmt, float eps,
                         float w_offset, void* stream);
 int cvb_fp8_norm_bwd(const float* dn, long long dn_stride, const void* h, long long h_stride, const void* w,
                      const float* rstd, const void* dh, long long dh_stride, void* dx, float* part, float* dw_acc,
@@ -37,8 +37,8 @@ struct Mat8 {      // [rows, cols] in a buffer; null buffer: absent
 int quantize(const void* x, int x_fp32, long long rows, long long cols, long long stride, int fmt, int extra,
              const Mat8& q, const Mat8& t, void* stream) {
   const int mode = (q.codes ? ROWS : 0) | (t.codes ? COLS : 0) | extra;
-  return cvb_fp8_quantize(x, x_fp32, rows, cols, stride, fmt, mode, q.codes, q.sf, q.ld, t.codes, t.sf, t.ld, nullptr,
-                          nullptr, 0.f, stream);
+  return cvb_fp8_quantize(x, x_fp32, rows, cols, stride, fmt, mode, q.codes, q.sf, nullptr, q.ld, t.codes, t.sf,
+                          nullptr, t.ld, nullptr, nullptr, 0.f, stream);
 }
 int product(const Mat8& a, int a_fmt, const Mat8& b, int b_fmt, int M, int N, int K, void* c, long long ldc,
             int out_kind, int* status, void* stream) {
@@ -69,7 +69,7 @@ extern "C" int cvb_fp8_norm_linear_fwd(const void* x, long long x_stride, const 
                                        int w_fp32, long long w_stride, int M, int N, int K, void* xq, void* wq, void* wt,
                                        void* y, long long ldy, int out_kind, int* status, void* stream) {
   const Mat8 mxq(xq, M, K);
-  const int rc = cvb_fp8_add_rmsnorm(x, x_stride, resid, r_stride, wn, h, mxq.codes, mxq.sf, mxq.ld, rstd, M, K, E4M3,
+  const int rc = cvb_fp8_add_rmsnorm(x, x_stride, resid, r_stride, wn, h, mxq.codes, mxq.sf, nullptr, mxq.ld, rstd, M, K, E4M3,
                                      eps, w_offset, stream);
   if (rc) return rc;
   return cvb_fp8_linear_fwd(nullptr, 0, 0, w, w_fp32, w_stride, M, N, K, xq, nullptr, wq, wt, y, ldy, out_kind, status,
@@ -88,7 +88,8 @@ extern "C" int cvb_fp8_linear_bwd(const void* dy, int dy_fp32, long long dy_stri
   if (rc) return rc;
   if (wt && (rc = product(mdq, grad_fmt, mwt, E4M3, M, K, N, dx, lddx, dx_kind, status, stream))) return rc;
   if (!dw) return 0;
-  if (h && (rc = cvb_fp8_quantize(h, 0, M, K, h_stride, E4M3, COLS, nullptr, nullptr, 0, mxt.codes, mxt.sf, mxt.ld,
+  if (h && (rc = cvb_fp8_quantize(h, 0, M, K, h_stride, E4M3, COLS, nullptr, nullptr, nullptr, 0, mxt.codes, mxt.sf,
+                                  nullptr, mxt.ld,
                                   rstd, wn, w_offset, stream)))
     return rc;
   return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, status, stream);

@@ -21,6 +21,7 @@ struct QuantArgs {
   long long q_ld;
   int kgroups;                     // ceil(ceil(cols / 128) / 4)
   uint8_t *qt, *sft;               // transposed form
+  uint8_t *ps, *pst;               // scale bytes of each form in plain order [row, block]; may be null
   long long qt_ld;
   int kgroups_t;
   int col_tiles;
@@ -234,9 +235,15 @@ fp8_quant_kernel(const QuantArgs p) {
       for (int w = 1; w < Q_THREADS / 32; ++w) m = __vmaxu2(m, s_max[w][threadIdx.x]);
       const uint32_t bytes = fp8_scale_bytes<FMT>(m);
       s_inv[threadIdx.x] = fp8_inverse_scales(bytes);
-      uint8_t* sf = p.sft + fp8_sf_offset(static_cast<long long>(tile_c) * QT + threadIdx.x * 2, tile_r, p.kgroups_t);
+      const long long col = static_cast<long long>(tile_c) * QT + threadIdx.x * 2;
+      uint8_t* sf = p.sft + fp8_sf_offset(col, tile_r, p.kgroups_t);
       sf[0] = static_cast<uint8_t>(bytes);
       sf[16] = static_cast<uint8_t>(bytes >> 16);
+      if (p.pst != nullptr) {
+        const long long nb = (p.rows + QT - 1) / QT;
+        if (col < p.cols) p.pst[col * nb + tile_r] = static_cast<uint8_t>(bytes);
+        if (col + 1 < p.cols) p.pst[(col + 1) * nb + tile_r] = static_cast<uint8_t>(bytes >> 16);
+      }
     }
   }
   if (ROWS) {
@@ -256,6 +263,12 @@ fp8_quant_kernel(const QuantArgs p) {
       uint8_t* sf = p.sf + fp8_sf_offset(r0, tile_c, p.kgroups);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sf[i * 16] = static_cast<uint8_t>(bytes[i >> 1] >> ((i & 1) * 16));
+      if (p.ps != nullptr) {
+        uint8_t* ps = p.ps + r0 * p.col_tiles + tile_c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i, ps += p.col_tiles)
+          if (i < nr) *ps = static_cast<uint8_t>(bytes[i >> 1] >> ((i & 1) * 16));
+      }
     }
     if (c0 < p.q_ld) {
       uint8_t* out = p.q + r0 * p.q_ld + c0;
@@ -284,9 +297,11 @@ fp8_quant_kernel(const QuantArgs p) {
     uint4 inv = make_uint4(0u, 0u, 0u, 0u);
     if (BLOCK) {
       inv.x = inv.y = inv.z = inv.w = fp8_inverse_scales(tile_bytes);
-      if (threadIdx.x < QT)
-        p.sft[fp8_sf_offset(static_cast<long long>(tile_c) * QT + threadIdx.x, tile_r, p.kgroups_t)] =
-            static_cast<uint8_t>(tile_bytes);
+      const long long col = static_cast<long long>(tile_c) * QT + threadIdx.x;
+      if (threadIdx.x < QT) {
+        p.sft[fp8_sf_offset(col, tile_r, p.kgroups_t)] = static_cast<uint8_t>(tile_bytes);
+        if (p.pst != nullptr && col < p.cols) p.pst[col * ((p.rows + QT - 1) / QT) + tile_r] = static_cast<uint8_t>(tile_bytes);
+      }
     } else {
       __syncthreads();
       inv = *reinterpret_cast<const uint4*>(&s_inv[cl * 4]);
@@ -325,16 +340,6 @@ fp8_quant_kernel(const QuantArgs p) {
   }
 }
 
-// scale bytes in the plain order [rows, blocks] for inspection and for other programs
-__global__ void fp8_scales_kernel(const uint8_t* __restrict__ sf, uint8_t* __restrict__ out, long long rows, int nb) {
-  const int kgroups = (nb + 3) / 4;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows * nb;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long r = i / nb;
-    out[i] = sf[fp8_sf_offset(r, static_cast<int>(i - r * nb), kgroups)];
-  }
-}
-
 template <typename T, int FMT>
 static void quant_launch(const QuantArgs& p, int mode, long long grid, cudaStream_t s) {
   const dim3 g(static_cast<unsigned>(grid));
@@ -356,7 +361,7 @@ static void quant_launch(const QuantArgs& p, int mode, long long grid, cudaStrea
 struct NormQuantArgs {
   const __nv_bfloat16 *x, *resid, *w;
   __nv_bfloat16* h;
-  uint8_t *q, *sf;
+  uint8_t *q, *sf, *ps;       // ps: scale bytes in plain order; may be null
   float* rstd;
   long long rows, x_stride, r_stride, h_stride, q_ld;
   int D, kgroups, vec;
@@ -429,6 +434,7 @@ fp8_norm_kernel(const NormQuantArgs p) {
   if (ok && t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
   uint8_t* q = p.q + row * p.q_ld;
   uint8_t* sf = p.sf + fp8_sf_offset(row, 0, p.kgroups);
+  uint8_t* ps = p.ps != nullptr ? p.ps + row * ((p.D + 127) / 128) : nullptr;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + t) * 8, n = max(0, min(8, p.D - c));
@@ -441,7 +447,10 @@ fp8_norm_kernel(const NormQuantArgs p) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const uint32_t byte = fp8_scale_bytes<FMT>(m) & 0xFFu;
-    if (ok && c < p.D && (t & 15) == 0) sf[(c >> 9) * 512 + ((c >> 7) & 3)] = static_cast<uint8_t>(byte);
+    if (ok && c < p.D && (t & 15) == 0) {
+      sf[(c >> 9) * 512 + ((c >> 7) & 3)] = static_cast<uint8_t>(byte);
+      if (ps != nullptr) ps[c >> 7] = static_cast<uint8_t>(byte);
+    }
     if (ok && c < p.q_ld) {
       *reinterpret_cast<uint2*>(q + c) = fp8_pack8<FMT>(v[i], fp8_low(fp8_inverse_scales(byte)));
       if (odd) fp8_fix_inf<FMT>(v[i], q + c, n);
@@ -644,10 +653,11 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 using namespace cvb;
 
+// ps, pst (may be null): the scale bytes once more, in plain order, for other programs to read
 // mode: 1 row form, 2 transposed form, 3 both, 5 row form with 128 x 128 blocks, 7 both with 128 x 128 blocks
 extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, long long x_stride, int fmt,
-                                int mode, void* q, void* sf, long long q_ld, void* qt, void* sft, long long qt_ld,
-                                const float* rstd, const void* w, float w_offset, void* stream) {
+                                int mode, void* q, void* sf, void* ps, long long q_ld, void* qt, void* sft, void* pst,
+                                long long qt_ld, const float* rstd, const void* w, float w_offset, void* stream) {
   if (rows <= 0 || cols <= 0) return 0;
   if ((fmt != FP8_E4M3 && fmt != FP8_E5M2) || (mode != 1 && mode != 2 && mode != 3 && mode != 5 && mode != 7)) return -1;
   if (mode > 3 && fmt != FP8_E4M3) return -1;
@@ -664,6 +674,7 @@ extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long 
   p.vec = aligned16(x) && (x_stride * elem) % 16 == 0;
   p.q = static_cast<uint8_t*>(q), p.sf = static_cast<uint8_t*>(sf), p.q_ld = q_ld;
   p.kgroups = static_cast<int>((col_tiles + 3) / 4);
+  p.ps = static_cast<uint8_t*>(ps), p.pst = static_cast<uint8_t*>(pst);
   p.qt = static_cast<uint8_t*>(qt), p.sft = static_cast<uint8_t*>(sft), p.qt_ld = qt_ld;
   p.kgroups_t = static_cast<int>((row_tiles + 3) / 4);
   p.col_tiles = static_cast<int>(col_tiles);
@@ -682,17 +693,8 @@ extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long 
   return static_cast<int>(cudaGetLastError());
 }
 
-extern "C" int cvb_fp8_scales(const void* sf, void* out, long long rows, int nb, void* stream) {
-  if (rows <= 0 || nb <= 0) return 0;
-  const long long n = rows * nb;
-  const unsigned grid = static_cast<unsigned>(n < 148ll * 8 * 256 ? (n + 255) / 256 : 148 * 8);
-  fp8_scales_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint8_t*>(sf),
-                                                                       static_cast<uint8_t*>(out), rows, nb);
-  return static_cast<int>(cudaGetLastError());
-}
-
 extern "C" int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride,
-                                   const void* w, void* h, void* q, void* sf, long long q_ld, float* rstd,
+                                   const void* w, void* h, void* q, void* sf, void* ps, long long q_ld, float* rstd,
                                    long long rows, int D, int fmt, float eps, float w_offset, void* stream) {
   if (rows <= 0 || D <= 0) return 0;
   if (fmt != FP8_E4M3 && fmt != FP8_E5M2) return -1;
@@ -701,7 +703,7 @@ extern "C" int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void
   NormQuantArgs p = {};
   p.x = static_cast<const __nv_bfloat16*>(x), p.resid = static_cast<const __nv_bfloat16*>(resid);
   p.w = static_cast<const __nv_bfloat16*>(w), p.h = static_cast<__nv_bfloat16*>(h);
-  p.q = static_cast<uint8_t*>(q), p.sf = static_cast<uint8_t*>(sf), p.rstd = rstd;
+  p.q = static_cast<uint8_t*>(q), p.sf = static_cast<uint8_t*>(sf), p.ps = static_cast<uint8_t*>(ps), p.rstd = rstd;
   p.rows = rows, p.x_stride = x_stride, p.r_stride = r_stride, p.h_stride = D, p.q_ld = q_ld;
   p.D = D, p.kgroups = ((D + 127) / 128 + 3) / 4;
   p.vec = aligned16(x) && aligned16(resid) && aligned16(w) && aligned16(h) && x_stride % 8 == 0 && r_stride % 8 == 0 &&

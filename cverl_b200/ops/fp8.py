@@ -90,18 +90,28 @@ def _alloc_rows(M: int, N: int, dtype: torch.dtype, device: torch.device) -> tor
 # the 8-bit matrix
 # ----------------------------------------------------------------------------
 def _nbytes(rows: int, cols: int) -> int:
+    """Codes and scale cells: what the products read."""
     return rows * ((cols + 15) // 16 * 16) + ((rows + 127) // 128) * ((cols + 511) // 512) * 512
 
 
+def _nbytes_plain(rows: int, cols: int) -> int:
+    """The scale bytes once more, in plain order ``[rows, blocks]``: what a caller reads."""
+    return rows * ((cols + 127) // 128)
+
+
 class Fp8Tensor:
-    """``[rows, cols]`` in 8 bits.  One buffer: codes, row-major with rows padded to 16 bytes, then the scale bytes in
-    the order in which the tensor core reads them (see ``cuda/fp8_common.cuh``)."""
+    """``[rows, cols]`` in 8 bits.  One buffer: codes, row-major with rows padded to 16 bytes; the scale bytes in the order
+    in which the tensor core reads them (see ``cuda/fp8_common.cuh``); the scale bytes in plain order."""
 
     __slots__ = ("buf", "rows", "cols", "dtype", "ld")
 
     def __init__(self, buf: torch.Tensor, rows: int, cols: int, dtype: torch.dtype):
         self.buf, self.rows, self.cols, self.dtype = buf, rows, cols, dtype
         self.ld = (cols + 15) // 16 * 16
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> "Fp8Tensor":
+        return cls(_bytes(_nbytes(rows, cols) + _nbytes_plain(rows, cols), device), rows, cols, dtype)
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -115,14 +125,19 @@ class Fp8Tensor:
     def sf_ptr(self) -> int:
         return self.buf.data_ptr() + self.rows * self.ld
 
+    def _pointers(self):
+        base = self.buf.data_ptr()
+        return base, base + self.rows * self.ld, base + _nbytes(self.rows, self.cols), self.ld
+
     @property
     def values(self) -> torch.Tensor:
         """The codes as an 8-bit float view ``[rows, cols]`` (in units of their scales)."""
         return self.buf.view(self.dtype).as_strided((self.rows, self.cols), (self.ld, 1))
 
     def scales(self) -> torch.Tensor:
-        """The scales ``[rows, ceil(cols / 128)]`` as ``torch.float8_e8m0fnu`` (powers of two)."""
-        return _scales(self).view(torch.float8_e8m0fnu)
+        """The scales as a view ``[rows, ceil(cols / 128)]`` of ``torch.float8_e8m0fnu`` (powers of two)."""
+        nb = _ceil(self.cols, BLOCK)
+        return self.buf.view(torch.float8_e8m0fnu).as_strided((self.rows, nb), (nb, 1), _nbytes(self.rows, self.cols))
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         s = self.scales().float().repeat_interleave(BLOCK, 1)[:, :self.cols]
@@ -141,21 +156,6 @@ class Fp8Weight:
         self.shape, self.device = w.shape, w.device
 
 
-@_on_device
-def _scales(q: Fp8Tensor) -> torch.Tensor:
-    nb = _ceil(q.cols, BLOCK)
-    out = torch.empty((q.rows, nb), dtype=torch.uint8, device=q.device)
-    if q.rows == 0 or nb == 0:
-        return out
-    if q.buf.is_cuda:
-        nv.check(nv.cuda().cvb_fp8_scales(q.sf_ptr, out.data_ptr(), q.rows, nb, _stream()), "cvb_fp8_scales")
-        count_launch()
-        return out
-    rt, kg = _ceil(q.rows, BLOCK), _ceil(q.cols, 4 * BLOCK)
-    cells = q.buf[q.rows * q.ld:].view(rt, kg, 32, 4, 4)                           # [.., r % 32, r / 32, b % 4]
-    return out.copy_(cells.permute(0, 3, 2, 1, 4).reshape(rt * BLOCK, kg * 4)[:q.rows, :nb])
-
-
 def _quantize_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1):
     """Codes (8-bit float ``[R, C]``) and scale bytes (uint8 ``[R, blocks]``) of a matrix, in PyTorch."""
     R, C = x.shape
@@ -172,15 +172,17 @@ def _quantize_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1):
 
 def _pack_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1) -> Fp8Tensor:
     R, C = x.shape
-    out = Fp8Tensor(torch.zeros(_nbytes(R, C), dtype=torch.uint8, device=x.device), R, C, dtype)
+    out = Fp8Tensor.empty(R, C, dtype, x.device)
+    out.buf.zero_()
     if R == 0 or C == 0:
         return out
     codes, byte = _quantize_ref(x, dtype, block_rows)
     out.buf[:R * out.ld].view(R, out.ld)[:, :C] = codes.contiguous().view(torch.uint8)
-    rt, kg = _ceil(R, BLOCK), _ceil(C, 4 * BLOCK)
+    rt, kg, at = _ceil(R, BLOCK), _ceil(C, 4 * BLOCK), _nbytes(R, C)
     cells = torch.ones((rt * BLOCK, kg * 4), dtype=torch.uint8, device=x.device)
     cells[:R, :byte.shape[1]] = byte
-    out.buf[R * out.ld:] = cells.view(rt, 4, 32, kg, 4).permute(0, 3, 2, 1, 4).reshape(-1)
+    out.buf[R * out.ld:at] = cells.view(rt, 4, 32, kg, 4).permute(0, 3, 2, 1, 4).reshape(-1)   # [.., r % 32, r / 32, b % 4]
+    out.buf[at:] = byte.reshape(-1)
     return out
 
 
@@ -212,13 +214,13 @@ def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int, rstd=None, w=None,
         return (_pack_ref(v, dtype, tall) if mode & _ROWS else None,
                 _pack_ref(v.t(), dtype, tall) if mode & _COLS else None)
     q = t = None
-    q_args = t_args = (None, None, 0)
+    q_args = t_args = (None, None, None, 0)
     if mode & _ROWS:
-        q = Fp8Tensor(_bytes(_nbytes(R, C), x.device), R, C, dtype)
-        q_args = (q.buf.data_ptr(), q.sf_ptr, q.ld)
+        q = Fp8Tensor.empty(R, C, dtype, x.device)
+        q_args = q._pointers()
     if mode & _COLS:
-        t = Fp8Tensor(_bytes(_nbytes(C, R), x.device), C, R, dtype)
-        t_args = (t.buf.data_ptr(), t.sf_ptr, t.ld)
+        t = Fp8Tensor.empty(C, R, dtype, x.device)
+        t_args = t._pointers()
     if R and C:
         nv.check(nv.cuda().cvb_fp8_quantize(
             x.data_ptr(), x.dtype == torch.float32, R, C, x.stride(0), _FMT[dtype], mode, *q_args, *t_args, None, None,
@@ -332,7 +334,7 @@ def _norm_forward(x2, r2, w, eps, w_offset, dtype, need_rstd: bool):
         h = x2 if r2 is None else (x2.float() + r2.detach().float()).to(x2.dtype)
         rstd = torch.rsqrt(h.float().pow(2).mean(-1) + eps)
         return _pack_ref(h.float() * rstd[:, None] * (w_offset + w.float()), dtype), h, rstd
-    q = Fp8Tensor(_bytes(_nbytes(R, D), x2.device), R, D, dtype)
+    q = Fp8Tensor.empty(R, D, dtype, x2.device)
     h = torch.empty((R, D), dtype=x2.dtype, device=x2.device) if r2 is not None else None
     rstd = torch.empty(R, dtype=torch.float32, device=x2.device) if need_rstd else None
     if R:
@@ -340,7 +342,7 @@ def _norm_forward(x2, r2, w, eps, w_offset, dtype, need_rstd: bool):
             w = w.contiguous()
         nv.check(nv.cuda().cvb_fp8_add_rmsnorm(
             x2.data_ptr(), x2.stride(0), nv.ptr(r2), r2.stride(0) if r2 is not None else 0, w.data_ptr(), nv.ptr(h),
-            q.buf.data_ptr(), q.sf_ptr, q.ld, nv.ptr(rstd), R, D, _FMT[dtype], eps, w_offset, _stream()),
+            *q._pointers(), nv.ptr(rstd), R, D, _FMT[dtype], eps, w_offset, _stream()),
             "cvb_fp8_add_rmsnorm")
         count_launch()
     return q, (h if h is not None else x2), rstd
