@@ -3,7 +3,9 @@
 ``cuda()`` returns ``libcverl_b200_cuda.so`` (sm_100a kernels, ``extern "C"``
 launchers taking raw device pointers and a ``cudaStream_t``); ``host()``
 returns ``libcverl.so`` (host runtime with the public C ABI).  Both are built
-by :mod:`cverl_b200._build` and live under ``cverl_b200/lib``.  On a machine
+by :mod:`cverl_b200._build` and live under ``cverl_b200/lib``.  ``torch_ext()``
+returns the extension module that keeps autograd nodes and workspaces of small
+layers out of Python; it calls the launchers of the first.  On a machine
 with a GPU a missing kernel library is a hard error: there is no silent eager
 fallback.
 """
@@ -18,6 +20,7 @@ import torch
 _LIB_DIR = Path(__file__).resolve().parent / "lib"
 _cuda_lib = None
 _host_lib = None
+_torch_ext = None
 
 c_void_p = C.c_void_p
 c_ll = C.c_longlong
@@ -174,6 +177,28 @@ def host():
             _build.build_host()
         _host_lib = C.CDLL(str(path))
     return _host_lib
+
+
+def torch_ext():
+    """The extension module in front of the kernel launchers; raises when it cannot be loaded."""
+    global _torch_ext
+    if _torch_ext is None:
+        import importlib.util
+
+        from .ops.gemm import launch_counter
+        lib = cuda()
+        path = _LIB_DIR / "_cverl_torch.so"
+        if not path.exists():
+            _ensure_built()
+        if not path.exists():
+            raise RuntimeError(f"native extension missing: {path} (run python -m cverl_b200._build)")
+        spec = importlib.util.spec_from_file_location("_cverl_torch", path)
+        ext = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ext)
+        ext.bind({n: C.cast(getattr(lib, n), c_void_p).value for n in _CUDA_PROTOS if n.startswith("cvb_fp8_")},
+                 launch_counter)
+        _torch_ext = ext
+    return _torch_ext
 
 
 def have_cuda_kernels() -> bool:

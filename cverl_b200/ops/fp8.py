@@ -16,12 +16,12 @@ Gradients pass through the roundings as if they were not there (straight-through
 
     y = Q(x) Q(w)^T       dx = Q(dy) Q(w)       dw = Q(dy^T) Q(x^T)^T
 
-with blocks of 128 along each product's own contraction.  CUDA tensors run the kernels; CPU tensors run the PyTorch
-statement of the same math, which is also the test oracle.  The reference has no 8-bit path.
+with blocks of 128 along each product's own contraction.  CUDA tensors run the kernels, with workspaces and autograd
+nodes in ``torch_ext/fp8_torch.cc``; CPU tensors run the PyTorch statement of the same math, which is also the test
+oracle.  The reference has no 8-bit path.
 """
 from __future__ import annotations
 
-import functools
 from typing import Optional, Tuple
 
 import torch
@@ -45,37 +45,11 @@ def _ceil(a: int, b: int) -> int:
     return (a + b - 1) // b
 
 
-def _current_device() -> int:
-    return torch._C._cuda_getDevice()
-
-
-def _on_device(fn):
-    """Runs ``fn`` with the device of its first argument as the current one: launches go to the tensors' device and to
-    that device's current stream."""
-    @functools.wraps(fn)
-    def call(x, *args, **kwargs):
-        t = x.buf if isinstance(x, Fp8Tensor) else x
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != _current_device():
-            with torch.cuda.device(t.device):
-                return fn(x, *args, **kwargs)
-        return fn(x, *args, **kwargs)
-    return call
-
-
-def _stream() -> int:
-    return nv.raw_stream(_current_device())
-
-
-def _status() -> int:
-    index = _current_device()
+def _status(index: int) -> int:
     p = _status_ptr.get(index)
     if p is None:
         p = _status_ptr[index] = nv.status_word(index).data_ptr()      # one per device, never replaced
     return p
-
-
-def _bytes(n: int, device: torch.device) -> torch.Tensor:
-    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _alloc_rows(M: int, N: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -109,10 +83,6 @@ class Fp8Tensor:
         self.buf, self.rows, self.cols, self.dtype = buf, rows, cols, dtype
         self.ld = (cols + 15) // 16 * 16
 
-    @classmethod
-    def empty(cls, rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> "Fp8Tensor":
-        return cls(_bytes(_nbytes(rows, cols) + _nbytes_plain(rows, cols), device), rows, cols, dtype)
-
     @property
     def shape(self) -> Tuple[int, int]:
         return (self.rows, self.cols)
@@ -124,10 +94,6 @@ class Fp8Tensor:
     @property
     def sf_ptr(self) -> int:
         return self.buf.data_ptr() + self.rows * self.ld
-
-    def _pointers(self):
-        base = self.buf.data_ptr()
-        return base, base + self.rows * self.ld, base + _nbytes(self.rows, self.cols), self.ld
 
     @property
     def values(self) -> torch.Tensor:
@@ -172,8 +138,7 @@ def _quantize_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1):
 
 def _pack_ref(x: torch.Tensor, dtype: torch.dtype, block_rows: int = 1) -> Fp8Tensor:
     R, C = x.shape
-    out = Fp8Tensor.empty(R, C, dtype, x.device)
-    out.buf.zero_()
+    out = Fp8Tensor(torch.zeros(_nbytes(R, C) + _nbytes_plain(R, C), dtype=torch.uint8, device=x.device), R, C, dtype)
     if R == 0 or C == 0:
         return out
     codes, byte = _quantize_ref(x, dtype, block_rows)
@@ -195,7 +160,7 @@ def _check_matrix(x: torch.Tensor, what: str) -> torch.Tensor:
         raise TypeError(f"{what}: bfloat16 or float32 is wanted, got {x.dtype}")
     if x.shape[0] > MAX_EXTENT or x.shape[1] > MAX_EXTENT:
         raise ValueError(f"{what}: at most {MAX_EXTENT} rows and columns, got {tuple(x.shape)}")
-    return x if x.stride(1) == 1 or x.shape[1] <= 1 else x.contiguous()
+    return x
 
 
 def _check_dtype(dtype: torch.dtype, what: str) -> None:
@@ -203,54 +168,35 @@ def _check_dtype(dtype: torch.dtype, what: str) -> None:
         raise TypeError(f"{what}: the 8-bit type is torch.float8_e4m3fn or torch.float8_e5m2, got {dtype}")
 
 
-def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int, rstd=None, w=None, w_offset: float = 0.0):
-    """(row form or None, transposed form or None) by the mode's bits.  With ``rstd`` (on the CPU) the values are
-    ``x * rstd[row] * (w_offset + w[col])``."""
+def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int):
+    """(row form or None, transposed form or None) by the mode's bits."""
     R, C = x.shape
-    if not x.is_cuda:
-        tall = BLOCK if mode & _TILES else 1
-        x = x.detach()
-        v = x.float() if rstd is None else x.float() * rstd[:, None] * (w_offset + w.float())
-        return (_pack_ref(v, dtype, tall) if mode & _ROWS else None,
-                _pack_ref(v.t(), dtype, tall) if mode & _COLS else None)
-    q = t = None
-    q_args = t_args = (None, None, None, 0)
-    if mode & _ROWS:
-        q = Fp8Tensor.empty(R, C, dtype, x.device)
-        q_args = q._pointers()
-    if mode & _COLS:
-        t = Fp8Tensor.empty(C, R, dtype, x.device)
-        t_args = t._pointers()
-    if R and C:
-        nv.check(nv.cuda().cvb_fp8_quantize(
-            x.data_ptr(), x.dtype == torch.float32, R, C, x.stride(0), _FMT[dtype], mode, *q_args, *t_args, None, None,
-            0.0, _stream()), "cvb_fp8_quantize")
-        count_launch()
-    return q, t
+    if x.is_cuda:
+        q, t = nv.torch_ext().quantize(x, _FMT[dtype], mode)
+        return (Fp8Tensor(q, R, C, dtype) if q is not None else None), (Fp8Tensor(t, C, R, dtype) if t is not None else None)
+    tall = BLOCK if mode & _TILES else 1
+    v = x.detach().float()
+    return (_pack_ref(v, dtype, tall) if mode & _ROWS else None), (_pack_ref(v.t(), dtype, tall) if mode & _COLS else None)
 
 
-@_on_device
 def quantize_fp8(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
     """``x [R, C]`` (bf16 or fp32) in 8 bits, one scale per 128 elements of a row."""
     _check_dtype(dtype, "quantize_fp8")
     return _quantize(_check_matrix(x, "quantize_fp8"), dtype, _ROWS)[0]
 
 
-@_on_device
 def quantize_fp8_t(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
     """``x.T [C, R]`` in 8 bits, one scale per 128 rows of ``x``."""
     _check_dtype(dtype, "quantize_fp8_t")
     return _quantize(_check_matrix(x, "quantize_fp8_t"), dtype, _COLS)[1]
 
 
-@_on_device
 def quantize_fp8_pair(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Tuple[Fp8Tensor, Fp8Tensor]:
     """``(quantize_fp8(x), quantize_fp8_t(x))`` from one read of ``x``."""
     _check_dtype(dtype, "quantize_fp8_pair")
     return _quantize(_check_matrix(x, "quantize_fp8_pair"), dtype, _ROWS | _COLS)
 
 
-@_on_device
 def quantize_fp8_weight(w: torch.Tensor, transposed: bool = True) -> Fp8Weight:
     """A weight ``[N, K]`` in e4m3 with one scale per 128 x 128 block.  ``transposed=False`` leaves the transpose out,
     which only gradients of the layer's input need."""
@@ -261,7 +207,6 @@ def quantize_fp8_weight(w: torch.Tensor, transposed: bool = True) -> Fp8Weight:
 # ----------------------------------------------------------------------------
 # product
 # ----------------------------------------------------------------------------
-@_on_device
 def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, *,
                 out_dtype: Optional[torch.dtype] = None, accumulate: bool = False) -> torch.Tensor:
     """``a [M, K] @ b [N, K].T -> [M, N]`` in bf16 (default) or fp32; ``accumulate`` adds to an fp32 ``out``.
@@ -296,10 +241,14 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
     if not a.buf.is_cuda:
         r = a.dequantize() @ b.dequantize().t()
         return out.add_(r) if accumulate else out.copy_(r)
-    nv.check(nv.cuda().cvb_fp8_gemm(
-        a.buf.data_ptr(), a.sf_ptr, a.ld, _FMT[a.dtype], b.buf.data_ptr(), b.sf_ptr, b.ld, _FMT[b.dtype], M, N, K,
-        out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype], _status(), _stream()),
-        "cvb_fp8_gemm")
+    index = out.get_device()
+    args = (a.buf.data_ptr(), a.sf_ptr, a.ld, _FMT[a.dtype], b.buf.data_ptr(), b.sf_ptr, b.ld, _FMT[b.dtype], M, N, K,
+            out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype], _status(index))
+    if index != torch._C._cuda_getDevice():       # launches go to the operands' device and its current stream
+        with torch.cuda.device(index):
+            nv.check(nv.cuda().cvb_fp8_gemm(*args, nv.raw_stream(index)), "cvb_fp8_gemm")
+    else:
+        nv.check(nv.cuda().cvb_fp8_gemm(*args, nv.raw_stream(index)), "cvb_fp8_gemm")
     count_launch()
     return out
 
@@ -321,34 +270,16 @@ def _check_norm(x, resid, w, what):
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+    return t if t.dim() == 2 else t.reshape(t.shape[:-1].numel(), t.shape[-1])
 
 
-def _norm_forward(x2, r2, w, eps, w_offset, dtype, need_rstd: bool):
-    """(8-bit rows, h or x2, rstd or None) of matrices."""
-    R, D = x2.shape
-    if not x2.is_cuda:
-        x2, w = x2.detach(), w.detach()
-        h = x2 if r2 is None else (x2.float() + r2.detach().float()).to(x2.dtype)
-        rstd = torch.rsqrt(h.float().pow(2).mean(-1) + eps)
-        return _pack_ref(h.float() * rstd[:, None] * (w_offset + w.float()), dtype), h, rstd
-    q = Fp8Tensor.empty(R, D, dtype, x2.device)
-    h = torch.empty((R, D), dtype=x2.dtype, device=x2.device) if r2 is not None else None
-    rstd = torch.empty(R, dtype=torch.float32, device=x2.device) if need_rstd else None
-    if R:
-        if w.stride(0) != 1:
-            w = w.contiguous()
-        nv.check(nv.cuda().cvb_fp8_add_rmsnorm(
-            x2.data_ptr(), x2.stride(0), nv.ptr(r2), r2.stride(0) if r2 is not None else 0, w.data_ptr(), nv.ptr(h),
-            *q._pointers(), nv.ptr(rstd), R, D, _FMT[dtype], eps, w_offset, _stream()),
-            "cvb_fp8_add_rmsnorm")
-        count_launch()
-    return q, (h if h is not None else x2), rstd
+def _norm_ref(x2, r2, w, eps, w_offset):
+    """(fp32 norm, h, rstd) of matrices in PyTorch."""
+    h = x2 if r2 is None else (x2.float() + r2.float()).to(x2.dtype)
+    rstd = torch.rsqrt(h.float().pow(2).mean(-1) + eps)
+    return h.float() * rstd[:, None] * (w_offset + w.float()), h, rstd
 
 
-@_on_device
 def add_rmsnorm_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], w: torch.Tensor, eps: float = 1e-6,
                     w_offset: float = 1.0, dtype: torch.dtype = E4M3) -> Tuple[Fp8Tensor, torch.Tensor]:
     """``(Q(rmsnorm(x + resid)), x + resid)``; ``resid`` may be None.  The norm is rounded once, from fp32 to 8 bits;
@@ -358,10 +289,13 @@ def add_rmsnorm_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], w: torch.Ten
     _check_norm(x, resid, w, "add_rmsnorm_fp8")
     if _needs_grad(x, resid, w):
         raise RuntimeError("add_rmsnorm_fp8 has no gradient: call it under torch.no_grad(), or add_rmsnorm_linear_fp8")
-    q, h, _ = _norm_forward(_rows2d(x), _rows2d(resid) if resid is not None else None, w, eps, w_offset, dtype, False)
-    if resid is None:
-        return q, x
-    return q, h if x.dim() == 2 else h.view(x.shape)
+    D = x.shape[-1]
+    if x.is_cuda:
+        q, h = nv.torch_ext().norm(x, resid, w, eps, w_offset, _FMT[dtype])
+        return Fp8Tensor(q, x.numel() // D, D, dtype), (x if h is None else h)
+    with torch.no_grad():
+        y, h, _ = _norm_ref(_rows2d(x), _rows2d(resid) if resid is not None else None, w, eps, w_offset)
+        return _pack_ref(y, dtype), (x if resid is None else h.view(x.shape))
 
 
 # ----------------------------------------------------------------------------
@@ -386,123 +320,88 @@ def _check_linear(rows: int, K: int, device, w, weight: Optional[Fp8Weight], gra
         raise ValueError(f"{what}: the 8-bit weight is given twice")
 
 
-def _quantised_within(M: int, K: int) -> bool:
-    """Whether the product quantises its bf16 rows itself (rows whose transpose nobody needs): every tile of 128 columns
-    does it for its share of K, in series, so for few rows of moderate length.  Back to back, against two kernels: one row,
-    K = 1024, N = 7168: 5.3 us against 6.6; 16 rows, K = 3584, N = 1024: 6.1 against 7.3; 32 rows, K = 2048: 7.2 against
-    7.5; 64 rows: 10.6 against 8.2; 16 rows, K = N = 8192: 14.2 against 11.9.  And one launch less."""
-    return M <= 16 and K <= 4096 or M <= 32 and K <= 2048
+# The PyTorch statement of the layers: the CPU path, and the oracle of the tests.  (CUDA: torch_ext/fp8_torch.cc.)
+def _gradients_ref(dy2, xt, wt, w, grad_dtype, dx_dtype):
+    """(dx or None, dw or None) from the transposed 8-bit forms; dw goes to the parameter's main_grad where it has one."""
+    dx = dw = None
+    if wt is not None:
+        dx = gemm_fp8_nt(_pack_ref(dy2, grad_dtype), wt, out_dtype=dx_dtype)
+    if w is not None:
+        main = getattr(w, "main_grad", None)
+        if main is None:
+            dw = gemm_fp8_nt(_pack_ref(dy2.t(), grad_dtype), xt, out_dtype=w.dtype)
+        elif main.dtype != torch.float32 or not main.is_contiguous() or main.numel() != w.numel():
+            raise TypeError("main_grad is a contiguous float32 tensor of the parameter's size")
+        else:
+            gemm_fp8_nt(_pack_ref(dy2.t(), grad_dtype), xt, main.view(w.shape), accumulate=True)
+    return dx, dw
 
 
-def _forward(x2, xq, w, weight: Optional[Fp8Weight], M, N, K, need_wt: bool, need_xt: bool, dtype):
-    """``(y, xt, wt, wt_off)``: the product, and the transposed 8-bit forms that gradients read: ``xt`` at the start of
-    its buffer, ``wt`` at ``wt_off`` bytes of its (buffers or None).  ``x2`` is the input's rows or None where ``xq`` is
-    its 8-bit form; ``w`` the weight or None where ``weight`` is."""
-    device = (x2 if x2 is not None else xq.buf).device
-    y = _alloc_rows(M, N, dtype, device)
-    if not y.is_cuda or not (M and N and K):
-        xt = None
-        if x2 is not None:
-            xq, xt = _quantize(x2, E4M3, _ROWS | (_COLS if need_xt else 0))
-        weight = weight or quantize_fp8_weight(w, transposed=need_wt)
-        gemm_fp8_nt(xq, weight.w, y)
-        return y, xt.buf if need_xt else None, weight.wt.buf if need_wt else None, 0
-    # workspaces: 8-bit x and w for this product; 8-bit x^T and w^T kept for the gradients
-    fused = xq is None and not need_xt and x2.dtype == torch.bfloat16 and _quantised_within(M, K)
-    xq_n = 0 if xq is not None or fused else _nbytes(M, K)
-    xt_n = _nbytes(K, M) if need_xt else 0
-    wq_n = wt_n = x_stride = w_stride = 0
-    x_fp32 = w_fp32 = False
-    if weight is None:
-        w = _check_matrix(w, "linear_fp8 weight")
-        wq_n, wt_n = _nbytes(N, K), _nbytes(K, N) if need_wt else 0
-        w_ptr, w_stride, w_fp32 = w.data_ptr(), w.stride(0), w.dtype == torch.float32
-    else:
-        w_ptr = None
-    temp = _bytes(xq_n + wq_n, device) if xq_n + wq_n else None
-    keep = _bytes(xt_n + wt_n, device) if xt_n + wt_n else None
-    temp_ptr = temp.data_ptr() if temp is not None else 0
-    keep_ptr = keep.data_ptr() if keep is not None else 0
-    if x2 is not None:
-        x_ptr, x_stride, x_fp32 = x2.data_ptr(), x2.stride(0), x2.dtype == torch.float32
-    else:
-        x_ptr = None
-    nv.check(nv.cuda().cvb_fp8_linear_fwd(
-        x_ptr, x_fp32, x_stride, w_ptr, w_fp32, w_stride, M, N, K,
-        None if fused else temp_ptr if xq_n else xq.buf.data_ptr(),
-        keep_ptr if xt_n else None, temp_ptr + xq_n if weight is None else weight.w.buf.data_ptr(),
-        keep_ptr + xt_n if wt_n else None, y.data_ptr(), max(y.stride(0), N), _OUT[dtype], _status(), _stream()),
-        "cvb_fp8_linear_fwd")
-    count_launch(1 + (x_ptr is not None and not fused) + (w_ptr is not None))
-    if need_wt and weight is not None:
-        return y, keep, weight.wt.buf, 0
-    return y, keep if need_xt else None, keep if need_wt else None, xt_n
-
-
-def _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, dx_dtype, norm=None):
-    """``(dx or None, dw or None)`` of ``y = x w^T``: dx where ``wt`` is given, dw where the parameter ``w`` is (added
-    to its fp32 ``main_grad`` where it has one, and then None).  ``norm = (h, rstd, wn, w_offset)`` stands for ``xt`` on the CPU."""
-    if dy.is_cuda and dy.get_device() != _current_device():
-        with torch.cuda.device(dy.device):
-            return _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, dx_dtype, norm)
-    dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N) if dy.numel() else dy.reshape(0, N), "linear_fp8 gradient")
-    dx = _alloc_rows(M, K, dx_dtype, dy.device) if wt is not None else None
-    target, is_main = _grad_target(w, N, K, "linear_fp8") if w is not None else (None, False)
-    if not (M and N and K):
-        if dx is not None:
-            dx.zero_()
-        if target is not None and not is_main:
-            target.zero_()
-    elif not dy2.is_cuda:
-        qdy, qdyt = _quantize(dy2, grad_dtype, (_ROWS if wt is not None else 0) | (_COLS if w is not None else 0))
-        if dx is not None:
-            gemm_fp8_nt(qdy, Fp8Tensor(wt, K, N, E4M3), dx)
-        if target is not None:
-            if norm is not None:
-                xt = _quantize(norm[0], E4M3, _COLS, *norm[1:])[1].buf
-            gemm_fp8_nt(qdyt, Fp8Tensor(xt, K, M, E4M3), target, accumulate=is_main)
-    else:
-        dyq_n = _nbytes(M, N) if wt is not None else 0
-        dyt_n = _nbytes(N, M) if w is not None else 0
-        temp = _bytes(dyq_n + dyt_n, dy.device)
-        base = temp.data_ptr()
-        dx_ptr = dw_ptr = wt_ptr = None
-        dx_stride = dw_stride = dw_kind = 0
-        if wt is not None:
-            wt_ptr, dx_ptr, dx_stride = wt.data_ptr() + wt_off, dx.data_ptr(), max(dx.stride(0), K)
-        if w is not None:
-            dw_ptr, dw_stride, dw_kind = target.data_ptr(), max(target.stride(0), K), 2 if is_main else _OUT[w.dtype]
-        nv.check(nv.cuda().cvb_fp8_linear_bwd(
-            dy2.data_ptr(), dy2.dtype == torch.float32, dy2.stride(0), _FMT[grad_dtype], M, N, K, base, base + dyq_n,
-            wt_ptr, nv.ptr(xt), None, 0, None, None, 0.0, dx_ptr, dx_stride, _OUT[dx_dtype], dw_ptr,
-            dw_stride, dw_kind, _status(), _stream()), "cvb_fp8_linear_bwd")
-        count_launch(1 + (wt is not None) + (w is not None))
-    return dx, (None if is_main else target)
-
-
-class _LinearFp8(torch.autograd.Function):
+class _LinearRef(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, weight, grad_dtype):
-        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        if need_dx and weight is not None and weight.wt is None:
-            raise ValueError("linear_fp8: the gradient of the input needs the transposed 8-bit weight")
         x2 = _rows2d(x)
-        (M, K), N = x2.shape, w.shape[0]
-        y, xt, wt, wt_off = _forward(x2, None, w, weight, M, N, K, need_dx, need_dw, x.dtype)
-        # what the gradients read: x^T and w^T in 8 bits, half of what the bf16 layer keeps of x
-        ctx.save_for_backward(w if need_dw else None, xt, wt)
-        ctx.cfg = (x.shape, x.dtype, M, N, K, grad_dtype, wt_off)
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
+        weight = weight or quantize_fp8_weight(w)
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        if need_dx and weight.wt is None:
+            raise ValueError("linear_fp8: the gradient of the input needs the transposed 8-bit weight")
+        ctx.forms = (_pack_ref(x2.t(), E4M3) if need_dw else None, weight.wt if need_dx else None)
+        ctx.save_for_backward(w if need_dw else None)
+        ctx.cfg = (x.shape, x.dtype, grad_dtype)
+        return gemm_fp8_nt(_pack_ref(x2, E4M3), weight.w, out_dtype=x.dtype).reshape(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        w, xt, wt = ctx.saved_tensors
-        shape, xdtype, M, N, K, grad_dtype, wt_off = ctx.cfg
-        dx, dw = _backward(dy, M, N, K, grad_dtype, wt, wt_off, xt, w, xdtype)
-        if dx is not None and len(shape) != 2:
-            dx = dx.reshape(shape)
-        return dx, dw, None, None
+        shape, dtype, grad_dtype = ctx.cfg
+        dx, dw = _gradients_ref(_rows2d(dy), *ctx.forms, ctx.saved_tensors[0], grad_dtype, dtype)
+        return (dx.reshape(shape) if dx is not None else None), dw, None, None
+
+
+class _NormLinearRef(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, resid, wn, w, weight, eps, w_offset, grad_dtype):
+        weight = weight or quantize_fp8_weight(w)
+        need_dn, need_dw = any(ctx.needs_input_grad[:3]), ctx.needs_input_grad[3]
+        if need_dn and weight.wt is None:
+            raise ValueError("add_rmsnorm_linear_fp8: the gradient of the input needs the transposed 8-bit weight")
+        n, h, rstd = _norm_ref(_rows2d(x), _rows2d(resid) if resid is not None else None, wn, eps, w_offset)
+        ctx.forms = (_pack_ref(n.t(), E4M3) if need_dw else None, weight.wt if need_dn else None)
+        ctx.save_for_backward(h, rstd, wn, w if need_dw else None)
+        ctx.cfg = (x.shape, w_offset, grad_dtype)
+        y = gemm_fp8_nt(_pack_ref(n, E4M3), weight.w, out_dtype=x.dtype).reshape(*x.shape[:-1], w.shape[0])
+        return y if resid is None else (y, h.view(x.shape))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, rstd, wn, w = ctx.saved_tensors
+        shape, w_offset, grad_dtype = ctx.cfg
+        dn, dw = _gradients_ref(_rows2d(dy), *ctx.forms, w, grad_dtype, torch.float32)
+        dx = dwn = None
+        if dn is not None:
+            xh, g = h.float() * rstd[:, None], dn * (w_offset + wn.float())
+            dx = rstd[:, None] * (g - xh * (g * xh).mean(-1, keepdim=True))
+            if dh is not None:
+                dx = dx + _rows2d(dh).float()
+            dx = dx.to(h.dtype).view(shape)
+            if ctx.needs_input_grad[2]:
+                dwn = (dn * xh).sum(0)
+                main = getattr(wn, "main_grad", None)
+                if main is not None:
+                    main.view(-1).add_(dwn)
+                    dwn = None
+                else:
+                    dwn = dwn.to(wn.dtype)
+        need_x, need_r = ctx.needs_input_grad[:2]
+        return (dx if need_x else None), (dx if need_r else None), dwn, dw, None, None, None, None
+
+
+def _parts(w, kept):
+    """What the extension takes for a weight: (parameter, 8-bit weight, its transpose), each None where there is none."""
+    if kept is None:
+        return w, None, None
+    return (None if kept is w else w), kept.w.buf, (kept.wt.buf if kept.wt is not None else None)
 
 
 class _Shape:
@@ -521,7 +420,6 @@ def _needs_grad(*tensors) -> bool:
     return False
 
 
-@_on_device
 def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dtype = E4M3) -> torch.Tensor:
     """``x [..., K] @ w [N, K].T`` with both operands rounded to 8 bits.
 
@@ -537,7 +435,10 @@ def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dt
             raise TypeError(f"{what}: inputs are torch.float8_e4m3fn, got {x.dtype}")
         if _needs_grad(w):
             raise RuntimeError(f"{what}: an 8-bit input carries no gradient: call it under torch.no_grad()")
-        return _forward(None, x, w, kept, x.rows, w.shape[0], x.cols, False, False, torch.bfloat16)[0]
+        if not x.buf.is_cuda:
+            return gemm_fp8_nt(x, (kept or quantize_fp8_weight(w, transposed=False)).w)
+        p, wq, _ = _parts(w, kept)
+        return nv.torch_ext().linear_rows8(x.buf, x.rows, x.cols, p, wq, w.shape[0], _status(x.buf.get_device()))
     shape = x.shape
     if not shape:
         raise ValueError(f"{what}: x has no dimensions")
@@ -545,163 +446,11 @@ def linear_fp8(x, w, *, weight: Optional[Fp8Weight] = None, grad_dtype: torch.dt
         raise TypeError(f"{what}: bfloat16 is wanted, got {x.dtype}")
     K = shape[-1]
     _check_linear(x.numel() // K if K else 0, K, x.device, w, weight, grad_dtype, what)
-    if not _needs_grad(x, w):
-        x2 = _rows2d(x)
-        N = w.shape[0]
-        y = _forward(x2, None, w, kept, x2.shape[0], N, K, False, False, x.dtype)[0]
-        return y if len(shape) == 2 else y.reshape(*shape[:-1], N)
-    if kept is w:
-        w = _Shape(w.shape)
-    return _LinearFp8.apply(x, w, kept, grad_dtype)
+    if x.is_cuda:
+        return nv.torch_ext().linear(x, *_parts(w, kept), w.shape[0], _FMT[grad_dtype], _status(x.get_device()))
+    return _LinearRef.apply(x, _Shape(w.shape) if kept is w else w, kept, grad_dtype)
 
 
-def _norm_linear_forward(x2, r2, wn, w, weight, eps, w_offset, need_wt: bool, need_rstd: bool):
-    """``(y, h, rstd, wt, wt_off)`` of matrices; ``h`` is ``x2`` without a residual, ``rstd`` None where not asked for."""
-    (M, K), N = x2.shape, w.shape[0]
-    if not x2.is_cuda or not (M and N and K):
-        q, h, rstd = _norm_forward(x2, r2, wn, eps, w_offset, E4M3, need_rstd)
-        y, _, wt, wt_off = _forward(None, q, w, weight, M, N, K, need_wt, False, x2.dtype)
-        return y, h, rstd, wt, wt_off
-    device = x2.device
-    y = _alloc_rows(M, N, x2.dtype, device)
-    h = torch.empty((M, K), dtype=x2.dtype, device=device) if r2 is not None else None
-    if wn.stride(0) != 1:
-        wn = wn.contiguous()
-    rstd = torch.empty(M, dtype=torch.float32, device=device) if need_rstd else None
-    xq_n = _nbytes(M, K)
-    w_ptr = wt_ptr = keep = None
-    wq_n = w_stride = 0
-    w_fp32 = False
-    if weight is None:
-        w = _check_matrix(w, "linear_fp8 weight")
-        w_ptr, w_stride, w_fp32, wq_n = w.data_ptr(), w.stride(0), w.dtype == torch.float32, _nbytes(N, K)
-        if need_wt:
-            keep = _bytes(_nbytes(K, N), device)
-            wt_ptr = keep.data_ptr()
-    temp = _bytes(xq_n + wq_n, device)
-    temp_ptr = temp.data_ptr()
-    nv.check(nv.cuda().cvb_fp8_norm_linear_fwd(
-        x2.data_ptr(), x2.stride(0), nv.ptr(r2), r2.stride(0) if r2 is not None else 0, wn.data_ptr(), nv.ptr(h),
-        nv.ptr(rstd), eps, w_offset, w_ptr, w_fp32, w_stride, M, N, K, temp_ptr,
-        temp_ptr + xq_n if weight is None else weight.w.buf.data_ptr(), wt_ptr, y.data_ptr(), max(y.stride(0), N),
-        _OUT[x2.dtype], _status(), _stream()), "cvb_fp8_norm_linear_fwd")
-    count_launch(2 + (w_ptr is not None))
-    if need_wt and weight is not None:
-        keep = weight.wt.buf
-    return y, (h if h is not None else x2), rstd, keep, 0
-
-
-class _NormLinearFp8(torch.autograd.Function):
-    """(linear(rmsnorm(x + resid)), x + resid) with the norm's result in 8 bits only."""
-
-    @staticmethod
-    def forward(ctx, x, resid, wn, w, weight, eps, w_offset, grad_dtype):
-        need_dn, need_dw = any(ctx.needs_input_grad[:3]), ctx.needs_input_grad[3]
-        if need_dn and weight is not None and weight.wt is None:
-            raise ValueError("add_rmsnorm_linear_fp8: the gradient of the input needs the transposed 8-bit weight")
-        y, h, rstd, wt, wt_off = _norm_linear_forward(
-            _rows2d(x), _rows2d(resid) if resid is not None else None, wn, w, weight, eps, w_offset, need_dn, True)
-        ctx.save_for_backward(h, rstd, wn, w if need_dw else None, wt)
-        ctx.cfg = (x.shape, h.shape[0], w.shape[0], h.shape[1], w_offset, grad_dtype, wt_off)
-        if x.dim() != 2:
-            y, h = y.reshape(*x.shape[:-1], w.shape[0]), h.view(x.shape)
-        return y if resid is None else (y, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, rstd, wn, w, wt = ctx.saved_tensors
-        shape, M, N, K, w_offset, grad_dtype, wt_off = ctx.cfg
-        need_x, need_r, need_wn = ctx.needs_input_grad[:3]
-        # The norm's result is formed again from h and rstd while its transpose is quantised: it is never stored.  Its
-        # gradient stays fp32 between the product and the norm's backward.
-        norm = (h, rstd, wn if wn.stride(0) == 1 else wn.contiguous(), w_offset)
-        if dy.is_cuda and M and N and K:
-            dx, dwn, dw = _norm_linear_backward(dy, dh, M, N, K, grad_dtype, wt, wt_off, w, norm, wn if need_wn else None)
-        else:
-            dn, dw = _backward(dy, M, N, K, grad_dtype, wt, wt_off, None, w, torch.float32, norm)
-            dx, dwn = _norm_backward_ref(dn, h, wn, rstd, dh, w_offset, need_wn) if dn is not None else (None, None)
-        if dx is not None and len(shape) != 2:
-            dx = dx.view(shape)
-        return (dx if need_x else None), (dx if need_r else None), dwn, dw, None, None, None, None
-
-
-def _grad_target(w, rows: int, cols: int, what: str):
-    """(where a weight's gradient goes, whether that is its main_grad)."""
-    main = getattr(w, "main_grad", None)
-    if main is None:
-        return _alloc_rows(rows, cols, w.dtype, w.device), False
-    if main.dtype != torch.float32 or not main.is_contiguous():
-        raise TypeError(f"{what}: main_grad is a contiguous float32 tensor")
-    return main.view(rows, cols), True
-
-
-def _norm_linear_backward(dy, dh, M, N, K, grad_dtype, wt, wt_off, w, norm, wn_param):
-    """``(dx, dwn, dw)``, each None where it is not wanted or went to a main_grad."""
-    if dy.get_device() != _current_device():
-        with torch.cuda.device(dy.device):
-            return _norm_linear_backward(dy, dh, M, N, K, grad_dtype, wt, wt_off, w, norm, wn_param)
-    h, rstd, wn, w_offset = norm
-    device = dy.device
-    dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N), "linear_fp8 gradient")
-    dh2 = _rows2d(dh) if dh is not None and wt is not None else None
-    lib = nv.cuda()
-    # one workspace: dy in both forms, the norm's result transposed, its gradient, and the parts of dwn
-    dyq_n = _nbytes(M, N) if wt is not None else 0
-    dyt_n, xt_n = (_nbytes(N, M), _nbytes(K, M)) if w is not None else (0, 0)
-    lddn = _ceil(K, 8) * 8
-    dn_n = M * lddn * 4 if wt is not None else 0
-    parts = min(M, lib.cvb_fp8_norm_bwd_parts()) if wn_param is not None else 0
-    temp = _bytes(_ceil(dyq_n + dyt_n + xt_n, 32) * 32 + dn_n + parts * K * 4, device)
-    base = temp.data_ptr()
-    dn_at = base + _ceil(dyq_n + dyt_n + xt_n, 32) * 32
-    wt_ptr = dx = dx_ptr = dw = dw_ptr = dwn = acc_ptr = dwn_ptr = part_ptr = None
-    dw_stride = dw_kind = 0
-    if wt is not None:
-        wt_ptr = wt.data_ptr() + wt_off
-        dx = torch.empty((M, K), dtype=h.dtype, device=device)
-        dx_ptr = dx.data_ptr()
-    if w is not None:
-        target, is_main = _grad_target(w, N, K, "linear_fp8")
-        dw_ptr, dw_stride, dw_kind = target.data_ptr(), max(target.stride(0), K), 2 if is_main else _OUT[w.dtype]
-        dw = None if is_main else target
-    if wn_param is not None:
-        part_ptr = dn_at + dn_n
-        if getattr(wn_param, "main_grad", None) is not None:
-            acc_ptr = _grad_target(wn_param, 1, K, "add_rmsnorm_linear_fp8")[0].data_ptr()
-        else:
-            dwn = torch.empty(K, dtype=wn_param.dtype, device=device)
-            dwn_ptr = dwn.data_ptr()
-    nv.check(lib.cvb_fp8_norm_linear_bwd(
-        dy2.data_ptr(), dy2.dtype == torch.float32, dy2.stride(0), _FMT[grad_dtype], M, N, K, base, base + dyq_n, wt_ptr,
-        base + dyq_n + dyt_n, h.data_ptr(), h.stride(0), rstd.data_ptr(), wn.data_ptr(), w_offset, dn_at, lddn, dw_ptr,
-        dw_stride, dw_kind, nv.ptr(dh2), dh2.stride(0) if dh2 is not None else 0, dx_ptr, part_ptr, acc_ptr, dwn_ptr,
-        _status(), _stream()), "cvb_fp8_norm_linear_bwd")
-    count_launch(1 + (2 if wt is not None else 0) + (2 if w is not None else 0) + (wn_param is not None))
-    return dx, dwn, dw
-
-
-def _norm_backward_ref(dn, h, wn, rstd, dh, w_offset, need_dwn):
-    """``(dx, dwn)`` of the norm in PyTorch; without rows on any device."""
-    D = h.shape[1]
-    xh, d32 = h.float() * rstd[:, None], dn.float()
-    g = d32 * (w_offset + wn.float())
-    dx = rstd[:, None] * (g - xh * (g * xh).mean(-1, keepdim=True))
-    if dh is not None:
-        dx = dx + _rows2d(dh).float()
-    dwn = None
-    if need_dwn:
-        dwn = (d32 * xh).sum(0)
-        main = getattr(wn, "main_grad", None)
-        if main is not None:
-            main.view(D).add_(dwn)
-            dwn = None
-        else:
-            dwn = dwn.to(wn.dtype)
-    return dx.to(h.dtype), dwn
-
-
-@_on_device
 def add_rmsnorm_linear_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], norm_w: torch.Tensor, w, eps: float = 1e-6,
                            w_offset: float = 1.0, *, weight: Optional[Fp8Weight] = None,
                            grad_dtype: torch.dtype = E4M3) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -712,11 +461,9 @@ def add_rmsnorm_linear_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], norm_
     K, N = x.shape[-1], w.shape[0] if len(w.shape) else 0
     _check_linear(x.numel() // K, K, x.device, w, weight, grad_dtype, what)
     kept = w if isinstance(w, Fp8Weight) else weight
-    if not _needs_grad(x, resid, norm_w, w):
-        y, h, *_ = _norm_linear_forward(_rows2d(x), _rows2d(resid) if resid is not None else None, norm_w, w, kept, eps,
-                                        w_offset, False, False)
-        if x.dim() != 2:
-            y, h = y.reshape(*x.shape[:-1], N), h.view(x.shape)
-        return y, x if resid is None else h
-    out = _NormLinearFp8.apply(x, resid, norm_w, _Shape(w.shape) if kept is w else w, kept, eps, w_offset, grad_dtype)
+    if x.is_cuda:
+        out = nv.torch_ext().norm_linear(x, resid, norm_w, *_parts(w, kept), N, eps, w_offset, _FMT[grad_dtype],
+                                         _status(x.get_device()))
+        return out[0], (x if resid is None else out[1])
+    out = _NormLinearRef.apply(x, resid, norm_w, _Shape(w.shape) if kept is w else w, kept, eps, w_offset, grad_dtype)
     return (out, x) if resid is None else out

@@ -429,6 +429,71 @@ def test_backward_twice_and_expanded_gradient():
     assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
+def test_batches_of_sequences_and_computed_weights():
+    """Leading dimensions are kept, a weight may be the result of an operation, a gradient may be missing or strided."""
+    x, r = _rand(3, 7, 260, seed=1).requires_grad_(), _rand(3, 7, 260, seed=2).requires_grad_()
+    w, wn = _rand(130, 260, seed=3).requires_grad_(), _rand(260, seed=4, std=0.1).requires_grad_()
+    dy = _rand(3, 7, 130, seed=5)
+    flat = torch.autograd.grad(ops.linear_fp8(x.view(21, 260), w), (x, w), dy.view(21, 130))
+    got = torch.autograd.grad(ops.linear_fp8(x, w * 1.0), (x, w), dy.transpose(0, 1).contiguous().transpose(0, 1))
+    assert got[0].shape == x.shape and all(torch.equal(a, b.view_as(a)) for a, b in zip(got, flat))
+    y, h = ops.add_rmsnorm_linear_fp8(x, r, wn, w)
+    assert y.shape == (3, 7, 130) and torch.equal(h, x + r)
+    y2, h2 = ops.add_rmsnorm_linear_fp8(x.view(21, 260), r.view(21, 260), wn, w)
+    assert torch.equal(y.view(21, 130), y2)
+    a = torch.autograd.grad(y, (x, r, wn, w), dy, retain_graph=True)
+    b = torch.autograd.grad(y2, (x, r, wn, w), dy.view(21, 130))
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
+    dh, = torch.autograd.grad(h, x, torch.ones_like(h))             # only h is used
+    assert torch.equal(dh, torch.ones_like(dh))
+    with torch.no_grad():
+        q, h3 = ops.add_rmsnorm_fp8(x, r, wn)
+        assert q.shape == (21, 260) and torch.equal(h3, h) and torch.equal(ops.linear_fp8(q, w), y2)
+    one = torch.autograd.grad(ops.linear_fp8(x[0, 0], w), w, dy[0, 0])[0]        # a single row without dimensions
+    assert one.shape == w.shape
+
+
+def test_only_some_gradients():
+    x, w, wn, r = _rand(40, 200, seed=1), _rand(30, 200, seed=2), _rand(200, seed=3), _rand(40, 200, seed=4)
+    full = [t.clone().requires_grad_() for t in (x, r, wn, w)]
+    dy = _rand(40, 30, seed=5)
+    want = torch.autograd.grad(ops.add_rmsnorm_linear_fp8(*full)[0], full, dy)
+    for i in range(4):
+        leaves = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, r, wn, w))]
+        got, = torch.autograd.grad(ops.add_rmsnorm_linear_fp8(*leaves)[0], leaves[i], dy)
+        assert torch.equal(got, want[i])
+    for t in (x, w):
+        t.requires_grad_()
+        g, = torch.autograd.grad(ops.linear_fp8(x, w), t, dy)
+        t.requires_grad_(False)
+        both = torch.autograd.grad(ops.linear_fp8(*(a := [v.clone().requires_grad_() for v in (x, w)])), a, dy)
+        assert torch.equal(g, both[0 if t is x else 1])
+
+
+def test_no_second_derivative():
+    x, w = _rand(4, 64, seed=1).requires_grad_(), _rand(8, 64, seed=2).requires_grad_()
+    g, = torch.autograd.grad(ops.linear_fp8(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.add_rmsnorm_fp8(x, None, _rand(64))
+    with pytest.raises(ValueError, match="transposed"):
+        ops.linear_fp8(x, ops.quantize_fp8_weight(w, transposed=False))
+
+
+def test_launches_are_counted():
+    from cverl_b200.ops.gemm import launch_counter
+    x, w, wn = _rand(200, 256, seed=1).requires_grad_(), _rand(300, 256, seed=2).requires_grad_(), _rand(256).requires_grad_()
+    n = launch_counter["n"]
+    y = ops.linear_fp8(x, w)                                # weight, input, product
+    assert launch_counter["n"] == n + 3
+    y.backward(torch.ones_like(y))                          # gradient, two products
+    assert launch_counter["n"] == n + 6
+    y, _ = ops.add_rmsnorm_linear_fp8(x, None, wn, w)       # weight, norm, product
+    y.backward(torch.ones_like(y))                          # gradient, norm's transpose, two products, norm, its weight
+    assert launch_counter["n"] == n + 15
+
+
 def test_empty_calls():
     w = _rand(30, 200, seed=2).requires_grad_()
     x = torch.empty(0, 200, dtype=torch.bfloat16, device="cuda", requires_grad=True)
