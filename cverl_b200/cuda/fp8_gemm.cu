@@ -348,11 +348,15 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const int n = n0 + lane * 4, nn = min(4, p.N - n);
   const uint32_t part = smem_u32(smem) + lane * 16;
   for (int r = rank + warp * p.split; r < min(TN, p.M - m0); r += (F8_THREADS / 32) * p.split) {
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.split; ++s) {
-      const float4 v = ld_cluster4(mapa_cluster(part + r * 512, s));
-      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-    }
+    // all of a row's loads are under way before the first is used (128 rows, N = 1024, K = 3584: 7.7 us against 8.1)
+    float4 v[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s < p.split) v[s] = ld_cluster4(mapa_cluster(part + r * 512, s));
+    float4 sum = v[0];
+#pragma unroll
+    for (int s = 1; s < 8; ++s)
+      if (s < p.split) sum.x += v[s].x, sum.y += v[s].y, sum.z += v[s].z, sum.w += v[s].w;
     if (nn > 0) fp8_store4(p, static_cast<long long>(m0 + r) * p.ldc + n, sum, nn);
   }
   cluster_sync_all();   // nobody leaves while a peer reads its tile
@@ -760,7 +764,7 @@ static int launch_small(const Fp8Operands& o, Fp8GemmParams p, cudaStream_t stre
   p.n_tiles = (p.N + 127) / 128;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
   // Fill the SMs: one CTA each (two where each still has 8 K blocks), clusters of eight only where few of them have to
-  // find room.  One token, N = 1024, K = 3584: 10.2 us with one CTA a tile, 4.5 with eight; 128 rows, N = K = 2048:
+  // find room.  One token, N = 1024, K = 3584: 10.2 us with one CTA a tile, 4.3 with eight; 128 rows, N = K = 2048:
   // 12.2 with one, 7.4 with four, 8.8 with eight; 128 rows, N = K = 8192: 27.0 with one, 17.6 with two, 14.6 with four.
   p.split = 1;
   while (p.split < 8) {
@@ -897,7 +901,7 @@ extern "C" int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int 
   const Fp8Operands o = {a, b, lda, ldb, M, N, K};
   const PairChoice pick = choose_pair(p.M, p.N, p.kblocks);
   // Above 128 rows always pairs; from 65 where tiles of 128 columns fill half of the SMs and K is short (128 rows,
-  // N = 7168, K = 1024: 6.4 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 7.9; N = K = 8192:
+  // N = 7168, K = 1024: 6.6 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 7.7; N = K = 8192:
   // 19.2 against 14.6).
   if (M > 128 || (M > 64 && N >= 37 * 128 && p.kblocks <= 12)) {
     if (pick.split == 2)
