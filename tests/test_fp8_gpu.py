@@ -74,7 +74,8 @@ def _whole(rows, cols, seed):
 PRODUCTS = [(1, 1, 1), (1, 128, 128), (1, 7168, 1024), (2, 129, 513), (15, 300, 130), (16, 256, 2048), (17, 65, 16),
             (33, 127, 640), (64, 1000, 1000), (65, 512, 129), (128, 1024, 3584), (129, 130, 4096), (200, 4000, 256),
             (333, 1003, 1111), (512, 512, 512), (1000, 257, 385), (2049, 260, 131), (257, 2304, 1024),
-            (1536, 1600, 640), (4100, 1024, 512), (300, 300, 9000)]
+            (1536, 1600, 640), (4100, 1024, 512), (300, 300, 9000), (300, 1, 200), (1000, 7, 129),
+            (129, 128, 1)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
