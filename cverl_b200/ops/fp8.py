@@ -80,6 +80,9 @@ class Fp8Tensor:
     __slots__ = ("buf", "rows", "cols", "dtype", "ld")
 
     def __init__(self, buf: torch.Tensor, rows: int, cols: int, dtype: torch.dtype):
+        if (buf.dtype != torch.uint8 or buf.dim() != 1 or buf.numel() != _nbytes(rows, cols) + _nbytes_plain(rows, cols)
+                or buf.storage_offset() or dtype not in _FMT):
+            raise ValueError(f"Fp8Tensor: not a buffer of a [{rows}, {cols}] matrix in {dtype}")
         self.buf, self.rows, self.cols, self.dtype = buf, rows, cols, dtype
         self.ld = (cols + 15) // 16 * 16
 

@@ -194,6 +194,8 @@ def test_refusals():
         (TypeError, lambda: ops.linear_fp8(torch.ones(2, 8).half(), torch.ones(4, 8))),
         (TypeError, lambda: ops.linear_fp8(torch.ones(2, 8), torch.ones(4, 8).half())),
         (ValueError, lambda: ops.linear_fp8(torch.ones(2, 8), torch.ones(4, 8), weight=ops.quantize_fp8_weight(torch.ones(5, 8)))),
+        (ValueError, lambda: ops.Fp8Tensor(torch.zeros(8, dtype=torch.uint8), 4, 8, E4M3)),
+        (ValueError, lambda: ops.Fp8Tensor(good.buf, 3, 17, E4M3)),
         (ValueError, lambda: ops.Fp8Weight(ops.quantize_fp8(torch.ones(4, 8), E5M2))),
         (ValueError, lambda: ops.Fp8Weight(good, a)),
         (TypeError, lambda: ops.linear_fp8(ops.quantize_fp8(torch.ones(2, 8), E5M2), ops.quantize_fp8_weight(torch.ones(4, 8)))),
