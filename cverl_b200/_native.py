@@ -126,6 +126,8 @@ _CUDA_PROTOS = {
     "cvb_fp8_norm_bwd_parts": "",
     "cvb_fp8_norm_bwd": "pl pl pp pl pp pp l i f p",
     "cvb_fp8_gemm": "ppli ppli iii p l i p p",
+    "cvb_fp8_gemm_grads": "ppl ppl ppl ppl i iii p l i p l i p p",
+    "cvb_fp8_gemm_grads_launches": "iii",
     "cvb_fp8_linear_fwd": "pil pil iii pppp p l i p p",
     "cvb_fp8_linear_bwd": "pil i iii pppp pl pp f pli pli p p",
     "cvb_fp8_norm_linear_fwd": "plpl pp p ff pil iii ppp p l i p p",

@@ -403,7 +403,7 @@ struct F8PairCfg {
   static constexpr int SF_GROUPS = BN == 128 ? 1 : 2;       // groups of 128 rows of B whose scales a tile reads
   static constexpr int SF_BYTES = (1 + SF_GROUPS) * 512;    // and those of A's rows of this CTA
   static constexpr int STAGES = OVERLAP ? 6 : BN == 192 ? 7 : 8;
-  static constexpr int SF_SLOTS = 3;                        // TMEM copies of the scales of four K blocks
+  static constexpr int SF_SLOTS = 4;                        // TMEM copies of the scales of four K blocks
   static constexpr int ACC1 = OVERLAP ? 192 : BN;
   static constexpr int SF_COL = ACC1 + BN;                  // 16 columns a slot
   static constexpr int THREADS = 64 + 32 * 8;
@@ -411,9 +411,11 @@ struct F8PairCfg {
   static constexpr int BAR_OFF = SF_OFF + STAGES * SF_BYTES;
   static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024;
   static_assert(SF_COL + 16 * SF_SLOTS <= 512, "tensor memory");
-  // A slot is written again SF_SLOTS groups of four K blocks later.  The stage that brings the new scales was filled
-  // after the MMAs STAGES blocks back had retired; the slot's last reader is at least 4 (SF_SLOTS - 1) + 1 back.
-  static_assert(4 * (SF_SLOTS - 1) + 1 >= STAGES, "scale slot reused before its readers retired");
+  // A slot is written again SF_SLOTS groups of up to four K blocks later, when its readers have retired: either they
+  // belong to the tile before the last (its accumulator has been read), or at most one of the groups between is the
+  // short one that ends a tile, so the last reader is at least 4 (SF_SLOTS - 2) + 1 + 1 blocks back, and the stage that
+  // brings the new scales was filled after the MMAs STAGES blocks back had retired.
+  static_assert(4 * (SF_SLOTS - 2) + 2 >= STAGES, "scale slot reused before its readers retired");
 };
 
 // Arrival that orders nothing but tensor memory (its reads are complete, tcgen05.fence::before_thread_sync precedes):
@@ -492,11 +494,37 @@ __device__ __forceinline__ void fp8_pair_tile(const Fp8GemmParams& p, int t, int
   *nb = r / size;
 }
 
-template <int BN, bool SPLIT>
+// One product, or two that a launch computes together: the first has the longer K.
+template <int PRODUCTS>
+struct Fp8PairArgs {
+  CUtensorMap a[PRODUCTS], b[PRODUCTS], sa[PRODUCTS], sb[PRODUCTS];
+  Fp8GemmParams p[PRODUCTS];
+  int head;                // two products: rounds of the second's tiles beside the last of the first's
+};
+
+// The tile that a pair computes as its l-th; false past its last.  Two products: the first's tiles in turn, as for one.
+// The pairs that get none in its last round take `head` tiles of the second meanwhile, then all pairs take the rest in
+// turn, so pairs that run at the same time work on neighbouring tiles all along.
+template <int PRODUCTS>
+__device__ __forceinline__ bool fp8_pair_next(const Fp8PairArgs<PRODUCTS>& g, int pair, int pairs, int l, int* which, int* t) {
+  *which = 0;
+  *t = pair + l * pairs;
+  if (*t < g.p[0].total) return true;
+  if (PRODUCTS == 1) return false;
+  constexpr int W = PRODUCTS - 1;
+  const int rest = g.p[0].total % pairs, m = l - (g.p[0].total / pairs + (pair < rest));
+  *which = W;
+  if (rest == 0) *t = pair + m * pairs;
+  else if (pair < rest) *t = g.head * (pairs - rest) + m * pairs + pair;
+  else if (m < g.head) *t = m * (pairs - rest) + pair - rest;
+  else *t = g.head * (pairs - rest) + (m - g.head) * pairs + pair;
+  return *t < g.p[W].total;
+}
+
+template <int BN, bool SPLIT, int PRODUCTS>
 __global__ void __launch_bounds__(F8PairCfg<BN>::THREADS, 1)
-fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                     const Fp8GemmParams p) {
+fp8_gemm_pair_kernel(const __grid_constant__ Fp8PairArgs<PRODUCTS> g) {
+  static_assert(!SPLIT || PRODUCTS == 1, "a split is of one product");
   using Cfg = F8PairCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -511,9 +539,9 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   const int crank = static_cast<int>(warp_uniform(cluster_ctarank()));
   const int rank = crank & 1, even = crank & ~1;                // within the pair; the pair's CTA that issues
   // first tile and stride of this pair's walk; SPLIT: the cluster's only tile, this pair's range of its K
-  const int pair = SPLIT ? blockIdx.x / (2 * p.split) : blockIdx.x >> 1, pairs = SPLIT ? p.total : gridDim.x >> 1;
-  const int kb0 = SPLIT ? (crank >> 1) * p.kb_per_split : 0;
-  const int kb1 = SPLIT ? min(p.kblocks, kb0 + p.kb_per_split) : p.kblocks;
+  const int pair = SPLIT ? blockIdx.x / (2 * g.p[0].split) : blockIdx.x >> 1;
+  const int pairs = SPLIT ? g.p[0].total : gridDim.x >> 1;
+  const int kb0 = SPLIT ? (crank >> 1) * g.p[0].kb_per_split : 0;
   const uint16_t both = static_cast<uint16_t>(3 << even);
 
   if (threadIdx.x == 0) {
@@ -528,10 +556,12 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     }
     *abort_flag = 0;
     mbar_fence_init();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
-    tma_prefetch_desc(&tmSA);
-    tma_prefetch_desc(&tmSB);
+    for (int w = 0; w < PRODUCTS; ++w) {
+      tma_prefetch_desc(&g.a[w]);
+      tma_prefetch_desc(&g.b[w]);
+      tma_prefetch_desc(&g.sa[w]);
+      tma_prefetch_desc(&g.sb[w]);
+    }
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -549,7 +579,10 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int t = pair; ok && t < p.total; t += pairs) {
+    int w, t;
+    for (int l = 0; ok && fp8_pair_next(g, pair, pairs, l, &w, &t); ++l) {
+      const Fp8GemmParams& p = g.p[w];
+      const int kb1 = SPLIT ? min(p.kblocks, kb0 + p.kb_per_split) : p.kblocks;
       int mb, nb;
       fp8_pair_tile(p, t, &mb, &nb);
       const int ra = mb * 2 + rank, rb = nb * BN / 128;         // groups of 128 rows
@@ -566,12 +599,12 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const int kg = kb >> 2;
         if (leader) {
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (Cfg::TILE_BYTES + (scales ? Cfg::SF_BYTES : 0)));
-          tma_load_2d_pair(sa, &tmA, fb, kb * 128, row_a);
-          tma_load_2d_pair(sa + Cfg::A_BYTES, &tmB, fb, kb * 128, row_b);
+          tma_load_2d_pair(sa, &g.a[w], fb, kb * 128, row_a);
+          tma_load_2d_pair(sa + Cfg::A_BYTES, &g.b[w], fb, kb * 128, row_b);
           if (scales) {   // rows of scale cells past the last read as zero: they belong to rows that are not stored
-            tma_load_2d_pair(sf, &tmSA, fb, 0, ra * p.kgroups + kg);
-            tma_load_2d_pair(sf + 512, &tmSB, fb, 0, rb * p.kgroups + kg);
-            if (Cfg::SF_GROUPS == 2) tma_load_2d_pair(sf + 1024, &tmSB, fb, 0, (rb + 1) * p.kgroups + kg);
+            tma_load_2d_pair(sf, &g.sa[w], fb, 0, ra * p.kgroups + kg);
+            tma_load_2d_pair(sf + 512, &g.sb[w], fb, 0, rb * p.kgroups + kg);
+            if (Cfg::SF_GROUPS == 2) tma_load_2d_pair(sf + 1024, &g.sb[w], fb, 0, (rb + 1) * p.kgroups + kg);
           }
         }
         __syncwarp();
@@ -590,16 +623,18 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      const uint32_t idesc = umma_idesc_mxf8(256, BN, p.a_fmt, p.b_fmt);
       const bool leader = elect_one();
       // descriptors of stage 0: a stage adds TILE_BYTES / 16 to the address field, 32 elements of K two
       const uint64_t da0 = umma_smem_desc(smem_u32(smem), 16, 1024);
       const uint64_t db0 = umma_smem_desc(smem_u32(smem) + Cfg::A_BYTES, 16, 1024);
       const uint64_t ds0 = umma_scale_desc(smem_u32(smem) + Cfg::SF_OFF);
-      int stage = 0, local = 0, slot = 0;
+      int stage = 0, slot = 0, w, t;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; ok && t < p.total; t += pairs, ++local) {
+      for (int local = 0; ok && fp8_pair_next(g, pair, pairs, local, &w, &t); ++local) {
+        const Fp8GemmParams& p = g.p[w];
+        const int kb1 = SPLIT ? min(p.kblocks, kb0 + p.kb_per_split) : p.kblocks;
+        const uint32_t idesc = umma_idesc_mxf8(256, BN, p.a_fmt, p.b_fmt);
         const int a = local & 1, use = local >> 1;
         // this accumulator's last tile has been read, and the other's where the two overlap
         if (use > 0 && !warp_wait(&tdone_bar[a], (use - 1) & 1, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY)) break;
@@ -652,6 +687,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     const uint32_t tfree = mapa_cluster(smem_u32(&tfree_bar[a]), even), tdone = mapa_cluster(smem_u32(&tdone_bar[a]), even);
     uint32_t use = 0;
     if (SPLIT) {
+      const Fp8GemmParams& p = g.p[0];
       const bool ok = warp_wait(&tfull_bar[0], 0, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
       tc_fence_after();
       // this pair's partial tile as [column][128 rows of this CTA]: the stages are free, every copy has been read.
@@ -667,7 +703,9 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         for (int i = 0; i < 32; ++i) part[(c + i) * 128] = __uint_as_float(r[i]);
       }
     }
-    for (int t = pair + a * pairs; !SPLIT && t < p.total; t += 2 * pairs, ++use) {
+    int w, t;
+    for (int l = a; !SPLIT && fp8_pair_next(g, pair, pairs, l, &w, &t); l += 2, ++use) {
+      const Fp8GemmParams& p = g.p[w];
       int mb, nb;
       fp8_pair_tile(p, t, &mb, &nb);
       bool ok = mbar_wait_bounded(&tfull_bar[a], use & 1, abort_flag);
@@ -710,6 +748,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   if (SPLIT) {
     // 64 columns at a time: chunk i belongs to pair i % split, there to the set of warps i / split
     if (warp >= 2) {
+      const Fp8GemmParams& p = g.p[0];
       const int q = warp & 3, a = (warp - 2) >> 2;
       int mb, nb;
       fp8_pair_tile(p, pair, &mb, &nb);
@@ -730,10 +769,10 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   }
 }
 
-struct Fp8Operands {
+struct Fp8Product {
   const void *a, *b;
   long long lda, ldb;
-  int M, N, K;
+  Fp8GemmParams p;
 };
 
 // The shared-memory opt-in of a kernel, made once per device: a call costs as much as an eighth of a small product.
@@ -767,12 +806,13 @@ static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, unsigned grid,
 }
 
 template <int TN, bool FUSE>
-static int launch_small(const Fp8Operands& o, Fp8GemmParams p, cudaStream_t stream) {
+static int launch_small(const Fp8Product& o, cudaStream_t stream) {
   using Cfg = F8SmallCfg<TN>;
   static_assert(TN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
   CUtensorMap ta = {}, tb;
-  if ((!FUSE && encode_tensor_map(&ta, o.a, 1, o.K, o.M, 0, o.lda, 0, 128, TN)) ||
-      encode_tensor_map(&tb, o.b, 1, o.K, o.N, 0, o.ldb, 0, 128, 128))
+  Fp8GemmParams p = o.p;
+  if ((!FUSE && encode_tensor_map(&ta, o.a, 1, p.K, p.M, 0, o.lda, 0, 128, TN)) ||
+      encode_tensor_map(&tb, o.b, 1, p.K, p.N, 0, o.ldb, 0, 128, 128))
     return -10;
   auto kern = fp8_gemm_small_kernel<TN, FUSE>;
   if (const int e = opt_in_smem<fp8_gemm_small_kernel<TN, FUSE>>(Cfg::SMEM_BYTES)) return e;
@@ -803,8 +843,8 @@ template <int BN>
 static int fp8_pair_capacity() {
   static const int cached = [] {
     using Cfg = F8PairCfg<BN>;
-    auto kern = fp8_gemm_pair_kernel<BN, false>;
-    if (opt_in_smem<fp8_gemm_pair_kernel<BN, false>>(Cfg::SMEM_BYTES)) return 0;
+    auto kern = fp8_gemm_pair_kernel<BN, false, 1>;
+    if (opt_in_smem<fp8_gemm_pair_kernel<BN, false, 1>>(Cfg::SMEM_BYTES)) return 0;
     cudaLaunchAttribute at;
     cudaLaunchConfig_t cfg = cluster_config(&at, 2 * 148, Cfg::THREADS, 2, Cfg::SMEM_BYTES, nullptr);
     int n = 0;
@@ -814,56 +854,148 @@ static int fp8_pair_capacity() {
   return cached;
 }
 
-template <int BN, bool SPLIT>
-static int launch_pair(const Fp8Operands& o, Fp8GemmParams p, int split, cudaStream_t stream) {
-  using Cfg = F8PairCfg<BN>;
-  static_assert(BN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
-  const int pairs = fp8_pair_capacity<BN>();
-  if (pairs <= 0) return -12;
-  CUtensorMap ta, tb, sa, sb;
-  const uint64_t ra = static_cast<uint64_t>((o.M + 127) / 128) * p.kgroups;
-  const uint64_t rb = static_cast<uint64_t>((o.N + 127) / 128) * p.kgroups;
-  if (encode_tensor_map(&ta, o.a, 1, o.K, o.M, 0, o.lda, 0, 128, 128) ||
-      encode_tensor_map(&tb, o.b, 1, o.K, o.N, 0, o.ldb, 0, 128, Cfg::HALF) ||
-      encode_tensor_map(&sa, p.a_sf, TMAP_U32_PLAIN, 128, ra, 0, 512, 0, 128, 1) ||
-      encode_tensor_map(&sb, p.b_sf, TMAP_U32_PLAIN, 128, rb, 0, 512, 0, 128, 1))
+// product w of a launch
+template <int BN, int PRODUCTS>
+static int pair_product(Fp8PairArgs<PRODUCTS>* g, int w, const Fp8Product& o) {
+  Fp8GemmParams& p = g->p[w];
+  p = o.p;
+  const uint64_t ra = static_cast<uint64_t>((p.M + 127) / 128) * p.kgroups;
+  const uint64_t rb = static_cast<uint64_t>((p.N + 127) / 128) * p.kgroups;
+  if (encode_tensor_map(&g->a[w], o.a, 1, p.K, p.M, 0, o.lda, 0, 128, 128) ||
+      encode_tensor_map(&g->b[w], o.b, 1, p.K, p.N, 0, o.ldb, 0, 128, F8PairCfg<BN>::HALF) ||
+      encode_tensor_map(&g->sa[w], p.a_sf, TMAP_U32_PLAIN, 128, ra, 0, 512, 0, 128, 1) ||
+      encode_tensor_map(&g->sb[w], p.b_sf, TMAP_U32_PLAIN, 128, rb, 0, 512, 0, 128, 1))
     return -10;
-  auto kern = fp8_gemm_pair_kernel<BN, SPLIT>;
-  if (const int e = opt_in_smem<fp8_gemm_pair_kernel<BN, SPLIT>>(Cfg::SMEM_BYTES)) return e;
   p.m_tiles = (p.M + 255) / 256;
   p.n_tiles = (p.N + BN - 1) / BN;
   if (static_cast<long long>(p.m_tiles) * p.n_tiles > 0x0fffffffll || ra > 0x7fffffffull || rb > 0x7fffffffull) return -11;
   p.total = p.m_tiles * p.n_tiles;
   p.group_m = p.m_tiles < 16 ? p.m_tiles : 16;
-  p.split = split;
+  return 0;
+}
+
+template <int BN, bool SPLIT, int PRODUCTS>
+static int launch_pairs(const Fp8PairArgs<PRODUCTS>& g, int clusters, int split, cudaStream_t stream) {
+  using Cfg = F8PairCfg<BN>;
+  static_assert(BN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
+  if (const int e = opt_in_smem<fp8_gemm_pair_kernel<BN, SPLIT, PRODUCTS>>(Cfg::SMEM_BYTES)) return e;
+  cudaLaunchAttribute at;
+  const cudaLaunchConfig_t cfg = cluster_config(&at, 2u * split * clusters, Cfg::THREADS, 2 * split, Cfg::SMEM_BYTES, stream);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<BN, SPLIT, PRODUCTS>, g));
+}
+
+template <int BN, bool SPLIT>
+static int launch_pair(const Fp8Product& o, int split, cudaStream_t stream) {
+  const int pairs = fp8_pair_capacity<BN>();
+  if (pairs <= 0) return -12;
+  Fp8PairArgs<1> g = {};
+  if (const int e = pair_product<BN>(&g, 0, o)) return e;
+  Fp8GemmParams& p = g.p[0];
   p.kb_per_split = (p.kblocks + split - 1) / split;
   p.split = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
-  const int n = SPLIT ? p.total * p.split : p.total < pairs ? p.total : pairs;
-  cudaLaunchAttribute at;
-  const cudaLaunchConfig_t cfg = cluster_config(&at, 2u * n, Cfg::THREADS, 2 * p.split, Cfg::SMEM_BYTES, stream);
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, sa, sb, p));
+  return launch_pairs<BN, SPLIT>(g, SPLIT ? p.total : p.total < pairs ? p.total : pairs, p.split, stream);
 }
 
 // Tile width and split for the pair kernel: the least of waves * (K blocks * c + o), in cycles.  c is what a K block
 // takes once the pipeline runs and o what a tile adds, both from timing the variants over K = 1024 ... 20480 at one and
 // at many waves; a split halves K and adds the meeting of the partial tiles.  Two pairs sharing K pay only while all
 // clusters are resident: [1024, 20480] x [2048, 20480]^T takes 53 us in 32 tiles of 256 columns, 36 with two pairs each.
-struct PairChoice {
-  int bn, split;
+struct PairCost {
+  int bn, split, c, o;
 };
-static PairChoice choose_pair(int M, int N, int kblocks) {
-  static const struct { int bn, split, c, o; } ways[] = {
-      {256, 1, 530, 1250}, {192, 1, 418, 750}, {128, 1, 408, 650}, {256, 2, 530, 5250}, {128, 2, 408, 3150}};
-  PairChoice best = {256, 1};
-  long long least = -1;
-  for (const auto& w : ways) {
-    const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + w.bn - 1) / w.bn);
-    if (w.split > 1 && (tiles * w.split > 74 || kblocks < 2 * w.split)) continue;
+static constexpr PairCost PAIR_COSTS[] = {
+    {256, 1, 530, 1250}, {192, 1, 418, 750}, {128, 1, 408, 650}, {256, 2, 530, 5250}, {128, 2, 408, 3150}};
+static long long pair_tiles(const Fp8GemmParams& p, int bn) {
+  return static_cast<long long>((p.M + 255) / 256) * ((p.N + bn - 1) / bn);
+}
+static PairCost choose_pair(const Fp8GemmParams& p, long long* least) {
+  PairCost best = PAIR_COSTS[0];
+  *least = -1;
+  for (const PairCost& w : PAIR_COSTS) {
+    const long long tiles = pair_tiles(p, w.bn);
+    if (w.split > 1 && (tiles * w.split > 74 || p.kblocks < 2 * w.split)) continue;
     const long long waves = (tiles * w.split + 73) / 74;
-    const long long cost = waves * (static_cast<long long>((kblocks + w.split - 1) / w.split) * w.c + w.o);
-    if (least < 0 || cost < least) least = cost, best = {w.bn, w.split};
+    const long long cost = waves * (static_cast<long long>((p.kblocks + w.split - 1) / w.split) * w.c + w.o);
+    if (*least < 0 || cost < *least) *least = cost, best = w;
   }
   return best;
+}
+// Above 128 rows always pairs; from 65 where tiles of 128 columns fill half of the SMs and K is short (128 rows,
+// N = 7168, K = 1024: 6.6 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 7.7; N = K = 8192:
+// 19.2 against 14.6).
+static bool takes_pairs(const Fp8GemmParams& p) {
+  return p.M > 128 || (p.M > 64 && p.N >= 37 * 128 && p.kblocks <= 12);
+}
+
+static int launch_product(const Fp8Product& o, cudaStream_t stream) {
+  const Fp8GemmParams& p = o.p;
+  if (takes_pairs(p)) {
+    long long cost;
+    const PairCost pick = choose_pair(p, &cost);
+    if (pick.split == 2)
+      return pick.bn == 256 ? launch_pair<256, true>(o, 2, stream) : launch_pair<128, true>(o, 2, stream);
+    if (pick.bn == 256) return launch_pair<256, false>(o, 1, stream);
+    if (pick.bn == 192) return launch_pair<192, false>(o, 1, stream);
+    return launch_pair<128, false>(o, 1, stream);
+  }
+  if (p.M <= 16) return launch_small<16, false>(o, stream);
+  if (p.M <= 32) return launch_small<32, false>(o, stream);
+  if (p.M <= 64) return launch_small<64, false>(o, stream);
+  return launch_small<128, false>(o, stream);
+}
+
+// Cycles of two products in one launch, by the same model, and the rounds `head` that make them fewest.
+static long long together_cost(const Fp8GemmParams& first, const Fp8GemmParams& second, const PairCost& w, int* head) {
+  const long long n1 = pair_tiles(first, w.bn), n2 = pair_tiles(second, w.bn), pairs = n1 + n2 < 74 ? n1 + n2 : 74;
+  const long long c1 = static_cast<long long>(first.kblocks) * w.c + w.o, c2 = static_cast<long long>(second.kblocks) * w.c + w.o;
+  const long long rest = n1 % pairs;
+  *head = 0;
+  if (rest == 0) return n1 / pairs * c1 + (n2 + pairs - 1) / pairs * c2;
+  long long least = -1;
+  for (long long h = c1 / c2; h <= c1 / c2 + 1; ++h) {
+    const long long left = n2 - h * (pairs - rest), more = left > 0 ? (left + pairs - 1) / pairs : 0;
+    const long long cost = n1 / pairs * c1 + (c1 > h * c2 ? c1 : h * c2) + more * c2;
+    if (least < 0 || cost < least) least = cost, *head = static_cast<int>(h < 0x0fffffff ? h : 0x0fffffff);
+  }
+  return least;
+}
+
+// How the two gradients of a layer [M, K] x [N, K] are computed: bn of one launch for both, 0 for a launch each.  A
+// launch costs the host and the drain of the one before about 4000 cycles.
+struct GradsPlan {
+  int bn, head;
+  bool x_first;
+};
+static GradsPlan plan_grads(int M, int N, int K) {
+  Fp8GemmParams x = {}, w = {};
+  x.M = M, x.N = K, x.kblocks = (N + 127) / 128;
+  w.M = N, w.N = K, w.kblocks = (M + 127) / 128;
+  GradsPlan plan = {0, 0, x.kblocks > w.kblocks};
+  if (!takes_pairs(x) || !takes_pairs(w)) return plan;
+  long long least, apart;
+  choose_pair(x, &least);
+  choose_pair(w, &apart);
+  least += apart + 4000;
+  for (const PairCost& way : PAIR_COSTS) {
+    if (way.split > 1 || way.bn == 192) continue;
+    int head;
+    const long long cost = plan.x_first ? together_cost(x, w, way, &head) : together_cost(w, x, way, &head);
+    if (cost <= least) least = cost, plan.bn = way.bn, plan.head = head;
+  }
+  return plan;
+}
+
+template <int BN>
+static int launch_together(const Fp8Product& first, const Fp8Product& second, int head, cudaStream_t stream) {
+  const int pairs = fp8_pair_capacity<BN>();
+  if (pairs <= 0) return -12;
+  Fp8PairArgs<2> g = {};
+  if (const int e = pair_product<BN>(&g, 0, first)) return e;
+  if (const int e = pair_product<BN>(&g, 1, second)) return e;
+  g.p[0].split = g.p[1].split = 1;
+  g.head = head;
+  const long long total = static_cast<long long>(g.p[0].total) + g.p[1].total;
+  return launch_pairs<BN, false>(g, total < pairs ? static_cast<int>(total) : pairs, 1, stream);
 }
 
 }  // namespace cvb
@@ -874,6 +1006,25 @@ static void output_params(Fp8GemmParams& p, void* c, long long ldc, int out_kind
   p.C = c, p.ldc = ldc, p.out_kind = out_kind, p.status = status;
   const uintptr_t at = reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(ldc * (out_kind == FP8_OUT_BF16 ? 2 : 4));
   p.vec = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
+}
+
+static int product_params(Fp8Product* o, const void* a, const void* a_sf, long long lda, int a_fmt, const void* b,
+                          const void* b_sf, long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc,
+                          int out_kind, int* status) {
+  if (a_fmt < 0 || a_fmt > 1 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
+  if (!status || !a || !b || !a_sf || !b_sf || !c) return -2;
+  // TMA and bulk copies start on 16-byte boundaries
+  if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(a_sf) |
+        reinterpret_cast<uintptr_t>(b_sf)) & 15) || lda % 16 || ldb % 16 || lda < K || ldb < K || ldc < N)
+    return -3;
+  *o = {a, b, lda, ldb, {}};
+  Fp8GemmParams& p = o->p;
+  p.a_sf = static_cast<const uint8_t*>(a_sf), p.b_sf = static_cast<const uint8_t*>(b_sf);
+  p.M = M, p.N = N, p.K = K;
+  p.kblocks = (K + 127) / 128, p.kgroups = (p.kblocks + 3) / 4;
+  p.a_fmt = a_fmt, p.b_fmt = b_fmt;
+  output_params(p, c, ldc, out_kind, status);
+  return 0;
 }
 
 // C = Q(x) B^T for up to 32 bf16 rows x, quantised to e4m3 within the product
@@ -892,42 +1043,43 @@ extern "C" int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* 
   p.M = M, p.N = N, p.kblocks = (K + 127) / 128, p.kgroups = (p.kblocks + 3) / 4;
   p.a_fmt = FP8_E4M3, p.b_fmt = b_fmt;
   output_params(p, c, ldc, out_kind, status);
-  const Fp8Operands o = {nullptr, b, 0, ldb, M, N, K};
-  if (M <= 16) return launch_small<16, true>(o, p, stream);
-  return launch_small<32, true>(o, p, stream);
+  const Fp8Product o = {nullptr, b, 0, ldb, p};
+  if (M <= 16) return launch_small<16, true>(o, stream);
+  return launch_small<32, true>(o, stream);
 }
 
 extern "C" int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                             long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind,
                             int* status, void* stream_v) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  Fp8Product o;
+  const int e = product_params(&o, a, a_sf, lda, a_fmt, b, b_sf, ldb, b_fmt, M, N, K, c, ldc, out_kind, status);
+  return e ? e : launch_product(o, static_cast<cudaStream_t>(stream_v));
+}
+
+// The two gradients of a linear layer, dx [M, K] = dy [M, N] wt [K, N]^T and dw [N, K] (+)= dyt [N, M] xt [K, M]^T, in
+// one launch where that fills the SMs better than one after the other.
+extern "C" int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long ld_dy, const void* wt, const void* wt_sf,
+                                  long long ld_wt, const void* dyt, const void* dyt_sf, long long ld_dyt,
+                                  const void* xt, const void* xt_sf, long long ld_xt, int grad_fmt, int M, int N, int K,
+                                  void* dx, long long lddx, int dx_kind, void* dw, long long lddw, int dw_kind,
+                                  int* status, void* stream_v) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (a_fmt < 0 || a_fmt > 1 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
-  if (!status || !a || !b || !a_sf || !b_sf || !c) return -2;
-  // TMA and bulk copies start on 16-byte boundaries
-  if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(a_sf) |
-        reinterpret_cast<uintptr_t>(b_sf)) & 15) || lda % 16 || ldb % 16 || lda < K || ldb < K || ldc < N)
-    return -3;
-  Fp8GemmParams p = {};
-  p.a_sf = static_cast<const uint8_t*>(a_sf), p.b_sf = static_cast<const uint8_t*>(b_sf);
-  p.M = M, p.N = N;
-  p.kblocks = (K + 127) / 128, p.kgroups = (p.kblocks + 3) / 4;
-  p.a_fmt = a_fmt, p.b_fmt = b_fmt;
-  output_params(p, c, ldc, out_kind, status);
-  const Fp8Operands o = {a, b, lda, ldb, M, N, K};
-  const PairChoice pick = choose_pair(p.M, p.N, p.kblocks);
-  // Above 128 rows always pairs; from 65 where tiles of 128 columns fill half of the SMs and K is short (128 rows,
-  // N = 7168, K = 1024: 6.6 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 7.7; N = K = 8192:
-  // 19.2 against 14.6).
-  if (M > 128 || (M > 64 && N >= 37 * 128 && p.kblocks <= 12)) {
-    if (pick.split == 2)
-      return pick.bn == 256 ? launch_pair<256, true>(o, p, 2, stream) : launch_pair<128, true>(o, p, 2, stream);
-    if (pick.bn == 256) return launch_pair<256, false>(o, p, 1, stream);
-    if (pick.bn == 192) return launch_pair<192, false>(o, p, 1, stream);
-    return launch_pair<128, false>(o, p, 1, stream);
-  }
-  if (M <= 16) return launch_small<16, false>(o, p, stream);
-  if (M <= 32) return launch_small<32, false>(o, p, stream);
-  if (M <= 64) return launch_small<64, false>(o, p, stream);
-  return launch_small<128, false>(o, p, stream);
+  Fp8Product x, w;
+  int e = product_params(&x, dy, dy_sf, ld_dy, grad_fmt, wt, wt_sf, ld_wt, FP8_E4M3, M, K, N, dx, lddx, dx_kind, status);
+  if (!e)
+    e = product_params(&w, dyt, dyt_sf, ld_dyt, grad_fmt, xt, xt_sf, ld_xt, FP8_E4M3, N, K, M, dw, lddw, dw_kind, status);
+  if (e) return e;
+  const GradsPlan plan = plan_grads(M, N, K);
+  if (plan.bn == 256) return launch_together<256>(plan.x_first ? x : w, plan.x_first ? w : x, plan.head, stream);
+  if (plan.bn == 128) return launch_together<128>(plan.x_first ? x : w, plan.x_first ? w : x, plan.head, stream);
+  if ((e = launch_product(x, stream))) return e;
+  return launch_product(w, stream);
+}
+
+// launches of cvb_fp8_gemm_grads
+extern "C" int cvb_fp8_gemm_grads_launches(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return plan_grads(M, N, K).bn ? 1 : 2;
 }

@@ -11,6 +11,10 @@ int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, 
 int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                  long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int* status,
                  void* stream);
+int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long ld_dy, const void* wt, const void* wt_sf,
+                       long long ld_wt, const void* dyt, const void* dyt_sf, long long ld_dyt, const void* xt,
+                       const void* xt_sf, long long ld_xt, int grad_fmt, int M, int N, int K, void* dx, long long lddx,
+                       int dx_kind, void* dw, long long lddw, int dw_kind, int* status, void* stream);
 int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* b, const void* b_sf, long long ldb, int b_fmt,
                       int M, int N, int K, void* c, long long ldc, int out_kind, int* status, void* stream);
 int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride, const void* w, void* h,
@@ -86,13 +90,14 @@ extern "C" int cvb_fp8_linear_bwd(const void* dy, int dy_fp32, long long dy_stri
   if (!mdq.codes && !mdt.codes) return 0;
   int rc = quantize(dy, dy_fp32, M, N, dy_stride, grad_fmt, 0, mdq, mdt, stream);
   if (rc) return rc;
-  if (wt && (rc = product(mdq, grad_fmt, mwt, E4M3, M, K, N, dx, lddx, dx_kind, status, stream))) return rc;
-  if (!dw) return 0;
+  if (!dw) return product(mdq, grad_fmt, mwt, E4M3, M, K, N, dx, lddx, dx_kind, status, stream);
   if (h && (rc = cvb_fp8_quantize(h, 0, M, K, h_stride, E4M3, COLS, nullptr, nullptr, nullptr, 0, mxt.codes, mxt.sf,
                                   nullptr, mxt.ld,
                                   rstd, wn, w_offset, stream)))
     return rc;
-  return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, status, stream);
+  if (!wt) return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, status, stream);
+  return cvb_fp8_gemm_grads(mdq.codes, mdq.sf, mdq.ld, mwt.codes, mwt.sf, mwt.ld, mdt.codes, mdt.sf, mdt.ld, mxt.codes,
+                            mxt.sf, mxt.ld, grad_fmt, M, N, K, dx, lddx, dx_kind, dw, lddw, dw_kind, status, stream);
 }
 
 // The gradients of the norm + linear layer.  wt given: `dn` (fp32 [M, lddn], a workspace) takes the gradient of the

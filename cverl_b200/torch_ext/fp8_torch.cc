@@ -39,6 +39,7 @@ struct Launchers {
                          const float*, const void*, float, float*, ll, void*, ll, int, const void*, ll, void*, float*,
                          float*, void*, int*, void*);
   int (*norm_bwd_parts)();
+  int (*gemm_grads_launches)(int, int, int);
 } fn;
 
 PyObject* launch_counter = nullptr;   // ops.gemm.launch_counter
@@ -55,6 +56,7 @@ void bind(const pybind11::dict& addresses, pybind11::dict counter) {
   take(fn.norm_linear_fwd, addresses, "cvb_fp8_norm_linear_fwd");
   take(fn.norm_linear_bwd, addresses, "cvb_fp8_norm_linear_bwd");
   take(fn.norm_bwd_parts, addresses, "cvb_fp8_norm_bwd_parts");
+  take(fn.gemm_grads_launches, addresses, "cvb_fp8_gemm_grads_launches");
   launch_counter = counter.release().ptr();
 }
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
@@ -235,6 +237,9 @@ void count_from_backward(long n) {
   count_launches(n);
 }
 
+// launches of the products of a backward pass
+long products(const Sizes& z, bool dx, bool dw) { return dx && dw ? fn.gemm_grads_launches(z.M, z.N, z.K) : dx + dw; }
+
 Tensor some(const OptTensor& t) { return t ? *t : Tensor(); }
 
 struct LinearFn : torch::autograd::Function<LinearFn> {
@@ -277,7 +282,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
                             needs[0] ? std::max<int64_t>(dx.stride(0), z.K) : 0, out_kind(dtype), ptr(g.target),
                             g.stride(z), g.kind, reinterpret_cast<int*>(z.status), stream_of(dy)),
               "cvb_fp8_linear_bwd");
-        count_from_backward(1 + needs[0] + needs[1]);
+        count_from_backward(1 + products(z, needs[0], needs[1]));
       }
       const auto shape = ctx->saved_data["shape"].toIntVector();
       if (dx.defined()) out[0] = shape.size() == 2 ? dx : dx.reshape(shape);
@@ -353,7 +358,7 @@ struct NormLinearFn : torch::autograd::Function<NormLinearFn> {
                                  reinterpret_cast<float*>(ptr(wn_main)), ptr(dwn), reinterpret_cast<int*>(z.status),
                                  stream_of(dy)),
               "cvb_fp8_norm_linear_bwd");
-        count_from_backward(1 + 2 * need_dn + 2 * need_dw + need_wn);
+        count_from_backward(1 + products(z, need_dn, need_dw) + need_dn + need_dw + need_wn);
       }
       if (dx.defined()) {
         const auto shape = ctx->saved_data["shape"].toIntVector();

@@ -242,6 +242,24 @@ def test_linear_and_gradients(m, k, n, grad):
     assert (w.main_grad.double() - 1 - want).norm() <= (m + 1) * 2.0 ** -24 * (want.norm() + (n * k) ** 0.5)
 
 
+# tiles of the longer and of the shorter product: less than a round of 74 CTA pairs together; more than one round each,
+# either product the longer; exactly one round; one tile; columns and rows that end inside a tile
+@pytest.mark.parametrize("m,k,n", [(200, 520, 2000), (5000, 1300, 4000), (2900, 1300, 6400), (300, 18900, 256),
+                                   (1301, 523, 1003), (129, 130, 131), (20000, 300, 260), (640, 5000, 8200)])
+def test_both_gradients_of_whole_numbers_are_exact(m, k, n):
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w, dy = (torch.randint(-8, 9, s, device="cuda", generator=g).bfloat16() for s in ((m, k), (n, k), (m, n)))
+    x.requires_grad_(), w.requires_grad_()
+    dx, dw = torch.autograd.grad(ops.linear_fp8(x, w), (x, w), dy)          # sums below 64 * 20000 < 2^24
+    assert torch.equal(dx, (dy.double() @ w.detach().double()).float().bfloat16())
+    assert torch.equal(dw, (dy.double().t() @ x.detach().double()).float().bfloat16())
+    w.main_grad = torch.ones(n, k, device="cuda")
+    sign = dy.sign()                                                        # e5m2 has three digits
+    ops.linear_fp8(x, w, grad_dtype=E5M2).backward(sign)
+    assert torch.equal(w.main_grad.double(), sign.double().t() @ x.detach().double() + 1)
+    assert torch.equal(x.grad, (sign.double() @ w.detach().double()).float().bfloat16())
+
+
 @pytest.mark.parametrize("m,k,n", LAYERS + [(40, 4100, 96), (9, 8192, 64), (6, 16384, 32)])
 @pytest.mark.parametrize("resid", [True, False])
 def test_norm_linear_and_gradients(m, k, n, resid):
@@ -488,11 +506,11 @@ def test_launches_are_counted():
     n = launch_counter["n"]
     y = ops.linear_fp8(x, w)                                # weight, input, product
     assert launch_counter["n"] == n + 3
-    y.backward(torch.ones_like(y))                          # gradient, two products
-    assert launch_counter["n"] == n + 6
+    y.backward(torch.ones_like(y))                          # gradient, both products
+    assert launch_counter["n"] == n + 5
     y, _ = ops.add_rmsnorm_linear_fp8(x, None, wn, w)       # weight, norm, product
-    y.backward(torch.ones_like(y))                          # gradient, norm's transpose, two products, norm, its weight
-    assert launch_counter["n"] == n + 15
+    y.backward(torch.ones_like(y))                          # gradient, norm's transpose, both products, norm, its weight
+    assert launch_counter["n"] == n + 13
 
 
 def test_empty_calls():
