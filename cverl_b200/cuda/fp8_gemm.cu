@@ -430,10 +430,42 @@ __device__ __forceinline__ void st_global_32b(void* p, uint32_t a, uint32_t b, u
                : "memory");
 }
 
+// C += a lane's 16 columns of its row, columns and rows of whole vectors: four lanes exchange vectors of four, so that
+// an instruction adds 64 bytes of a row from four lanes.
+__device__ __forceinline__ void fp8_quad_add(const Fp8GemmParams& p, const uint32_t* r, int row, int col) {
+  const int j = threadIdx.x & 3;
+  uint32_t x[4][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = r[i];
+#pragma unroll
+  for (int m = 1; m <= 2; m <<= 1)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      if (v & m) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, j & m ? x[v][i] : x[v | m][i], m);
+        if (j & m) x[v][i] = got;
+        else x[v | m][i] = got;
+      }
+    }
+  row &= ~3;                    // lane j has vector j of rows row + 0 ... 3
+  float* dst = reinterpret_cast<float*>(p.C) + static_cast<long long>(row) * p.ldc + col + j * 4;
+#pragma unroll
+  for (int k = 0; k < 4; ++k, dst += p.ldc)
+    if (row + k < p.M)
+      red_add_v4_f32(dst, __uint_as_float(x[k][0]), __uint_as_float(x[k][1]), __uint_as_float(x[k][2]), __uint_as_float(x[k][3]));
+}
+
 // 32 rows x 64 columns of one epilogue warp, lane = row, straight from registers: a lane's 64 results are 128 (or
 // 256) bytes of its row, stored as whole 32-byte sectors.  An accumulating product adds by reduction, one addition an
 // element: the result does not depend on the order.  Value by value where C is not aligned or the columns end.
 __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const uint32_t (&r)[64], int row, int col) {
+  if (p.out_kind == FP8_OUT_F32_ACC && p.vec >= 16 && col + 64 <= p.N) {
+#pragma unroll
+    for (int g = 0; g < 64; g += 16) fp8_quad_add(p, r + g, row, col + g);
+    return;
+  }
   if (row >= p.M) return;
   const long long off = static_cast<long long>(row) * p.ldc + col;
   const int n = p.N - col;
