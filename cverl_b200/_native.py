@@ -125,7 +125,7 @@ _CUDA_PROTOS = {
     "cvb_fp8_add_rmsnorm": "plpl p p pppl p l i i ff p",
     "cvb_fp8_norm_bwd_parts": "",
     "cvb_fp8_norm_bwd": "pl pl pp pl pp pp l i f p",
-    "cvb_fp8_gemm": "ppli ppli iii p l i p p",
+    "cvb_fp8_gemm": "ppli ppli iii p l i i p p",
     "cvb_fp8_gemm_grads": "ppl ppl ppl ppl i iii p l i p l i p p",
     "cvb_fp8_gemm_grads_launches": "iii",
     "cvb_fp8_linear_fwd": "pil pil iii pppp p l i p p",

@@ -15,6 +15,16 @@ namespace cvb {
 
 enum : int { FP8_OUT_BF16 = 0, FP8_OUT_F32 = 1, FP8_OUT_F32_ACC = 2 };
 
+// What a launch may assume of the kernel before it in the stream.  Where that is the kernel that quantised the
+// operands, the product is placed while it still runs (programmatic dependent launch), sets up its barriers, tensor
+// memory and first loads of what that kernel does not write, and waits for its end.  128 rows, N = 1024, K = 3584,
+// quantised and multiplied: 8.6 us, 9.4 one after the other; 16 rows, N = 7168, K = 1024 after a norm: 6.3 and 7.9.
+enum Fp8After {
+  AFTER_ANY = 0,           // nothing: an ordinary launch
+  AFTER_OPERANDS = 1,      // it, or one before it, wrote A and B; none of its writes is C
+  AFTER_A = 2,             // it wrote A; B was complete before it started
+};
+
 struct Fp8GemmParams {
   const uint8_t *a_sf, *b_sf;
   const __nv_bfloat16* x;  // small kernel, FUSE: A as bf16 rows, quantised on the way
@@ -28,6 +38,7 @@ struct Fp8GemmParams {
   int m_tiles, n_tiles;
   int split, kb_per_split; // CTAs (or CTA pairs) of a cluster that share a tile's K, and K blocks of each
   int group_m, total;      // pair kernel: M tiles walked per N tile, tiles in all
+  int after;               // Fp8After
   int* status;
 };
 
@@ -134,6 +145,7 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
 // to back against 6.6 for two kernels; at 64 rows 11.5 against 8.8).  A stage's scale cells hold this block's byte only,
 // so they move to tensor memory once a block.
 // ---------------------------------------------------------------------------------------------------
+constexpr int F8_SMEM_ALONE = 117 * 1024;     // more than half of an SM: no second CTA beside
 template <int TN>
 struct F8SmallCfg {
   static constexpr int B_BYTES = 128 * 128;
@@ -196,22 +208,26 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     const uint8_t* b_sf = p.b_sf + static_cast<long long>(n0 >> 7) * p.kgroups * 512;
     const uint8_t* a_sf = FUSE ? nullptr : p.a_sf + static_cast<long long>(m0 >> 7) * p.kgroups * 512;
     constexpr uint32_t BYTES = FUSE ? Cfg::B_BYTES : Cfg::TILE_BYTES, SF = FUSE ? 512 : 1024;
-    auto fill = [&](int kb, int stage) {
-      uint8_t* sb = smem + stage * Cfg::TILE_BYTES;
-      uint8_t* sf = sf_smem + stage * Cfg::SF_BYTES;
+    auto fill_b = [&](int kb, int stage) {
       const bool scales = kb == kb0 || (kb & 3) == 0;
-      const long long kg = static_cast<long long>(kb >> 2) * 512;
       mbar_arrive_expect_tx(&full_bar[stage], BYTES + (scales ? SF : 0));
-      tma_load_2d(sb, &tmB, &full_bar[stage], kb * 128, n0);
-      if (!FUSE) tma_load_2d(sb + Cfg::B_BYTES, &tmA, &full_bar[stage], kb * 128, m0);
-      if (scales) {
-        bulk_load(sf, b_sf + kg, 512, &full_bar[stage]);
-        if (!FUSE) bulk_load(sf + 512, a_sf + kg, 512, &full_bar[stage]);
-      }
+      tma_load_2d(smem + stage * Cfg::TILE_BYTES, &tmB, &full_bar[stage], kb * 128, n0);
+      if (scales)
+        bulk_load(sf_smem + stage * Cfg::SF_BYTES, b_sf + static_cast<long long>(kb >> 2) * 512, 512, &full_bar[stage]);
+    };
+    auto fill_a = [&](int kb, int stage) {
+      if (FUSE) return;
+      tma_load_2d(smem + stage * Cfg::TILE_BYTES + Cfg::B_BYTES, &tmA, &full_bar[stage], kb * 128, m0);
+      if (kb == kb0 || (kb & 3) == 0)
+        bulk_load(sf_smem + stage * Cfg::SF_BYTES + 512, a_sf + static_cast<long long>(kb >> 2) * 512, 512, &full_bar[stage]);
     };
     // The first fill of every stage waits for nothing: one lane a stage.  One after the other they took 560 cycles each
     // (one row, N = K = 1024: 3.7 us against 3.4).
-    if (lane < Cfg::STAGES && kb0 + lane < kb1) fill(kb0 + lane, lane);
+    const bool first = lane < Cfg::STAGES && kb0 + lane < kb1;
+    if (p.after != AFTER_A) wait_for_previous_kernel();
+    if (first) fill_b(kb0 + lane, lane);
+    if (p.after == AFTER_A) wait_for_previous_kernel();
+    if (first) fill_a(kb0 + lane, lane);
     __syncwarp();
     int stage = 0;
     uint32_t phase = 0;
@@ -221,7 +237,10 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         ok = false;
         break;
       }
-      if (leader) fill(kb, stage);
+      if (leader) {
+        fill_b(kb, stage);
+        fill_a(kb, stage);
+      }
       __syncwarp();
       if (++stage == Cfg::STAGES) {
         stage = 0;
@@ -608,6 +627,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ Fp8PairArgs<PRODUCTS> g) {
   if (warp == 0) {
     const bool leader = elect_one();
     const uint32_t full0 = mapa_cluster(smem_u32(full_bar), even);
+    wait_for_previous_kernel();
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -821,19 +841,21 @@ static int opt_in_smem(int bytes) {
   return static_cast<int>(e);
 }
 
-static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, unsigned grid, int threads, int cluster, size_t smem,
-                                         cudaStream_t stream) {
-  at->id = cudaLaunchAttributeClusterDimension;
-  at->val.clusterDim.x = cluster;
-  at->val.clusterDim.y = 1;
-  at->val.clusterDim.z = 1;
+static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute (&at)[2], unsigned grid, int threads, int cluster,
+                                         size_t smem, int after, cudaStream_t stream) {
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after == AFTER_ANY ? 1 : 2;
   return cfg;
 }
 
@@ -841,13 +863,14 @@ template <int TN, bool FUSE>
 static int launch_small(const Fp8Product& o, cudaStream_t stream) {
   using Cfg = F8SmallCfg<TN>;
   static_assert(TN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
+  static_assert(Cfg::SMEM_BYTES <= F8_SMEM_ALONE, "opted in");
   CUtensorMap ta = {}, tb;
   Fp8GemmParams p = o.p;
   if ((!FUSE && encode_tensor_map(&ta, o.a, 1, p.K, p.M, 0, o.lda, 0, 128, TN)) ||
       encode_tensor_map(&tb, o.b, 1, p.K, p.N, 0, o.ldb, 0, 128, 128))
     return -10;
   auto kern = fp8_gemm_small_kernel<TN, FUSE>;
-  if (const int e = opt_in_smem<fp8_gemm_small_kernel<TN, FUSE>>(Cfg::SMEM_BYTES)) return e;
+  if (const int e = opt_in_smem<fp8_gemm_small_kernel<TN, FUSE>>(F8_SMEM_ALONE)) return e;
   p.m_tiles = (p.M + TN - 1) / TN;
   p.n_tiles = (p.N + 127) / 128;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
@@ -864,9 +887,13 @@ static int launch_small(const Fp8Product& o, cudaStream_t stream) {
   p.kb_per_split = (p.kblocks + p.split - 1) / p.split;
   p.split = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
   if (tiles * p.split > 0x7fffffffll) return -11;
-  cudaLaunchAttribute at;
+  // Placed beside a kernel that still runs, CTAs would gather in pairs on the SMs that it leaves free: where there is
+  // an SM for each, too much shared memory for two (128 rows, N = K = 4096: 10.3 us with the quantisation, 12.6 in
+  // pairs).  128: clusters of four do not find 148 SMs.
+  const int smem = p.after != AFTER_ANY && tiles * p.split <= 128 ? F8_SMEM_ALONE : Cfg::SMEM_BYTES;
+  cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg =
-      cluster_config(&at, static_cast<unsigned>(tiles * p.split), F8_THREADS, p.split, Cfg::SMEM_BYTES, stream);
+      cluster_config(at, static_cast<unsigned>(tiles * p.split), F8_THREADS, p.split, smem, p.after, stream);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, p));
 }
 
@@ -877,8 +904,8 @@ static int fp8_pair_capacity() {
     using Cfg = F8PairCfg<BN>;
     auto kern = fp8_gemm_pair_kernel<BN, false, 1>;
     if (opt_in_smem<fp8_gemm_pair_kernel<BN, false, 1>>(Cfg::SMEM_BYTES)) return 0;
-    cudaLaunchAttribute at;
-    cudaLaunchConfig_t cfg = cluster_config(&at, 2 * 148, Cfg::THREADS, 2, Cfg::SMEM_BYTES, nullptr);
+    cudaLaunchAttribute at[2];
+    cudaLaunchConfig_t cfg = cluster_config(at, 2 * 148, Cfg::THREADS, 2, Cfg::SMEM_BYTES, AFTER_ANY, nullptr);
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
     return n;
@@ -911,8 +938,9 @@ static int launch_pairs(const Fp8PairArgs<PRODUCTS>& g, int clusters, int split,
   using Cfg = F8PairCfg<BN>;
   static_assert(BN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
   if (const int e = opt_in_smem<fp8_gemm_pair_kernel<BN, SPLIT, PRODUCTS>>(Cfg::SMEM_BYTES)) return e;
-  cudaLaunchAttribute at;
-  const cudaLaunchConfig_t cfg = cluster_config(&at, 2u * split * clusters, Cfg::THREADS, 2 * split, Cfg::SMEM_BYTES, stream);
+  cudaLaunchAttribute at[2];
+  const cudaLaunchConfig_t cfg =
+      cluster_config(at, 2u * split * clusters, Cfg::THREADS, 2 * split, Cfg::SMEM_BYTES, g.p[0].after, stream);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<BN, SPLIT, PRODUCTS>, g));
 }
 
@@ -1042,8 +1070,8 @@ static void output_params(Fp8GemmParams& p, void* c, long long ldc, int out_kind
 
 static int product_params(Fp8Product* o, const void* a, const void* a_sf, long long lda, int a_fmt, const void* b,
                           const void* b_sf, long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc,
-                          int out_kind, int* status) {
-  if (a_fmt < 0 || a_fmt > 1 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
+                          int out_kind, int after, int* status) {
+  if (a_fmt < 0 || after < AFTER_ANY || after > AFTER_A || a_fmt > 1 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
   if (!status || !a || !b || !a_sf || !b_sf || !c) return -2;
   // TMA and bulk copies start on 16-byte boundaries
   if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(a_sf) |
@@ -1054,7 +1082,7 @@ static int product_params(Fp8Product* o, const void* a, const void* a_sf, long l
   p.a_sf = static_cast<const uint8_t*>(a_sf), p.b_sf = static_cast<const uint8_t*>(b_sf);
   p.M = M, p.N = N, p.K = K;
   p.kblocks = (K + 127) / 128, p.kgroups = (p.kblocks + 3) / 4;
-  p.a_fmt = a_fmt, p.b_fmt = b_fmt;
+  p.a_fmt = a_fmt, p.b_fmt = b_fmt, p.after = after;
   output_params(p, c, ldc, out_kind, status);
   return 0;
 }
@@ -1082,15 +1110,16 @@ extern "C" int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* 
 
 extern "C" int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                             long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind,
-                            int* status, void* stream_v) {
+                            int after, int* status, void* stream_v) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   Fp8Product o;
-  const int e = product_params(&o, a, a_sf, lda, a_fmt, b, b_sf, ldb, b_fmt, M, N, K, c, ldc, out_kind, status);
+  const int e = product_params(&o, a, a_sf, lda, a_fmt, b, b_sf, ldb, b_fmt, M, N, K, c, ldc, out_kind, after, status);
   return e ? e : launch_product(o, static_cast<cudaStream_t>(stream_v));
 }
 
 // The two gradients of a linear layer, dx [M, K] = dy [M, N] wt [K, N]^T and dw [N, K] (+)= dyt [N, M] xt [K, M]^T, in
-// one launch where that fills the SMs better than one after the other.
+// one launch where that fills the SMs better than one after the other.  The stream's last launch wrote some of the
+// operands and neither result.
 extern "C" int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long ld_dy, const void* wt, const void* wt_sf,
                                   long long ld_wt, const void* dyt, const void* dyt_sf, long long ld_dyt,
                                   const void* xt, const void* xt_sf, long long ld_xt, int grad_fmt, int M, int N, int K,
@@ -1099,11 +1128,14 @@ extern "C" int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long l
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   Fp8Product x, w;
-  int e = product_params(&x, dy, dy_sf, ld_dy, grad_fmt, wt, wt_sf, ld_wt, FP8_E4M3, M, K, N, dx, lddx, dx_kind, status);
+  int e = product_params(&x, dy, dy_sf, ld_dy, grad_fmt, wt, wt_sf, ld_wt, FP8_E4M3, M, K, N, dx, lddx, dx_kind,
+                         AFTER_OPERANDS, status);
   if (!e)
-    e = product_params(&w, dyt, dyt_sf, ld_dyt, grad_fmt, xt, xt_sf, ld_xt, FP8_E4M3, N, K, M, dw, lddw, dw_kind, status);
+    e = product_params(&w, dyt, dyt_sf, ld_dyt, grad_fmt, xt, xt_sf, ld_xt, FP8_E4M3, N, K, M, dw, lddw, dw_kind,
+                       AFTER_ANY, status);
   if (e) return e;
   const GradsPlan plan = plan_grads(M, N, K);
+  if (plan.bn) w.p.after = AFTER_OPERANDS;
   if (plan.bn == 256) return launch_together<256>(plan.x_first ? x : w, plan.x_first ? w : x, plan.head, stream);
   if (plan.bn == 128) return launch_together<128>(plan.x_first ? x : w, plan.x_first ? w : x, plan.head, stream);
   if ((e = launch_product(x, stream))) return e;

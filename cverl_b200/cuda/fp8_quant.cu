@@ -199,6 +199,7 @@ __device__ __forceinline__ bool piece_maxima(const Piece<__nv_bfloat16, false>& 
 template <typename T, int FMT, bool NORM, bool ROWS, bool COLS, bool BLOCK>
 __global__ void __launch_bounds__(Q_THREADS, sizeof(T) == 4 ? 1 : NORM ? 2 : 3)
 fp8_quant_kernel(const QuantArgs p) {
+  launch_dependents();             // a product that follows sets itself up meanwhile
   __shared__ __align__(16) uint32_t s_max[COLS || BLOCK ? Q_THREADS / 32 : 1][QT / 2];   // column maxima by warp
   __shared__ __align__(16) uint32_t s_inv[COLS ? QT / 2 : 4];      // 2^-e of two columns a word, as bf16
   __shared__ __align__(16) uint8_t s_t[COLS ? QT * QT : 16];       // transposed codes, 8-byte units XOR-swizzled
@@ -392,6 +393,7 @@ struct RowBlock {
 template <int TPR, int NV, int FMT, bool VEC>
 __global__ void __launch_bounds__(RowBlock<TPR>::THREADS)
 fp8_norm_kernel(const NormQuantArgs p) {
+  launch_dependents();
   constexpr int ROWS = RowBlock<TPR>::ROWS;
   __shared__ float s_part[ROWS][TPR / 32];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, lane = threadIdx.x & 31;

@@ -387,6 +387,14 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t cta_mas
 }
 
 // ---------------------------------------------------------------------------
+// overlap of a kernel with the next one in its stream (programmatic dependent launch)
+// ---------------------------------------------------------------------------
+// The next kernel's CTAs may be placed once every CTA of this one has said so.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Until the kernel before has ended and its writes are visible; returns at once in an ordinary launch.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
 // misc
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {

@@ -246,7 +246,7 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
         return out.add_(r) if accumulate else out.copy_(r)
     index = out.get_device()
     args = (a.buf.data_ptr(), a.sf_ptr, a.ld, _FMT[a.dtype], b.buf.data_ptr(), b.sf_ptr, b.ld, _FMT[b.dtype], M, N, K,
-            out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype], _status(index))
+            out.data_ptr(), max(out.stride(0), N), 2 if accumulate else _OUT[out.dtype], 0, _status(index))
     if index != torch._C._cuda_getDevice():       # launches go to the operands' device and its current stream
         with torch.cuda.device(index):
             nv.check(nv.cuda().cvb_fp8_gemm(*args, nv.raw_stream(index)), "cvb_fp8_gemm")
