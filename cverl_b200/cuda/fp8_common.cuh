@@ -64,6 +64,12 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
         : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
   return r;
 }
+// two bf16 by a power of two each: exact, or so small that its code is zero; subnormal inputs count
+__device__ __forceinline__ uint32_t fp8_mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 template <int FMT>
 __device__ __forceinline__ uint2 fp8_pack8(const float (&v)[8], float inv) {
   uint2 o;
