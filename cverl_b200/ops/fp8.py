@@ -101,10 +101,14 @@ class Fp8Tensor:
     @property
     def values(self) -> torch.Tensor:
         """The codes as an 8-bit float view ``[rows, cols]`` (in units of their scales)."""
+        if self.buf.is_cuda:
+            return nv.torch_ext().view8(self.buf, self.rows, self.cols, _FMT[self.dtype])
         return self.buf.view(self.dtype).as_strided((self.rows, self.cols), (self.ld, 1))
 
     def scales(self) -> torch.Tensor:
         """The scales as a view ``[rows, ceil(cols / 128)]`` of ``torch.float8_e8m0fnu`` (powers of two)."""
+        if self.buf.is_cuda:
+            return nv.torch_ext().view8(self.buf, self.rows, self.cols, 2)
         nb = _ceil(self.cols, BLOCK)
         return self.buf.view(torch.float8_e8m0fnu).as_strided((self.rows, nb), (nb, 1), _nbytes(self.rows, self.cols))
 

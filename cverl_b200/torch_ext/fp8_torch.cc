@@ -5,6 +5,7 @@
 // The arguments are checked by the Python functions that call in here (ops/fp8.py); the launchers' addresses come from
 // the ctypes library, so that it is loaded once.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/stl.h>
@@ -79,15 +80,19 @@ int64_t nbytes(int64_t rows, int64_t cols) { return rows * up(cols, 16) + up(row
 // the scale bytes once more, in plain order
 int64_t nbytes_plain(int64_t rows, int64_t cols) { return rows * (up(cols, 128) / 128); }
 
-Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
+// straight from the allocator: the way through the dispatcher takes as long again
+Tensor fresh(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(size, type, like.device(), std::nullopt);
+}
+Tensor bytes(int64_t n, const Tensor& like) { return fresh({n}, at::kByte, like); }
 char* ptr(const Tensor& t) { return t.defined() ? static_cast<char*>(t.data_ptr()) : nullptr; }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // [M, N] whose rows start on 32 bytes (what the vector stores of the product want)
 Tensor alloc_rows(int64_t M, int64_t N, at::ScalarType dtype, const Tensor& like) {
   const int64_t per32 = dtype == at::kBFloat16 ? 16 : 8;
-  if (N % per32 == 0) return at::empty({M, N}, like.options().dtype(dtype));
-  return at::empty({M, up(N, per32)}, like.options().dtype(dtype)).narrow(1, 0, N);
+  if (N % per32 == 0) return fresh({M, N}, dtype, like);
+  return fresh({M, up(N, per32)}, dtype, like).narrow(1, 0, N);
 }
 Tensor matrix(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
 Tensor rows2d(const Tensor& t) {
@@ -137,8 +142,8 @@ Forward forward(const Tensor& x, const Tensor& xq, int64_t M, int64_t K, const W
   f.y = alloc_rows(M, N, dtype, like);
   const bool has_resid = resid && resid->defined();
   if (wn) {
-    f.h = has_resid ? at::empty({M, K}, x.options()) : x;
-    if (need_rstd) f.rstd = at::empty({M}, x.options().dtype(at::kFloat));
+    f.h = has_resid ? fresh({M, K}, x.scalar_type(), x) : x;
+    if (need_rstd) f.rstd = fresh({M}, at::kFloat, x);
   }
   if (M == 0 || N == 0 || K == 0) {
     f.y.zero_();
@@ -333,9 +338,9 @@ struct NormLinearFn : torch::autograd::Function<NormLinearFn> {
       if (need_wn) {
         pybind11::gil_scoped_acquire gil;
         wn_main = main_grad(wn);
-        if (!wn_main.defined()) dwn = at::empty({z.K}, wn.options());
+        if (!wn_main.defined()) dwn = fresh({z.K}, wn.scalar_type(), wn);
       }
-      if (need_dn) dx = at::empty({z.M, z.K}, h.options());
+      if (need_dn) dx = fresh({z.M, z.K}, h.scalar_type(), h);
       if (z.empty()) {      // no rows, or no columns in y: only dh is left
         if (dx.defined()) dh.defined() ? dx.copy_(dh) : dx.zero_();
         if (dwn.defined()) dwn.zero_();
@@ -441,6 +446,21 @@ std::pair<OptTensor, OptTensor> quantize(const Tensor& x_in, int64_t fmt, int64_
   return {q, t};
 }
 
+// The codes (fmt 0, 1) or plain scales (fmt 2) of a [rows, cols] matrix as a view of its buffer, without the two calls
+// through the dispatcher that a view of another type takes from Python.
+Tensor view8(const Tensor& buf, int64_t rows, int64_t cols, int64_t fmt) {
+  constexpr at::ScalarType types[] = {at::kFloat8_e4m3fn, at::kFloat8_e5m2, at::kFloat8_e8m0fnu};
+  TORCH_CHECK_VALUE(fmt >= 0 && fmt < 3 && rows >= 0 && cols >= 0 && buf.scalar_type() == at::kByte &&
+                        buf.numel() == nbytes(rows, cols) + nbytes_plain(rows, cols),
+                    "not a buffer of a [", rows, ", ", cols, "] matrix");
+  Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()), buf.key_set(),
+                                                      c10::scalarTypeToTypeMeta(types[fmt]));
+  const int64_t width = fmt == 2 ? up(cols, 128) / 128 : cols, ld = fmt == 2 ? width : up(cols, 16);
+  const int64_t sizes[] = {rows, width}, strides[] = {ld, 1};
+  v.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides, buf.storage_offset() + (fmt == 2 ? nbytes(rows, cols) : 0));
+  return v;
+}
+
 // (buffer of the 8-bit rows, x + resid or None)
 std::pair<Tensor, OptTensor> norm(const Tensor& x_in, const OptTensor& resid, const Tensor& w, double eps, double off, int64_t fmt) {
   const c10::cuda::CUDAGuard guard(x_in.device());
@@ -448,7 +468,7 @@ std::pair<Tensor, OptTensor> norm(const Tensor& x_in, const OptTensor& resid, co
   const Tensor x = rows2d(x_in), r = resid ? rows2d(*resid) : Tensor(), wn = unit_stride(w);
   const int64_t R = x.size(0), D = x.size(1);
   const Tensor q = bytes(nbytes(R, D) + nbytes_plain(R, D), x);
-  const Tensor h = r.defined() ? at::empty({R, D}, x.options()) : Tensor();
+  const Tensor h = r.defined() ? fresh({R, D}, x.scalar_type(), x) : Tensor();
   if (R) {
     check(fn.add_rmsnorm(ptr(x), x.stride(0), ptr(r), r.defined() ? r.stride(0) : 0, ptr(wn), ptr(h), ptr(q),
                          ptr(q) + R * up(D, 16), ptr(q) + nbytes(R, D), up(D, 16), nullptr, R, D, fmt, eps, off, stream_of(x)),
@@ -469,4 +489,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_linear", &norm_linear);
   m.def("quantize", &quantize);
   m.def("norm", &norm);
+  m.def("view8", &view8);
 }

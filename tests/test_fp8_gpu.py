@@ -538,3 +538,18 @@ def test_refusals():
                  lambda: ops.add_rmsnorm_fp8(_rand(4, 64), None, torch.ones(64))):
         with pytest.raises((TypeError, ValueError)):
             call()
+
+
+def test_values_and_scales_are_views_of_the_buffer():
+    q = ops.quantize_fp8(_rand(3, 200), E5M2)
+    v, s = q.values, q.scales()
+    assert v.dtype == E5M2 and v.shape == (3, 200) and v.stride() == (208, 1) and v.device == q.device
+    assert s.dtype == torch.float8_e8m0fnu and s.shape == (3, 2) and s.is_contiguous()
+    assert v.untyped_storage().data_ptr() == s.untyped_storage().data_ptr() == q.buf.data_ptr()
+    del q                                                    # the views keep the memory
+    kept = v.float().clone()
+    torch.empty(3 * 208 + 1024, dtype=torch.uint8, device="cuda").fill_(255)
+    assert torch.equal(v.float(), kept) and not v.requires_grad and not v.clone().requires_grad
+    assert torch.equal(torch.cat([v.view(torch.uint8), v.view(torch.uint8)])[3:], v.view(torch.uint8))
+    e = ops.quantize_fp8(torch.empty(0, 5, device="cuda"))
+    assert e.values.shape == (0, 5) and e.scales().shape == (0, 1)
