@@ -121,8 +121,8 @@ _CUDA_PROTOS = {
     "cvb_moe_dispatch": "ppppp l iii p",
     "cvb_moe_combine": "pppp l ii p",
     "cvb_moe_combine_bwd": "pppppppp l iii p",
-    "cvb_fp8_quantize": "p i lll ii pppl pppl pp f p",
-    "cvb_fp8_add_rmsnorm": "plpl p p pppl p l i i ff p",
+    "cvb_fp8_quantize": "p i lll ii pppl pppl pp f i p",
+    "cvb_fp8_add_rmsnorm": "plpl p p pppl p l i i ff i p",
     "cvb_fp8_norm_bwd_parts": "",
     "cvb_fp8_norm_bwd": "pl pl pp pl pp pp l i f p",
     "cvb_fp8_gemm": "ppli ppli iii p l i i p p",

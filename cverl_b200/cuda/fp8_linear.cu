@@ -7,7 +7,7 @@
 extern "C" {
 int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, long long x_stride, int fmt, int mode,
                      void* q, void* sf, void* ps, long long q_ld, void* qt, void* sft, void* pst, long long qt_ld,
-                     const float* rstd, const void* w, float w_offset, void* stream);
+                     const float* rstd, const void* w, float w_offset, int beside, void* stream);
 int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                  long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int after,
                  int* status, void* stream);
@@ -19,7 +19,7 @@ int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* b, const vo
                       int M, int N, int K, void* c, long long ldc, int out_kind, int* status, void* stream);
 int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride, const void* w, void* h,
                         void* q, void* sf, void* ps, long long q_ld, float* rstd, long long rows, int D, int fmt, float eps,
-                        float w_offset, void* stream);
+                        float w_offset, int beside, void* stream);
 int cvb_fp8_norm_bwd(const float* dn, long long dn_stride, const void* h, long long h_stride, const void* w,
                      const float* rstd, const void* dh, long long dh_stride, void* dx, float* part, float* dw_acc,
                      void* dw, long long rows, int D, float w_offset, void* stream);
@@ -40,10 +40,10 @@ struct Mat8 {      // [rows, cols] in a buffer; null buffer: absent
 };
 
 int quantize(const void* x, int x_fp32, long long rows, long long cols, long long stride, int fmt, int extra,
-             const Mat8& q, const Mat8& t, void* stream) {
+             const Mat8& q, const Mat8& t, int beside, void* stream) {
   const int mode = (q.codes ? ROWS : 0) | (t.codes ? COLS : 0) | extra;
   return cvb_fp8_quantize(x, x_fp32, rows, cols, stride, fmt, mode, q.codes, q.sf, nullptr, q.ld, t.codes, t.sf,
-                          nullptr, t.ld, nullptr, nullptr, 0.f, stream);
+                          nullptr, t.ld, nullptr, nullptr, 0.f, beside, stream);
 }
 int product(const Mat8& a, int a_fmt, const Mat8& b, int b_fmt, int M, int N, int K, void* c, long long ldc,
             int out_kind, int after, int* status, void* stream) {
@@ -60,14 +60,13 @@ extern "C" int cvb_fp8_linear_fwd(const void* x, int x_fp32, long long x_stride,
                                   void* y, long long ldy, int out_kind, int* status, void* stream) {
   const Mat8 mxq(xq, M, K), mxt(xt, K, M), mwq(wq, N, K), mwt(wt, K, N);
   int rc = 0;
-  if (w && (rc = quantize(w, w_fp32, N, K, w_stride, E4M3, BLOCKS, mwq, mwt, stream))) return rc;
+  if (w && (rc = quantize(w, w_fp32, N, K, w_stride, E4M3, BLOCKS, mwq, mwt, 0, stream))) return rc;
   if (x && !xq) {
     if (x_fp32 || xt) return -1;
     return cvb_fp8_gemm_rows(x, x_stride, mwq.codes, mwq.sf, mwq.ld, E4M3, M, N, K, y, ldy, out_kind, status, stream);
   }
-  if (x && (rc = quantize(x, x_fp32, M, K, x_stride, E4M3, 0, mxq, mxt, stream))) return rc;
-  // x: the launch before wrote it and not the weight; w alone: it wrote the weight
-  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, x ? AFTER_A : w ? AFTER_OPERANDS : AFTER_ANY, status,
+  if (x && (rc = quantize(x, x_fp32, M, K, x_stride, E4M3, 0, mxq, mxt, w != nullptr, stream))) return rc;
+  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, w ? AFTER_OPERANDS : x ? AFTER_A : AFTER_ANY, status,
                  stream);
 }
 
@@ -78,11 +77,11 @@ extern "C" int cvb_fp8_norm_linear_fwd(const void* x, long long x_stride, const 
                                        void* y, long long ldy, int out_kind, int* status, void* stream) {
   const Mat8 mxq(xq, M, K), mwq(wq, N, K), mwt(wt, K, N);
   int rc = 0;
-  if (w && (rc = quantize(w, w_fp32, N, K, w_stride, E4M3, BLOCKS, mwq, mwt, stream))) return rc;
+  if (w && (rc = quantize(w, w_fp32, N, K, w_stride, E4M3, BLOCKS, mwq, mwt, 0, stream))) return rc;
   if ((rc = cvb_fp8_add_rmsnorm(x, x_stride, resid, r_stride, wn, h, mxq.codes, mxq.sf, nullptr, mxq.ld, rstd, M, K, E4M3,
-                                eps, w_offset, stream)))
+                                eps, w_offset, w != nullptr, stream)))
     return rc;
-  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, AFTER_A, status, stream);
+  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, w ? AFTER_OPERANDS : AFTER_A, status, stream);
 }
 
 // dx [M, K] = dy w (where wt is given) and dw [N, K] (+)= dy^T x (where dw is given).  `dyq` and `dyt` are workspaces
@@ -93,12 +92,12 @@ extern "C" int cvb_fp8_linear_bwd(const void* dy, int dy_fp32, long long dy_stri
                                   int dx_kind, void* dw, long long lddw, int dw_kind, int* status, void* stream) {
   const Mat8 mdq(wt ? dyq : nullptr, M, N), mdt(dw ? dyt : nullptr, N, M), mwt(wt, K, N), mxt(xt, K, M);
   if (!mdq.codes && !mdt.codes) return 0;
-  int rc = quantize(dy, dy_fp32, M, N, dy_stride, grad_fmt, 0, mdq, mdt, stream);
+  int rc = quantize(dy, dy_fp32, M, N, dy_stride, grad_fmt, 0, mdq, mdt, 0, stream);
   if (rc) return rc;
   if (!dw) return product(mdq, grad_fmt, mwt, E4M3, M, K, N, dx, lddx, dx_kind, AFTER_A, status, stream);
   if (h && (rc = cvb_fp8_quantize(h, 0, M, K, h_stride, E4M3, COLS, nullptr, nullptr, nullptr, 0, mxt.codes, mxt.sf,
                                   nullptr, mxt.ld,
-                                  rstd, wn, w_offset, stream)))
+                                  rstd, wn, w_offset, 1, stream)))
     return rc;
   if (!wt) return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, AFTER_OPERANDS, status, stream);
   return cvb_fp8_gemm_grads(mdq.codes, mdq.sf, mdq.ld, mwt.codes, mwt.sf, mwt.ld, mdt.codes, mdt.sf, mdt.ld, mxt.codes,

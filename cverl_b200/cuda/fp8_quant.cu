@@ -10,6 +10,23 @@
 
 namespace cvb {
 
+// `beside`: the kernel reads nothing that the launch before it writes, nor writes what that touches, and runs beside it;
+// it ends after it, so that what follows may rely on both.  All kernels here therefore end with a wait, which returns at
+// once in an ordinary launch.  1301 x 1000 with a weight of 520 rows, forward: 9.9 us, 12.3 one after the other.
+template <typename Args>
+static void launch_rows(void (*kernel)(const Args), const Args& p, long long grid, int threads, int beside, cudaStream_t s) {
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cfg.attrs = &at;
+  cfg.numAttrs = beside ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 constexpr int QT = 128;            // tile edge
 constexpr int Q_THREADS = 256;
 
@@ -108,7 +125,7 @@ struct Piece<__nv_bfloat16, NORM> {
     else return v;
   }
   // codes of row i with the scale in the half i & 1 of `inv`; of columns j and j + 1 with those in its low and high half.
-  // bf16 are scaled as they are read, two to an instruction: 20480 x 3584, both forms, XX us, YY value by value.
+  // bf16 are scaled as they are read, two to an instruction: 20480 x 7168, both forms, 117 us, 123 value by value.
   template <int FMT>
   __device__ __forceinline__ uint2 row_codes(int i, uint32_t inv) const {
     if constexpr (NORM) return fp8_row_codes<FMT>(*this, i, inv);
@@ -389,17 +406,17 @@ fp8_quant_kernel(const QuantArgs p) {
       }
     }
   }
+  wait_for_previous_kernel();      // see launch_rows
 }
 
 template <typename T, int FMT>
-static void quant_launch(const QuantArgs& p, int mode, long long grid, cudaStream_t s) {
-  const dim3 g(static_cast<unsigned>(grid));
+static void quant_launch(const QuantArgs& p, int mode, long long grid, int beside, cudaStream_t s) {
   switch (mode) {
-    case 1: fp8_quant_kernel<T, FMT, false, true, false, false><<<g, Q_THREADS, 0, s>>>(p); break;
-    case 2: fp8_quant_kernel<T, FMT, false, false, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
-    case 3: fp8_quant_kernel<T, FMT, false, true, true, false><<<g, Q_THREADS, 0, s>>>(p); break;
-    case 5: fp8_quant_kernel<T, FP8_E4M3, false, true, false, true><<<g, Q_THREADS, 0, s>>>(p); break;
-    default: fp8_quant_kernel<T, FP8_E4M3, false, true, true, true><<<g, Q_THREADS, 0, s>>>(p); break;
+    case 1: launch_rows(fp8_quant_kernel<T, FMT, false, true, false, false>, p, grid, Q_THREADS, beside, s); break;
+    case 2: launch_rows(fp8_quant_kernel<T, FMT, false, false, true, false>, p, grid, Q_THREADS, beside, s); break;
+    case 3: launch_rows(fp8_quant_kernel<T, FMT, false, true, true, false>, p, grid, Q_THREADS, beside, s); break;
+    case 5: launch_rows(fp8_quant_kernel<T, FP8_E4M3, false, true, false, true>, p, grid, Q_THREADS, beside, s); break;
+    default: launch_rows(fp8_quant_kernel<T, FP8_E4M3, false, true, true, true>, p, grid, Q_THREADS, beside, s); break;
   }
 }
 
@@ -508,18 +525,19 @@ fp8_norm_kernel(const NormQuantArgs p) {
       if (odd) fp8_fix_inf<FMT>(v[i], q + c, n);
     }
   }
+  wait_for_previous_kernel();
 }
 
 template <int TPR, int NV>
-static void norm_launch(const NormQuantArgs& p, int fmt, cudaStream_t s) {
+static void norm_launch(const NormQuantArgs& p, int fmt, int beside, cudaStream_t s) {
   constexpr int THREADS = RowBlock<TPR>::THREADS;
   const unsigned grid = static_cast<unsigned>((p.rows + THREADS / TPR - 1) / (THREADS / TPR));
   if (p.vec) {
-    if (fmt == FP8_E4M3) fp8_norm_kernel<TPR, NV, FP8_E4M3, true><<<grid, THREADS, 0, s>>>(p);
-    else fp8_norm_kernel<TPR, NV, FP8_E5M2, true><<<grid, THREADS, 0, s>>>(p);
+    if (fmt == FP8_E4M3) launch_rows(fp8_norm_kernel<TPR, NV, FP8_E4M3, true>, p, grid, THREADS, beside, s);
+    else launch_rows(fp8_norm_kernel<TPR, NV, FP8_E5M2, true>, p, grid, THREADS, beside, s);
   } else {
-    if (fmt == FP8_E4M3) fp8_norm_kernel<TPR, NV, FP8_E4M3, false><<<grid, THREADS, 0, s>>>(p);
-    else fp8_norm_kernel<TPR, NV, FP8_E5M2, false><<<grid, THREADS, 0, s>>>(p);
+    if (fmt == FP8_E4M3) launch_rows(fp8_norm_kernel<TPR, NV, FP8_E4M3, false>, p, grid, THREADS, beside, s);
+    else launch_rows(fp8_norm_kernel<TPR, NV, FP8_E5M2, false>, p, grid, THREADS, beside, s);
   }
 }
 
@@ -709,7 +727,7 @@ using namespace cvb;
 // mode: 1 row form, 2 transposed form, 3 both, 5 row form with 128 x 128 blocks, 7 both with 128 x 128 blocks
 extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, long long x_stride, int fmt,
                                 int mode, void* q, void* sf, void* ps, long long q_ld, void* qt, void* sft, void* pst,
-                                long long qt_ld, const float* rstd, const void* w, float w_offset, void* stream) {
+                                long long qt_ld, const float* rstd, const void* w, float w_offset, int beside, void* stream) {
   if (rows <= 0 || cols <= 0) return 0;
   if ((fmt != FP8_E4M3 && fmt != FP8_E5M2) || (mode != 1 && mode != 2 && mode != 3 && mode != 5 && mode != 7)) return -1;
   if (mode > 3 && fmt != FP8_E4M3) return -1;
@@ -734,20 +752,21 @@ extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long grid = row_tiles * col_tiles;
   if (rstd != nullptr) {     // the transposed form of a norm's result: what a weight gradient reads
-    fp8_quant_kernel<__nv_bfloat16, FP8_E4M3, true, false, true, false><<<static_cast<unsigned>(grid), Q_THREADS, 0, s>>>(p);
+    launch_rows(fp8_quant_kernel<__nv_bfloat16, FP8_E4M3, true, false, true, false>, p, grid, Q_THREADS, beside, s);
   } else if (x_fp32) {
-    if (fmt == FP8_E4M3) quant_launch<float, FP8_E4M3>(p, mode, grid, s);
-    else quant_launch<float, FP8_E5M2>(p, mode, grid, s);
+    if (fmt == FP8_E4M3) quant_launch<float, FP8_E4M3>(p, mode, grid, beside, s);
+    else quant_launch<float, FP8_E5M2>(p, mode, grid, beside, s);
   } else {
-    if (fmt == FP8_E4M3) quant_launch<__nv_bfloat16, FP8_E4M3>(p, mode, grid, s);
-    else quant_launch<__nv_bfloat16, FP8_E5M2>(p, mode, grid, s);
+    if (fmt == FP8_E4M3) quant_launch<__nv_bfloat16, FP8_E4M3>(p, mode, grid, beside, s);
+    else quant_launch<__nv_bfloat16, FP8_E5M2>(p, mode, grid, beside, s);
   }
   return static_cast<int>(cudaGetLastError());
 }
 
 extern "C" int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride,
                                    const void* w, void* h, void* q, void* sf, void* ps, long long q_ld, float* rstd,
-                                   long long rows, int D, int fmt, float eps, float w_offset, void* stream) {
+                                   long long rows, int D, int fmt, float eps, float w_offset, int beside,
+                                   void* stream) {
   if (rows <= 0 || D <= 0) return 0;
   if (fmt != FP8_E4M3 && fmt != FP8_E5M2) return -1;
   if (!aligned16(q) || q_ld % 16 || q_ld < D || (resid != nullptr) != (h != nullptr)) return -2;
@@ -763,13 +782,13 @@ extern "C" int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void
   p.eps = eps, p.w_offset = w_offset;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // the fewest threads that hold a row with at most four vectors each
-  if (D <= 256) norm_launch<32, 1>(p, fmt, s);
-  else if (D <= 512) norm_launch<32, 2>(p, fmt, s);
-  else if (D <= 1024) norm_launch<32, 4>(p, fmt, s);
-  else if (D <= 2048) norm_launch<128, 2>(p, fmt, s);
-  else if (D <= 4096) norm_launch<128, 4>(p, fmt, s);
-  else if (D <= 8192) norm_launch<256, 4>(p, fmt, s);
-  else norm_launch<512, 4>(p, fmt, s);
+  if (D <= 256) norm_launch<32, 1>(p, fmt, beside, s);
+  else if (D <= 512) norm_launch<32, 2>(p, fmt, beside, s);
+  else if (D <= 1024) norm_launch<32, 4>(p, fmt, beside, s);
+  else if (D <= 2048) norm_launch<128, 2>(p, fmt, beside, s);
+  else if (D <= 4096) norm_launch<128, 4>(p, fmt, beside, s);
+  else if (D <= 8192) norm_launch<256, 4>(p, fmt, beside, s);
+  else norm_launch<512, 4>(p, fmt, beside, s);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -27,9 +27,9 @@ typedef long long ll;
 // ---------------------------------------------------------------------------------------------------------------
 struct Launchers {
   int (*quantize)(const void*, int, ll, ll, ll, int, int, void*, void*, void*, ll, void*, void*, void*, ll, const float*,
-                  const void*, float, void*);
+                  const void*, float, int, void*);
   int (*add_rmsnorm)(const void*, ll, const void*, ll, const void*, void*, void*, void*, void*, ll, float*, ll, int, int,
-                     float, float, void*);
+                     float, float, int, void*);
   int (*linear_fwd)(const void*, int, ll, const void*, int, ll, int, int, int, void*, void*, void*, void*, void*, ll, int,
                     int*, void*);
   int (*linear_bwd)(const void*, int, ll, int, int, int, int, void*, void*, void*, void*, const void*, ll, const float*,
@@ -439,7 +439,7 @@ std::pair<OptTensor, OptTensor> quantize(const Tensor& x_in, int64_t fmt, int64_
   if (R && C) {
     check(fn.quantize(ptr(x), fp32(x), R, C, x.stride(0), fmt, mode, qp, qp ? qp + R * up(C, 16) : nullptr,
                       qp ? qp + nbytes(R, C) : nullptr, up(C, 16), tp, tp ? tp + C * up(R, 16) : nullptr,
-                      tp ? tp + nbytes(C, R) : nullptr, up(R, 16), nullptr, nullptr, 0.f, stream_of(x)),
+                      tp ? tp + nbytes(C, R) : nullptr, up(R, 16), nullptr, nullptr, 0.f, 0, stream_of(x)),
           "cvb_fp8_quantize");
     count_launches(1);
   }
@@ -471,7 +471,8 @@ std::pair<Tensor, OptTensor> norm(const Tensor& x_in, const OptTensor& resid, co
   const Tensor h = r.defined() ? fresh({R, D}, x.scalar_type(), x) : Tensor();
   if (R) {
     check(fn.add_rmsnorm(ptr(x), x.stride(0), ptr(r), r.defined() ? r.stride(0) : 0, ptr(wn), ptr(h), ptr(q),
-                         ptr(q) + R * up(D, 16), ptr(q) + nbytes(R, D), up(D, 16), nullptr, R, D, fmt, eps, off, stream_of(x)),
+                         ptr(q) + R * up(D, 16), ptr(q) + nbytes(R, D), up(D, 16), nullptr, R, D, fmt, eps, off, 0,
+                         stream_of(x)),
           "cvb_fp8_add_rmsnorm");
     count_launches(1);
   }
