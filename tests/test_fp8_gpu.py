@@ -553,3 +553,93 @@ def test_values_and_scales_are_views_of_the_buffer():
     assert torch.equal(torch.cat([v.view(torch.uint8), v.view(torch.uint8)])[3:], v.view(torch.uint8))
     e = ops.quantize_fp8(torch.empty(0, 5, device="cuda"))
     assert e.values.shape == (0, 5) and e.scales().shape == (0, 1)
+
+
+@pytest.mark.parametrize("m", [1, 24, 40, 128, 300, 2048])
+def test_overlapped_launches_give_what_separate_ones_give(m):
+    """Layers without a pause, weights changed in between, against the same operators one at a time."""
+    d, f = 1024, 2560
+    x0, r0, wn = _rand(m, d, seed=1), _rand(m, d, seed=2), _rand(d, seed=3, std=0.1)
+    up0, down0 = _rand(f, d, seed=4, std=d ** -0.5), _rand(d, f, seed=5, std=f ** -0.5)
+    kept = ops.quantize_fp8_weight(_rand(d, d, seed=6, std=d ** -0.5))
+
+    def fast():
+        x, r, up, down = x0.clone(), r0.clone(), up0.clone(), down0.clone()
+        for i in range(30):
+            y, r = ops.add_rmsnorm_linear_fp8(x, r, wn, up)
+            up.mul_(-1.001)
+            x = ops.linear_fp8(y, down)
+            down.mul_(-0.999)
+            x = ops.linear_fp8(x, kept)
+        return x, r, y
+
+    def one_at_a_time():
+        def product(q, w):
+            torch.cuda.synchronize()
+            y = ops.gemm_fp8_nt(q, w if isinstance(w, ops.Fp8Tensor) else ops.quantize_fp8_weight(w).w)
+            torch.cuda.synchronize()
+            return y
+        x, r, up, down = x0.clone(), r0.clone(), up0.clone(), down0.clone()
+        for i in range(30):
+            q, r = ops.add_rmsnorm_fp8(x, r, wn)
+            y = product(q, up)
+            up.mul_(-1.001)
+            x = product(ops.quantize_fp8(y), down)
+            down.mul_(-0.999)
+            x = product(ops.quantize_fp8(x), kept.w)
+        return x, r, y
+
+    with torch.no_grad():
+        want = one_at_a_time()
+        for got in (fast(), fast()):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            got = fast()
+        for _ in range(2):
+            g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_overlapped_backward_passes():
+    """Training steps without a pause: whole numbers, so that every result is exact; and a norm in front, against the
+    same steps with a pause before and after each."""
+    m, k, n = 1500, 1024, 1280
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, w0, dy = (torch.randint(-8, 9, s, device="cuda", generator=g).bfloat16() for s in ((m, k), (n, k), (m, n)))
+    x.requires_grad_()
+    w = w0.clone().requires_grad_()
+    w.main_grad = torch.zeros(n, k, device="cuda")
+    got = []
+    for i in range(30):
+        got.append(torch.autograd.grad(ops.linear_fp8(x, w), (x, w), dy, allow_unused=True)[0])
+        with torch.no_grad():
+            w.mul_(-1.0 if i % 3 else 0.5 ** (i % 2))
+            dy = dy.neg()
+    want, main = [], torch.zeros(n, k, device="cuda", dtype=torch.float64)
+    scale, sign = 1.0, 1.0
+    dx0, dw0 = dy.double() @ w0.double(), dy.double().t() @ x.detach().double()
+    for i in range(30):
+        assert torch.equal(got[i], (dx0 * scale * sign).float().bfloat16())
+        main += sign * dw0
+        scale, sign = scale * (-1.0 if i % 3 else 0.5 ** (i % 2)), -sign
+    assert torch.equal(w.main_grad.double(), main)
+
+    r, wn, d = _rand(m, k, seed=4), _rand(k, seed=5, std=0.1), _rand(m, n, seed=6, std=1e-2)
+
+    def steps(pause):
+        a, b, c, e = (t.detach().clone().requires_grad_() for t in (_rand(m, k, seed=7), r, wn, _rand(n, k, seed=8)))
+        for i in range(15):
+            pause()
+            y, h = ops.add_rmsnorm_linear_fp8(a, b, c, e)
+            pause()
+            grads = torch.autograd.grad((y, h), (a, b, c, e), (d, r))
+            pause()
+            with torch.no_grad():
+                for t, u in zip((a, b, c, e), grads):
+                    t.add_(u, alpha=-0.1)
+        return y, h, a, b, c, e
+
+    for u, v in zip(steps(lambda: None), steps(torch.cuda.synchronize)):
+        assert torch.equal(u, v)
