@@ -18,7 +18,7 @@ enum : int { FP8_OUT_BF16 = 0, FP8_OUT_F32 = 1, FP8_OUT_F32_ACC = 2 };
 // What a launch may assume of the kernel before it in the stream.  Where that is the kernel that quantised the
 // operands, the product is placed while it still runs (programmatic dependent launch), sets up its barriers, tensor
 // memory and first loads of what that kernel does not write, and waits for its end.  128 rows, N = 1024, K = 3584,
-// quantised and multiplied: 8.6 us, 9.4 one after the other; 16 rows, N = 7168, K = 1024 after a norm: 6.3 and 7.9.
+// quantised and multiplied: 7.7 us, 8.6 one after the other; 16 rows, N = 7168, K = 1024 after a norm: 6.3 and 7.9.
 enum Fp8After {
   AFTER_ANY = 0,           // nothing: an ordinary launch
   AFTER_OPERANDS = 1,      // it, or one before it, wrote A and B; none of its writes is C
@@ -145,7 +145,6 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
 // to back against 6.6 for two kernels; at 64 rows 11.5 against 8.8).  A stage's scale cells hold this block's byte only,
 // so they move to tensor memory once a block.
 // ---------------------------------------------------------------------------------------------------
-constexpr int F8_SMEM_ALONE = 117 * 1024;     // more than half of an SM: no second CTA beside
 template <int TN>
 struct F8SmallCfg {
   static constexpr int B_BYTES = 128 * 128;
@@ -255,6 +254,9 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     }
   } else if (warp == 1) {
     const uint32_t idesc = umma_idesc_mxf8(128, TN, p.b_fmt, p.a_fmt);
+    // where the tile's rows begin in their group's scales (copied whole): 0, or 2 columns for the second 64 of 128 rows.
+    // Narrower tiles are the only one of their group: the operand may not begin at an odd column.
+    const uint32_t a_col = TN == 64 ? (m0 & 127) >> 5 : 0;
     const bool leader = elect_one();
     const uint64_t db0 = umma_smem_desc(smem_u32(smem), 16, 1024);
     const uint64_t da0 = umma_smem_desc(smem_u32(smem) + Cfg::B_BYTES, 16, 1024);
@@ -270,12 +272,13 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       const uint64_t ds = ds0 + stage * (Cfg::SF_BYTES >> 4);
       const uint32_t id = umma_idesc_scale_id(idesc, kb & 3);
       const uint32_t sfb = tmem + Cfg::SFB_COL + slot * 4, sfa = tmem + Cfg::SFA_COL + (FUSE ? stage : slot) * 4;
+      const uint32_t rows_a = sfa + a_col;
       if (leader) {
         if (scales) tmem_cp_scales(sfb, ds);
         if (scales || FUSE) tmem_cp_scales(sfa, ds + 32);
-        umma_mxf8(tmem, db, da, id, sfb, sfa, kb > kb0 ? 1u : 0u);
+        umma_mxf8(tmem, db, da, id, sfb, rows_a, kb > kb0 ? 1u : 0u);
 #pragma unroll
-        for (int k = 1; k < 4; ++k) umma_mxf8(tmem, db + 2 * k, da + 2 * k, id, sfb, sfa, 1u);
+        for (int k = 1; k < 4; ++k) umma_mxf8(tmem, db + 2 * k, da + 2 * k, id, sfb, rows_a, 1u);
         umma_commit(&empty_bar[stage]);
         if (last) umma_commit(done_bar);
       }
@@ -863,37 +866,33 @@ template <int TN, bool FUSE>
 static int launch_small(const Fp8Product& o, cudaStream_t stream) {
   using Cfg = F8SmallCfg<TN>;
   static_assert(TN * 512 <= Cfg::STAGES * Cfg::TILE_BYTES, "the partial tile fits the stages");
-  static_assert(Cfg::SMEM_BYTES <= F8_SMEM_ALONE, "opted in");
   CUtensorMap ta = {}, tb;
   Fp8GemmParams p = o.p;
   if ((!FUSE && encode_tensor_map(&ta, o.a, 1, p.K, p.M, 0, o.lda, 0, 128, TN)) ||
       encode_tensor_map(&tb, o.b, 1, p.K, p.N, 0, o.ldb, 0, 128, 128))
     return -10;
   auto kern = fp8_gemm_small_kernel<TN, FUSE>;
-  if (const int e = opt_in_smem<fp8_gemm_small_kernel<TN, FUSE>>(F8_SMEM_ALONE)) return e;
+  if (const int e = opt_in_smem<fp8_gemm_small_kernel<TN, FUSE>>(Cfg::SMEM_BYTES)) return e;
   p.m_tiles = (p.M + TN - 1) / TN;
   p.n_tiles = (p.N + 127) / 128;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-  // Fill the SMs: one CTA each (two where each still has 8 K blocks), clusters of eight only where few of them have to
-  // find room.  One token, N = 1024, K = 3584: 10.2 us with one CTA a tile, 4.3 with eight; 128 rows, N = K = 2048:
-  // 12.2 with one, 7.4 with four, 8.8 with eight; 128 rows, N = K = 8192: 27.0 with one, 17.6 with two, 14.6 with four.
+  // Fill the SMs: one CTA each (two where each still has 8 K blocks), clusters of eight only where there are few of them
+  // or each CTA still has 6 K blocks.  One token, N = 1024, K = 3584: 10.2 us with one CTA a tile, 4.3 with eight; 128
+  // rows, N = 1024, K = 3584: 6.5 with four, 6.8 with eight; 16 rows, N = 2048, K = 8192: 7.4 with four, 6.2 with eight;
+  // 128 rows, N = K = 8192: 27.0 with one, 17.6 with two, 14.6 with four.
   p.split = 1;
   while (p.split < 8) {
     const int next = p.split * 2, per = p.kblocks / next;
-    const long long room = next == 8 ? 74 : per >= 8 ? 296 : 148;
+    const long long room = next == 8 ? (per >= 6 ? 128 : 74) : per >= 8 ? 296 : 148;
     if (per < 1 || tiles * next > room) break;
     p.split = next;
   }
   p.kb_per_split = (p.kblocks + p.split - 1) / p.split;
   p.split = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
   if (tiles * p.split > 0x7fffffffll) return -11;
-  // Placed beside a kernel that still runs, CTAs would gather in pairs on the SMs that it leaves free: where there is
-  // an SM for each, too much shared memory for two (128 rows, N = K = 4096: 10.3 us with the quantisation, 12.6 in
-  // pairs).  128: clusters of four do not find 148 SMs.
-  const int smem = p.after != AFTER_ANY && tiles * p.split <= 128 ? F8_SMEM_ALONE : Cfg::SMEM_BYTES;
   cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg =
-      cluster_config(at, static_cast<unsigned>(tiles * p.split), F8_THREADS, p.split, smem, p.after, stream);
+      cluster_config(at, static_cast<unsigned>(tiles * p.split), F8_THREADS, p.split, Cfg::SMEM_BYTES, p.after, stream);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, p));
 }
 
@@ -981,7 +980,7 @@ static PairCost choose_pair(const Fp8GemmParams& p, long long* least) {
   return best;
 }
 // Above 128 rows always pairs; from 65 where tiles of 128 columns fill half of the SMs and K is short (128 rows,
-// N = 7168, K = 1024: 6.6 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 7.7; N = K = 8192:
+// N = 7168, K = 1024: 6.6 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 6.6; N = K = 8192:
 // 19.2 against 14.6).
 static bool takes_pairs(const Fp8GemmParams& p) {
   return p.M > 128 || (p.M > 64 && p.N >= 37 * 128 && p.kblocks <= 12);
@@ -1000,7 +999,9 @@ static int launch_product(const Fp8Product& o, cudaStream_t stream) {
   }
   if (p.M <= 16) return launch_small<16, false>(o, stream);
   if (p.M <= 32) return launch_small<32, false>(o, stream);
-  if (p.M <= 64) return launch_small<64, false>(o, stream);
+  // two tiles of 64 rows instead of one of 128 while their CTAs find an SM each: half as much to meet and to store
+  // (128 rows, N = 1024, K = 3584: 6.6 us against 7.1; N = K = 2048: 6.3 against 7.5; N = K = 8192: 17.3 against 14.5)
+  if (p.M <= 64 || p.N <= 37 * 128) return launch_small<64, false>(o, stream);
   return launch_small<128, false>(o, stream);
 }
 
