@@ -982,8 +982,14 @@ static PairCost choose_pair(const Fp8GemmParams& p, long long* least) {
 // Above 128 rows always pairs; from 65 where tiles of 128 columns fill half of the SMs and K is short (128 rows,
 // N = 7168, K = 1024: 6.6 us against 8.8 with the other kernel; N = 1024, K = 3584: 9.3 against 6.6; N = K = 8192:
 // 19.2 against 14.6).
-static bool takes_pairs(const Fp8GemmParams& p) {
+static bool fills_pairs(const Fp8GemmParams& p) {
   return p.M > 128 || (p.M > 64 && p.N >= 37 * 128 && p.kblocks <= 12);
+}
+// But tiles of 64 x 128 while four CTAs of a cluster each find an SM: 256 rows, N = 1024, K = 3584: 6.9 us against 9.3
+// in pairs; 512 rows, N = 512, K = 4096: 7.4 against 9.9; 512 rows, N = K = 1024 (64 tiles): 6.9 against 6.4.
+static bool takes_pairs(const Fp8GemmParams& p) {
+  const long long tiles = static_cast<long long>((p.M + 63) / 64) * ((p.N + 127) / 128);
+  return fills_pairs(p) && (p.M <= 128 || tiles > 37);
 }
 
 static int launch_product(const Fp8Product& o, cudaStream_t stream) {
@@ -1032,7 +1038,7 @@ static GradsPlan plan_grads(int M, int N, int K) {
   x.M = M, x.N = K, x.kblocks = (N + 127) / 128;
   w.M = N, w.N = K, w.kblocks = (M + 127) / 128;
   GradsPlan plan = {0, 0, x.kblocks > w.kblocks};
-  if (!takes_pairs(x) || !takes_pairs(w)) return plan;
+  if (!fills_pairs(x) || !fills_pairs(w)) return plan;
   long long least, apart;
   choose_pair(x, &least);
   choose_pair(w, &apart);
