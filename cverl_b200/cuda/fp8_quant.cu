@@ -125,7 +125,7 @@ struct Piece<__nv_bfloat16, NORM> {
     else return v;
   }
   // codes of row i with the scale in the half i & 1 of `inv`; of columns j and j + 1 with those in its low and high half.
-  // bf16 are scaled as they are read, two to an instruction: 20480 x 7168, both forms, 117 us, 123 value by value.
+  // bf16 are scaled as they are read, two to an instruction: 20480 x 3584, both forms, 57.4 us, 59.7 value by value.
   template <int FMT>
   __device__ __forceinline__ uint2 row_codes(int i, uint32_t inv) const {
     if constexpr (NORM) return fp8_row_codes<FMT>(*this, i, inv);
@@ -266,8 +266,8 @@ __device__ __forceinline__ bool piece_maxima(const Piece<__nv_bfloat16, false>& 
 // Instructions bound this kernel before HBM does (71 % of the issue slots and 65 % of the integer pipe at 4.1 TB/s in
 // an earlier form), so scales are computed two to a word, a column's once for the tile, addresses advance by a stride,
 // and an infinity costs nothing where there is none.
-template <typename T, int FMT, bool NORM, bool ROWS, bool COLS, bool BLOCK>
-__global__ void __launch_bounds__(Q_THREADS, sizeof(T) == 4 ? 1 : NORM ? 2 : 3)
+template <typename T, int FMT, bool NORM, bool ROWS, bool COLS, bool BLOCK, int CTAS = sizeof(T) == 4 ? 1 : NORM ? 2 : 3>
+__global__ void __launch_bounds__(Q_THREADS, CTAS)
 fp8_quant_kernel(const QuantArgs p) {
   launch_dependents();             // a product that follows sets itself up meanwhile
   __shared__ __align__(16) uint32_t s_max[COLS || BLOCK ? Q_THREADS / 32 : 1][QT / 2];   // column maxima by warp
@@ -409,8 +409,17 @@ fp8_quant_kernel(const QuantArgs p) {
   wait_for_previous_kernel();      // see launch_rows
 }
 
+// Four CTAs an SM (64 registers, some spilled) where rows are written and there are eight tiles an SM or more, else three:
+// both forms of 20480 x 3584 57.4 us with three, 53.2 with four; its rows 38.6 and 36.5; its transpose alone 40.2 and 42.1;
+// both forms of 20480 x 1024 (1,280 tiles) 16.6 either way; of 4096 x 2048 (512 tiles) 8.2 and 8.9.
 template <typename T, int FMT>
 static void quant_launch(const QuantArgs& p, int mode, long long grid, int beside, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (grid > 8 * 148 && mode == 1)
+      return launch_rows(fp8_quant_kernel<T, FMT, false, true, false, false, 4>, p, grid, Q_THREADS, beside, s);
+    if (grid > 8 * 148 && mode == 3)
+      return launch_rows(fp8_quant_kernel<T, FMT, false, true, true, false, 4>, p, grid, Q_THREADS, beside, s);
+  }
   switch (mode) {
     case 1: launch_rows(fp8_quant_kernel<T, FMT, false, true, false, false>, p, grid, Q_THREADS, beside, s); break;
     case 2: launch_rows(fp8_quant_kernel<T, FMT, false, false, true, false>, p, grid, Q_THREADS, beside, s); break;
