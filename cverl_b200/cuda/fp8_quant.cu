@@ -118,11 +118,15 @@ struct Piece<__nv_bfloat16, NORM> {
         if (a == i && b == j) v = get(a, b);
     return v;
   }
-  __device__ __forceinline__ float get(int i, int j) const {
+  __device__ __forceinline__ float scaled(int i, int j) const {       // x, or x rstd
     const uint32_t w = raw[i][j >> 1];
     const float v = __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
-    if constexpr (NORM) return v * rstd[i] * gain[j];
+    if constexpr (NORM) return v * rstd[i];
     else return v;
+  }
+  __device__ __forceinline__ float get(int i, int j) const {
+    if constexpr (NORM) return scaled(i, j) * gain[j];
+    else return scaled(i, j);
   }
   // codes of row i with the scale in the half i & 1 of `inv`; of columns j and j + 1 with those in its low and high half.
   // bf16 are scaled as they are read, two to an instruction: 20480 x 3584, both forms, 57.4 us, 59.7 value by value.
@@ -220,6 +224,36 @@ __device__ __forceinline__ bool piece_maxima(const Piece<T, NORM>& x, uint32_t (
     rmax[i] = fp8_max16(__float_as_uint(rm[2 * i])) | (fp8_max16(__float_as_uint(rm[2 * i + 1])) << 16);
     cmax[i] = fp8_max16(__float_as_uint(cm[2 * i])) | (fp8_max16(__float_as_uint(cm[2 * i + 1])) << 16);
   }
+  return odd;
+}
+
+// The norm's result, columns alone (rmax is not written).  Rounding keeps the order of magnitudes, so a column's maximum
+// of |x rstd gain| is the gain's product with that of |x rstd|; NaN, a gain's among them, is passed over by fmaxf.
+__device__ __forceinline__ bool piece_maxima(const Piece<__nv_bfloat16, true>& x, uint32_t (&)[4], uint32_t (&cmax)[4]) {
+  float cm[8], all = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    cm[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cm[j] = fmaxf(cm[j], fabsf(x.scaled(i, j)));
+    cm[j] = fmaxf(0.f, cm[j] * fabsf(x.gain[j]));
+    all = fmaxf(all, cm[j]);
+  }
+  const bool odd = __float_as_uint(all) >= 0x7F800000u;
+  if (odd) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      cm[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(x.get(i, j));
+        if (__float_as_uint(a) < 0x7F800000u) cm[j] = fmaxf(cm[j], a);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    cmax[j] = fp8_max16(__float_as_uint(cm[2 * j])) | (fp8_max16(__float_as_uint(cm[2 * j + 1])) << 16);
   return odd;
 }
 
