@@ -141,9 +141,9 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
 //
 // FUSE: A comes as bf16 rows.  The four epilogue warps, idle until the MMAs end, read 128 columns at a time, find each
 // row's scale and write codes and scale bytes where TMA would have put them; every column of tiles does so for itself,
-// which for up to 32 rows costs less than a launch and a pass through memory (one token, N = 7168, K = 1024: 5.3 us back
-// to back against 6.6 for two kernels; at 64 rows 11.5 against 8.8).  A stage's scale cells hold this block's byte only,
-// so they move to tensor memory once a block.
+// which for up to 16 rows costs less than a launch and a pass through memory (one token, N = 7168, K = 1024: 5.0 us back
+// to back against 5.4 for two kernels that overlap; 24 rows 6.9 against 5.8).  A stage's scale cells hold this block's
+// byte only, so they move to tensor memory once a block.
 // ---------------------------------------------------------------------------------------------------
 template <int TN>
 struct F8SmallCfg {
@@ -291,12 +291,11 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   } else {
     const int q = warp & 3;
     if constexpr (FUSE) {
-      // 16 rows at a time: eight threads a row, 16 columns each
-      constexpr int PASSES = TN / 16;
-      const int r16 = (threadIdx.x - 64) >> 3, j = threadIdx.x & 7;
-      uint4 raw[PASSES][2], next[PASSES][2];           // this block's values and the next one's
-      auto load = [&](int kb, int pass, uint4(&out)[2]) {
-        const int row = m0 + pass * 16 + r16, c = kb * 128 + j * 16;
+      static_assert(TN == 16, "eight threads a row, 16 columns each");
+      const int r = (threadIdx.x - 64) >> 3, j = threadIdx.x & 7, row = m0 + r;
+      uint4 raw[2], next[2];                            // this block's values and the next one's
+      auto load = [&](int kb, uint4(&out)[2]) {
+        const int c = kb * 128 + j * 16;
         const __nv_bfloat16* src = p.x + row * p.x_stride + c;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -304,39 +303,29 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           out[h] = p.x_vec ? load_raw8<true>(src + h * 8, n) : load_raw8<false>(src + h * 8, n);
         }
       };
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) load(kb0, i, raw[i]);
+      load(kb0, raw);
       int stage = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (kb + 1 < kb1) {
-#pragma unroll
-          for (int i = 0; i < PASSES; ++i) load(kb + 1, i, next[i]);
-        }
+        if (kb + 1 < kb1) load(kb + 1, next);
         if (!warp_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, ERR_WAIT_EMPTY)) break;
-        uint8_t* sa = smem + stage * Cfg::TILE_BYTES + Cfg::B_BYTES;
-        uint8_t* sf = sf_smem + stage * Cfg::SF_BYTES + 512 + (kb & 3);
+        float lo[8], hi[8];
+        widen8(raw[0], lo);
+        widen8(raw[1], hi);
+        bool odd = false;
+        uint32_t m = fp8_max16(max(fp8_finite_max(lo, &odd), fp8_finite_max(hi, &odd)));
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          float lo[8], hi[8];
-          widen8(raw[i][0], lo);
-          widen8(raw[i][1], hi);
-          bool odd = false;
-          uint32_t m = fp8_max16(max(fp8_finite_max(lo, &odd), fp8_finite_max(hi, &odd)));
-#pragma unroll
-          for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const uint32_t byte = fp8_scale_bytes<FP8_E4M3>(m) & 0xFFu;
-          const float inv = fp8_low(fp8_inverse_scales(byte));
-          const uint2 a = fp8_pack8<FP8_E4M3>(lo, inv), b = fp8_pack8<FP8_E4M3>(hi, inv);
-          const int r = i * 16 + r16;
-          uint8_t* dst = sa + r * 128 + ((j ^ (r & 7)) << 4);      // the 128-byte swizzle
-          *reinterpret_cast<uint4*>(dst) = make_uint4(a.x, a.y, b.x, b.y);
-          if (odd) {
-            fp8_fix_inf<FP8_E4M3>(lo, dst, 8);
-            fp8_fix_inf<FP8_E4M3>(hi, dst + 8, 8);
-          }
-          if (j == 0) sf[(r & 31) * 16 + (r >> 5) * 4] = static_cast<uint8_t>(byte);
+        for (int o = 4; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const uint32_t byte = fp8_scale_bytes<FP8_E4M3>(m) & 0xFFu;
+        const float inv = fp8_low(fp8_inverse_scales(byte));
+        const uint2 a = fp8_pack8<FP8_E4M3>(lo, inv), b = fp8_pack8<FP8_E4M3>(hi, inv);
+        uint8_t* dst = smem + stage * Cfg::TILE_BYTES + Cfg::B_BYTES + r * 128 + ((j ^ (r & 7)) << 4);   // 128-byte swizzle
+        *reinterpret_cast<uint4*>(dst) = make_uint4(a.x, a.y, b.x, b.y);
+        if (odd) {
+          fp8_fix_inf<FP8_E4M3>(lo, dst, 8);
+          fp8_fix_inf<FP8_E4M3>(hi, dst + 8, 8);
         }
+        if (j == 0) sf_smem[stage * Cfg::SF_BYTES + 512 + r * 16 + (kb & 3)] = static_cast<uint8_t>(byte);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full_bar[stage]);
@@ -344,8 +333,7 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           stage = 0;
           phase ^= 1;
         }
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) raw[i][0] = next[i][0], raw[i][1] = next[i][1];
+        raw[0] = next[0], raw[1] = next[1];
       }
     }
     bool ok = mbar_wait_bounded(done_bar, 0, abort_flag);
@@ -1094,13 +1082,13 @@ static int product_params(Fp8Product* o, const void* a, const void* a_sf, long l
   return 0;
 }
 
-// C = Q(x) B^T for up to 32 bf16 rows x, quantised to e4m3 within the product
+// C = Q(x) B^T for up to 16 bf16 rows x, quantised to e4m3 within the product
 extern "C" int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* b, const void* b_sf, long long ldb,
                                  int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int* status,
                                  void* stream_v) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (M > 32 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
+  if (M > 16 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
   if (!status || !x || !b || !b_sf || !c) return -2;
   if (((reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(b_sf)) & 15) || ldb % 16 || ldb < K || ldc < N) return -3;
   Fp8GemmParams p = {};
@@ -1111,8 +1099,7 @@ extern "C" int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* 
   p.a_fmt = FP8_E4M3, p.b_fmt = b_fmt;
   output_params(p, c, ldc, out_kind, status);
   const Fp8Product o = {nullptr, b, 0, ldb, p};
-  if (M <= 16) return launch_small<16, true>(o, stream);
-  return launch_small<32, true>(o, stream);
+  return launch_small<16, true>(o, stream);
 }
 
 extern "C" int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,

@@ -53,7 +53,7 @@ int product(const Mat8& a, int a_fmt, const Mat8& b, int b_fmt, int M, int N, in
 }  // namespace
 
 // y [M, N] = x [M, K] w [N, K]^T.  x null: `xq` holds its 8-bit form already.  w null: `wq` does.  `xt` and `wt`
-// (both may be null) take the transposed forms that the backward pass reads.  xq null: up to 32 bf16 rows, quantised
+// (both may be null) take the transposed forms that the backward pass reads.  xq null: up to 16 bf16 rows, quantised
 // within the product.
 extern "C" int cvb_fp8_linear_fwd(const void* x, int x_fp32, long long x_stride, const void* w, int w_fp32,
                                   long long w_stride, int M, int N, int K, void* xq, void* xt, void* wq, void* wt,

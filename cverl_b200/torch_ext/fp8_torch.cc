@@ -112,10 +112,10 @@ Tensor shaped(const Tensor& y, at::IntArrayRef x_shape) {
 }
 
 // Whether the product quantises its bf16 rows itself (rows whose transpose nobody needs): every tile of 128 columns
-// does it for its share of K, in series, so for few rows of moderate length.  Back to back, against two kernels: one
-// row, K = 1024, N = 7168: 5.3 us against 6.6; 16 rows, K = 3584, N = 1024: 6.1 against 7.3; 32 rows, K = 2048: 7.2
-// against 7.5; 64 rows: 10.6 against 8.2; 16 rows, K = N = 8192: 14.2 against 11.9.  And one launch less.
-bool quantised_within(int64_t M, int64_t K) { return (M <= 16 && K <= 4096) || (M <= 32 && K <= 2048); }
+// does it for its share of K, in series, so for few rows of moderate length.  Back to back, against two kernels that
+// overlap: one row, K = 1024, N = 7168: 5.0 us against 5.4; 16 rows, K = 3584, N = 1024: 5.2 against 5.4; 24 rows: 6.6
+// against 5.7; 16 rows, K = N = 4096: 7.6 against 6.9, with K = 6144, N = 2048 6.9 against 6.7.  And one launch less.
+bool quantised_within(int64_t M, int64_t K) { return M <= 16 && K <= 4096; }
 
 // ---------------------------------------------------------------------------------------------------------------
 // weights: a parameter to convert in the call, or 8-bit forms that the caller keeps
