@@ -141,7 +141,7 @@ template <bool VEC>
 __device__ __forceinline__ uint4 load_raw8(const __nv_bfloat16* p, int n) {
   uint4 u = make_uint4(0u, 0u, 0u, 0u);
   if (VEC) {
-    if (n > 0) u = __ldg(reinterpret_cast<const uint4*>(p));
+    if (n > 0) u = *reinterpret_cast<const uint4*>(p);
   } else {
     const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
     u.x = (n > 0 ? e[0] : 0u) | ((n > 1 ? e[1] : 0u) << 16);

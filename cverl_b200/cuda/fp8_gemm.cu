@@ -15,16 +15,11 @@ namespace cvb {
 
 enum : int { FP8_OUT_BF16 = 0, FP8_OUT_F32 = 1, FP8_OUT_F32_ACC = 2 };
 
-// What a launch may assume of the kernel before it in the stream.  Where that is the kernel that quantised the
-// operands, the product is placed while it still runs (programmatic dependent launch), sets up its barriers, tensor
-// memory and first loads of what that kernel does not write, and waits for its end.  128 rows, N = 1024, K = 3584,
-// quantised and multiplied: 7.7 us, 8.6 one after the other; 16 rows, N = 7168, K = 1024 after a norm: 6.3 and 7.9.
-enum Fp8After {
-  AFTER_ANY = 0,           // nothing: an ordinary launch
-  AFTER_OPERANDS = 1,      // it, or one before it, wrote A and B; none of its writes is C
-  AFTER_A = 2,             // it wrote A; B was complete before it started
-};
-
+// Products, like the quantisations and the norm's forward pass, are launched so that they may be placed while the kernel
+// before them in the stream still runs (programmatic dependent launch).  A product sets up its barriers and tensor memory
+// meanwhile, loads B where the caller says that nobody writes it, and touches no other global memory before that kernel
+// has ended.  128 rows, N = 1024,
+// K = 3584, quantised and multiplied: 7.7 us, 8.6 one after the other; 16 rows, N = 7168, K = 1024 after a norm: 6.3, 7.9.
 struct Fp8GemmParams {
   const uint8_t *a_sf, *b_sf;
   const __nv_bfloat16* x;  // small kernel, FUSE: A as bf16 rows, quantised on the way
@@ -38,7 +33,7 @@ struct Fp8GemmParams {
   int m_tiles, n_tiles;
   int split, kb_per_split; // CTAs (or CTA pairs) of a cluster that share a tile's K, and K blocks of each
   int group_m, total;      // pair kernel: M tiles walked per N tile, tiles in all
-  int after;               // Fp8After
+  int b_ready;             // B was complete before the kernel before this one started
   int* status;
 };
 
@@ -223,9 +218,9 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     // The first fill of every stage waits for nothing: one lane a stage.  One after the other they took 560 cycles each
     // (one row, N = K = 1024: 3.7 us against 3.4).
     const bool first = lane < Cfg::STAGES && kb0 + lane < kb1;
-    if (p.after != AFTER_A) wait_for_previous_kernel();
+    if (!p.b_ready) wait_for_previous_kernel();
     if (first) fill_b(kb0 + lane, lane);
-    if (p.after == AFTER_A) wait_for_previous_kernel();
+    if (p.b_ready) wait_for_previous_kernel();
     if (first) fill_a(kb0 + lane, lane);
     __syncwarp();
     int stage = 0;
@@ -303,6 +298,7 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           out[h] = p.x_vec ? load_raw8<true>(src + h * 8, n) : load_raw8<false>(src + h * 8, n);
         }
       };
+      wait_for_previous_kernel();
       load(kb0, raw);
       int stage = 0;
       uint32_t phase = 0;
@@ -621,7 +617,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ Fp8PairArgs<PRODUCTS> g) {
   if (warp == 0) {
     const bool leader = elect_one();
     const uint32_t full0 = mapa_cluster(smem_u32(full_bar), even);
-    wait_for_previous_kernel();
+    wait_for_previous_kernel();          // the stores of this pair follow on its loads
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -836,7 +832,7 @@ static int opt_in_smem(int bytes) {
 }
 
 static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute (&at)[2], unsigned grid, int threads, int cluster,
-                                         size_t smem, int after, cudaStream_t stream) {
+                                         size_t smem, cudaStream_t stream) {
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = cluster;
   at[0].val.clusterDim.y = 1;
@@ -849,7 +845,7 @@ static cudaLaunchConfig_t cluster_config(cudaLaunchAttribute (&at)[2], unsigned 
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = at;
-  cfg.numAttrs = after == AFTER_ANY ? 1 : 2;
+  cfg.numAttrs = 2;
   return cfg;
 }
 
@@ -883,7 +879,7 @@ static int launch_small(const Fp8Product& o, cudaStream_t stream) {
   if (tiles * p.split > 0x7fffffffll) return -11;
   cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg =
-      cluster_config(at, static_cast<unsigned>(tiles * p.split), F8_THREADS, p.split, Cfg::SMEM_BYTES, p.after, stream);
+      cluster_config(at, static_cast<unsigned>(tiles * p.split), F8_THREADS, p.split, Cfg::SMEM_BYTES, stream);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, p));
 }
 
@@ -895,7 +891,7 @@ static int fp8_pair_capacity() {
     auto kern = fp8_gemm_pair_kernel<BN, false, 1>;
     if (opt_in_smem<fp8_gemm_pair_kernel<BN, false, 1>>(Cfg::SMEM_BYTES)) return 0;
     cudaLaunchAttribute at[2];
-    cudaLaunchConfig_t cfg = cluster_config(at, 2 * 148, Cfg::THREADS, 2, Cfg::SMEM_BYTES, AFTER_ANY, nullptr);
+    cudaLaunchConfig_t cfg = cluster_config(at, 2 * 148, Cfg::THREADS, 2, Cfg::SMEM_BYTES, nullptr);
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
     return n;
@@ -930,7 +926,7 @@ static int launch_pairs(const Fp8PairArgs<PRODUCTS>& g, int clusters, int split,
   if (const int e = opt_in_smem<fp8_gemm_pair_kernel<BN, SPLIT, PRODUCTS>>(Cfg::SMEM_BYTES)) return e;
   cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg =
-      cluster_config(at, 2u * split * clusters, Cfg::THREADS, 2 * split, Cfg::SMEM_BYTES, g.p[0].after, stream);
+      cluster_config(at, 2u * split * clusters, Cfg::THREADS, 2 * split, Cfg::SMEM_BYTES, stream);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<BN, SPLIT, PRODUCTS>, g));
 }
 
@@ -1068,8 +1064,8 @@ static void output_params(Fp8GemmParams& p, void* c, long long ldc, int out_kind
 
 static int product_params(Fp8Product* o, const void* a, const void* a_sf, long long lda, int a_fmt, const void* b,
                           const void* b_sf, long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc,
-                          int out_kind, int after, int* status) {
-  if (a_fmt < 0 || after < AFTER_ANY || after > AFTER_A || a_fmt > 1 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
+                          int out_kind, int b_ready, int* status) {
+  if (a_fmt < 0 || a_fmt > 1 || b_fmt < 0 || b_fmt > 1 || out_kind < 0 || out_kind > 2) return -1;
   if (!status || !a || !b || !a_sf || !b_sf || !c) return -2;
   // TMA and bulk copies start on 16-byte boundaries
   if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(a_sf) |
@@ -1080,7 +1076,7 @@ static int product_params(Fp8Product* o, const void* a, const void* a_sf, long l
   p.a_sf = static_cast<const uint8_t*>(a_sf), p.b_sf = static_cast<const uint8_t*>(b_sf);
   p.M = M, p.N = N, p.K = K;
   p.kblocks = (K + 127) / 128, p.kgroups = (p.kblocks + 3) / 4;
-  p.a_fmt = a_fmt, p.b_fmt = b_fmt, p.after = after;
+  p.a_fmt = a_fmt, p.b_fmt = b_fmt, p.b_ready = b_ready;
   output_params(p, c, ldc, out_kind, status);
   return 0;
 }
@@ -1105,18 +1101,18 @@ extern "C" int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* 
   return launch_small<16, true>(o, stream);
 }
 
+// b_ready: B is not written by the kernel before this one, and was complete before that started
 extern "C" int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
                             long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind,
-                            int after, int* status, void* stream_v) {
+                            int b_ready, int* status, void* stream_v) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   Fp8Product o;
-  const int e = product_params(&o, a, a_sf, lda, a_fmt, b, b_sf, ldb, b_fmt, M, N, K, c, ldc, out_kind, after, status);
+  const int e = product_params(&o, a, a_sf, lda, a_fmt, b, b_sf, ldb, b_fmt, M, N, K, c, ldc, out_kind, b_ready, status);
   return e ? e : launch_product(o, static_cast<cudaStream_t>(stream_v));
 }
 
 // The two gradients of a linear layer, dx [M, K] = dy [M, N] wt [K, N]^T and dw [N, K] (+)= dyt [N, M] xt [K, M]^T, in
-// one launch where that fills the SMs better than one after the other.  The stream's last launch wrote some of the
-// operands and neither result.
+// one launch where that fills the SMs better than one after the other.
 extern "C" int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long ld_dy, const void* wt, const void* wt_sf,
                                   long long ld_wt, const void* dyt, const void* dyt_sf, long long ld_dyt,
                                   const void* xt, const void* xt_sf, long long ld_xt, int grad_fmt, int M, int N, int K,
@@ -1126,13 +1122,12 @@ extern "C" int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long l
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   Fp8Product x, w;
   int e = product_params(&x, dy, dy_sf, ld_dy, grad_fmt, wt, wt_sf, ld_wt, FP8_E4M3, M, K, N, dx, lddx, dx_kind,
-                         AFTER_OPERANDS, status);
+                         0, status);
   if (!e)
     e = product_params(&w, dyt, dyt_sf, ld_dyt, grad_fmt, xt, xt_sf, ld_xt, FP8_E4M3, N, K, M, dw, lddw, dw_kind,
-                       AFTER_ANY, status);
+                       0, status);
   if (e) return e;
   const GradsPlan plan = plan_grads(M, N, K);
-  if (plan.bn) w.p.after = AFTER_OPERANDS;
   if (plan.bn == 256) return launch_together<256>(plan.x_first ? x : w, plan.x_first ? w : x, plan.head, stream);
   if (plan.bn == 128) return launch_together<128>(plan.x_first ? x : w, plan.x_first ? w : x, plan.head, stream);
   if ((e = launch_product(x, stream))) return e;

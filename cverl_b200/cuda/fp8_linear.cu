@@ -9,7 +9,7 @@ int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, 
                      void* q, void* sf, void* ps, long long q_ld, void* qt, void* sft, void* pst, long long qt_ld,
                      const float* rstd, const void* w, float w_offset, int beside, void* stream);
 int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
-                 long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int after,
+                 long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int b_ready,
                  int* status, void* stream);
 int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long ld_dy, const void* wt, const void* wt_sf,
                        long long ld_wt, const void* dyt, const void* dyt_sf, long long ld_dyt, const void* xt,
@@ -28,7 +28,6 @@ int cvb_fp8_norm_bwd(const float* dn, long long dn_stride, const void* h, long l
 namespace {
 constexpr int E4M3 = 0;
 enum { ROWS = 1, COLS = 2, BLOCKS = 4 };
-enum { AFTER_ANY = 0, AFTER_OPERANDS = 1, AFTER_A = 2 };      // what the launch before a product wrote
 
 struct Mat8 {      // [rows, cols] in a buffer; null buffer: absent
   char* codes;
@@ -46,8 +45,8 @@ int quantize(const void* x, int x_fp32, long long rows, long long cols, long lon
                           nullptr, t.ld, nullptr, nullptr, 0.f, beside, stream);
 }
 int product(const Mat8& a, int a_fmt, const Mat8& b, int b_fmt, int M, int N, int K, void* c, long long ldc,
-            int out_kind, int after, int* status, void* stream) {
-  return cvb_fp8_gemm(a.codes, a.sf, a.ld, a_fmt, b.codes, b.sf, b.ld, b_fmt, M, N, K, c, ldc, out_kind, after, status,
+            int out_kind, bool b_ready, int* status, void* stream) {
+  return cvb_fp8_gemm(a.codes, a.sf, a.ld, a_fmt, b.codes, b.sf, b.ld, b_fmt, M, N, K, c, ldc, out_kind, b_ready, status,
                       stream);
 }
 }  // namespace
@@ -66,7 +65,7 @@ extern "C" int cvb_fp8_linear_fwd(const void* x, int x_fp32, long long x_stride,
     return cvb_fp8_gemm_rows(x, x_stride, mwq.codes, mwq.sf, mwq.ld, E4M3, M, N, K, y, ldy, out_kind, status, stream);
   }
   if (x && (rc = quantize(x, x_fp32, M, K, x_stride, E4M3, 0, mxq, mxt, w != nullptr, stream))) return rc;
-  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, w ? AFTER_OPERANDS : x ? AFTER_A : AFTER_ANY, status,
+  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, x && !w, status,
                  stream);
 }
 
@@ -81,7 +80,7 @@ extern "C" int cvb_fp8_norm_linear_fwd(const void* x, long long x_stride, const 
   if ((rc = cvb_fp8_add_rmsnorm(x, x_stride, resid, r_stride, wn, h, mxq.codes, mxq.sf, nullptr, mxq.ld, rstd, M, K, E4M3,
                                 eps, w_offset, w != nullptr, stream)))
     return rc;
-  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, w ? AFTER_OPERANDS : AFTER_A, status, stream);
+  return product(mxq, E4M3, mwq, E4M3, M, N, K, y, ldy, out_kind, !w, status, stream);
 }
 
 // dx [M, K] = dy w (where wt is given) and dw [N, K] (+)= dy^T x (where dw is given).  `dyq` and `dyt` are workspaces
@@ -94,12 +93,12 @@ extern "C" int cvb_fp8_linear_bwd(const void* dy, int dy_fp32, long long dy_stri
   if (!mdq.codes && !mdt.codes) return 0;
   int rc = quantize(dy, dy_fp32, M, N, dy_stride, grad_fmt, 0, mdq, mdt, 0, stream);
   if (rc) return rc;
-  if (!dw) return product(mdq, grad_fmt, mwt, E4M3, M, K, N, dx, lddx, dx_kind, AFTER_A, status, stream);
+  if (!dw) return product(mdq, grad_fmt, mwt, E4M3, M, K, N, dx, lddx, dx_kind, true, status, stream);
   if (h && (rc = cvb_fp8_quantize(h, 0, M, K, h_stride, E4M3, COLS, nullptr, nullptr, nullptr, 0, mxt.codes, mxt.sf,
                                   nullptr, mxt.ld,
                                   rstd, wn, w_offset, 1, stream)))
     return rc;
-  if (!wt) return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, AFTER_OPERANDS, status, stream);
+  if (!wt) return product(mdt, grad_fmt, mxt, E4M3, N, K, M, dw, lddw, dw_kind, false, status, stream);
   return cvb_fp8_gemm_grads(mdq.codes, mdq.sf, mdq.ld, mwt.codes, mwt.sf, mwt.ld, mdt.codes, mdt.sf, mdt.ld, mxt.codes,
                             mxt.sf, mxt.ld, grad_fmt, M, N, K, dx, lddx, dx_kind, dw, lddw, dw_kind, status, stream);
 }

@@ -10,11 +10,13 @@
 
 namespace cvb {
 
-// `beside`: the kernel reads nothing that the launch before it writes, nor writes what that touches, and runs beside it;
-// it ends after it, so that what follows may rely on both.  All kernels here therefore end with a wait, which returns at
-// once in an ordinary launch.  1301 x 1000 with a weight of 520 rows, forward: 9.9 us, 12.3 one after the other.
+// A kernel may be placed while the one before it in the stream still runs, and lets the next one be placed as soon as it
+// may itself begin.  Ordinarily it begins when that has ended: all that was launched before is then complete, and its own
+// loads are not of the read-only kind, which would allow them to be served from before that.  `beside`: it reads nothing
+// that the launch before it writes, nor writes what that touches, and begins at once; it ends after it, so that what
+// follows may rely on both.  1301 x 1000 with a weight of 520 rows, forward: 9.9 us, 12.3 one after the other.
 template <typename Args>
-static void launch_rows(void (*kernel)(const Args), const Args& p, long long grid, int threads, int beside, cudaStream_t s) {
+static void launch_rows(void (*kernel)(const Args), const Args& p, long long grid, int threads, cudaStream_t s) {
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
@@ -23,7 +25,7 @@ static void launch_rows(void (*kernel)(const Args), const Args& p, long long gri
   cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cfg.attrs = &at;
-  cfg.numAttrs = beside ? 1 : 0;
+  cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -41,7 +43,7 @@ struct QuantArgs {
   uint8_t *ps, *pst;               // scale bytes of each form in plain order [row, block]; may be null
   long long qt_ld;
   int kgroups_t;
-  int col_tiles;
+  int col_tiles, beside;
   // values are x * rstd[row] * (w_offset + w[col]) where rstd is given
   const float* rstd;
   const __nv_bfloat16* w;
@@ -81,7 +83,7 @@ struct Piece<__nv_bfloat16, NORM> {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (r0 + i < p.rows) u = __ldg(reinterpret_cast<const uint4*>(x + i * p.x_stride));
+        if (r0 + i < p.rows) u = *reinterpret_cast<const uint4*>(x + i * p.x_stride);
         raw[i][0] = u.x, raw[i][1] = u.y, raw[i][2] = u.z, raw[i][3] = u.w;
       }
     } else {
@@ -303,7 +305,8 @@ __device__ __forceinline__ bool piece_maxima(const Piece<__nv_bfloat16, false>& 
 template <typename T, int FMT, bool NORM, bool ROWS, bool COLS, bool BLOCK, int CTAS = sizeof(T) == 4 ? 1 : NORM ? 2 : 3>
 __global__ void __launch_bounds__(Q_THREADS, CTAS)
 fp8_quant_kernel(const QuantArgs p) {
-  launch_dependents();             // a product that follows sets itself up meanwhile
+  if (!p.beside) wait_for_previous_kernel();      // see launch_rows
+  launch_dependents();
   __shared__ __align__(16) uint32_t s_max[COLS || BLOCK ? Q_THREADS / 32 : 1][QT / 2];   // column maxima by warp
   __shared__ __align__(16) uint32_t s_inv[COLS ? QT / 2 : 4];      // 2^-e of two columns a word, as bf16
   __shared__ __align__(16) uint8_t s_t[COLS ? QT * QT : 16];       // transposed codes, 8-byte units XOR-swizzled
@@ -440,26 +443,26 @@ fp8_quant_kernel(const QuantArgs p) {
       }
     }
   }
-  wait_for_previous_kernel();      // see launch_rows
+  if (p.beside) wait_for_previous_kernel();
 }
 
 // Four CTAs an SM (64 registers, some spilled) where rows are written and there are eight tiles an SM or more, else three:
 // both forms of 20480 x 3584 57.4 us with three, 53.2 with four; its rows 38.6 and 36.5; its transpose alone 40.2 and 42.1;
 // both forms of 20480 x 1024 (1,280 tiles) 16.6 either way; of 4096 x 2048 (512 tiles) 8.2 and 8.9.
 template <typename T, int FMT>
-static void quant_launch(const QuantArgs& p, int mode, long long grid, int beside, cudaStream_t s) {
+static void quant_launch(const QuantArgs& p, int mode, long long grid, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {
     if (grid > 8 * 148 && mode == 1)
-      return launch_rows(fp8_quant_kernel<T, FMT, false, true, false, false, 4>, p, grid, Q_THREADS, beside, s);
+      return launch_rows(fp8_quant_kernel<T, FMT, false, true, false, false, 4>, p, grid, Q_THREADS, s);
     if (grid > 8 * 148 && mode == 3)
-      return launch_rows(fp8_quant_kernel<T, FMT, false, true, true, false, 4>, p, grid, Q_THREADS, beside, s);
+      return launch_rows(fp8_quant_kernel<T, FMT, false, true, true, false, 4>, p, grid, Q_THREADS, s);
   }
   switch (mode) {
-    case 1: launch_rows(fp8_quant_kernel<T, FMT, false, true, false, false>, p, grid, Q_THREADS, beside, s); break;
-    case 2: launch_rows(fp8_quant_kernel<T, FMT, false, false, true, false>, p, grid, Q_THREADS, beside, s); break;
-    case 3: launch_rows(fp8_quant_kernel<T, FMT, false, true, true, false>, p, grid, Q_THREADS, beside, s); break;
-    case 5: launch_rows(fp8_quant_kernel<T, FP8_E4M3, false, true, false, true>, p, grid, Q_THREADS, beside, s); break;
-    default: launch_rows(fp8_quant_kernel<T, FP8_E4M3, false, true, true, true>, p, grid, Q_THREADS, beside, s); break;
+    case 1: launch_rows(fp8_quant_kernel<T, FMT, false, true, false, false>, p, grid, Q_THREADS, s); break;
+    case 2: launch_rows(fp8_quant_kernel<T, FMT, false, false, true, false>, p, grid, Q_THREADS, s); break;
+    case 3: launch_rows(fp8_quant_kernel<T, FMT, false, true, true, false>, p, grid, Q_THREADS, s); break;
+    case 5: launch_rows(fp8_quant_kernel<T, FP8_E4M3, false, true, false, true>, p, grid, Q_THREADS, s); break;
+    default: launch_rows(fp8_quant_kernel<T, FP8_E4M3, false, true, true, true>, p, grid, Q_THREADS, s); break;
   }
 }
 
@@ -475,7 +478,7 @@ struct NormQuantArgs {
   uint8_t *q, *sf, *ps;       // ps: scale bytes in plain order; may be null
   float* rstd;
   long long rows, x_stride, r_stride, h_stride, q_ld;
-  int D, kgroups, vec;
+  int D, kgroups, vec, beside;
   float eps, w_offset;
 };
 
@@ -503,6 +506,7 @@ struct RowBlock {
 template <int TPR, int NV, int FMT, bool VEC>
 __global__ void __launch_bounds__(RowBlock<TPR>::THREADS)
 fp8_norm_kernel(const NormQuantArgs p) {
+  if (!p.beside) wait_for_previous_kernel();
   launch_dependents();
   constexpr int ROWS = RowBlock<TPR>::ROWS;
   __shared__ float s_part[ROWS][TPR / 32];
@@ -568,19 +572,19 @@ fp8_norm_kernel(const NormQuantArgs p) {
       if (odd) fp8_fix_inf<FMT>(v[i], q + c, n);
     }
   }
-  wait_for_previous_kernel();
+  if (p.beside) wait_for_previous_kernel();
 }
 
 template <int TPR, int NV>
-static void norm_launch(const NormQuantArgs& p, int fmt, int beside, cudaStream_t s) {
+static void norm_launch(const NormQuantArgs& p, int fmt, cudaStream_t s) {
   constexpr int THREADS = RowBlock<TPR>::THREADS;
   const unsigned grid = static_cast<unsigned>((p.rows + THREADS / TPR - 1) / (THREADS / TPR));
   if (p.vec) {
-    if (fmt == FP8_E4M3) launch_rows(fp8_norm_kernel<TPR, NV, FP8_E4M3, true>, p, grid, THREADS, beside, s);
-    else launch_rows(fp8_norm_kernel<TPR, NV, FP8_E5M2, true>, p, grid, THREADS, beside, s);
+    if (fmt == FP8_E4M3) launch_rows(fp8_norm_kernel<TPR, NV, FP8_E4M3, true>, p, grid, THREADS, s);
+    else launch_rows(fp8_norm_kernel<TPR, NV, FP8_E5M2, true>, p, grid, THREADS, s);
   } else {
-    if (fmt == FP8_E4M3) launch_rows(fp8_norm_kernel<TPR, NV, FP8_E4M3, false>, p, grid, THREADS, beside, s);
-    else launch_rows(fp8_norm_kernel<TPR, NV, FP8_E5M2, false>, p, grid, THREADS, beside, s);
+    if (fmt == FP8_E4M3) launch_rows(fp8_norm_kernel<TPR, NV, FP8_E4M3, false>, p, grid, THREADS, s);
+    else launch_rows(fp8_norm_kernel<TPR, NV, FP8_E5M2, false>, p, grid, THREADS, s);
   }
 }
 
@@ -791,17 +795,17 @@ extern "C" int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long 
   p.qt = static_cast<uint8_t*>(qt), p.sft = static_cast<uint8_t*>(sft), p.qt_ld = qt_ld;
   p.kgroups_t = static_cast<int>((row_tiles + 3) / 4);
   p.col_tiles = static_cast<int>(col_tiles);
-  p.rstd = rstd, p.w = static_cast<const __nv_bfloat16*>(w), p.w_offset = w_offset;
+  p.rstd = rstd, p.w = static_cast<const __nv_bfloat16*>(w), p.w_offset = w_offset, p.beside = beside;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long grid = row_tiles * col_tiles;
   if (rstd != nullptr) {     // the transposed form of a norm's result: what a weight gradient reads
-    launch_rows(fp8_quant_kernel<__nv_bfloat16, FP8_E4M3, true, false, true, false>, p, grid, Q_THREADS, beside, s);
+    launch_rows(fp8_quant_kernel<__nv_bfloat16, FP8_E4M3, true, false, true, false>, p, grid, Q_THREADS, s);
   } else if (x_fp32) {
-    if (fmt == FP8_E4M3) quant_launch<float, FP8_E4M3>(p, mode, grid, beside, s);
-    else quant_launch<float, FP8_E5M2>(p, mode, grid, beside, s);
+    if (fmt == FP8_E4M3) quant_launch<float, FP8_E4M3>(p, mode, grid, s);
+    else quant_launch<float, FP8_E5M2>(p, mode, grid, s);
   } else {
-    if (fmt == FP8_E4M3) quant_launch<__nv_bfloat16, FP8_E4M3>(p, mode, grid, beside, s);
-    else quant_launch<__nv_bfloat16, FP8_E5M2>(p, mode, grid, beside, s);
+    if (fmt == FP8_E4M3) quant_launch<__nv_bfloat16, FP8_E4M3>(p, mode, grid, s);
+    else quant_launch<__nv_bfloat16, FP8_E5M2>(p, mode, grid, s);
   }
   return static_cast<int>(cudaGetLastError());
 }
@@ -822,16 +826,16 @@ extern "C" int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void
   p.D = D, p.kgroups = ((D + 127) / 128 + 3) / 4;
   p.vec = aligned16(x) && aligned16(resid) && aligned16(w) && aligned16(h) && x_stride % 8 == 0 && r_stride % 8 == 0 &&
           D % 8 == 0;
-  p.eps = eps, p.w_offset = w_offset;
+  p.eps = eps, p.w_offset = w_offset, p.beside = beside;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // the fewest threads that hold a row with at most four vectors each
-  if (D <= 256) norm_launch<32, 1>(p, fmt, beside, s);
-  else if (D <= 512) norm_launch<32, 2>(p, fmt, beside, s);
-  else if (D <= 1024) norm_launch<32, 4>(p, fmt, beside, s);
-  else if (D <= 2048) norm_launch<128, 2>(p, fmt, beside, s);
-  else if (D <= 4096) norm_launch<128, 4>(p, fmt, beside, s);
-  else if (D <= 8192) norm_launch<256, 4>(p, fmt, beside, s);
-  else norm_launch<512, 4>(p, fmt, beside, s);
+  if (D <= 256) norm_launch<32, 1>(p, fmt, s);
+  else if (D <= 512) norm_launch<32, 2>(p, fmt, s);
+  else if (D <= 1024) norm_launch<32, 4>(p, fmt, s);
+  else if (D <= 2048) norm_launch<128, 2>(p, fmt, s);
+  else if (D <= 4096) norm_launch<128, 4>(p, fmt, s);
+  else if (D <= 8192) norm_launch<256, 4>(p, fmt, s);
+  else norm_launch<512, 4>(p, fmt, s);
   return static_cast<int>(cudaGetLastError());
 }
 
