@@ -187,6 +187,7 @@ fp8_gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
     tmem_relinquish();
   }
+  launch_dependents();       // there is room for a quantisation or a norm beside these CTAs, to wait for their end
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
