@@ -643,3 +643,31 @@ def test_overlapped_backward_passes():
 
     for u, v in zip(steps(lambda: None), steps(torch.cuda.synchronize)):
         assert torch.equal(u, v)
+
+
+def test_two_threads_launch_into_one_stream():
+    """Forward and backward passes of two host threads mix their launches in one stream."""
+    import threading
+
+    def work(m, seed, steps, out):
+        x, w = _rand(m, 512, seed=seed).requires_grad_(), _rand(640, 512, seed=seed + 1, std=0.05).requires_grad_()
+        wn, dy = _rand(512, seed=seed + 2, std=0.1).requires_grad_(), _rand(m, 640, seed=seed + 3)
+        for i in range(steps):
+            y = ops.linear_fp8(x, w)
+            g = torch.autograd.grad(y, (x, w), dy)
+            z, h = ops.add_rmsnorm_linear_fp8(x, None, wn, w)
+            k = torch.autograd.grad(z, (x, wn, w), dy)
+            out[:] = [y.detach(), z.detach(), *g, *k]
+
+    want, got = {}, {}
+    for m in (40, 600):
+        work(m, m, 1, want.setdefault(m, []))
+    for _ in range(3):
+        threads = [threading.Thread(target=work, args=(m, m, 40, got.setdefault(m, []))) for m in (40, 600)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        for m in want:
+            assert len(got[m]) == len(want[m]) == 7 and all(torch.equal(a, b) for a, b in zip(got[m], want[m]))
