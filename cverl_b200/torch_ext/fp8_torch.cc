@@ -147,6 +147,7 @@ Forward forward(const Tensor& x, const Tensor& xq, int64_t M, int64_t K, const W
   }
   if (M == 0 || N == 0 || K == 0) {
     f.y.zero_();
+    if (has_resid && M && K) at::add_out(f.h, x, *resid);   // no columns in y: the sum is a result all the same
     return f;
   }
   const bool convert = !wt.wq.defined();

@@ -671,3 +671,26 @@ def test_two_threads_launch_into_one_stream():
         torch.cuda.synchronize()
         for m in want:
             assert len(got[m]) == len(want[m]) == 7 and all(torch.equal(a, b) for a, b in zip(got[m], want[m]))
+
+
+@pytest.mark.parametrize("shape", [(40, 96), (2, 3, 129)])
+def test_a_weight_without_rows_leaves_the_sum(shape):
+    """y has no columns; x + resid and its gradients are what they always are."""
+    def poison():                       # what the allocator hands out next
+        torch.full(shape, 7.0, dtype=torch.bfloat16, device="cuda")
+
+    x, r, wn = _rand(*shape, seed=1), _rand(*shape, seed=2), _rand(shape[-1], seed=3, std=0.1)
+    w, dh = torch.empty(0, shape[-1], dtype=torch.bfloat16, device="cuda"), _rand(*shape, seed=4)
+    for weight in (w, ops.quantize_fp8_weight(w)):
+        poison()
+        with torch.no_grad():
+            y, h = ops.add_rmsnorm_linear_fp8(x, r, wn, weight)
+        assert y.shape == (*shape[:-1], 0) and torch.equal(h, x + r)
+    leaves = [t.clone().requires_grad_() for t in (x, r, wn, w)]
+    poison()
+    y, h = ops.add_rmsnorm_linear_fp8(*leaves)
+    assert torch.equal(h, x + r)
+    dx, dr, dwn, dw = torch.autograd.grad((y, h), leaves, (torch.empty_like(y), dh))
+    assert torch.equal(dx, dh) and torch.equal(dr, dh) and not dwn.any() and dw.shape == w.shape
+    y, h = ops.add_rmsnorm_linear_fp8(x, None, wn, w)
+    assert h is x and y.numel() == 0
