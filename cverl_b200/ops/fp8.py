@@ -81,7 +81,7 @@ class Fp8Tensor:
 
     def __init__(self, buf: torch.Tensor, rows: int, cols: int, dtype: torch.dtype):
         if (buf.dtype != torch.uint8 or buf.dim() != 1 or buf.numel() != _nbytes(rows, cols) + _nbytes_plain(rows, cols)
-                or buf.storage_offset() or dtype not in _FMT):
+                or not buf.is_contiguous() or buf.storage_offset() or dtype not in _FMT):
             raise ValueError(f"Fp8Tensor: not a buffer of a [{rows}, {cols}] matrix in {dtype}")
         self.buf, self.rows, self.cols, self.dtype = buf, rows, cols, dtype
         self.ld = (cols + 15) // 16 * 16

@@ -207,3 +207,14 @@ def test_refusals():
     for err, call in bad:
         with pytest.raises(err):
             call()
+
+
+def test_a_buffer_that_is_not_one_run_of_bytes_is_refused():
+    """The kernels read a buffer from its first byte on, whatever its strides say."""
+    q = ops.quantize_fp8(torch.ones(3, 8))
+    n = q.buf.numel()
+    for buf in (torch.zeros(1, dtype=torch.uint8).expand(n), torch.zeros(2 * n, dtype=torch.uint8)[::2],
+                torch.zeros(n + 16, dtype=torch.uint8)[16:], q.buf.view(1, n), q.buf.view(torch.int8)):
+        with pytest.raises(ValueError, match="not a buffer"):
+            ops.Fp8Tensor(buf, 3, 8, E4M3)
+    assert torch.equal(ops.Fp8Tensor(q.buf.clone(), 3, 8, E4M3).dequantize(), torch.ones(3, 8))
