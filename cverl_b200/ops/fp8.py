@@ -80,6 +80,8 @@ class Fp8Tensor:
     __slots__ = ("buf", "rows", "cols", "dtype", "ld")
 
     def __init__(self, buf: torch.Tensor, rows: int, cols: int, dtype: torch.dtype):
+        if not (0 <= rows <= MAX_EXTENT and 0 <= cols <= MAX_EXTENT):
+            raise ValueError(f"Fp8Tensor: at most {MAX_EXTENT} rows and columns, got [{rows}, {cols}]")
         if (buf.dtype != torch.uint8 or buf.dim() != 1 or buf.numel() != _nbytes(rows, cols) + _nbytes_plain(rows, cols)
                 or not buf.is_contiguous() or buf.storage_offset() or dtype not in _FMT):
             raise ValueError(f"Fp8Tensor: not a buffer of a [{rows}, {cols}] matrix in {dtype}")
@@ -267,6 +269,8 @@ def _check_norm(x, resid, w, what):
     shape = x.shape
     if not shape or not 1 <= shape[-1] <= MAX_NORM_WIDTH:
         raise ValueError(f"{what}: a last dimension of 1 to {MAX_NORM_WIDTH} is wanted, got shape {tuple(shape)}")
+    if x.numel() // shape[-1] > MAX_EXTENT:
+        raise ValueError(f"{what}: at most {MAX_EXTENT} rows, got shape {tuple(shape)}")
     if (x.is_cuda or w.is_cuda) and (x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16):
         raise TypeError(f"{what}: bfloat16 is wanted on the GPU, got {x.dtype} and a weight in {w.dtype}")
     if w.dim() != 1 or w.shape[0] != shape[-1] or w.device != x.device:

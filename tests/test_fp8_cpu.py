@@ -218,3 +218,16 @@ def test_a_buffer_that_is_not_one_run_of_bytes_is_refused():
         with pytest.raises(ValueError, match="not a buffer"):
             ops.Fp8Tensor(buf, 3, 8, E4M3)
     assert torch.equal(ops.Fp8Tensor(q.buf.clone(), 3, 8, E4M3).dequantize(), torch.ones(3, 8))
+
+
+@pytest.mark.parametrize("rows", [2 ** 31 - 1023, 2 ** 31, -1])
+def test_sizes_beyond_32_bits_are_refused_wherever_a_matrix_is_made(rows):
+    n = max(rows, 0)
+    with pytest.raises(ValueError):
+        ops.Fp8Tensor(torch.empty(n * 16 + -(-n // 128) * 512 + n, dtype=torch.uint8, device="meta"), rows, 1, E4M3)
+    with pytest.raises(ValueError):
+        ops.Fp8Tensor(torch.empty(0, dtype=torch.uint8, device="meta"), 0, rows, E4M3)
+    if rows > 0:
+        x = torch.empty((1, 1), device="meta").expand(rows, 1)
+        with pytest.raises(ValueError, match="rows"):
+            ops.add_rmsnorm_fp8(x, None, torch.empty(1, device="meta"))
