@@ -188,27 +188,34 @@ def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int):
     return (_pack_ref(v, dtype, tall) if mode & _ROWS else None), (_pack_ref(v.t(), dtype, tall) if mode & _COLS else None)
 
 
+def _check_activations(x: torch.Tensor, dtype: torch.dtype, what: str) -> torch.Tensor:
+    _check_dtype(dtype, what)
+    _check_matrix(x, what)
+    if _needs_grad(x):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or linear_fp8 on the tensor itself")
+    return x
+
+
 def quantize_fp8(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
-    """``x [R, C]`` (bf16 or fp32) in 8 bits, one scale per 128 elements of a row."""
-    _check_dtype(dtype, "quantize_fp8")
-    return _quantize(_check_matrix(x, "quantize_fp8"), dtype, _ROWS)[0]
+    """``x [R, C]`` (bf16 or fp32) in 8 bits, one scale per 128 elements of a row.  This, the transpose and the pair have
+    no gradient and refuse an input that asks for one: ``linear_fp8`` rounds and differentiates."""
+    return _quantize(_check_activations(x, dtype, "quantize_fp8"), dtype, _ROWS)[0]
 
 
 def quantize_fp8_t(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Fp8Tensor:
     """``x.T [C, R]`` in 8 bits, one scale per 128 rows of ``x``."""
-    _check_dtype(dtype, "quantize_fp8_t")
-    return _quantize(_check_matrix(x, "quantize_fp8_t"), dtype, _COLS)[1]
+    return _quantize(_check_activations(x, dtype, "quantize_fp8_t"), dtype, _COLS)[1]
 
 
 def quantize_fp8_pair(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Tuple[Fp8Tensor, Fp8Tensor]:
     """``(quantize_fp8(x), quantize_fp8_t(x))`` from one read of ``x``."""
-    _check_dtype(dtype, "quantize_fp8_pair")
-    return _quantize(_check_matrix(x, "quantize_fp8_pair"), dtype, _ROWS | _COLS)
+    return _quantize(_check_activations(x, dtype, "quantize_fp8_pair"), dtype, _ROWS | _COLS)
 
 
 def quantize_fp8_weight(w: torch.Tensor, transposed: bool = True) -> Fp8Weight:
     """A weight ``[N, K]`` in e4m3 with one scale per 128 x 128 block.  ``transposed=False`` leaves the transpose out,
-    which only gradients of the layer's input need."""
+    which only gradients of the layer's input need.  A copy without history, of a parameter too: ``linear_fp8`` takes
+    both where the parameter trains."""
     q, t = _quantize(_check_matrix(w, "quantize_fp8_weight"), E4M3, _ROWS | _TILES | (_COLS if transposed else 0))
     return Fp8Weight(q, t)
 

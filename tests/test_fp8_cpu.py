@@ -231,3 +231,16 @@ def test_sizes_beyond_32_bits_are_refused_wherever_a_matrix_is_made(rows):
         x = torch.empty((1, 1), device="meta").expand(rows, 1)
         with pytest.raises(ValueError, match="rows"):
             ops.add_rmsnorm_fp8(x, None, torch.empty(1, device="meta"))
+
+
+@pytest.mark.parametrize("quantize", [ops.quantize_fp8, ops.quantize_fp8_t, ops.quantize_fp8_pair])
+def test_quantising_what_asks_for_a_gradient_is_refused(quantize):
+    """The 8-bit form has no history: a product of it would drop the gradient without a word."""
+    x, w = torch.ones(4, 8, requires_grad=True), torch.ones(3, 8, requires_grad=True)
+    for t in (x, x * 2):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            quantize(t)
+        with torch.no_grad():
+            quantize(t)
+        quantize(t.detach())
+    assert not ops.linear_fp8(ops.quantize_fp8(x.detach()), ops.quantize_fp8_weight(w)).requires_grad    # kept weights are copies
