@@ -248,6 +248,8 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
             raise TypeError(f"gemm_fp8_nt: out has dtype {out.dtype}")
         if accumulate and out.dtype != torch.float32:
             raise TypeError("gemm_fp8_nt: accumulate needs a float32 out")
+        if _needs_grad(out):
+            raise RuntimeError("gemm_fp8_nt has no gradient: call it under torch.no_grad() for an out that asks for one")
         if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"gemm_fp8_nt: out has strides {out.stride()}: rows of unit stride that do not overlap are wanted")
     if M == 0 or N == 0:

@@ -244,3 +244,14 @@ def test_quantising_what_asks_for_a_gradient_is_refused(quantize):
             quantize(t)
         quantize(t.detach())
     assert not ops.linear_fp8(ops.quantize_fp8(x.detach()), ops.quantize_fp8_weight(w)).requires_grad    # kept weights are copies
+
+
+def test_a_product_into_what_asks_for_a_gradient_is_refused():
+    a, b = ops.quantize_fp8(torch.ones(4, 8)), ops.quantize_fp8(torch.ones(3, 8))
+    leaf = torch.zeros(4, 3, requires_grad=True)
+    for out in (leaf, leaf * 1):
+        for acc in (False, True):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                ops.gemm_fp8_nt(a, b, out, accumulate=acc)
+    with torch.no_grad():
+        assert (ops.gemm_fp8_nt(a, b, leaf) == 8).all()
