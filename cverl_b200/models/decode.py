@@ -336,7 +336,8 @@ class GraphedDecoder:
     ``step(tokens)`` copies the tokens into the graph's input buffer, replays, and returns the graph's logits
     buffer (valid until the next ``step``).  The caches, the recurrent states, the length counter and the position
     vector are the tensors of ``state``; the graph updates them in place.  ``fp8`` takes the result of
-    ``fp8_decode_weights(model)``: the projections then read 8-bit weights, half the bytes of a step.
+    ``fp8_decode_weights(model)``: the projections then read 8-bit weights, half the bytes of a step.  They are those of
+    the capture for as long as the decoder lives; after the parameters change, make another.
     """
 
     def __init__(self, model, state: DecodeState, batch: int, warmup: int = 2, fp8: Optional[dict] = None):
@@ -347,6 +348,7 @@ class GraphedDecoder:
         if state.dev is None:
             state.to_native(model)
         self.model, self.state = model, state
+        self.fp8 = None if state.fp8 is None else dict(state.fp8)      # the graph holds the weights' addresses
         dev = model.flat.flat.device
         self.tokens = torch.zeros(batch, dtype=torch.long, device=dev)
         # warm-up steps run for real on a side stream (lazy initialisation, allocator pools) and are then undone:

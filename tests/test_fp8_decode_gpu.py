@@ -110,3 +110,20 @@ def test_models_without_the_native_step_are_refused():
     model = Qwen35Model(Qwen35TextConfig.tiny(), dtype=torch.bfloat16, device=torch.device("cuda", 0), with_main_grad=False)
     with pytest.raises(RuntimeError, match="native decode"):
         decode.fp8_decode_weights(model)
+
+
+def test_a_captured_decoder_keeps_its_weights():
+    """The graph reads the weights that it was captured with, also after the state has been given others."""
+    from cverl_b200.models import decode
+    model, ids = _model(), _ids(2)
+    want = _steps(model, ids, decode.fp8_decode_weights(model), graphed=True)
+    with torch.no_grad():
+        state, _ = decode.prefill(model, ids[:, :64], max_len=70)
+        runner = decode.GraphedDecoder(model, state, 2, fp8=decode.fp8_decode_weights(model))
+        sizes = [w.w.buf.numel() for w in state.fp8.values()]
+        state.fp8 = None
+        waste = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in sizes]     # what freed memory would become
+        got = [runner.step(ids[:, t]).clone() for t in range(64, 70)]
+    del waste
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
