@@ -133,8 +133,9 @@ class PolicyRolloutWorker(RolloutWorker):
 
 class CachedQwenRolloutWorker(RolloutWorker):
     """Cached decode over a ``Qwen35Model`` (see ``cverl_b200.models.decode``).  With ``fp8`` the decode steps read the
-    projections' weights in 8 bits, converted from the parameters at the start of every ``generate``; the log-probs
-    are then those of the 8-bit policy."""
+    projections' weights in 8 bits, converted from the parameters at the start of every ``generate``.  The prompt is run
+    on the bf16 weights all the same: the first token and its log-prob are the bf16 policy's, those after it come from
+    8-bit projections over the caches and recurrent states that the bf16 prompt pass left."""
 
     def __init__(self, model, pad_id: int = 0, fp8: bool = False):
         self.model = model

@@ -127,3 +127,22 @@ def test_a_captured_decoder_keeps_its_weights():
     del waste
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_which_policy_the_log_probs_come_from():
+    """The first from the prompt's pass on the bf16 weights, the others from 8-bit steps over the caches it left."""
+    from cverl_b200.models import decode
+    from cverl_b200.rollout.worker import CachedQwenRolloutWorker, GenerationConfig, TokenBatch, sample_next_tokens
+    model, ids = _model(), _ids(3)[:, :64].contiguous()
+    batch = TokenBatch(ids, torch.ones_like(ids), torch.full((3,), 64, device="cuda"))
+    cfg = GenerationConfig(max_new_tokens=3, temperature=0.0, eos_token_id=-1, seed=0)
+    eight, sixteen = (CachedQwenRolloutWorker(model, fp8=f).generate(batch, cfg) for f in (True, False))
+    assert torch.equal(eight.logprobs[:, 0], sixteen.logprobs[:, 0])
+    assert not torch.equal(eight.logprobs[:, 1], sixteen.logprobs[:, 1])
+    with torch.no_grad():
+        state, logits = decode.prefill(model, ids, max_len=67)
+        state.fp8 = decode.fp8_decode_weights(model)
+        for t in range(3):
+            tok, lp = sample_next_tokens(logits, cfg, None)
+            assert torch.equal(eight.token_ids[:, t], tok) and torch.equal(eight.logprobs[:, t], lp)
+            logits = decode.decode_step(model, state, tok)
