@@ -694,3 +694,47 @@ def test_a_weight_without_rows_leaves_the_sum(shape):
     assert torch.equal(dx, dh) and torch.equal(dr, dh) and not dwn.any() and dw.shape == w.shape
     y, h = ops.add_rmsnorm_linear_fp8(x, None, wn, w)
     assert h is x and y.numel() == 0
+
+
+# rows per CTA 8, 4, 2 and 1 of the norm's backward pass, one row to more than its CTAs hold at once
+@pytest.mark.parametrize("m,k", [(1, 200), (1301, 200), (37, 400), (900, 1000), (2100, 1024), (150, 2048), (40, 4100),
+                                 (9, 8192), (300, 16384)])
+def test_norm_gradients_keep_fp32_between_product_and_norm(m, k):
+    """dy and w are whole numbers that 8 bits hold, so dn = dy w is exact in fp32, and mostly not in bf16."""
+    n = 600
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    dy, w = (torch.randint(-8, 9, s, device="cuda", generator=g).bfloat16() for s in ((m, n), (n, k)))
+    x, r, wn, dh = _rand(m, k, seed=1), _rand(m, k, seed=2), _rand(k, seed=3, std=0.1), _rand(m, k, seed=4)
+    dn = dy.double() @ w.double()
+    assert dn.abs().max() < 2 ** 24
+    _, h, rstd = orc.norm(x, r, wn, EPS, 1.0)
+    xh, gain = h.double() * rstd, 1.0 + wn.double()
+    # rstd: k / 2 + 8 half steps (see test_norm); the mean of g xh: k additions; a handful of products and sums
+    fp32 = (1.5 * k + 16) * 2.0 ** -24
+    size = (rstd * dn * gain).abs() + rstd * xh.abs() * (dn * gain * xh).abs().mean(-1, keepdim=True) + dh.double().abs()
+    want, dwn = orc.norm_grads(h, rstd, wn, 1.0, dn, dh)
+    near = 2.0 ** -8 * want.abs() + fp32 * (1 + 2.0 ** -8) * size
+    leaves = [t.requires_grad_() for t in (x, r, wn)]
+    y, h_out = ops.add_rmsnorm_linear_fp8(*leaves, ops.quantize_fp8_weight(w), EPS, 1.0)
+    dx, dr, dw16 = torch.autograd.grad((y, h_out), leaves, (dy, dh), retain_graph=True)
+    assert torch.equal(dx, dr) and ((dx.double() - want).abs() <= near).all()
+    if m * k > 10000:                              # a bf16 rounding of dn would show
+        rounded, _ = orc.norm_grads(h, rstd, wn, 1.0, dn.bfloat16().double(), dh)
+        assert not ((rounded.bfloat16().double() - want).abs() <= near).all()
+    # m additions, and rstd's half steps
+    sums = (m + k / 2 + 16) * 2.0 ** -24 * (dn * xh).abs().sum(0)
+    assert ((dw16.double() - dwn).abs() <= 2.0 ** -8 * dwn.abs() + (1 + 2.0 ** -8) * sums).all()
+    wn.main_grad = torch.zeros(k, device="cuda")
+    torch.autograd.backward((y, h_out), (dy, dh), inputs=[wn], retain_graph=True)
+    assert ((wn.main_grad.double() - dwn).abs() <= sums).all()
+    # one row at a time: every share of the weight's gradient arrives, and none of it in another row's dx
+    for row in {0, m // 3, m // 2, max(m - 2, 0), m - 1}:
+        one = torch.zeros_like(dy)
+        one[row] = dy[row]
+        wn.main_grad.zero_()                       # every pass through the layer adds to it
+        dx, = torch.autograd.grad((y, h_out), (x,), (one, dh), retain_graph=True)
+        e = dn[row] * xh[row]
+        assert ((wn.main_grad.double() - e).abs() <= (k / 2 + 16) * 2.0 ** -24 * e.abs()).all()
+        assert ((dx[row].double() - want[row]).abs() <= near[row]).all()
+        dx[row] = dh[row]
+        assert torch.equal(dx, dh)
