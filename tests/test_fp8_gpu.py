@@ -738,3 +738,38 @@ def test_norm_gradients_keep_fp32_between_product_and_norm(m, k):
         assert ((dx[row].double() - want[row]).abs() <= near[row]).all()
         dx[row] = dh[row]
         assert torch.equal(dx, dh)
+
+
+# the few-rows kernel with tiles of 16 (three), 32, 64 (two, one more last) and 128 rows, K shared by up to eight CTAs, and
+# once CTA pairs
+@pytest.mark.parametrize("m,n,k", [(1, 1000, 640), (16, 513, 3584), (5, 30000, 300), (24, 256, 2048), (40, 1024, 4000),
+                                   (100, 300, 4096), (100, 5000, 1800), (128, 8192, 512), (300, 513, 700)])
+@pytest.mark.parametrize("beside", [0, 3])
+def test_overlapped_accumulating_products(m, n, k, beside):
+    """Products that add to one matrix without a pause between them, their operands and their sum changed on the way."""
+    steps = 30
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = (torch.randint(-8, 9, s, device="cuda", generator=g).bfloat16() for s in ((m, k), (n, k)))
+    step = x.double() @ w.double().t()
+    assert 2 * steps * step.abs().max() < 2 ** 24
+    b = ops.quantize_fp8(w)
+    wide = torch.full((m, n + beside), 5.0, device="cuda")
+    out = wide[:, beside:]
+    out.zero_()
+    want, sign = torch.zeros_like(step), 1
+    torch.cuda.synchronize()
+    for i in range(steps):
+        a = ops.quantize_fp8(x)
+        ops.gemm_fp8_nt(a, b, out, accumulate=True)
+        want += sign * step
+        if i % 4 != 3:
+            ops.gemm_fp8_nt(a, b, out, accumulate=True)
+            want += sign * step
+        if i % 3 == 1:
+            x.neg_()
+            sign = -sign
+        if i % 5 == 2:
+            out.neg_()
+            want.neg_()
+    assert torch.equal(out.double(), want)
+    assert (wide[:, :beside] == 5.0).all()
