@@ -125,6 +125,8 @@ def decode_step(model, state: DecodeState, tokens: torch.Tensor) -> torch.Tensor
         if state.dev is None:
             state.to_native(model)
         return decode_step_native(model, state, tokens)
+    if state.fp8 is not None:
+        raise RuntimeError("8-bit projections need the native decode path, which does not support this model / device")
     cfg = model.cfg
     B = tokens.shape[0]
     pos = state.length

@@ -255,3 +255,19 @@ def test_a_product_into_what_asks_for_a_gradient_is_refused():
                 ops.gemm_fp8_nt(a, b, out, accumulate=acc)
     with torch.no_grad():
         assert (ops.gemm_fp8_nt(a, b, leaf) == 8).all()
+
+
+def test_8_bit_weights_without_the_native_step_are_refused():
+    """The PyTorch step reads the parameters: with 8-bit weights in the state it would not do what was asked for."""
+    from cverl_b200.models import decode
+    from cverl_b200.models.config import Qwen35TextConfig
+    from cverl_b200.models.qwen3_5 import Qwen35Model
+    model = Qwen35Model(Qwen35TextConfig.tiny(), dtype=torch.float32, with_main_grad=False)
+    model.init_weights(seed=1)
+    with torch.no_grad():
+        state, logits = decode.prefill(model, torch.arange(8).view(1, 8), max_len=12)
+        decode.decode_step(model, state, logits.argmax(-1))
+        state.fp8 = {}
+        with pytest.raises(RuntimeError, match="native decode"):
+            decode.decode_step(model, state, logits.argmax(-1))
+        assert state.length == 9
