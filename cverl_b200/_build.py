@@ -7,9 +7,9 @@ Shared libraries are produced under ``cverl_b200/lib``:
 * ``libcverl.so`` - the host-side C/C++ runtime (public C ABI of the RL math,
   topology, pipeline schedule, safetensors, tokenizers, reward, transports,
   plugin loader);
-* ``_cverl_torch.so`` - autograd nodes and workspaces in front of the kernel launchers
-  (``torch_ext/*.cc``), a Python extension built against the headers and libraries of the
-  installed ``torch``;
+* ``_cverl_torch.<torch and Python version>.so`` - autograd nodes and workspaces in front of
+  the kernel launchers (``torch_ext/*.cc``), a Python extension built against the headers and
+  libraries of the installed ``torch``;
 * ``libcverl_nccl.so`` - the native NCCL communicator (``nccl/nccl_backend.cc``),
   built against the ``nccl.h`` / ``libnccl.so.2`` of the installed ``nvidia-nccl``
   wheel (the library ``torch`` itself loads), skipped when that wheel is absent.
@@ -22,6 +22,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -32,7 +33,6 @@ OBJ_DIR = ROOT / "build" / "obj"
 CUDA_LIB = LIB_DIR / "libcverl_b200_cuda.so"
 HOST_LIB = LIB_DIR / "libcverl.so"
 NCCL_LIB = LIB_DIR / "libcverl_nccl.so"
-TORCH_EXT = LIB_DIR / "_cverl_torch.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -203,24 +203,30 @@ def build_nccl(force: bool = False, verbose: bool = False) -> Path | None:
     return NCCL_LIB
 
 
-def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
-    import sysconfig
+def torch_ext_path() -> Path:
+    """The extension's file.  It fits one torch and one Python, so their versions are part of its name: after either
+    changes it is built anew instead of being loaded with another layout of their objects."""
+    import torch
+    return LIB_DIR / f"_cverl_torch.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so"
 
+
+def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     import torch
     srcs = sorted((PKG / "torch_ext").glob("*.cc"))
+    path = torch_ext_path()
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    if not force and TORCH_EXT.exists() and TORCH_EXT.stat().st_mtime >= _newest(srcs):
-        return TORCH_EXT
+    if not force and path.exists() and path.stat().st_mtime >= _newest(srcs):
+        return path
     if verbose:
         print("[g++] torch_ext", flush=True)
     root = Path(torch.__file__).resolve().parent
     cuda_home = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
     inc = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_path("include"), cuda_home / "include"]
-    _run([os.environ.get("CXX", "g++"), *CXX_FLAGS, "-shared", f"-DTORCH_EXTENSION_NAME={TORCH_EXT.stem}",
+    _run([os.environ.get("CXX", "g++"), *CXX_FLAGS, "-shared", "-DTORCH_EXTENSION_NAME=_cverl_torch",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{p}" for p in inc), *map(str, srcs),
-          "-o", str(TORCH_EXT), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+          "-o", str(path), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
           "-ltorch", "-ltorch_python"])
-    return TORCH_EXT
+    return path
 
 
 def build_all(force: bool = False, verbose: bool = False) -> None:

@@ -187,9 +187,10 @@ def torch_ext():
     if _torch_ext is None:
         import importlib.util
 
+        from ._build import torch_ext_path
         from .ops.gemm import launch_counter
         lib = cuda()
-        path = _LIB_DIR / "_cverl_torch.so"
+        path = torch_ext_path()
         if not path.exists():
             _ensure_built()
         if not path.exists():

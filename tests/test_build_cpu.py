@@ -1,0 +1,48 @@
+"""Which built files count as current."""
+import os
+
+import pytest
+import torch
+
+from cverl_b200 import _build
+from cverl_b200 import _native as nv
+
+
+@pytest.fixture
+def builds(monkeypatch, tmp_path):
+    """Output paths of the compilations that build_torch_ext starts, in a folder of its own."""
+    made = []
+
+    def run(cmd, log_path=None):
+        out = cmd[cmd.index("-o") + 1]
+        made.append(out)
+        open(out, "w").close()
+
+    monkeypatch.setattr(_build, "LIB_DIR", tmp_path)
+    monkeypatch.setattr(_build, "_run", run)
+    return made
+
+
+def test_the_extension_is_built_once(builds):
+    first = _build.build_torch_ext()
+    assert builds == [str(first)] and first == _build.torch_ext_path()
+    assert _build.build_torch_ext() == first and len(builds) == 1
+    os.utime(first, (0, 0))                                        # older than its sources
+    assert _build.build_torch_ext() == first and len(builds) == 2
+
+
+def test_another_torch_or_python_takes_another_extension(builds, monkeypatch):
+    first = _build.build_torch_ext()
+    monkeypatch.setattr(torch, "__version__", "9.9.9+other")
+    second = _build.build_torch_ext()
+    assert second != first and len(builds) == 2
+    monkeypatch.setattr(_build.sysconfig, "get_config_var", lambda name: "cpython-399-other")
+    assert _build.build_torch_ext() not in (first, second) and len(builds) == 3
+
+
+def test_an_extension_of_another_torch_is_not_loaded(monkeypatch):
+    monkeypatch.setattr(nv, "_torch_ext", None)
+    monkeypatch.setattr(torch, "__version__", "9.9.9+other")
+    monkeypatch.setenv("CVERL_B200_NO_AUTOBUILD", "1")
+    with pytest.raises(RuntimeError, match="native extension missing"):
+        nv.torch_ext()
