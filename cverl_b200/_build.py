@@ -215,13 +215,14 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     srcs = sorted((PKG / "torch_ext").glob("*.cc"))
     path = torch_ext_path()
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    if not force and path.exists() and path.stat().st_mtime >= _newest(srcs):
+    if not force and path.exists() and path.stat().st_mtime >= _newest([*srcs, PKG / "cuda" / "fp8_launch.h"]):
         return path
     if verbose:
         print("[g++] torch_ext", flush=True)
     root = Path(torch.__file__).resolve().parent
     cuda_home = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
-    inc = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_path("include"), cuda_home / "include"]
+    inc = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_path("include"), cuda_home / "include",
+           PKG / "cuda"]
     _run([os.environ.get("CXX", "g++"), *CXX_FLAGS, "-shared", "-DTORCH_EXTENSION_NAME=_cverl_torch",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{p}" for p in inc), *map(str, srcs),
           "-o", str(path), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",

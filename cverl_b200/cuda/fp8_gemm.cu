@@ -8,6 +8,7 @@
 // four instructions that name the same scale byte.  Nothing is rescaled outside the tensor core, so the accumulator
 // stays in TMEM over all of K.
 #include "fp8_common.cuh"
+#include "fp8_launch.h"
 #include "gemm_tcgen05.h"
 #include <atomic>
 

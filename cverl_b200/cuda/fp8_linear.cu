@@ -2,28 +2,7 @@
 // the calls than in the kernels (five ctypes calls of a 77-token layer's step took longer than its ten launches).
 //
 // Buffers of 8-bit matrices are codes (rows padded to 16 bytes) followed by the scale cells.
-#include <cuda_runtime.h>
-
-extern "C" {
-int cvb_fp8_quantize(const void* x, int x_fp32, long long rows, long long cols, long long x_stride, int fmt, int mode,
-                     void* q, void* sf, void* ps, long long q_ld, void* qt, void* sft, void* pst, long long qt_ld,
-                     const float* rstd, const void* w, float w_offset, int beside, void* stream);
-int cvb_fp8_gemm(const void* a, const void* a_sf, long long lda, int a_fmt, const void* b, const void* b_sf,
-                 long long ldb, int b_fmt, int M, int N, int K, void* c, long long ldc, int out_kind, int b_ready,
-                 int* status, void* stream);
-int cvb_fp8_gemm_grads(const void* dy, const void* dy_sf, long long ld_dy, const void* wt, const void* wt_sf,
-                       long long ld_wt, const void* dyt, const void* dyt_sf, long long ld_dyt, const void* xt,
-                       const void* xt_sf, long long ld_xt, int grad_fmt, int M, int N, int K, void* dx, long long lddx,
-                       int dx_kind, void* dw, long long lddw, int dw_kind, int* status, void* stream);
-int cvb_fp8_gemm_rows(const void* x, long long x_stride, const void* b, const void* b_sf, long long ldb, int b_fmt,
-                      int M, int N, int K, void* c, long long ldc, int out_kind, int* status, void* stream);
-int cvb_fp8_add_rmsnorm(const void* x, long long x_stride, const void* resid, long long r_stride, const void* w, void* h,
-                        void* q, void* sf, void* ps, long long q_ld, float* rstd, long long rows, int D, int fmt, float eps,
-                        float w_offset, int beside, void* stream);
-int cvb_fp8_norm_bwd(const float* dn, long long dn_stride, const void* h, long long h_stride, const void* w,
-                     const float* rstd, const void* dh, long long dh_stride, void* dx, float* part, float* dw_acc,
-                     void* dw, long long rows, int D, float w_offset, void* stream);
-}
+#include "fp8_launch.h"
 
 namespace {
 constexpr int E4M3 = 0;

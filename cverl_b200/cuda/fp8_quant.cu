@@ -7,6 +7,7 @@
 // shuffles and a column block's is eight values per thread and one shared-memory maximum.  Both forms come from the
 // registers of the one read; only the transposed codes pass through shared memory.
 #include "fp8_common.cuh"
+#include "fp8_launch.h"
 
 namespace cvb {
 

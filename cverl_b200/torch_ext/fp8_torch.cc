@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
+#include "fp8_launch.h"
 
 namespace {
 
@@ -20,27 +21,19 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
-typedef long long ll;
 
 // ---------------------------------------------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------------------------------------------
 struct Launchers {
-  int (*quantize)(const void*, int, ll, ll, ll, int, int, void*, void*, void*, ll, void*, void*, void*, ll, const float*,
-                  const void*, float, int, void*);
-  int (*add_rmsnorm)(const void*, ll, const void*, ll, const void*, void*, void*, void*, void*, ll, float*, ll, int, int,
-                     float, float, int, void*);
-  int (*linear_fwd)(const void*, int, ll, const void*, int, ll, int, int, int, void*, void*, void*, void*, void*, ll, int,
-                    int*, void*);
-  int (*linear_bwd)(const void*, int, ll, int, int, int, int, void*, void*, void*, void*, const void*, ll, const float*,
-                    const void*, float, void*, ll, int, void*, ll, int, int*, void*);
-  int (*norm_linear_fwd)(const void*, ll, const void*, ll, const void*, void*, float*, float, float, const void*, int, ll,
-                         int, int, int, void*, void*, void*, void*, ll, int, int*, void*);
-  int (*norm_linear_bwd)(const void*, int, ll, int, int, int, int, void*, void*, void*, void*, const void*, ll,
-                         const float*, const void*, float, float*, ll, void*, ll, int, const void*, ll, void*, float*,
-                         float*, void*, int*, void*);
-  int (*norm_bwd_parts)();
-  int (*gemm_grads_launches)(int, int, int);
+  decltype(&cvb_fp8_quantize) quantize;
+  decltype(&cvb_fp8_add_rmsnorm) add_rmsnorm;
+  decltype(&cvb_fp8_linear_fwd) linear_fwd;
+  decltype(&cvb_fp8_linear_bwd) linear_bwd;
+  decltype(&cvb_fp8_norm_linear_fwd) norm_linear_fwd;
+  decltype(&cvb_fp8_norm_linear_bwd) norm_linear_bwd;
+  decltype(&cvb_fp8_norm_bwd_parts) norm_bwd_parts;
+  decltype(&cvb_fp8_gemm_grads_launches) gemm_grads_launches;
 } fn;
 
 PyObject* launch_counter = nullptr;   // ops.gemm.launch_counter

@@ -46,3 +46,25 @@ def test_an_extension_of_another_torch_is_not_loaded(monkeypatch):
     monkeypatch.setenv("CVERL_B200_NO_AUTOBUILD", "1")
     with pytest.raises(RuntimeError, match="native extension missing"):
         nv.torch_ext()
+
+
+def test_8_bit_launchers_are_declared_once_and_bound_as_declared():
+    """The header that the kernels and the extension are compiled against, letter by letter against the ctypes binding."""
+    import re
+    text = re.sub(r"//.*", "", (_build.PKG / "cuda" / "fp8_launch.h").read_text())
+    letters = {"int": "i", "long long": "l", "float": "f"}
+    declared = {}
+    for name, args in re.findall(r"\bint (cvb_fp8_\w+)\(([^)]*)\);", text):
+        kinds = [re.sub(r"\s*\w+$", "", a.strip()) for a in args.split(",") if a.strip() not in ("", "void")]
+        declared[name] = "".join("p" if k.endswith("*") else letters[k] for k in kinds)
+    bound = {n: c.replace(" ", "") for n, c in nv._CUDA_PROTOS.items() if n.startswith("cvb_fp8_")}
+    assert set(bound) <= set(declared) and {n: declared[n] for n in bound} == bound
+    for path in [*(_build.PKG / "cuda").glob("fp8_*.cu"), *(_build.PKG / "torch_ext").glob("*.cc")]:
+        assert '#include "fp8_launch.h"' in path.read_text(), path.name
+
+
+def test_the_extension_is_built_anew_when_a_launcher_changes(builds):
+    first = _build.build_torch_ext()
+    at = (_build.PKG / "cuda" / "fp8_launch.h").stat().st_mtime
+    os.utime(first, (at - 1, at - 1))
+    assert _build.build_torch_ext() == first and len(builds) == 2
