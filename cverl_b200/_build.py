@@ -226,7 +226,10 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     _run([os.environ.get("CXX", "g++"), *CXX_FLAGS, "-shared", "-DTORCH_EXTENSION_NAME=_cverl_torch",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{p}" for p in inc), *map(str, srcs),
           "-o", str(path), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
-          "-ltorch", "-ltorch_python"])
+          "-ltorch", "-ltorch_python",
+          # torch's own C++ runtime, by its file: strings, streams and exceptions pass between the two, and a compiler that
+          # finds only the static one would link a second copy in (the first error message with a number crashed)
+          "-l:libstdc++.so.6"])
     return path
 
 

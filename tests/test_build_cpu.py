@@ -68,3 +68,14 @@ def test_the_extension_is_built_anew_when_a_launcher_changes(builds):
     at = (_build.PKG / "cuda" / "fp8_launch.h").stat().st_mtime
     os.utime(first, (at - 1, at - 1))
     assert _build.build_torch_ext() == first and len(builds) == 2
+
+
+def test_errors_of_the_extension_are_python_exceptions():
+    """Messages with numbers in them end the process where the extension brings a C++ runtime of its own beside torch's."""
+    import subprocess
+    import sys
+    code = ("import torch; from cverl_b200 import _native as nv\n"
+            "try: nv.torch_ext().view8(torch.zeros(5, dtype=torch.uint8), 3, 7, 0)\n"
+            "except ValueError as e: print(e)")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=_build.ROOT)
+    assert r.returncode == 0 and "[3, 7] matrix" in r.stdout, (r.returncode, r.stderr[-500:])

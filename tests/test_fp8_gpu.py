@@ -773,3 +773,16 @@ def test_overlapped_accumulating_products(m, n, k, beside):
             want.neg_()
     assert torch.equal(out.double(), want)
     assert (wide[:, :beside] == 5.0).all()
+
+
+def test_a_refusal_of_a_launcher_is_an_exception():
+    """A buffer that does not start on 16 bytes: the launchers refuse it before anything runs."""
+    q, kept = ops.quantize_fp8(_rand(20, 64, seed=1)), ops.quantize_fp8_weight(_rand(30, 64, seed=2))
+    room = torch.empty(q.buf.numel() + 8, dtype=torch.uint8, device="cuda")
+    room[8:] = q.buf
+    odd = ops.Fp8Tensor(torch.from_dlpack(room[8:]), 20, 64, E4M3)
+    assert odd.buf.data_ptr() % 16 == 8
+    for call in (lambda: ops.gemm_fp8_nt(odd, kept.w), lambda: ops.linear_fp8(odd, kept)):
+        with pytest.raises(RuntimeError, match="failed with code -3"):
+            call()
+    assert torch.equal(ops.linear_fp8(q, kept), ops.gemm_fp8_nt(q, kept.w))
