@@ -3,6 +3,15 @@
 // compile where it is not followed.  Every launcher returns 0 or an error code; arguments are explained at the definitions.
 #pragma once
 
+// Buffer of an 8-bit matrix [rows, cols]: codes, row-major with rows padded to 16 bytes; the scale cells, 512 bytes per 128
+// rows and 512 columns; and, in buffers that leave the extension, the scale bytes once more in plain order.
+inline long long fp8_row_bytes(long long cols) { return (cols + 15) / 16 * 16; }
+inline long long fp8_code_bytes(long long rows, long long cols) { return rows * fp8_row_bytes(cols); }
+inline long long fp8_operand_bytes(long long rows, long long cols) {      // what the products read
+  return fp8_code_bytes(rows, cols) + (rows + 127) / 128 * ((cols + 511) / 512) * 512;
+}
+inline long long fp8_plain_scale_bytes(long long rows, long long cols) { return rows * ((cols + 127) / 128); }
+
 extern "C" {
 
 // fp8_quant.cu

@@ -1,7 +1,5 @@
 // The launches of an 8-bit linear layer, forward and backward, each behind one call: a small layer spends more time in
 // the calls than in the kernels (five ctypes calls of a 77-token layer's step took longer than its ten launches).
-//
-// Buffers of 8-bit matrices are codes (rows padded to 16 bytes) followed by the scale cells.
 #include "fp8_launch.h"
 
 namespace {
@@ -12,8 +10,8 @@ struct Mat8 {      // [rows, cols] in a buffer; null buffer: absent
   char* codes;
   char* sf;
   long long ld;
-  Mat8(void* buf, long long rows, long long cols) : codes(static_cast<char*>(buf)), sf(nullptr), ld((cols + 15) / 16 * 16) {
-    if (codes) sf = codes + rows * ld;
+  Mat8(void* buf, long long rows, long long cols) : codes(static_cast<char*>(buf)), sf(nullptr), ld(fp8_row_bytes(cols)) {
+    if (codes) sf = codes + fp8_code_bytes(rows, cols);
   }
 };
 

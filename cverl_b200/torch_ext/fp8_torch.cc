@@ -68,10 +68,8 @@ enum { ROWS = 1, COLS = 2 };
 enum { OUT_BF16 = 0, OUT_F32 = 1, OUT_F32_ACC = 2 };
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-// codes and scale cells of an 8-bit matrix: what the products read
-int64_t nbytes(int64_t rows, int64_t cols) { return rows * up(cols, 16) + up(rows, 128) / 128 * (up(cols, 512) / 512) * 512; }
-// the scale bytes once more, in plain order
-int64_t nbytes_plain(int64_t rows, int64_t cols) { return rows * (up(cols, 128) / 128); }
+int64_t nbytes(int64_t rows, int64_t cols) { return fp8_operand_bytes(rows, cols); }
+int64_t nbytes_whole(int64_t rows, int64_t cols) { return nbytes(rows, cols) + fp8_plain_scale_bytes(rows, cols); }
 
 // straight from the allocator: the way through the dispatcher takes as long again
 Tensor fresh(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
@@ -428,12 +426,12 @@ std::pair<OptTensor, OptTensor> quantize(const Tensor& x_in, int64_t fmt, int64_
   const int64_t R = x.size(0), C = x.size(1);
   OptTensor q, t;
   char *qp = nullptr, *tp = nullptr;
-  if (mode & ROWS) q = bytes(nbytes(R, C) + nbytes_plain(R, C), x), qp = ptr(*q);
-  if (mode & COLS) t = bytes(nbytes(C, R) + nbytes_plain(C, R), x), tp = ptr(*t);
+  if (mode & ROWS) q = bytes(nbytes_whole(R, C), x), qp = ptr(*q);
+  if (mode & COLS) t = bytes(nbytes_whole(C, R), x), tp = ptr(*t);
   if (R && C) {
-    check(fn.quantize(ptr(x), fp32(x), R, C, x.stride(0), fmt, mode, qp, qp ? qp + R * up(C, 16) : nullptr,
-                      qp ? qp + nbytes(R, C) : nullptr, up(C, 16), tp, tp ? tp + C * up(R, 16) : nullptr,
-                      tp ? tp + nbytes(C, R) : nullptr, up(R, 16), nullptr, nullptr, 0.f, 0, stream_of(x)),
+    check(fn.quantize(ptr(x), fp32(x), R, C, x.stride(0), fmt, mode, qp, qp ? qp + fp8_code_bytes(R, C) : nullptr,
+                      qp ? qp + nbytes(R, C) : nullptr, fp8_row_bytes(C), tp, tp ? tp + fp8_code_bytes(C, R) : nullptr,
+                      tp ? tp + nbytes(C, R) : nullptr, fp8_row_bytes(R), nullptr, nullptr, 0.f, 0, stream_of(x)),
           "cvb_fp8_quantize");
     count_launches(1);
   }
@@ -445,11 +443,11 @@ std::pair<OptTensor, OptTensor> quantize(const Tensor& x_in, int64_t fmt, int64_
 Tensor view8(const Tensor& buf, int64_t rows, int64_t cols, int64_t fmt) {
   constexpr at::ScalarType types[] = {at::kFloat8_e4m3fn, at::kFloat8_e5m2, at::kFloat8_e8m0fnu};
   TORCH_CHECK_VALUE(fmt >= 0 && fmt < 3 && rows >= 0 && cols >= 0 && buf.scalar_type() == at::kByte &&
-                        buf.numel() == nbytes(rows, cols) + nbytes_plain(rows, cols),
+                        buf.numel() == nbytes_whole(rows, cols),
                     "not a buffer of a [", rows, ", ", cols, "] matrix");
   Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()), buf.key_set(),
                                                       c10::scalarTypeToTypeMeta(types[fmt]));
-  const int64_t width = fmt == 2 ? up(cols, 128) / 128 : cols, ld = fmt == 2 ? width : up(cols, 16);
+  const int64_t width = fmt == 2 ? up(cols, 128) / 128 : cols, ld = fmt == 2 ? width : fp8_row_bytes(cols);
   const int64_t sizes[] = {rows, width}, strides[] = {ld, 1};
   v.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides, buf.storage_offset() + (fmt == 2 ? nbytes(rows, cols) : 0));
   return v;
@@ -461,11 +459,11 @@ std::pair<Tensor, OptTensor> norm(const Tensor& x_in, const OptTensor& resid, co
   at::NoGradGuard no_grad;
   const Tensor x = rows2d(x_in), r = resid ? rows2d(*resid) : Tensor(), wn = unit_stride(w);
   const int64_t R = x.size(0), D = x.size(1);
-  const Tensor q = bytes(nbytes(R, D) + nbytes_plain(R, D), x);
+  const Tensor q = bytes(nbytes_whole(R, D), x);
   const Tensor h = r.defined() ? fresh({R, D}, x.scalar_type(), x) : Tensor();
   if (R) {
     check(fn.add_rmsnorm(ptr(x), x.stride(0), ptr(r), r.defined() ? r.stride(0) : 0, ptr(wn), ptr(h), ptr(q),
-                         ptr(q) + R * up(D, 16), ptr(q) + nbytes(R, D), up(D, 16), nullptr, R, D, fmt, eps, off, 0,
+                         ptr(q) + fp8_code_bytes(R, D), ptr(q) + nbytes(R, D), fp8_row_bytes(D), nullptr, R, D, fmt, eps, off, 0,
                          stream_of(x)),
           "cvb_fp8_add_rmsnorm");
     count_launches(1);

@@ -4,6 +4,7 @@ import torch
 
 import fp8_oracle as orc
 from cverl_b200 import ops
+from cverl_b200.ops import fp8
 from fp8_oracle import E4M3, E5M2
 
 
@@ -271,3 +272,17 @@ def test_8_bit_weights_without_the_native_step_are_refused():
         with pytest.raises(RuntimeError, match="native decode"):
             decode.decode_step(model, state, logits.argmax(-1))
         assert state.length == 9
+
+
+def test_the_buffer_is_laid_out_as_the_kernels_lay_it_out():
+    """Sizes and offsets of the Python side against those that the extension and the launchers are compiled with."""
+    from cverl_b200 import _native as nv
+    view = nv.torch_ext().view8
+    for rows in (0, 1, 3, 127, 128, 129, 1000):
+        for cols in (0, 1, 15, 16, 17, 128, 129, 511, 512, 513, 4100):
+            q = ops.Fp8Tensor(torch.zeros(fp8._nbytes(rows, cols) + fp8._nbytes_plain(rows, cols), dtype=torch.uint8), rows, cols, E4M3)
+            for got, want in ((view(q.buf, rows, cols, 0), q.values), (view(q.buf, rows, cols, 2), q.scales())):
+                assert got.dtype == want.dtype and got.shape == want.shape and got.stride() == want.stride()
+                assert got.storage_offset() == want.storage_offset()
+            with pytest.raises(ValueError, match="not a buffer"):
+                view(torch.zeros(q.buf.numel() + 1, dtype=torch.uint8), rows, cols, 0)
