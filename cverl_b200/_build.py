@@ -215,7 +215,7 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     srcs = sorted((PKG / "torch_ext").glob("*.cc"))
     path = torch_ext_path()
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    if not force and path.exists() and path.stat().st_mtime >= _newest([*srcs, PKG / "cuda" / "fp8_launch.h"]):
+    if not force and path.exists() and path.stat().st_mtime >= _newest([*srcs, PKG / "cuda" / "fp8_launch.h", Path(__file__)]):
         return path
     if verbose:
         print("[g++] torch_ext", flush=True)

@@ -70,6 +70,13 @@ def test_the_extension_is_built_anew_when_a_launcher_changes(builds):
     assert _build.build_torch_ext() == first and len(builds) == 2
 
 
+def test_the_extension_is_built_anew_when_its_recipe_changes(builds):
+    first = _build.build_torch_ext()
+    at = os.stat(_build.__file__).st_mtime
+    os.utime(first, (at - 1, at - 1))
+    assert _build.build_torch_ext() == first and len(builds) == 2
+
+
 def test_errors_of_the_extension_are_python_exceptions():
     """Messages with numbers in them end the process where the extension brings a C++ runtime of its own beside torch's."""
     import subprocess
