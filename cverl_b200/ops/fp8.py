@@ -88,6 +88,13 @@ class Fp8Tensor:
         self.buf, self.rows, self.cols, self.dtype = buf, rows, cols, dtype
         self.ld = (cols + 15) // 16 * 16
 
+    @classmethod
+    def _made(cls, buf: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> "Fp8Tensor":
+        """Around a buffer that the extension has just made for these sizes: the checks take a tenth of a small call."""
+        t = cls.__new__(cls)
+        t.buf, t.rows, t.cols, t.dtype, t.ld = buf, rows, cols, dtype, (cols + 15) // 16 * 16
+        return t
+
     @property
     def shape(self) -> Tuple[int, int]:
         return (self.rows, self.cols)
@@ -182,7 +189,8 @@ def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int):
     R, C = x.shape
     if x.is_cuda:
         q, t = nv.torch_ext().quantize(x, _FMT[dtype], mode)
-        return (Fp8Tensor(q, R, C, dtype) if q is not None else None), (Fp8Tensor(t, C, R, dtype) if t is not None else None)
+        return (Fp8Tensor._made(q, R, C, dtype) if q is not None else None,
+                Fp8Tensor._made(t, C, R, dtype) if t is not None else None)
     tall = BLOCK if mode & _TILES else 1
     v = x.detach().float()
     return (_pack_ref(v, dtype, tall) if mode & _ROWS else None), (_pack_ref(v.t(), dtype, tall) if mode & _COLS else None)
@@ -191,7 +199,7 @@ def _quantize(x: torch.Tensor, dtype: torch.dtype, mode: int):
 def _check_activations(x: torch.Tensor, dtype: torch.dtype, what: str) -> torch.Tensor:
     _check_dtype(dtype, what)
     _check_matrix(x, what)
-    if _needs_grad(x):
+    if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or linear_fp8 on the tensor itself")
     return x
 
@@ -248,7 +256,7 @@ def gemm_fp8_nt(a: Fp8Tensor, b: Fp8Tensor, out: Optional[torch.Tensor] = None, 
             raise TypeError(f"gemm_fp8_nt: out has dtype {out.dtype}")
         if accumulate and out.dtype != torch.float32:
             raise TypeError("gemm_fp8_nt: accumulate needs a float32 out")
-        if _needs_grad(out):
+        if out.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("gemm_fp8_nt has no gradient: call it under torch.no_grad() for an out that asks for one")
         if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"gemm_fp8_nt: out has strides {out.stride()}: rows of unit stride that do not overlap are wanted")
@@ -312,7 +320,7 @@ def add_rmsnorm_fp8(x: torch.Tensor, resid: Optional[torch.Tensor], w: torch.Ten
     D = x.shape[-1]
     if x.is_cuda:
         q, h = nv.torch_ext().norm(x, resid, w, eps, w_offset, _FMT[dtype])
-        return Fp8Tensor(q, x.numel() // D, D, dtype), (x if h is None else h)
+        return Fp8Tensor._made(q, x.numel() // D, D, dtype), (x if h is None else h)
     with torch.no_grad():
         y, h, _ = _norm_ref(_rows2d(x), _rows2d(resid) if resid is not None else None, w, eps, w_offset)
         return _pack_ref(y, dtype), (x if resid is None else h.view(x.shape))
