@@ -868,7 +868,7 @@ static int launch_small(const Fp8Product& o, cudaStream_t stream) {
   // Fill the SMs: one CTA each (two where each still has 8 K blocks), clusters of eight only where there are few of them
   // or each CTA still has 6 K blocks.  One token, N = 1024, K = 3584: 10.2 us with one CTA a tile, 4.3 with eight; 128
   // rows, N = 1024, K = 3584: 6.5 with four, 6.8 with eight; 16 rows, N = 2048, K = 8192: 7.4 with four, 6.2 with eight;
-  // 128 rows, N = K = 8192: 27.0 with one, 17.6 with two, 14.6 with four.
+  // 128 rows, N = K = 8192, weights in L2: 27.0 with one, 17.6 with two, 14.6 with four (19.2 with weights from HBM).
   p.split = 1;
   while (p.split < 8) {
     const int next = p.split * 2, per = p.kblocks / next;
