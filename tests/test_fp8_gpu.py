@@ -786,3 +786,22 @@ def test_a_refusal_of_a_launcher_is_an_exception():
         with pytest.raises(RuntimeError, match="failed with code -3"):
             call()
     assert torch.equal(ops.linear_fp8(q, kept), ops.gemm_fp8_nt(q, kept.w))
+
+
+def test_a_main_grad_that_does_not_fit_is_an_exception():
+    """Raised from the backward pass, before anything is added anywhere."""
+    x, w, wn = _rand(20, 64, seed=1).requires_grad_(), _rand(30, 64, seed=2).requires_grad_(), _rand(64, seed=3).requires_grad_()
+    good, good_n = torch.zeros(30, 64, device="cuda"), torch.zeros(64, device="cuda")
+    for bad, bad_n, err in ((good.bfloat16(), good_n, TypeError), (good.t().contiguous().t(), good_n, TypeError),
+                            (good[:29], good_n, TypeError), (good.cpu(), good_n, TypeError), ("no tensor", good_n, RuntimeError),
+                            (good, good_n.bfloat16(), TypeError)):
+        w.main_grad, wn.main_grad = bad, bad_n
+        if bad is not good:
+            with pytest.raises(err):
+                ops.linear_fp8(x, w).sum().backward()
+        with pytest.raises(err):
+            ops.add_rmsnorm_linear_fp8(x, None, wn, w)[0].sum().backward()
+        assert not good.any() and not good_n.any() and x.grad is None
+    w.main_grad, wn.main_grad = good, good_n
+    ops.add_rmsnorm_linear_fp8(x, None, wn, w)[0].sum().backward()
+    assert good.any() and good_n.any() and x.grad is not None
